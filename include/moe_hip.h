@@ -267,6 +267,113 @@ moe_status moe_plan_set_shared_overlap(moe_plan* plan, int32_t on);
  * and launch counts per stage since the last reset (arrays of MOE_NUM_STAGES). */
 moe_status moe_plan_stage_times(moe_plan* plan, float* ms, int32_t* calls, int32_t reset);
 
+/* ---- Operators beside the layer
+ *
+ * The pieces of a Mixture-of-Experts layer whose experts are not the plan's
+ * SwiGLU (adapted experts, src/model.rs:1416-1446, other activations, biases,
+ * norms on both sides of the block), as calls of their own: no plan, no state.
+ * `device` is the device of every pointer and of `stream`; the caller's current
+ * device is left as it was.  dtype: a moe_dtype of the activations, weights and
+ * gradients.  Alignment, ownership, streams, errors and reproducibility as above;
+ * a workspace is used only while the call's kernels run. */
+
+/* Stable counting sort of the T k assignments by expert: expert ascending, then
+ * t k + j ascending.  topk_idx [T, k]: int32 (index_bytes 4) or int64 (8); an index
+ * outside [0, E) is an assignment without an expert (padding) and is sorted behind
+ * every expert.  The same expert may occur several times in a token.  counts [E],
+ * offsets [E + 1] (offsets[E] = assignments that have an expert), perm [T k]
+ * (position -> t k + j), inv_perm [T k] (t k + j -> position).  1 <= E <= 1024, 1 <= k
+ * <= 16, T k < 2^31.  The workspace may be NULL where
+ * moe_sort_workspace_bytes is 0. */
+size_t moe_sort_workspace_bytes(int64_t num_tokens, int32_t experts_per_tok, int32_t num_experts);
+moe_status moe_sort_tokens(int32_t device, void* stream, int64_t num_tokens,
+                           int32_t experts_per_tok, int32_t num_experts, int32_t index_bytes,
+                           const void* topk_idx, int32_t* counts, int32_t* offsets, int32_t* perm,
+                           int32_t* inv_perm, void* workspace);
+
+/* x_perm[inv_perm[t, j]] = x[t]; rows at or beyond *num_kept (a device int: the
+ * sort's offsets + E) are zeros.  x [T, H], x_perm [T k, H], H a multiple of 8.  The
+ * backward of x is moe_unpermute of the rows' gradient without weights. */
+moe_status moe_permute(int32_t device, void* stream, int32_t dtype, int64_t num_tokens,
+                       int32_t experts_per_tok, int32_t hidden, const int32_t* inv_perm,
+                       const int32_t* num_kept, const void* x, void* x_perm);
+
+/* out[t] = sum_j weights[t, j] y[inv_perm[t, j]] over the assignments that have an
+ * expert, j ascending, in fp32, rounded once.  weights [T, k] fp32, or NULL: 1. */
+moe_status moe_unpermute(int32_t device, void* stream, int32_t dtype, int64_t num_tokens,
+                         int32_t experts_per_tok, int32_t hidden, const int32_t* inv_perm,
+                         const int32_t* num_kept, const void* y, const float* weights, void* out);
+
+/* Backward of moe_unpermute: d_y[inv_perm[t, j]] = weights[t, j] d_out[t] (zeros for an
+ * assignment without an expert) and, when d_weights [T, k] is not NULL, d_weights[t, j] =
+ * <d_out[t], y[inv_perm[t, j]]> (0 without an expert), in fp32. */
+moe_status moe_unpermute_backward(int32_t device, void* stream, int32_t dtype, int64_t num_tokens,
+                                  int32_t experts_per_tok, int32_t hidden,
+                                  const int32_t* inv_perm, const int32_t* num_kept,
+                                  const void* d_out, const void* y, const float* weights,
+                                  void* d_y, float* d_weights);
+
+/* Activations of moe_linear_forward: gelu with the error function, gelu_tanh with
+ * its tanh approximation. */
+typedef enum {
+  MOE_ACT_NONE = 0, MOE_ACT_RELU, MOE_ACT_SILU, MOE_ACT_GELU, MOE_ACT_GELU_TANH
+} moe_activation;
+
+/* y[r] = act(x[r] W_g^T + b_g) + residual[r] for the rows offsets[g] <= r < offsets[g + 1]
+ * of each group g.  x [M, K], weight [G, N, K], bias [G, N] or NULL, residual [M, N] or
+ * NULL, y [M, N]; K = in_features and N = out_features are multiples of 8.  Rows behind
+ * the last group's get y = residual (or 0).  offsets NULL: one weight [N, K] for every
+ * row (num_groups 1).  pre_act [M, N] (or NULL) receives the pre-activation for a
+ * backward.  Offsets that descend or leave [0, M] read as clamped to the running
+ * maximum.  Refused with MOE_ERR_UNSUPPORTED: a weight matrix of 2^31 bytes, more than
+ * 2^26 rows or operands of 2^34 bytes (2^31 in the backward). */
+size_t moe_linear_workspace_bytes(int32_t dtype, int64_t num_rows, int32_t in_features,
+                                  int32_t out_features, int32_t num_groups, int32_t grouped,
+                                  int32_t activation, int32_t backward);
+moe_status moe_linear_forward(int32_t device, void* stream, int32_t dtype, int64_t num_rows,
+                              int32_t in_features, int32_t out_features, int32_t num_groups,
+                              const int32_t* offsets, const void* x, const void* weight,
+                              const void* bias, const void* residual, int32_t activation, void* y,
+                              void* pre_act, void* workspace);
+/* dx [M, K] (0 behind the last group's rows), d_weight [G, N, K] and d_bias [G, N] (0 for a
+ * group without rows), each written unless NULL.  The residual's gradient is d_y. */
+moe_status moe_linear_backward(int32_t device, void* stream, int32_t dtype, int64_t num_rows,
+                               int32_t in_features, int32_t out_features, int32_t num_groups,
+                               const int32_t* offsets, const void* d_y, const void* x,
+                               const void* weight, const void* pre_act, int32_t activation,
+                               void* dx, void* d_weight, void* d_bias, void* workspace);
+
+/* The norms before and after a block, its gate and its residual, in one pass:
+ *   u = RMSNorm(y) post_weight (u = y without post_weight),
+ *   h_out = residual_scale h + gate u,  n_out = RMSNorm(h_out) next_weight,
+ * with RMSNorm(v) = v / sqrt(mean(v^2) + eps), fp32 statistics, one rounding of h_out and
+ * one of n_out (which is formed from the unrounded h_out).  All [T, H]; weights [H]; H a
+ * multiple of 8 up to 32768.  gate: [H], [T] or [T, H] by gate_kind.  Without next_weight no
+ * n_out is written.  Without y the call is a plain RMSNorm of h (no post_weight, no
+ * gate, residual_scale 1): n_out = RMSNorm(h) next_weight, h_out is not written.
+ * rstd_post, rstd_next [T] fp32: kept for a backward, or NULL. */
+typedef enum {
+  MOE_GATE_NONE = 0, MOE_GATE_CHANNEL, MOE_GATE_TOKEN, MOE_GATE_FULL
+} moe_gate_kind;
+moe_status moe_residual_norm(int32_t device, void* stream, int32_t dtype, int64_t num_tokens,
+                             int32_t hidden, const void* h, const void* y,
+                             const void* post_weight, const void* gate, int32_t gate_kind,
+                             const void* next_weight, float residual_scale, float eps,
+                             void* h_out, void* n_out, float* rstd_post, float* rstd_next);
+/* Backward: d_h, d_y [T, H] and the gradients of post_weight, gate and next_weight, each in
+ * its tensor's shape, for what the forward was given.  d_h_out may be NULL (0) where
+ * d_n_out is given.  h_out is the forward's (without y: h). */
+size_t moe_residual_norm_workspace_bytes(int64_t num_tokens, int32_t hidden);
+moe_status moe_residual_norm_backward(int32_t device, void* stream, int32_t dtype,
+                                      int64_t num_tokens, int32_t hidden, const void* d_h_out,
+                                      const void* d_n_out, const void* h_out, const void* y,
+                                      const void* post_weight, const void* gate,
+                                      int32_t gate_kind, const void* next_weight,
+                                      float residual_scale, const float* rstd_post,
+                                      const float* rstd_next, void* d_h, void* d_y,
+                                      void* d_post_weight, void* d_gate, void* d_next_weight,
+                                      void* workspace);
+
 const char* moe_last_error(void);
 const char* moe_version(void);
 

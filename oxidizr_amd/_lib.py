@@ -22,7 +22,10 @@ EXPORTED = [
     "moe_saved_field_range", "moe_stage_name", "moe_plan_set_profiling", "moe_plan_stage_times",
     "moe_plan_set_shared_overlap", "moe_block_forward", "moe_block_backward",
     "moe_last_error", "moe_version", "moe_check_tokens", "moe_forward_noalloc",
-    "moe_workspace_check",
+    "moe_workspace_check", "moe_sort_workspace_bytes", "moe_sort_tokens", "moe_permute",
+    "moe_unpermute", "moe_unpermute_backward", "moe_linear_workspace_bytes",
+    "moe_linear_forward", "moe_linear_backward", "moe_residual_norm",
+    "moe_residual_norm_workspace_bytes", "moe_residual_norm_backward",
 ]
 NUM_STAGES = 20
 
@@ -71,7 +74,7 @@ def load():
         raise RuntimeError(f"{LIB_PATH} is missing: build it with `python -c 'import "
                            f"__graft_entry__ as g; g.build()'` (hipcc, gfx950)")
     L = ctypes.CDLL(LIB_PATH)
-    i32, sz, i64 = ctypes.c_int32, ctypes.c_size_t, ctypes.c_int64
+    i32, sz, i64, f32 = ctypes.c_int32, ctypes.c_size_t, ctypes.c_int64, ctypes.c_float
     P = ctypes.POINTER
     L.moe_config_default.argtypes = [P(MoeConfigC), i32, i32, i32, i32, i32]
     L.moe_config_default.restype = None
@@ -112,6 +115,33 @@ def load():
     L.moe_plan_set_shared_overlap.restype = i32
     L.moe_plan_stage_times.argtypes = [_vp, P(ctypes.c_float), P(i32), i32]
     L.moe_plan_stage_times.restype = i32
+    L.moe_sort_workspace_bytes.argtypes = [i64, i32, i32]
+    L.moe_sort_workspace_bytes.restype = sz
+    L.moe_sort_tokens.argtypes = [i32, _vp, i64, i32, i32, i32, _vp, _vp, _vp, _vp, _vp, _vp]
+    L.moe_sort_tokens.restype = i32
+    L.moe_permute.argtypes = [i32, _vp, i32, i64, i32, i32, _vp, _vp, _vp, _vp]
+    L.moe_permute.restype = i32
+    L.moe_unpermute.argtypes = [i32, _vp, i32, i64, i32, i32, _vp, _vp, _vp, _vp, _vp]
+    L.moe_unpermute.restype = i32
+    L.moe_unpermute_backward.argtypes = [i32, _vp, i32, i64, i32, i32, _vp, _vp, _vp, _vp, _vp, _vp,
+                                         _vp]
+    L.moe_unpermute_backward.restype = i32
+    L.moe_linear_workspace_bytes.argtypes = [i32, i64, i32, i32, i32, i32, i32, i32]
+    L.moe_linear_workspace_bytes.restype = sz
+    L.moe_linear_forward.argtypes = [i32, _vp, i32, i64, i32, i32, i32, _vp, _vp, _vp, _vp, _vp,
+                                     i32, _vp, _vp, _vp]
+    L.moe_linear_forward.restype = i32
+    L.moe_linear_backward.argtypes = [i32, _vp, i32, i64, i32, i32, i32, _vp, _vp, _vp, _vp, _vp,
+                                      i32, _vp, _vp, _vp, _vp]
+    L.moe_linear_backward.restype = i32
+    L.moe_residual_norm.argtypes = [i32, _vp, i32, i64, i32, _vp, _vp, _vp, _vp, i32, _vp, f32, f32,
+                                    _vp, _vp, _vp, _vp]
+    L.moe_residual_norm.restype = i32
+    L.moe_residual_norm_workspace_bytes.argtypes = [i64, i32]
+    L.moe_residual_norm_workspace_bytes.restype = sz
+    L.moe_residual_norm_backward.argtypes = [i32, _vp, i32, i64, i32, _vp, _vp, _vp, _vp, _vp, _vp,
+                                             i32, _vp, f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]
+    L.moe_residual_norm_backward.restype = i32
     L.moe_last_error.argtypes = []
     L.moe_last_error.restype = ctypes.c_char_p
     L.moe_version.argtypes = []

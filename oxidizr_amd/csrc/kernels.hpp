@@ -309,7 +309,7 @@ MOE_DEV bool resolve_k(const KGroups& g, int blk, int M, int N, int BM, int BN, 
 // already split over the XCDs, it measured slower).  order[E] = 1 when the
 // busiest XCD holds at most 8 % more rows than the mean, else 0 (the kernels
 // then deal every expert's tiles over all XCDs).  Integer arithmetic only.
-__global__ __launch_bounds__(1024) void k_xcd_order(const int* __restrict__ counts, int E,
+static __global__ __launch_bounds__(1024) void k_xcd_order(const int* __restrict__ counts, int E,
                                                     int* __restrict__ order) {
   __shared__ int cnt[1024];
   __shared__ int load[8];
@@ -414,7 +414,7 @@ __global__ __launch_bounds__(C::THREADS) void k_router_logits_split(const T* __r
 }
 
 // logits[i] = ((partial[0][i] + partial[1][i]) + ...) + bias[i % E]
-__global__ __launch_bounds__(256) void k_router_reduce(const float* __restrict__ partial,
+static __global__ __launch_bounds__(256) void k_router_reduce(const float* __restrict__ partial,
                                                        int nsplit, int64_t TE, int E,
                                                        const float* __restrict__ bias,
                                                        float* __restrict__ logits) {
@@ -708,7 +708,7 @@ MOE_DEV void colsum_unit(const float* __restrict__ a, int Tn, int E, float* __re
   if (r == 0 && e < E && t0 < Tn)
     part[(int64_t)rb * E + e] = ((red[0][c] + red[1][c]) + red[2][c]) + red[3][c];
 }
-__global__ __launch_bounds__(256) void k_colsum_partial(const float* __restrict__ a, int Tn, int E,
+static __global__ __launch_bounds__(256) void k_colsum_partial(const float* __restrict__ a, int Tn, int E,
                                                         float* __restrict__ part) {
   __shared__ float red[4][64];
   colsum_unit(a, Tn, E, part, (int)blockIdx.x, threadIdx.x, red);
@@ -725,7 +725,7 @@ MOE_DEV float colsum_final(const float* __restrict__ part, int nrb, int E, int e
   for (; rb < nrb; ++rb) s[rb & 3] += part[(int64_t)rb * E + e];
   return (((s[0] + s[1]) + s[2]) + s[3]) * scale;
 }
-__global__ void k_colsum_final(const float* __restrict__ part, int nrb, int E, float scale,
+static __global__ void k_colsum_final(const float* __restrict__ part, int nrb, int E, float scale,
                                float* __restrict__ out) {
   const int e = blockIdx.x * blockDim.x + threadIdx.x;
   if (e < E) out[e] = colsum_final(part, nrb, E, e, scale);
@@ -795,7 +795,7 @@ MOE_DEV void loss_stats(const LossArgs& a) {
 constexpr int kRouteSmallTokens = 64;
 
 // Per-block expert histogram of 256 tokens' k assignments.
-__global__ __launch_bounds__(256) void k_hist(const int* __restrict__ idx, int Tn, int k, int E,
+static __global__ __launch_bounds__(256) void k_hist(const int* __restrict__ idx, int Tn, int k, int E,
                                               int* __restrict__ block_hist) {
   extern __shared__ int hist[];
   for (int e = threadIdx.x; e < E; e += 256) hist[e] = 0;
@@ -975,7 +975,7 @@ MOE_DEV void scan_histograms(const int* __restrict__ block_hist, int nb, int E,
 // chunk in 8 registers where that holds it and the DPP prefix sums (T = 200, E =
 // 16 forward 120 -> 102 us; T = 300, E = 500 317 -> 296; T = 1500, E = 64 368 ->
 // 358; fp32 training step of T = 1024, E = 8 256 -> 242).
-__global__ __launch_bounds__(1024) void k_scan(const int* __restrict__ block_hist, int nb, int E,
+static __global__ __launch_bounds__(1024) void k_scan(const int* __restrict__ block_hist, int nb, int E,
                                                int* __restrict__ block_base,
                                                int* __restrict__ counts,
                                                int* __restrict__ offsets,
@@ -1014,7 +1014,7 @@ inline int scan_grid(int rows, int E) {
 // ORs (order-independent), so a lane's rank is a popcount of the mask below
 // it; across the block's 4 waves the offsets come from per-wave counts.  A
 // token picks distinct experts, so each lane is in a mask at most once.
-__global__ __launch_bounds__(256) void k_scatter(const int* __restrict__ idx, int Tn, int k,
+static __global__ __launch_bounds__(256) void k_scatter(const int* __restrict__ idx, int Tn, int k,
                                                  int E, const int* __restrict__ block_base,
                                                  int* __restrict__ perm,
                                                  int* __restrict__ inv_perm) {
@@ -1113,7 +1113,7 @@ __global__ __launch_bounds__(256) void k_gather(const T* __restrict__ x,
 // inv_perm for choice j.  A position outside [0, T k) (which valid routing
 // never makes) is skipped.  No row is copied: the expert GEMMs read token
 // rows through perm.
-__global__ __launch_bounds__(256) void k_scatter_groups(const int* __restrict__ idx, int Tn,
+static __global__ __launch_bounds__(256) void k_scatter_groups(const int* __restrict__ idx, int Tn,
                                                         int k, int E,
                                                         const int* __restrict__ group_base,
                                                         int* __restrict__ perm,
@@ -1608,7 +1608,7 @@ __global__ __launch_bounds__(C::THREADS) void k_down_dgrad(const T* __restrict__
 // dw[perm[r]] = sum over the 32-column blocks c < nb of dwp[c][r] (c ascending):
 // the combine weights' gradient in (token, slot) order.  Block 0 also writes the
 // has_grad mask when asked for.
-__global__ __launch_bounds__(256) void k_dw_sum(const float* __restrict__ dwp, int nb, int TK,
+static __global__ __launch_bounds__(256) void k_dw_sum(const float* __restrict__ dwp, int nb, int TK,
                                                 const int* __restrict__ perm,
                                                 float* __restrict__ dw,
                                                 const int* __restrict__ counts, int E,
@@ -1996,7 +1996,7 @@ __global__ __launch_bounds__(256) void k_router_dgrad(const T* __restrict__ dl, 
 // Sets n bytes at p to zero: 16-byte stores where p + i is 16-byte aligned
 // and whole, single bytes otherwise.  A kernel rather than hipMemsetAsync, so
 // a caller may capture the call in a HIP graph.
-__global__ __launch_bounds__(256) void k_zero(uint8_t* __restrict__ p, int64_t n) {
+static __global__ __launch_bounds__(256) void k_zero(uint8_t* __restrict__ p, int64_t n) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 16;
   if (i >= n) return;
   if ((((uintptr_t)(p + i)) & 15u) == 0 && i + 16 <= n) {
@@ -2572,7 +2572,7 @@ __global__ __launch_bounds__(1024) void k_small_route(
 
 // The list of touched experts alone, from the kept offsets (a recomputing
 // backward, whose forward's list is gone): one block of 1024 threads.
-__global__ __launch_bounds__(1024) void k_small_slots(const int* __restrict__ offsets, int E,
+static __global__ __launch_bounds__(1024) void k_small_slots(const int* __restrict__ offsets, int E,
                                                       const bf16_t* const* gate_tab,
                                                       const bf16_t* const* up_tab,
                                                       const bf16_t* const* down_tab,

@@ -1,0 +1,461 @@
+// HIP kernels of expert_linear (gfx950 / CDNA4): a matrix product with bias,
+// activation and residual in its epilogue, over rows sorted by expert or with one
+// weight for all rows.
+//   z[r] = x[r] W_e^T + b_e,  y[r] = act(z[r]) + res[r]   for r in expert e's rows,
+//   dz = dy act'(z),  dx = dz W_e,  dW_e = dz^T x,  db_e = sum_r dz[r],  dres = dy.
+// W_e is [N, K] row-major (out, in).  Rows behind the last expert's have y = res (or
+// 0), dx = 0 and no part in dW and db.  The GEMM main loop is gemm.hpp's.
+#pragma once
+#include "kernels.hpp"
+
+namespace moe {
+
+enum { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3, kActGeluTanh = 4, kNumActs = 5 };
+
+// Activations and their derivatives in fp32.  gelu: z Phi(z) with the error
+// function; gelu_tanh: 0.5 z (1 + tanh(c (z + 0.044715 z^3))), written with the
+// logistic function: 0.5 (1 + tanh(v)) = 1 / (1 + exp(-2 v)).
+constexpr float kGeluC = 0.7978845608028654f;  // sqrt(2 / pi)
+MOE_DEV float act_value(float z, int act) {
+  switch (act) {
+    case kActRelu: return z > 0.0f ? z : 0.0f;
+    case kActSilu: return z * sigmoid_f(z);
+    case kActGelu: return 0.5f * z * (1.0f + erff(z * 0.7071067811865476f));
+    case kActGeluTanh: return z * sigmoid_f(2.0f * kGeluC * (z + 0.044715f * z * z * z));
+    default: return z;
+  }
+}
+MOE_DEV float act_slope(float z, int act) {
+  switch (act) {
+    case kActRelu: return z > 0.0f ? 1.0f : 0.0f;
+    case kActSilu: {
+      const float s = sigmoid_f(z);
+      return s * (1.0f + z * (1.0f - s));
+    }
+    case kActGelu:
+      return 0.5f * (1.0f + erff(z * 0.7071067811865476f)) +
+             z * 0.3989422804014327f * __expf(-0.5f * z * z);
+    case kActGeluTanh: {
+      const float s = sigmoid_f(2.0f * kGeluC * (z + 0.044715f * z * z * z));
+      return s + 2.0f * z * s * (1.0f - s) * kGeluC * (1.0f + 3.0f * 0.044715f * z * z);
+    }
+    default: return 1.0f;
+  }
+}
+
+// What the epilogue of a forward needs.  bias: [G, N] (or [N]) or null; res, pre: row r
+// at r N, or null.
+template <typename T>
+struct LinearEpi {
+  const T *bias, *res;
+  T *y, *pre;
+  int act, N;
+};
+
+// Eight outputs of row r from column n on.  The pre-activation is kept in the
+// dtype: a bf16 z is off by at most 2^-9 of itself, which moves act'(z) by less than
+// the rounding of dz behind it.
+template <typename T>
+MOE_DEV void linear_store8(const LinearEpi<T>& e, int64_t r, int n, const float* acc,
+                           const float* bias, const float* res) {
+  const int64_t o = r * e.N + n;
+  float z[8], y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) z[i] = bias ? acc[i] + bias[i] : acc[i];
+  if (e.pre) store8(e.pre + o, z);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = act_value(z[i], e.act);
+  if (res) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] += res[i];
+  }
+  store8(e.y + o, y);
+}
+
+// ------------------------------------------------------------------ preparation
+// Before the tiled launches of a grouped call.  Block 0: a clean copy of the offsets
+// (clamped to [0, M] and made ascending, so that no offsets make a launch leave its
+// buffers), the tile prefixes, and the experts' weight (and weight gradient)
+// addresses.  The blocks after it: rows behind the last expert's, which are out =
+// res (or zeros), `cols` wide, and out2 = 0.
+template <typename T>
+__global__ __launch_bounds__(1024) void k_linear_prep(const int* __restrict__ offsets, int E, int M,
+                                                      int* __restrict__ offs_out,
+                                                      int* __restrict__ prefixes,
+                                                      const T* w, T* dw, int64_t stride,
+                                                      const T** __restrict__ w_tab,
+                                                      T** __restrict__ dw_tab,
+                                                      const T* __restrict__ res,
+                                                      T* __restrict__ out, T* __restrict__ out2,
+                                                      int cols) {
+  if (blockIdx.x > 0) {
+    // a clean last offset: the largest of the offsets, as block 0 makes it
+    int m = 0;
+    for (int e = threadIdx.x; e <= E; e += 1024) m = max(m, offsets[e]);
+    __shared__ int top[16];
+    m = wave_max(m);
+    if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max(m, top[i]);
+    const int64_t v0 = (int64_t)min(m, M) * cols / 8, v1 = (int64_t)M * cols / 8;
+    const int64_t step = (int64_t)(gridDim.x - 1) * 1024;
+    const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int64_t v = v0 + (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x; v < v1; v += step) {
+      float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (res) load8(res + v * 8, f);
+      store8(out + v * 8, f);
+      if (out2) store8(out2 + v * 8, zero);
+    }
+    return;
+  }
+  __shared__ int cnt[1024], offs[1024], wsum[16 * kScanCount], wmaxs[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // running maximum of the offsets clamped to [0, M]: offset e + 1 in thread e
+  const int o0 = min(max(offsets[0], 0), M);
+  int v = tid < E ? min(max(offsets[tid + 1], o0), M) : o0;
+  for (int d = 1; d < 64; d <<= 1) {
+    const int u = __shfl_up(v, d, 64);
+    if (lane >= d) v = max(v, u);
+  }
+  if (lane == 63) wmaxs[wave] = v;
+  __syncthreads();
+  for (int i = 0; i < wave; ++i) v = max(v, wmaxs[i]);
+  offs[tid] = v;
+  __syncthreads();
+  const int lo = tid == 0 ? o0 : offs[tid - 1];
+  if (tid < E) {
+    cnt[tid] = v - lo;
+    w_tab[tid] = w + tid * stride;
+    if (dw) dw_tab[tid] = dw + tid * stride;
+  }
+  __syncthreads();
+  // the scan writes offsets from zero; rows before the first offset are none's
+  scan_counts(cnt, E, offs_out, prefixes, offs, wsum);
+  if (tid < E) offs_out[tid] += o0;
+  if (tid == 1023) offs_out[E] += o0;  // the thread that wrote it
+}
+
+// ------------------------------------------------------------------ tiled products
+// y tile by tile; the residual of a pass is requested one pass ahead.
+template <typename T, class C>
+__global__ __launch_bounds__(C::THREADS) void k_linear_fwd(const T* __restrict__ X, RowGroups groups,
+                                                           const T* const* w_tab, const T* w_one,
+                                                           int K, LinearEpi<T> epi) {
+  __shared__ __align__(16) T smem[rowgroup_smem_elems<T, C, 1, 1, 1>()];
+  int grp, row0, mv, n0;
+  const int N = epi.N;
+  if (!resolve_rows(groups, N, C::AR, C::BN, grp, row0, mv, n0)) return;
+  const T* w = pick(w_tab, w_one, grp);
+  const T* bias = epi.bias ? epi.bias + (int64_t)grp * N + n0 : nullptr;
+  with_tile_rows<T, C, 1>(mv, [&](auto ct) {
+    using CT = decltype(ct);
+    OpDesc<T> a[1] = {{X + (int64_t)row0 * K, K, mv, K}};
+    OpDesc<T> b[1] = {{w + (int64_t)n0 * K, K, N - n0, K}};
+    f32x16 acc[1][CT::TN][CT::TM], xacc[1][CT::XTN];
+    zero_acc<CT, 1>(acc, xacc);
+    mainloop_x<CT, T, false, false, 1, 1>(acc, xacc, a, b, K, smem);
+    static_assert(epi_lds_floats<CT, 1>() * 4 <= (int)sizeof(smem), "epilogue LDS");
+    auto visit = [&](int m, int n, const float* v, const float* res) {
+      if (m >= mv || n0 + n >= N) return;
+      float bv[8];
+      if (bias) load8(bias + n, bv);
+      linear_store8(epi, (int64_t)row0 + m, n0 + n, v, bias ? bv : nullptr, res);
+    };
+    if (epi.res) {
+      constexpr int V = Vec16<T>::N;
+      struct Pre { u32x4 r[8 / V]; };
+      for_each_row8_xpre<CT, 1, Pre>(acc, xacc, reinterpret_cast<float*>(smem),
+                                     [&](int m, int n, Pre& q) {
+        if (m >= mv || n0 + n >= N) return;
+        const T* p = epi.res + ((int64_t)row0 + m) * N + n0 + n;
+#pragma unroll
+        for (int i = 0; i < 8 / V; ++i) q.r[i] = *gptr(reinterpret_cast<const u32x4*>(p + i * V));
+      }, [&](int m, int n, auto& v, const Pre& q) {
+        float r[8];
+#pragma unroll
+        for (int i = 0; i < 8 / V; ++i) unpack16(q.r[i], r + i * V, T());
+        visit(m, n, v[0], r);
+      });
+    } else {
+      for_each_row8_x<CT, 1>(acc, xacc, reinterpret_cast<float*>(smem),
+                             [&](int m, int n, auto& v) { visit(m, n, v[0], nullptr); });
+    }
+  });
+}
+
+// dx = dz W (K-major weight operand).
+template <typename T, class C>
+__global__ __launch_bounds__(C::THREADS) void k_linear_dgrad(const T* __restrict__ dZ,
+                                                             RowGroups groups,
+                                                             const T* const* w_tab, const T* w_one,
+                                                             int N, int K, T* __restrict__ dX) {
+  __shared__ __align__(16) T smem[rowgroup_smem_elems<T, C, 1, 1, 1>()];
+  int grp, row0, mv, k0;
+  if (!resolve_rows(groups, K, C::AR, C::BN, grp, row0, mv, k0)) return;
+  const T* w = pick(w_tab, w_one, grp);  // element (k, n) of the operand at w + n K + k
+  with_tile_rows<T, C, 1>(mv, [&](auto ct) {
+    using CT = decltype(ct);
+    OpDesc<T> a[1] = {{dZ + (int64_t)row0 * N, N, mv, N}};
+    OpDesc<T> b[1] = {{w + k0, K, K - k0, N}};
+    f32x16 acc[1][CT::TN][CT::TM], xacc[1][CT::XTN];
+    zero_acc<CT, 1>(acc, xacc);
+    mainloop_x<CT, T, false, true, 1, 1>(acc, xacc, a, b, N, smem);
+    static_assert(epi_lds_floats<CT, 1>() * 4 <= (int)sizeof(smem), "epilogue LDS");
+    for_each_row8_x<CT, 1>(acc, xacc, reinterpret_cast<float*>(smem), [&](int m, int n, auto& v) {
+      if (m >= mv || k0 + n >= K) return;
+      store8(dX + ((int64_t)row0 + m) * K + k0 + n, v[0]);
+    });
+  });
+}
+
+// ------------------------------------------------------------------ few rows
+// A launch with few rows to an expert is the stream of the weights that it
+// touches.  As in the layer's small-batch kernels a wave multiplies 16 weight rows
+// with the rows of the expert (up to four chunks of 16) by 16 x 16 MFMAs straight
+// from memory: lane l supplies 16-byte vector l / 16 + 4 q of weight row l % 16 and
+// of token row l % 16 in step q, so four lanes read 64 contiguous bytes.  KS waves of
+// a workgroup share a block of 16 weight rows and take every KS-th k-chunk of 8
+// steps; their sums are added through LDS in wave order.
+constexpr int kLinearSkinnyRows = 64;  // rows of an expert that one workgroup takes
+// Slot s of a launch: the s-th (expert, 64 rows of it) pair with rows, experts
+// ascending.  Every wave finds its own from the offsets: lane l counts the chunks of
+// experts l E/64 .., a prefix sum over the lanes finds the lane that holds slot s.
+// False for a slot past the last.
+MOE_DEV bool skinny_slot(const int* __restrict__ offsets, int E, int M, int s, int& grp, int& r0,
+                         int& rows) {
+  const int lane = threadIdx.x & 63;
+  const int per = (E + 63) >> 6, e0 = lane * per;
+  constexpr int R = kLinearSkinnyRows;
+  int n = 0;
+  for (int i = 0; i < per; ++i) {
+    const int e = e0 + i;
+    if (e < E) {
+      const int a = min(max(offsets[e], 0), M), b = min(max(offsets[e + 1], a), M);
+      n += (b - a + R - 1) / R;
+    }
+  }
+  const int incl = wave_incl_scan(n);
+  const uint64_t m = __ballot(incl > s);
+  if (m == 0) return false;
+  const int l = __ffsll((unsigned long long)m) - 1;
+  int left = s - (__builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(n, l));
+  // the experts of lane l, walked by every lane (uniform)
+  for (int i = 0; i < per; ++i) {
+    const int e = l * per + i;
+    if (e >= E) break;
+    const int a = uni(min(max(offsets[e], 0), M)), b = uni(min(max(offsets[e + 1], a), M));
+    const int c = (b - a + R - 1) / R;
+    if (left < c) {
+      grp = e;
+      r0 = a + left * R;
+      rows = min(R, b - r0);
+      return true;
+    }
+    left -= c;
+  }
+  return false;
+}
+
+// NC: chunks of 16 rows (1 for calls of at most 16 rows, else 4).  Blocks below
+// nslot x nNb are (slot, row blocks) pairs; the others write the rows behind the
+// last expert's.  offsets null: one weight, rows s 64 .. .
+template <typename T, int NC, int KS>
+__global__ __launch_bounds__(256) void k_linear_skinny(const T* __restrict__ X,
+                                                       const int* __restrict__ offsets, int E,
+                                                       int M, int nslot, const T* __restrict__ W,
+                                                       int K, LinearEpi<T> epi) {
+  constexpr int RB = 4 / KS, V = Vec16<T>::N, KC = 32 * V;
+  __shared__ f32x4 red[KS > 1 ? (KS - 1) * RB * NC * 64 : 1];
+  const int N = epi.N;
+  const int nNb = (N + 16 * RB - 1) / (16 * RB);
+  const int slot = uni(blockIdx.x / nNb), nb = uni(blockIdx.x % nNb);
+  if (slot >= nslot) {
+    int m = 0;
+    for (int e = threadIdx.x & 63; e <= E; e += 64) m = max(m, offsets[e]);
+    m = min(wave_max(m), M);
+    const int64_t v0 = (int64_t)m * N / 8, v1 = (int64_t)M * N / 8;
+    const int64_t step = ((int64_t)gridDim.x - (int64_t)nslot * nNb) * 256;
+    for (int64_t v = v0 + ((int64_t)blockIdx.x - (int64_t)nslot * nNb) * 256 + threadIdx.x; v < v1;
+         v += step) {
+      float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (epi.res) load8(epi.res + v * 8, f);
+      store8(epi.y + v * 8, f);
+      if (epi.pre) store8(epi.pre + v * 8, zero);
+    }
+    return;
+  }
+  int grp = 0, r0 = slot * kLinearSkinnyRows, rows = min(kLinearSkinnyRows, M - r0);
+  if (offsets && !skinny_slot(offsets, E, M, slot, grp, r0, rows)) return;  // workgroup-uniform
+  grp = uni(grp); r0 = uni(r0); rows = uni(rows);
+  const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int rb = wave / KS, ks = wave % KS;
+  const int n0 = (nb * RB + rb) * 16;
+  const int nrows = uni(min(16, N - n0));
+  const int g = lane >> 4, rl = lane & 15;
+  const int nch = (rows + 15) / 16;
+  f32x4 acc[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) acc[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (nrows > 0) {
+    const rsrc_t rx = make_rsrc(uni_ptr(X + (int64_t)r0 * K), (uint32_t)uni(rows * K * (int)sizeof(T)));
+    const rsrc_t rw = make_rsrc(uni_ptr(W + ((int64_t)grp * N + n0) * K),
+                                (uint32_t)uni(nrows * K * (int)sizeof(T)));
+    const uint32_t vw = (uint32_t)((rl * K + V * g) * (int)sizeof(T));
+    uint32_t vx[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      vx[c] = c * 16 + rl < rows ? (uint32_t)(((c * 16 + rl) * K + V * g) * (int)sizeof(T)) : kOobOffset;
+    for (int kc = ks; kc * KC < K; kc += KS) {
+      const uint32_t soff = (uint32_t)kc * 512;
+      u32x4 wa[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const bool kin = kc * KC + 4 * V * q + V * g < K;
+        wa[q] = buf_ld16(rw, kin ? vw + 64 * q : kOobOffset, soff);
+      }
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        if (c >= nch) break;
+        u32x4 xa[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const bool kin = kc * KC + 4 * V * q + V * g < K;
+          xa[q] = buf_ld16(rx, kin ? vx[c] + 64 * q : kOobOffset, soff);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) mfma16(acc[c], xa[q], wa[q], T());
+      }
+    }
+  }
+  if constexpr (KS > 1) {
+    if (ks > 0) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        if (c < nch) red[((ks - 1) * RB + rb) * NC * 64 + c * 64 + lane] = acc[c];
+    }
+    __syncthreads();
+    if (ks > 0) return;
+#pragma unroll
+    for (int q = 1; q < KS; ++q)
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        if (c < nch) acc[c] += red[((q - 1) * RB + rb) * NC * 64 + c * 64 + lane];
+  }
+  // lane holds row 16 c + 4 g + r, column n0 + rl
+  if (rl >= nrows) return;
+  const int n = n0 + rl;
+  const float bias = epi.bias ? to_f<T>(epi.bias[(int64_t)grp * N + n]) : 0.0f;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    if (c >= nch) break;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int t = c * 16 + 4 * g + r;
+      if (t >= rows) continue;
+      const int64_t o = ((int64_t)r0 + t) * N + n;
+      const float z = acc[c][r] + bias;
+      if (epi.pre) epi.pre[o] = from_f<T>(z);
+      const float y = act_value(z, epi.act);
+      epi.y[o] = from_f<T>(epi.res ? y + to_f<T>(epi.res[o]) : y);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ backward, element-wise part
+// dz = dy act'(z) (written when act is not none) and, per 64-row chunk of a group,
+// the column sums of dz for the bias gradient, from the unrounded products.  Block
+// (chunk, 256 columns): thread (r, c) takes rows r, r + 8, .. of 8 columns; the eight
+// row lanes are added in order.
+constexpr int kDzRows = kF32RowTile;  // rows of a chunk: the prefix of 64-row tiles counts them
+template <typename T>
+__global__ __launch_bounds__(256) void k_linear_dz(const T* __restrict__ dY,
+                                                   const T* __restrict__ pre, int act, RowGroups g,
+                                                   int N, T* __restrict__ dZ,
+                                                   float* __restrict__ part) {
+  __shared__ float col[8][256 + 8];
+  int r0, rows;
+  const int chunk = blockIdx.x;
+  if (g.offsets) {
+    if (chunk >= g.tile_prefix[g.G]) return;
+    const int grp = uni(find_group(g.tile_prefix, g.G, chunk));
+    r0 = g.offsets[grp] + (chunk - g.tile_prefix[grp]) * kDzRows;
+    rows = min(kDzRows, g.offsets[grp + 1] - r0);
+  } else {
+    r0 = chunk * kDzRows;
+    rows = min(kDzRows, g.M - r0);
+  }
+  const int rl = threadIdx.x >> 5, c8 = (threadIdx.x & 31) * 8;
+  const int n = blockIdx.y * 256 + c8;
+  float s[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s[i] = 0.0f;
+  if (n < N) {
+#pragma unroll
+    for (int j = 0; j < kDzRows / 8; ++j) {
+      const int r = rl + 8 * j;
+      if (r >= rows) continue;
+      const int64_t o = ((int64_t)r0 + r) * N + n;
+      float d[8];
+      load8(dY + o, d);
+      if (act != kActNone) {
+        float z[8];
+        load8(pre + o, z);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[i] *= act_slope(z[i], act);
+        store8(dZ + o, d);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] += d[i];
+    }
+  }
+  if (!part) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) col[rl][c8 + i] = s[i];
+  __syncthreads();
+  const int cc = blockIdx.y * 256 + threadIdx.x;
+  if (cc >= N) return;
+  float t = 0.0f;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) t += col[r][threadIdx.x];
+  part[(int64_t)chunk * N + cc] = t;
+}
+
+// db[g] = the sum of group g's chunks, in order (zeros for a group without rows);
+// and zeros for the weight gradient of a group without rows.  Block (group, 64
+// columns): four row lanes of 64 columns each.
+template <typename T>
+__global__ __launch_bounds__(256) void k_linear_db(const float* __restrict__ part, RowGroups g,
+                                                   int N, T* __restrict__ db) {
+  __shared__ float col[4][64];
+  const int grp = blockIdx.y;
+  const int p0 = g.offsets ? g.tile_prefix[grp] : 0;
+  const int p1 = g.offsets ? g.tile_prefix[grp + 1] : (g.M + kDzRows - 1) / kDzRows;
+  const int n = blockIdx.x * 64 + (threadIdx.x & 63), rl = threadIdx.x >> 6;
+  float s = 0.0f;
+  if (n < N) {
+#pragma unroll 8
+    for (int p = p0 + rl; p < p1; p += 4) s += part[(int64_t)p * N + n];
+  }
+  col[rl][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (rl != 0 || n >= N) return;
+  db[(int64_t)grp * N + n] =
+      from_f<T>((col[0][n & 63] + col[1][n & 63]) + (col[2][n & 63] + col[3][n & 63]));
+}
+
+// Zeros the weight gradient of every group without rows: block (part, group).
+template <typename T>
+__global__ __launch_bounds__(256) void k_linear_zero_dw(const int* __restrict__ offsets,
+                                                        int64_t stride, T* __restrict__ dw) {
+  const int grp = blockIdx.y;
+  if (offsets[grp + 1] > offsets[grp]) return;
+  const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < stride / 8;
+       i += (int64_t)gridDim.x * 256)
+    store8(dw + grp * stride + i * 8, zero);
+}
+
+}  // namespace moe

@@ -1,0 +1,642 @@
+// C ABI of the operators beside the MoE layer: tokens sorted by expert and back,
+// expert products with bias, activation and residual, norms around a block.
+// Declared in include/moe_hip.h.  The calls keep no state: sizes in, device
+// pointers in, launches on the call's stream.
+#include "host.hpp"
+#include "linear.hpp"
+#include "ops.hpp"
+
+using namespace moe;
+
+namespace {
+
+// Makes `device` current for one call and the caller's device current after it.
+struct DeviceScope {
+  int before = -1, device;
+  bool changed = false;
+  explicit DeviceScope(int d) : device(d) {}
+  hipError_t enter() {
+    hipError_t e = hipGetDevice(&before);
+    if (e != hipSuccess || before == device) return e;
+    e = hipSetDevice(device);
+    changed = e == hipSuccess;
+    return e;
+  }
+  ~DeviceScope() {
+    if (changed) (void)hipSetDevice(before);
+  }
+};
+
+moe_status check_pointers(std::initializer_list<const void*> needed,
+                          std::initializer_list<const void*> optional = {}) {
+  for (const void* p : needed) {
+    if (!p) return fail(MOE_ERR_INVALID, "a required pointer is NULL");
+    if (!aligned16(p)) return fail(MOE_ERR_INVALID, "device pointers must be 16-byte aligned");
+  }
+  for (const void* p : optional)
+    if (p && !aligned16(p)) return fail(MOE_ERR_INVALID, "device pointers must be 16-byte aligned");
+  return MOE_OK;
+}
+
+moe_status check_dtype(int dtype) {
+  if (dtype != MOE_DTYPE_F32 && dtype != MOE_DTYPE_BF16)
+    return fail(MOE_ERR_INVALID, "unknown dtype %d", dtype);
+  return MOE_OK;
+}
+
+// Blocks of a launch of `waves` waves, four to a block; 0 when the grid would not
+// hold them.
+unsigned wave_grid(int64_t waves) {
+  const int64_t g = (waves + 3) / 4;
+  return g <= INT32_MAX ? (unsigned)g : 0u;
+}
+
+// ---- sort by expert
+constexpr int64_t kMaxAssignments = (int64_t(1) << 31) - 1;  // positions are int32
+struct SortPlan {
+  int64_t N, chunk;
+  int blocks;
+  size_t bytes;
+};
+SortPlan sort_plan(int64_t T, int k, int E) {
+  SortPlan p{};
+  p.N = T * k;
+  const int64_t tiles = (p.N + kSortTile - 1) / kSortTile;
+  p.chunk = kSortTile * std::max<int64_t>(1, (tiles + kSortMaxBlocks - 1) / kSortMaxBlocks);
+  p.blocks = (int)std::max<int64_t>(1, (p.N + p.chunk - 1) / p.chunk);
+  p.bytes = p.blocks > 1 ? align_up((size_t)p.blocks * (E + 1) * sizeof(int)) : 0;
+  return p;
+}
+moe_status check_sort(int64_t T, int k, int E) {
+  if (T < 0) return fail(MOE_ERR_INVALID, "num_tokens is negative");
+  if (k < 1 || k > kMaxPerTok)
+    return fail(MOE_ERR_INVALID, "experts_per_tok %d is outside 1..%d", k, kMaxPerTok);
+  if (E < 1 || E > 1024) return fail(MOE_ERR_INVALID, "num_experts %d is outside 1..1024", E);
+  if (T > kMaxAssignments / k)
+    return fail(MOE_ERR_UNSUPPORTED, "num_tokens x experts_per_tok reaches 2^31");
+  return MOE_OK;
+}
+
+template <typename I>
+moe_status launch_sort(hipStream_t s, const SortPlan& p, int E, const I* idx, int* counts,
+                       int* offsets, int* perm, int* inv, int* hist) {
+  const size_t row = (size_t)(E + 1) * sizeof(int);
+  if (p.blocks > 1)
+    hipLaunchKernelGGL(k_sort_hist<I>, dim3(p.blocks), dim3(kSortThreads), row, s, idx, p.N, E,
+                       p.chunk, hist);
+  hipLaunchKernelGGL(k_sort_scatter<I>, dim3(p.blocks), dim3(kSortThreads), kSortWaves * row, s,
+                     idx, p.N, E, p.chunk, hist, counts, offsets, perm, inv);
+  LAUNCH_CHECK();
+  return MOE_OK;
+}
+
+// ---- rows to experts and back
+moe_status check_rows(int dtype, int64_t T, int k, int H) {
+  moe_status st = check_dtype(dtype);
+  if (st != MOE_OK) return st;
+  if ((st = check_sort(T, k, 1)) != MOE_OK) return st;
+  if (H < 8 || H % 8 != 0) return fail(MOE_ERR_INVALID, "hidden %d is not a positive multiple of 8", H);
+  return MOE_OK;
+}
+
+// Calls f(integral constant >= k): the k rows of a token are held in registers.
+template <class F>
+void with_k(int k, F&& f) {
+  if (k <= 2) f(std::integral_constant<int, 2>());
+  else if (k <= 4) f(std::integral_constant<int, 4>());
+  else if (k <= 8) f(std::integral_constant<int, 8>());
+  else f(std::integral_constant<int, 16>());
+}
+
+template <typename D>
+moe_status launch_permute(hipStream_t s, int64_t T, int k, int H, const int* inv, const int* kept,
+                          const D* x, D* xp) {
+  const int per = 64 * kPermuteVecs * Vec16<D>::N;
+  const unsigned grid = wave_grid(T * ceil_div(H, per));
+  if (!grid) return fail(MOE_ERR_UNSUPPORTED, "too many tokens for one launch");
+  hipLaunchKernelGGL(k_permute<D>, dim3(grid), dim3(256), 0, s, x, inv, kept, T, k, H, xp);
+  LAUNCH_CHECK();
+  return MOE_OK;
+}
+
+template <typename D>
+moe_status launch_unpermute(hipStream_t s, int64_t T, int k, int H, const int* inv,
+                            const int* kept, const D* y, const float* w, D* out) {
+  const unsigned grid = wave_grid(T * ceil_div(H, 64 * Vec16<D>::N));
+  if (!grid) return fail(MOE_ERR_UNSUPPORTED, "too many tokens for one launch");
+  with_k(k, [&](auto kc) {
+    hipLaunchKernelGGL((k_unpermute<D, decltype(kc)::value>), dim3(grid), dim3(256), 0, s, y, inv,
+                       kept, w, T, k, H, out);
+  });
+  LAUNCH_CHECK();
+  return MOE_OK;
+}
+
+template <typename D>
+moe_status launch_unpermute_bwd(hipStream_t s, int64_t T, int k, int H, const int* inv,
+                                const int* kept, const D* dout, const D* y, const float* w, D* dy,
+                                float* dw) {
+  const int slices = ceil_div(H, 64 * Vec16<D>::N);
+  with_k(k, [&](auto kc) {
+    constexpr int KM = decltype(kc)::value;
+    auto go = [&](auto wpt) {
+      constexpr int W = decltype(wpt)::value;
+      hipLaunchKernelGGL((k_unpermute_bwd<D, W, KM>), dim3((unsigned)((T + 4 / W - 1) / (4 / W))),
+                         dim3(256), 0, s, dout, y, inv, kept, w, T, k, H, dy, dw);
+    };
+    if (slices == 1) go(std::integral_constant<int, 1>());
+    else if (slices == 2) go(std::integral_constant<int, 2>());
+    else go(std::integral_constant<int, 4>());
+  });
+  LAUNCH_CHECK();
+  return MOE_OK;
+}
+
+// ---- norms around a block
+constexpr int kNormMaxHidden = 32768;
+moe_status check_norm(int dtype, int64_t T, int H, int gate_kind, bool y, bool post, bool gate,
+                      bool next, float scale) {
+  moe_status st = check_dtype(dtype);
+  if (st != MOE_OK) return st;
+  if (T < 0 || T >= (int64_t(1) << 31)) return fail(MOE_ERR_INVALID, "num_tokens is outside 0..2^31-1");
+  if (H < 8 || H % 8 != 0) return fail(MOE_ERR_INVALID, "hidden %d is not a positive multiple of 8", H);
+  if (H > kNormMaxHidden)
+    return fail(MOE_ERR_UNSUPPORTED, "hidden %d is above %d", H, kNormMaxHidden);
+  if (gate_kind < kGateNone || gate_kind > kGateFull)
+    return fail(MOE_ERR_INVALID, "unknown gate kind %d", gate_kind);
+  if ((gate_kind != kGateNone) != gate)
+    return fail(MOE_ERR_INVALID, "gate and gate_kind do not go together");
+  if (!y && (post || gate))
+    return fail(MOE_ERR_INVALID, "a post norm or a gate needs the block's output y");
+  if (!y && !next) return fail(MOE_ERR_INVALID, "neither y nor next_weight: nothing to compute");
+  if (!y && scale != 1.0f) return fail(MOE_ERR_INVALID, "residual_scale needs the block's output y");
+  return MOE_OK;
+}
+
+// Calls f(waves to a row, chunks to a thread) with 64 * 8 * WPR * NCH >= H.
+template <class F>
+void with_norm_shape(int H, F&& f) {
+  using std::integral_constant;
+  if (H <= 512) f(integral_constant<int, 1>(), integral_constant<int, 1>());
+  else if (H <= 2048) f(integral_constant<int, 4>(), integral_constant<int, 1>());
+  else if (H <= 4096) f(integral_constant<int, 8>(), integral_constant<int, 1>());
+  else if (H <= 8192) f(integral_constant<int, 8>(), integral_constant<int, 2>());
+  else if (H <= 16384) f(integral_constant<int, 16>(), integral_constant<int, 2>());
+  else f(integral_constant<int, 16>(), integral_constant<int, 4>());
+}
+constexpr int norm_threads(int wpr) { return wpr > 4 ? 64 * wpr : 256; }
+constexpr int norm_rows(int wpr) { return wpr > 4 ? 1 : 4 / wpr; }
+
+// Blocks of the backward: enough to fill the CUs twice; each adds its rows' column
+// sums in registers and writes one partial row.
+constexpr int kNormBwdBlocks = 512;
+int norm_bwd_blocks(int64_t T, int H) {
+  int rows = 1;
+  with_norm_shape(H, [&](auto wpr, auto) { rows = norm_rows(decltype(wpr)::value); });
+  return (int)std::min<int64_t>(kNormBwdBlocks, (T + rows - 1) / rows);
+}
+
+template <typename D>
+moe_status launch_norm_fwd(hipStream_t s, const NormArgs<D>& a) {
+  with_norm_shape(a.H, [&](auto wpr, auto nch) {
+    constexpr int W = decltype(wpr)::value;
+    const int64_t grid = (a.Tn + norm_rows(W) - 1) / norm_rows(W);
+    hipLaunchKernelGGL((k_norm_fwd<D, W, decltype(nch)::value>), dim3((unsigned)grid),
+                       dim3(norm_threads(W)), 0, s, a);
+  });
+  LAUNCH_CHECK();
+  return MOE_OK;
+}
+
+template <typename D>
+moe_status launch_norm_bwd(hipStream_t s, const NormBwdArgs<D>& a, D* dw2, D* dgate_chan, D* dw3) {
+  const int nb = norm_bwd_blocks(a.Tn, a.H);
+  with_norm_shape(a.H, [&](auto wpr, auto nch) {
+    constexpr int W = decltype(wpr)::value;
+    hipLaunchKernelGGL((k_norm_bwd<D, W, decltype(nch)::value>), dim3(nb), dim3(norm_threads(W)), 0,
+                       s, a);
+  });
+  if (a.need_a + a.need_b > 0)
+    hipLaunchKernelGGL(k_norm_colsum<D>, dim3(ceil_div(a.H, 64), a.need_a + a.need_b), dim3(256), 0,
+                       s, a.part, nb, a.H, a.need_a, a.need_b, a.w2,
+                       a.gate_kind == kGateChannel ? a.gate : nullptr, dw2, dgate_chan, dw3);
+  LAUNCH_CHECK();
+  return MOE_OK;
+}
+
+// ---- expert products
+moe_status check_linear(int dtype, int64_t M, int K, int N, int E, bool grouped, int act) {
+  moe_status st = check_dtype(dtype);
+  if (st != MOE_OK) return st;
+  if (M < 0) return fail(MOE_ERR_INVALID, "num_rows is negative");
+  if (K < 8 || K % 8 != 0 || N < 8 || N % 8 != 0)
+    return fail(MOE_ERR_INVALID, "in_features %d and out_features %d must be positive multiples of 8",
+                K, N);
+  if (grouped ? (E < 1 || E > 1024) : E != 1)
+    return fail(MOE_ERR_INVALID, grouped ? "num_groups %d is outside 1..1024"
+                                         : "num_groups %d without offsets is not 1", E);
+  if (act < 0 || act >= kNumActs) return fail(MOE_ERR_INVALID, "unknown activation %d", act);
+  const int64_t b = elt_size(dtype);
+  if ((int64_t)K * N * b >= kMaxExtentBytes)
+    return fail(MOE_ERR_UNSUPPORTED, "a weight matrix reaches 2^31 bytes");
+  if (M > (int64_t(1) << 26) || M * std::max(K, N) * b >= kMaxExtentBytes * 8)
+    return fail(MOE_ERR_UNSUPPORTED, "num_rows x max(in, out features) reaches 2^34 bytes");
+  return MOE_OK;
+}
+
+struct LinearWs {
+  size_t offs, prefixes, w_tab, dw_tab, dz, part, splitk, splitk_bytes, total;
+};
+int64_t dz_chunks(int64_t M, int E, bool grouped) {
+  return (M + kDzRows - 1) / kDzRows + (grouped ? E : 0);
+}
+LinearWs linear_ws(int dtype, int64_t M, int K, int N, int E, bool grouped, int act, bool backward) {
+  LinearWs w{};
+  Carve c;
+  const size_t b = elt_size(dtype);
+  if (grouped) {
+    w.offs = c.take((size_t)(E + 1) * 4);
+    w.prefixes = c.take((size_t)kNumTilePrefixes * (E + 1) * 4);
+    w.w_tab = c.take((size_t)E * sizeof(void*));
+    w.dw_tab = c.take((size_t)E * sizeof(void*));
+  }
+  if (backward) {
+    if (act != kActNone) w.dz = c.take((size_t)M * N * b);
+    w.part = c.take((size_t)dz_chunks(M, E, grouped) * N * 4);
+    if (!grouped) {
+      w.splitk_bytes = dtype == MOE_DTYPE_BF16
+                           ? dense_wgrad_partial_bytes<bf16_t, 1>(N, K, (int)M)
+                           : dense_wgrad_partial_bytes<float, 1>(N, K, (int)M);
+      w.splitk = c.take(w.splitk_bytes);
+    }
+  }
+  w.total = c.off;
+  return w;
+}
+
+// Whether a forward runs as the stream of its weights (k_linear_skinny): few rows to
+// an expert.  Rows are counted as evenly spread over the experts that can have any.
+constexpr int kSkinnyRowsPerGroup = 16;
+bool linear_skinny(int64_t M, int E, bool grouped) {
+  const int64_t groups = grouped ? std::min<int64_t>(E, M) : 1;
+  return grouped ? M <= kSkinnyRowsPerGroup * groups : M <= kLinearSkinnyRows;
+}
+
+// Row tilings of a product alone on the GPU, in tenths of a round of 256-row tiles
+// (measured on dense launches, see with_dense_tiling's table): 128 x 128 and 64 x 128
+// tiles where those leave CUs idle, 384-row tiles where they fill more rounds.
+constexpr TileCosts kLinearCosts{10.0, {6.8, 8.2}, {4.4, 5.7}};
+constexpr double kTallCost = 1.4;  // a 384-row tile against a 256-row one
+
+// Calls f(tiling, row groups, grid) for a launch of M rows in E groups (offsets and
+// prefixes of k_linear_prep), or dense (offsets null), with N output columns.
+template <typename D, class F>
+void with_linear_tiling(const int* offsets, const int* prefixes, int E, int64_t M, int N, F&& f) {
+  using C = typename Tilings<D>::Big;
+  const bool grouped = offsets != nullptr;
+  auto go = [&](auto c, int half_last, int tall) {
+    using CC = decltype(c);
+    const int rows = CC::XR == 128 ? CC::AR : CC::BM;
+    if (!grouped) {
+      f(c, RowGroups{nullptr, nullptr, nullptr, nullptr, 1, (int)M, 0, 0},
+        (int)((int64_t)ceil_div(M, CC::AR) * ceil_div(N, CC::BN)));
+      return;
+    }
+    const int* tp = prefixes + prefix_slot(rows) * (E + 1);
+    const int64_t mt = ceil_div(M, rows) + E;
+    f(c, RowGroups{offsets, tp, tp + (E + 1), tp + 2 * (E + 1), E, (int)M, half_last, tall},
+      8 * ceil_div(mt * ceil_div(N, CC::BN), 8));
+  };
+  if constexpr (has_half_rows<D, C>()) {
+    using C3 = Rows384<C>;
+    using CM = typename LowTilings<C>::Mid;
+    using CS = typename LowTilings<C>::Small;
+    const int groups = grouped ? (int)std::min<int64_t>(E, M) : 1;
+    const double r = (double)M / groups;
+    auto tiles = [&](int bm, int bn) {
+      return (grouped ? group_row_tiles(groups, r, bm) : (double)ceil_div(M, bm)) * ceil_div(N, bn);
+    };
+    const double big = big_cost(tiles(C::BM, C::BN), kLinearCosts.big) / (grouped ? 1.15 : 1.0);
+    const double mid = round_cost(tiles(CM::BM, CM::BN), kLinearCosts.mid);
+    const double small = round_cost(tiles(CS::BM, CS::BN), kLinearCosts.small);
+    const bool tall_ok = !grouped || M >= 2 * (int64_t)C3::AR * E;
+    const double tall = tall_ok ? big_cost(tiles(C3::AR, C3::BN), kLinearCosts.big * kTallCost) : 1e30;
+    if (std::min(mid, small) < std::min(big, tall))
+      return mid <= small ? go(CM{}, 0, 0) : go(CS{}, 0, 0);
+    if (tall < big) return go(C3{}, 1, 0);
+    return go(C{}, grouped && M >= 2 * (int64_t)C::BM * E, tall_rows_for(C::BM));
+  }
+  go(C{}, 0, 0);
+}
+
+// Blocks of k_linear_prep: one for the prefixes, the others for the rows behind the
+// last expert's.
+constexpr int kPrepBlocks = 1 + 128;
+
+template <typename D>
+moe_status linear_forward(hipStream_t s, int64_t M, int K, int N, int E, const int* offsets,
+                          const D* x, const D* w, const LinearEpi<D>& epi, char* ws) {
+  const bool grouped = offsets != nullptr;
+  if (linear_skinny(M, E, grouped)) {
+    const int64_t nslot = grouped ? std::min<int64_t>(E, M) + M / kLinearSkinnyRows
+                                  : ceil_div(M, kLinearSkinnyRows);
+    constexpr int KS = 2, RB = 4 / KS;
+    const int nNb = ceil_div(N, 16 * RB);
+    const unsigned grid = (unsigned)(nslot * nNb + (grouped ? 64 : 0));
+    auto go = [&](auto nc) {
+      hipLaunchKernelGGL((k_linear_skinny<D, decltype(nc)::value, KS>), dim3(grid), dim3(256), 0, s,
+                         x, offsets, E, (int)M, (int)nslot, w, K, epi);
+    };
+    if (M <= 16) go(std::integral_constant<int, 1>());
+    else go(std::integral_constant<int, 4>());
+    LAUNCH_CHECK();
+    return MOE_OK;
+  }
+  const LinearWs L = linear_ws(sizeof(D) == 2 ? MOE_DTYPE_BF16 : MOE_DTYPE_F32, M, K, N, E, grouped,
+                               epi.act, false);
+  int* offs = grouped ? (int*)(ws + L.offs) : nullptr;
+  int* prefixes = grouped ? (int*)(ws + L.prefixes) : nullptr;
+  const D** w_tab = grouped ? (const D**)(ws + L.w_tab) : nullptr;
+  if (grouped)
+    hipLaunchKernelGGL(k_linear_prep<D>, dim3(kPrepBlocks), dim3(1024), 0, s, offsets, E, (int)M,
+                       offs, prefixes, w, (D*)nullptr, (int64_t)N * K, w_tab, (D**)nullptr, epi.res,
+                       epi.y, epi.pre, N);
+  with_linear_tiling<D>(offs, prefixes, E, M, N, [&](auto c, const RowGroups& r, int grid) {
+    using C = decltype(c);
+    hipLaunchKernelGGL((k_linear_fwd<D, C>), dim3(grid), dim3(C::THREADS), 0, s, x, r,
+                       (const D* const*)w_tab, w, K, epi);
+  });
+  LAUNCH_CHECK();
+  return MOE_OK;
+}
+
+template <typename D>
+moe_status linear_backward(hipStream_t s, int64_t M, int K, int N, int E, const int* offsets,
+                           const D* dy, const D* x, const D* w, const D* pre, int act, D* dx, D* dw,
+                           D* db, char* ws) {
+  const bool grouped = offsets != nullptr;
+  const LinearWs L = linear_ws(sizeof(D) == 2 ? MOE_DTYPE_BF16 : MOE_DTYPE_F32, M, K, N, E, grouped,
+                               act, true);
+  int* offs = grouped ? (int*)(ws + L.offs) : nullptr;
+  int* prefixes = grouped ? (int*)(ws + L.prefixes) : nullptr;
+  const D** w_tab = grouped ? (const D**)(ws + L.w_tab) : nullptr;
+  D** dw_tab = grouped ? (D**)(ws + L.dw_tab) : nullptr;
+  if (grouped)
+    hipLaunchKernelGGL(k_linear_prep<D>, dim3(dx ? kPrepBlocks : 1), dim3(1024), 0, s, offsets, E,
+                       (int)M, offs, prefixes, w, dw, (int64_t)N * K, w_tab, dw_tab,
+                       (const D*)nullptr, dx, (D*)nullptr, K);
+  const RowGroups chunks{offs, prefixes, nullptr, nullptr, E, (int)M, 0, 0};
+  static_assert(prefix_slot(kDzRows) == 0, "the chunks' prefix is the first");
+  const D* dz = dy;
+  if (act != kActNone || db) {
+    D* out = (D*)(ws + L.dz);
+    float* part = db ? (float*)(ws + L.part) : nullptr;
+    hipLaunchKernelGGL(k_linear_dz<D>, dim3((unsigned)dz_chunks(M, E, grouped), ceil_div(N, 256)),
+                       dim3(256), 0, s, dy, pre, act, chunks, N, out, part);
+    if (act != kActNone) dz = out;
+    if (db)
+      hipLaunchKernelGGL(k_linear_db<D>, dim3(ceil_div(N, 64), E), dim3(256), 0, s, part, chunks, N,
+                         db);
+  }
+  LAUNCH_CHECK();
+  if (dx)
+    with_linear_tiling<D>(offs, prefixes, E, M, K, [&](auto c, const RowGroups& r, int grid) {
+      using C = decltype(c);
+      hipLaunchKernelGGL((k_linear_dgrad<D, C>), dim3(grid), dim3(C::THREADS), 0, s, dz, r,
+                         (const D* const*)w_tab, w, N, K, dx);
+    });
+  LAUNCH_CHECK();
+  if (!dw) return MOE_OK;
+  if (!grouped)
+    return launch_dense_wgrad<D, 1>(s, dz, nullptr, N, x, K, (int)M, N, K, 1.0f, dw, nullptr,
+                                    (float*)(ws + L.splitk), L.splitk_bytes);
+  using C = WgradTiling<D, 1>;
+  hipLaunchKernelGGL(k_linear_zero_dw<D>, dim3(8, E), dim3(256), 0, s, offs, (int64_t)N * K, dw);
+  const KGroups kg{offs, E, (int)M, 1, 0, 1, nullptr};
+  const int grid = kgrouped_grid(E, N, K, C::BM, C::BN);
+  hipLaunchKernelGGL((k_wgrad<D, 1, true>), dim3(grid), dim3(C::THREADS), 0, s, dz,
+                     (const D*)nullptr, (int64_t)N, x, (int64_t)K, kg, N, K, 1.0f,
+                     (D* const*)dw_tab, (D*)nullptr, (D* const*)nullptr, (D*)nullptr,
+                     (float*)nullptr, grid, 0);
+  LAUNCH_CHECK();
+  return MOE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t moe_sort_workspace_bytes(int64_t T, int32_t k, int32_t E) {
+  return check_sort(T, k, E) == MOE_OK ? sort_plan(T, k, E).bytes : 0;
+}
+
+moe_status moe_sort_tokens(int32_t device, void* stream, int64_t T, int32_t k, int32_t E,
+                           int32_t index_bytes, const void* topk_idx, int32_t* counts,
+                           int32_t* offsets, int32_t* perm, int32_t* inv_perm, void* workspace) {
+  moe_status st = check_sort(T, k, E);
+  if (st != MOE_OK) return st;
+  if (index_bytes != 4 && index_bytes != 8)
+    return fail(MOE_ERR_INVALID, "index_bytes %d is neither 4 nor 8", index_bytes);
+  if ((st = check_pointers({counts, offsets})) != MOE_OK) return st;
+  const SortPlan p = sort_plan(T, k, E);
+  if (T > 0 && (st = check_pointers({topk_idx, perm, inv_perm})) != MOE_OK) return st;
+  if (p.bytes && (st = check_pointers({workspace})) != MOE_OK) return st;
+  DeviceScope dev(device);
+  HIP_TRY(dev.enter());
+  hipStream_t s = (hipStream_t)stream;
+  if (index_bytes == 4)
+    return launch_sort<int32_t>(s, p, E, (const int32_t*)topk_idx, counts, offsets, perm, inv_perm,
+                                (int*)workspace);
+  return launch_sort<int64_t>(s, p, E, (const int64_t*)topk_idx, counts, offsets, perm, inv_perm,
+                              (int*)workspace);
+}
+
+moe_status moe_permute(int32_t device, void* stream, int32_t dtype, int64_t T, int32_t k,
+                       int32_t H, const int32_t* inv_perm, const int32_t* num_kept, const void* x,
+                       void* x_perm) {
+  moe_status st = check_rows(dtype, T, k, H);
+  if (st != MOE_OK || T == 0) return st;
+  if ((st = check_pointers({inv_perm, x, x_perm})) != MOE_OK) return st;
+  if (!num_kept) return fail(MOE_ERR_INVALID, "a required pointer is NULL");
+  DeviceScope dev(device);
+  HIP_TRY(dev.enter());
+  if (dtype == MOE_DTYPE_BF16)
+    return launch_permute<bf16_t>((hipStream_t)stream, T, k, H, inv_perm, num_kept,
+                                  (const bf16_t*)x, (bf16_t*)x_perm);
+  return launch_permute<float>((hipStream_t)stream, T, k, H, inv_perm, num_kept, (const float*)x,
+                               (float*)x_perm);
+}
+
+moe_status moe_unpermute(int32_t device, void* stream, int32_t dtype, int64_t T, int32_t k,
+                         int32_t H, const int32_t* inv_perm, const int32_t* num_kept,
+                         const void* y, const float* weights, void* out) {
+  moe_status st = check_rows(dtype, T, k, H);
+  if (st != MOE_OK || T == 0) return st;
+  if ((st = check_pointers({inv_perm, y, out}, {weights})) != MOE_OK) return st;
+  if (!num_kept) return fail(MOE_ERR_INVALID, "a required pointer is NULL");
+  DeviceScope dev(device);
+  HIP_TRY(dev.enter());
+  if (dtype == MOE_DTYPE_BF16)
+    return launch_unpermute<bf16_t>((hipStream_t)stream, T, k, H, inv_perm, num_kept,
+                                    (const bf16_t*)y, weights, (bf16_t*)out);
+  return launch_unpermute<float>((hipStream_t)stream, T, k, H, inv_perm, num_kept, (const float*)y,
+                                 weights, (float*)out);
+}
+
+moe_status moe_unpermute_backward(int32_t device, void* stream, int32_t dtype, int64_t T,
+                                  int32_t k, int32_t H, const int32_t* inv_perm,
+                                  const int32_t* num_kept, const void* d_out, const void* y,
+                                  const float* weights, void* d_y, float* d_weights) {
+  moe_status st = check_rows(dtype, T, k, H);
+  if (st != MOE_OK || T == 0) return st;
+  if ((st = check_pointers({inv_perm, d_out, d_y}, {y, weights, d_weights})) != MOE_OK) return st;
+  if (!num_kept) return fail(MOE_ERR_INVALID, "a required pointer is NULL");
+  if (d_weights && !y) return fail(MOE_ERR_INVALID, "d_weights needs y");
+  DeviceScope dev(device);
+  HIP_TRY(dev.enter());
+  if (dtype == MOE_DTYPE_BF16)
+    return launch_unpermute_bwd<bf16_t>((hipStream_t)stream, T, k, H, inv_perm, num_kept,
+                                        (const bf16_t*)d_out, (const bf16_t*)y, weights,
+                                        (bf16_t*)d_y, d_weights);
+  return launch_unpermute_bwd<float>((hipStream_t)stream, T, k, H, inv_perm, num_kept,
+                                     (const float*)d_out, (const float*)y, weights, (float*)d_y,
+                                     d_weights);
+}
+
+size_t moe_linear_workspace_bytes(int32_t dtype, int64_t M, int32_t K, int32_t N, int32_t E,
+                                  int32_t grouped, int32_t activation, int32_t backward) {
+  if (check_linear(dtype, M, K, N, E, grouped != 0, activation) != MOE_OK) return 0;
+  return linear_ws(dtype, M, K, N, E, grouped != 0, activation, backward != 0).total;
+}
+
+moe_status moe_linear_forward(int32_t device, void* stream, int32_t dtype, int64_t M, int32_t K,
+                              int32_t N, int32_t E, const int32_t* offsets, const void* x,
+                              const void* weight, const void* bias, const void* residual,
+                              int32_t activation, void* y, void* pre_act, void* workspace) {
+  moe_status st = check_linear(dtype, M, K, N, E, offsets != nullptr, activation);
+  if (st != MOE_OK || M == 0) return st;
+  if ((st = check_pointers({x, weight, y}, {bias, residual, pre_act})) != MOE_OK) return st;
+  if (offsets && (st = check_pointers({offsets, workspace})) != MOE_OK) return st;
+  DeviceScope dev(device);
+  HIP_TRY(dev.enter());
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == MOE_DTYPE_BF16)
+    return linear_forward<bf16_t>(s, M, K, N, E, offsets, (const bf16_t*)x, (const bf16_t*)weight,
+                                  {(const bf16_t*)bias, (const bf16_t*)residual, (bf16_t*)y,
+                                   (bf16_t*)pre_act, activation, N},
+                                  (char*)workspace);
+  return linear_forward<float>(s, M, K, N, E, offsets, (const float*)x, (const float*)weight,
+                               {(const float*)bias, (const float*)residual, (float*)y,
+                                (float*)pre_act, activation, N},
+                               (char*)workspace);
+}
+
+moe_status moe_linear_backward(int32_t device, void* stream, int32_t dtype, int64_t M, int32_t K,
+                               int32_t N, int32_t E, const int32_t* offsets, const void* d_y,
+                               const void* x, const void* weight, const void* pre_act,
+                               int32_t activation, void* dx, void* d_weight, void* d_bias,
+                               void* workspace) {
+  moe_status st = check_linear(dtype, M, K, N, E, offsets != nullptr, activation);
+  if (st != MOE_OK) return st;
+  const int64_t b = elt_size(dtype);
+  // the weight gradient's operands reach over all rows of a group
+  if (M * std::max(K, N) * b >= kMaxExtentBytes)
+    return fail(MOE_ERR_UNSUPPORTED, "num_rows x max(in, out features) reaches 2^31 bytes");
+  if ((st = check_pointers({}, {dx, d_weight, d_bias, workspace})) != MOE_OK) return st;
+  DeviceScope dev(device);
+  HIP_TRY(dev.enter());
+  hipStream_t s = (hipStream_t)stream;
+  if (M == 0) {  // sums over no row
+    if ((st = zero_async(s, d_weight, (size_t)E * N * K * b)) != MOE_OK) return st;
+    return zero_async(s, d_bias, (size_t)E * N * b);
+  }
+  if ((st = check_pointers({d_y, x, weight}, {pre_act})) != MOE_OK) return st;
+  if (activation != kActNone && !pre_act)
+    return fail(MOE_ERR_INVALID, "the activation's backward needs pre_act");
+  if (offsets && (st = check_pointers({offsets})) != MOE_OK) return st;
+  if (linear_ws(dtype, M, K, N, E, offsets != nullptr, activation, true).total && !workspace)
+    return fail(MOE_ERR_INVALID, "a required pointer is NULL");
+  if (dtype == MOE_DTYPE_BF16)
+    return linear_backward<bf16_t>(s, M, K, N, E, offsets, (const bf16_t*)d_y, (const bf16_t*)x,
+                                   (const bf16_t*)weight, (const bf16_t*)pre_act, activation,
+                                   (bf16_t*)dx, (bf16_t*)d_weight, (bf16_t*)d_bias,
+                                   (char*)workspace);
+  return linear_backward<float>(s, M, K, N, E, offsets, (const float*)d_y, (const float*)x,
+                                (const float*)weight, (const float*)pre_act, activation, (float*)dx,
+                                (float*)d_weight, (float*)d_bias, (char*)workspace);
+}
+
+moe_status moe_residual_norm(int32_t device, void* stream, int32_t dtype, int64_t T, int32_t H,
+                             const void* h, const void* y, const void* post_weight,
+                             const void* gate, int32_t gate_kind, const void* next_weight,
+                             float residual_scale, float eps, void* h_out, void* n_out,
+                             float* rstd_post, float* rstd_next) {
+  moe_status st = check_norm(dtype, T, H, gate_kind, y, post_weight, gate, next_weight,
+                             residual_scale);
+  if (st != MOE_OK || T == 0) return st;
+  if ((st = check_pointers({h}, {y, post_weight, gate, next_weight, h_out, n_out, rstd_post,
+                                 rstd_next})) != MOE_OK)
+    return st;
+  if ((y && !h_out) || (next_weight && !n_out))
+    return fail(MOE_ERR_INVALID, "a required pointer is NULL");
+  DeviceScope dev(device);
+  HIP_TRY(dev.enter());
+  auto go = [&](auto d) {
+    using D = decltype(d);
+    return launch_norm_fwd<D>((hipStream_t)stream,
+                              {(const D*)h, (const D*)y, (const D*)post_weight, (const D*)gate,
+                               (const D*)next_weight, gate_kind, residual_scale, eps, T, H,
+                               (D*)h_out, (D*)n_out, rstd_post, rstd_next});
+  };
+  return dtype == MOE_DTYPE_BF16 ? go(bf16_t()) : go(float());
+}
+
+size_t moe_residual_norm_workspace_bytes(int64_t T, int32_t H) {
+  if (check_norm(MOE_DTYPE_F32, T, H, kGateNone, false, false, false, true, 1.0f) != MOE_OK) return 0;
+  return (size_t)norm_bwd_blocks(T, H) * 2 * H * sizeof(float);
+}
+
+moe_status moe_residual_norm_backward(int32_t device, void* stream, int32_t dtype, int64_t T,
+                                      int32_t H, const void* d_h_out, const void* d_n_out,
+                                      const void* h_out, const void* y, const void* post_weight,
+                                      const void* gate, int32_t gate_kind, const void* next_weight,
+                                      float residual_scale, const float* rstd_post,
+                                      const float* rstd_next, void* d_h, void* d_y,
+                                      void* d_post_weight, void* d_gate, void* d_next_weight,
+                                      void* workspace) {
+  moe_status st = check_norm(dtype, T, H, gate_kind, y, post_weight, gate, next_weight,
+                             residual_scale);
+  if (st != MOE_OK) return st;
+  if ((st = check_pointers({}, {d_h_out, d_n_out, h_out, y, post_weight, gate, next_weight,
+                                rstd_post, rstd_next, d_h, d_y, d_post_weight, d_gate,
+                                d_next_weight, workspace})) != MOE_OK)
+    return st;
+  if ((post_weight && !d_post_weight) || (gate && !d_gate) || (next_weight && !d_next_weight))
+    return fail(MOE_ERR_INVALID, "a required pointer is NULL");
+  const size_t b = elt_size(dtype);
+  DeviceScope dev(device);
+  HIP_TRY(dev.enter());
+  hipStream_t s = (hipStream_t)stream;
+  if (T == 0) {  // sums over no row
+    if ((st = zero_async(s, d_post_weight, H * b)) != MOE_OK) return st;
+    if ((st = zero_async(s, gate_kind == kGateChannel ? d_gate : nullptr, H * b)) != MOE_OK) return st;
+    return zero_async(s, d_next_weight, H * b);
+  }
+  if (!d_h || (y && !d_y) || !workspace || (post_weight && !rstd_post) ||
+      (next_weight && (!rstd_next || !h_out || !d_n_out)) || (!next_weight && !d_h_out))
+    return fail(MOE_ERR_INVALID, "a required pointer is NULL");
+  const bool chan = gate_kind == kGateChannel;
+  auto go = [&](auto d) {
+    using D = decltype(d);
+    const NormBwdArgs<D> a{(const D*)d_h_out, (const D*)d_n_out, (const D*)h_out, (const D*)y,
+                           (const D*)post_weight, (const D*)gate, (const D*)next_weight, gate_kind,
+                           residual_scale, T, H, rstd_post, rstd_next, (D*)d_h, (D*)d_y,
+                           chan ? nullptr : (D*)d_gate, (float*)workspace,
+                           post_weight || chan ? 1 : 0, next_weight ? 1 : 0};
+    return launch_norm_bwd<D>(s, a, (D*)d_post_weight, chan ? (D*)d_gate : nullptr,
+                              (D*)d_next_weight);
+  };
+  return dtype == MOE_DTYPE_BF16 ? go(bf16_t()) : go(float());
+}
+
+}  // extern "C"

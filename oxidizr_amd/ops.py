@@ -1,0 +1,416 @@
+"""Operators beside the MoE layer, for layers whose experts are not the plan's SwiGLU: adapted
+experts (src/model.rs:1416-1446), biases, other activations, norms on both sides of the block.
+
+    order = sort_tokens(topk_idx, num_experts)            # assignments sorted by expert
+    rows = permute_tokens(x, order)                       # [T, H] -> [T k, H], expert by expert
+    a = expert_linear(rows, w1, b1, offsets=order.offsets, activation="gelu")
+    b = expert_linear(a, w2, b2, offsets=order.offsets)
+    y = unpermute_tokens(b, order, weights)               # back to [T, H], weighted
+    h, n = residual_norm(h, y, post_weight, gate=g, next_weight=w)
+
+Every function takes float32 or bfloat16 CUDA tensors (one dtype to a call; routing weights are
+float32), runs on the current stream of their device, sums in fp32 in a fixed order and is
+differentiable once.  Tensors that are not contiguous or not 16-byte aligned are copied first.
+Wrong arguments raise ModelError, what the library refuses MoeError.  The arithmetic runs in
+libmoe_hip.so; PyTorch provides memory, streams and the autograd nodes.
+"""
+from typing import NamedTuple, Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .moe import ModelError, _dtype_code
+
+ACTIVATIONS = ("none", "relu", "silu", "gelu", "gelu_tanh")  # moe_activation's order
+_GATE_NONE, _GATE_CHANNEL, _GATE_TOKEN, _GATE_FULL = range(4)
+MAX_EXPERTS_PER_TOK = 16
+MAX_EXPERTS = 1024
+
+
+class TokenOrder(NamedTuple):
+    """The T k assignments of a routing sorted by expert (int32 tensors)."""
+    counts: torch.Tensor    # [E] assignments of each expert
+    offsets: torch.Tensor   # [E + 1] their exclusive prefix; offsets[E]: assignments with an expert
+    perm: torch.Tensor      # [T k] position -> t * k + j
+    inv_perm: torch.Tensor  # [T, k] t * k + j -> position
+
+
+def _require(ok, message):
+    if not ok:
+        raise ModelError(message)
+
+
+def _ready(t):
+    """t as the library reads it: contiguous and 16-byte aligned."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _on_device(first, *others):
+    """The device index of a call's tensors (the first is always there)."""
+    _require(first.is_cuda, f"expected CUDA tensors, got one on {first.device}")
+    for t in others:
+        _require(t is None or t.device == first.device,
+                 f"tensors on different devices: {first.device} and {t.device if t is not None else None}")
+    return first.device.index
+
+
+def _call(fn, device, *args):
+    _lib.check(fn(device, torch.cuda.current_stream(device).cuda_stream, *args))
+
+
+def _workspace(nbytes, like):
+    """Scratch of one call, from the caching allocator: its stream hands the memory out again only
+    behind the call's kernels, and a captured call keeps its own in the graph's pool."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+
+
+def _tracked(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+# ---------------------------------------------------------------- tokens sorted by expert and back
+
+def sort_tokens(topk_idx, num_experts: int) -> TokenOrder:
+    """Stable sort of topk_idx [T, k] (int32 or int64) by expert, then by t * k + j. An index outside
+    [0, num_experts) has no expert (a padding token) and comes behind every expert."""
+    _require(topk_idx.dim() == 2, f"topk_idx must be [T, k], got {list(topk_idx.shape)}")
+    _require(topk_idx.dtype in (torch.int32, torch.int64),
+             f"topk_idx must be int32 or int64, got {topk_idx.dtype}")
+    T, k = topk_idx.shape
+    _require(1 <= k <= MAX_EXPERTS_PER_TOK, f"experts per token must be 1..{MAX_EXPERTS_PER_TOK}, got {k}")
+    _require(1 <= num_experts <= MAX_EXPERTS, f"num_experts must be 1..{MAX_EXPERTS}, got {num_experts}")
+    dev = _on_device(topk_idx)
+    idx = _ready(topk_idx)
+    L = _lib.load()
+
+    def ints(*shape):
+        return torch.empty(shape, dtype=torch.int32, device=idx.device)
+    order = TokenOrder(ints(num_experts), ints(num_experts + 1), ints(T * k), ints(T, k))
+    ws = _workspace(L.moe_sort_workspace_bytes(T, k, num_experts), idx)
+    _call(L.moe_sort_tokens, dev, T, k, num_experts, idx.element_size(), _ptr(idx), _ptr(order.counts),
+          _ptr(order.offsets), _ptr(order.perm), _ptr(order.inv_perm), _ptr(ws))
+    return order
+
+
+def _check_order(order):
+    _require(isinstance(order, TokenOrder), "order must be a TokenOrder (sort_tokens)")
+    _require(order.inv_perm.dim() == 2, "order.inv_perm must be [T, k]")
+    for t in (order.offsets, order.inv_perm):
+        _require(t.dtype == torch.int32, f"a TokenOrder holds int32 tensors, got {t.dtype}")
+    _require(1 <= order.inv_perm.shape[1] <= MAX_EXPERTS_PER_TOK,
+             f"experts per token must be 1..{MAX_EXPERTS_PER_TOK}, got {order.inv_perm.shape[1]}")
+    _require(order.offsets.dim() == 1 and order.offsets.numel() >= 2, "order.offsets must be [E + 1]")
+    return order.inv_perm.shape
+
+
+def _check_hidden(H):
+    _require(H >= 8 and H % 8 == 0, f"the hidden size must be a positive multiple of 8, got {H}")
+
+
+class _Slots:
+    """What the row kernels read of a TokenOrder."""
+
+    def __init__(self, order):
+        self.inv, self.offsets = _ready(order.inv_perm), _ready(order.offsets)
+        self.T, self.k = order.inv_perm.shape
+        self.kept = self.offsets.data_ptr() + 4 * (self.offsets.numel() - 1)
+
+
+def _permute(x, slots):
+    out = x.new_empty(slots.T * slots.k, x.shape[1])
+    _call(_lib.load().moe_permute, x.device.index, _dtype_code(x.dtype), slots.T, slots.k, x.shape[1],
+          _ptr(slots.inv), slots.kept, _ptr(x), _ptr(out))
+    return out
+
+
+def _unpermute(y, slots, weights):
+    out = y.new_empty(slots.T, y.shape[1])
+    _call(_lib.load().moe_unpermute, y.device.index, _dtype_code(y.dtype), slots.T, slots.k, y.shape[1],
+          _ptr(slots.inv), slots.kept, _ptr(y), _ptr(weights), _ptr(out))
+    return out
+
+
+class _Permute(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, slots):
+        ctx.slots = slots
+        return _permute(_ready(x), slots)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dxp):
+        return _unpermute(_ready(dxp), ctx.slots, None), None
+
+
+def permute_tokens(x, order: TokenOrder):
+    """Rows of x [T, H] in the order's positions: out[inv_perm[t, j]] = x[t] [T k, H]; the rows behind
+    the last expert's (assignments without one) are zeros."""
+    T, k = _check_order(order)
+    _require(x.dim() == 2 and x.shape[0] == T, f"x must be [{T}, H], got {list(x.shape)}")
+    _check_hidden(x.shape[1])
+    _dtype_code(x.dtype)
+    _on_device(x, order.inv_perm, order.offsets)
+    slots = _Slots(order)
+    if _tracked(x):
+        return _Permute.apply(x, slots)
+    return _permute(_ready(x), slots)
+
+
+class _Unpermute(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weights, slots):
+        y = _ready(y)
+        weights = None if weights is None else _ready(weights)
+        need_dw = weights is not None and ctx.needs_input_grad[1]
+        # the rows are read again only for the gradient of the weights
+        ctx.save_for_backward(y if need_dw else None, weights)
+        ctx.slots = slots
+        return _unpermute(y, slots, weights)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        y, weights = ctx.saved_tensors
+        slots, dout = ctx.slots, _ready(dout)
+        dy = dout.new_empty(slots.T * slots.k, dout.shape[1])
+        dw = torch.empty_like(weights) if y is not None else None
+        _call(_lib.load().moe_unpermute_backward, dout.device.index, _dtype_code(dout.dtype), slots.T,
+              slots.k, dout.shape[1], _ptr(slots.inv), slots.kept, _ptr(dout), _ptr(y), _ptr(weights),
+              _ptr(dy), _ptr(dw))
+        return dy, dw, None
+
+
+def unpermute_tokens(y, order: TokenOrder, weights: Optional[torch.Tensor] = None):
+    """out[t] = sum_j weights[t, j] * y[inv_perm[t, j]] [T, H] over the assignments that have an expert,
+    j ascending; weights [T, k] float32, or None for a plain sum."""
+    T, k = _check_order(order)
+    _require(y.dim() == 2 and y.shape[0] == T * k, f"y must be [{T * k}, H], got {list(y.shape)}")
+    _check_hidden(y.shape[1])
+    _dtype_code(y.dtype)
+    if weights is not None:
+        _require(weights.dtype == torch.float32 and weights.shape == (T, k),
+                 f"weights must be float32 [{T}, {k}], got {weights.dtype} {list(weights.shape)}")
+    _on_device(y, order.inv_perm, order.offsets, weights)
+    slots = _Slots(order)
+    if _tracked(y, weights):
+        return _Unpermute.apply(y, weights, slots)
+    return _unpermute(_ready(y), slots, None if weights is None else _ready(weights))
+
+
+# ---------------------------------------------------------------- expert products
+
+class _LinearShape(NamedTuple):
+    M: int
+    K: int
+    N: int
+    groups: int
+    grouped: bool
+    act: int
+
+
+def _linear(x, weight, bias, offsets, residual, s, keep):
+    L = _lib.load()
+    code = _dtype_code(x.dtype)
+    y = x.new_empty(s.M, s.N)
+    pre = torch.empty_like(y) if keep else None
+    ws = _workspace(L.moe_linear_workspace_bytes(code, s.M, s.K, s.N, s.groups, s.grouped, s.act, 0), x)
+    _call(L.moe_linear_forward, x.device.index, code, s.M, s.K, s.N, s.groups, _ptr(offsets), _ptr(x),
+          _ptr(weight), _ptr(bias), _ptr(residual), s.act, _ptr(y), _ptr(pre), _ptr(ws))
+    return y, pre
+
+
+class _ExpertLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, offsets, s):
+        x, weight = _ready(x), _ready(weight)
+        bias = None if bias is None else _ready(bias)
+        residual = None if residual is None else _ready(residual)
+        products = any(ctx.needs_input_grad[:3])  # any gradient that reads the pre-activation
+        y, pre = _linear(x, weight, bias, offsets, residual, s, products and s.act != 0)
+        ctx.save_for_backward(x, weight, pre, offsets)
+        ctx.s = s
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, pre, offsets = ctx.saved_tensors
+        s, (need_x, need_w, need_b, need_r) = ctx.s, ctx.needs_input_grad[:4]
+        dx = dw = db = None
+        if need_x or need_w or need_b:
+            up = _ready(dy)
+            L = _lib.load()
+            code = _dtype_code(up.dtype)
+            dx = torch.empty_like(x) if need_x else None
+            dw = torch.empty_like(weight) if need_w else None
+            db = up.new_empty((s.groups, s.N) if s.grouped else (s.N,)) if need_b else None
+            ws = _workspace(L.moe_linear_workspace_bytes(code, s.M, s.K, s.N, s.groups, s.grouped,
+                                                         s.act, 1), up)
+            _call(L.moe_linear_backward, up.device.index, code, s.M, s.K, s.N, s.groups, _ptr(offsets),
+                  _ptr(up), _ptr(x), _ptr(weight), _ptr(pre), s.act, _ptr(dx), _ptr(dw), _ptr(db),
+                  _ptr(ws))
+        return dx, dw, db, dy if need_r else None, None, None
+
+
+def expert_linear(x, weight, bias=None, *, offsets=None, activation: str = "none", residual=None):
+    """activation(x W^T + bias) + residual, [M, N].
+
+    With offsets (int32 [E + 1], as sort_tokens gives them) rows offsets[e] .. offsets[e + 1] of x [M, K]
+    take weight[e] of weight [E, N, K] and bias[e] of bias [E, N]; rows behind the last expert's are the
+    residual's, or zeros. Without offsets weight is [N, K] and bias [N]. K and N are multiples of 8.
+    activation: one of ACTIVATIONS ("gelu" with the error function, "gelu_tanh" approximated)."""
+    _require(activation in ACTIVATIONS, f"activation must be one of {ACTIVATIONS}, got {activation!r}")
+    _require(x.dim() == 2, f"x must be [M, K], got {list(x.shape)}")
+    M, K = x.shape
+    grouped = offsets is not None
+    _require(weight.dim() == (3 if grouped else 2) and weight.shape[-1] == K,
+             f"weight must be {'[E, N' if grouped else '[N'}, {K}], got {list(weight.shape)}")
+    groups, N = (weight.shape[0], weight.shape[1]) if grouped else (1, weight.shape[0])
+    _require(K >= 8 and K % 8 == 0 and N >= 8 and N % 8 == 0,
+             f"input and output widths must be positive multiples of 8, got {K} and {N}")
+    if grouped:
+        _require(1 <= groups <= MAX_EXPERTS, f"num_experts must be 1..{MAX_EXPERTS}, got {groups}")
+        _require(offsets.dtype == torch.int32 and offsets.shape == (groups + 1,),
+                 f"offsets must be int32 [{groups + 1}], got {offsets.dtype} {list(offsets.shape)}")
+    if bias is not None:
+        want = (groups, N) if grouped else (N,)
+        _require(bias.shape == want, f"bias must be {list(want)}, got {list(bias.shape)}")
+    if residual is not None:
+        _require(residual.shape == (M, N), f"residual must be [{M}, {N}], got {list(residual.shape)}")
+    _dtype_code(x.dtype)
+    for t in (weight, bias, residual):
+        _require(t is None or t.dtype == x.dtype, "x, weight, bias and residual must have one dtype")
+    _on_device(x, weight, bias, residual, offsets)
+    s = _LinearShape(M, K, N, groups, grouped, ACTIVATIONS.index(activation))
+    offsets = _ready(offsets) if grouped else None
+    if _tracked(x, weight, bias, residual):
+        return _ExpertLinear.apply(x, weight, bias, residual, offsets, s)
+    return _linear(_ready(x), _ready(weight), None if bias is None else _ready(bias), offsets,
+                   None if residual is None else _ready(residual), s, False)[0]
+
+
+# ---------------------------------------------------------------- norms around a block
+
+class _NormShape(NamedTuple):
+    T: int
+    H: int
+    gate_kind: int
+    scale: float
+    eps: float
+
+
+def _norm(h, y, post_weight, gate, next_weight, s, keep):
+    out = torch.empty_like(h) if y is not None else None
+    n = torch.empty_like(h) if next_weight is not None else None
+    r2 = h.new_empty(s.T, dtype=torch.float32) if keep and post_weight is not None else None
+    r3 = h.new_empty(s.T, dtype=torch.float32) if keep and next_weight is not None else None
+    _call(_lib.load().moe_residual_norm, h.device.index, _dtype_code(h.dtype), s.T, s.H, _ptr(h), _ptr(y),
+          _ptr(post_weight), _ptr(gate), s.gate_kind, _ptr(next_weight), s.scale, s.eps, _ptr(out), _ptr(n),
+          _ptr(r2), _ptr(r3))
+    return out, n, r2, r3
+
+
+class _ResidualNorm(torch.autograd.Function):
+    """(h_out, n) of a block's output y, or n alone without y (a plain RMSNorm of h)."""
+
+    @staticmethod
+    def forward(ctx, h, y, post_weight, gate, next_weight, s):
+        ctx.set_materialize_grads(False)
+        h, y, post_weight, gate, next_weight = (None if t is None else _ready(t)
+                                                for t in (h, y, post_weight, gate, next_weight))
+        out, n, r2, r3 = _norm(h, y, post_weight, gate, next_weight, s, True)
+        after = h if y is None else out  # what the second norm is taken of
+        ctx.save_for_backward(after if n is not None else None, y, post_weight, gate, next_weight, r2, r3)
+        ctx.s = s
+        return (out, n) if y is not None and n is not None else out if n is None else n
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *up):
+        after, y, post_weight, gate, next_weight, r2, r3 = ctx.saved_tensors
+        s = ctx.s
+        d_out = up[0] if y is not None else None
+        d_n = up[-1] if next_weight is not None else None
+        d_out, d_n = (None if t is None else _ready(t) for t in (d_out, d_n))
+        like = d_out if d_out is not None else d_n
+        if like is None:
+            return (None,) * 6
+        d_next = None
+        if next_weight is not None:
+            # without a gradient of n the second norm has none
+            d_next = torch.zeros_like(next_weight) if d_n is None else torch.empty_like(next_weight)
+        used = next_weight if d_n is not None else None
+        d_h = torch.empty_like(like)
+        d_y = None if y is None else torch.empty_like(like)
+        d_post = None if post_weight is None else torch.empty_like(post_weight)
+        d_gate = None if gate is None else torch.empty_like(gate)
+        L = _lib.load()
+        ws = _workspace(L.moe_residual_norm_workspace_bytes(s.T, s.H), like)
+        _call(L.moe_residual_norm_backward, like.device.index, _dtype_code(like.dtype), s.T, s.H,
+              _ptr(d_out), _ptr(d_n), _ptr(after), _ptr(y), _ptr(post_weight), _ptr(gate), s.gate_kind,
+              _ptr(used), s.scale, _ptr(r2), _ptr(r3), _ptr(d_h), _ptr(d_y), _ptr(d_post), _ptr(d_gate),
+              _ptr(d_next) if used is not None else None, _ptr(ws))
+        return d_h, d_y, d_post, d_gate, d_next, None
+
+
+def _gate_kind(gate, h):
+    if gate is None:
+        return _GATE_NONE
+    if gate.shape == h.shape:
+        return _GATE_FULL
+    if gate.shape == h.shape[-1:]:
+        return _GATE_CHANNEL
+    _require(gate.shape == h.shape[:-1] + (1,),
+             f"gate must be {list(h.shape[-1:])}, {list(h.shape[:-1]) + [1]} or {list(h.shape)}, "
+             f"got {list(gate.shape)}")
+    return _GATE_TOKEN
+
+
+def _check_norm(h, *weights):
+    _require(h.dim() >= 2, f"expected [..., T, H], got {list(h.shape)}")
+    H = h.shape[-1]
+    _check_hidden(H)
+    _dtype_code(h.dtype)
+    for w in weights:
+        _require(w is None or w.shape == (H,), f"a norm's weight must be [{H}]")
+        _require(w is None or w.dtype == h.dtype, "activations and norm weights must have one dtype")
+    return H
+
+
+def rms_norm(x, weight, eps: float = 1e-6):
+    """x / sqrt(mean(x^2) + eps) * weight over the last dimension."""
+    H = _check_norm(x, weight)
+    _on_device(x, weight)
+    s = _NormShape(x.numel() // H, H, _GATE_NONE, 1.0, eps)
+    if _tracked(x, weight):
+        return _ResidualNorm.apply(x, None, None, None, weight, s)
+    return _norm(_ready(x), None, None, None, _ready(weight), s, False)[1]
+
+
+def residual_norm(h, y, post_weight=None, *, gate=None, next_weight=None, residual_scale: float = 1.0,
+                  eps: float = 1e-6):
+    """A block's output y added to its input h, with the norms on both sides, in one pass:
+
+        h_out = residual_scale * h + gate * RMSNorm(y) * post_weight   (y itself without post_weight)
+        n     = RMSNorm(h_out) * next_weight                           (the next block's input)
+
+    h, y [..., H]; post_weight, next_weight [H]; gate [H], [..., 1] or [..., H]. Returns h_out, or
+    (h_out, n) with a next_weight."""
+    H = _check_norm(h, post_weight, next_weight)
+    _require(y.shape == h.shape, f"y must be {list(h.shape)}, got {list(y.shape)}")
+    _require(y.dtype == h.dtype and (gate is None or gate.dtype == h.dtype),
+             "h, y and gate must have one dtype")
+    kind = _gate_kind(gate, h)
+    _on_device(h, y, post_weight, gate, next_weight)
+    s = _NormShape(h.numel() // H, H, kind, float(residual_scale), eps)
+    if _tracked(h, y, post_weight, gate, next_weight):
+        return _ResidualNorm.apply(h, y, post_weight, gate, next_weight, s)
+    out, n, _, _ = _norm(*(None if t is None else _ready(t) for t in (h, y, post_weight, gate, next_weight)),
+                         s, False)
+    return out if n is None else (out, n)

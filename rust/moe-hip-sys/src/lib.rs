@@ -54,6 +54,19 @@ pub mod ffi {
     pub const MOE_SAVED_MEAN_PROB: i32 = 9;
     pub const MOE_NUM_STAGES: usize = 20;
 
+    /// `moe_activation`: the epilogue of `moe_linear_forward`.
+    pub const MOE_ACT_NONE: i32 = 0;
+    pub const MOE_ACT_RELU: i32 = 1;
+    pub const MOE_ACT_SILU: i32 = 2;
+    pub const MOE_ACT_GELU: i32 = 3;
+    pub const MOE_ACT_GELU_TANH: i32 = 4;
+
+    /// `moe_gate_kind`: the shape of `moe_residual_norm`'s gate.
+    pub const MOE_GATE_NONE: i32 = 0;
+    pub const MOE_GATE_CHANNEL: i32 = 1;
+    pub const MOE_GATE_TOKEN: i32 = 2;
+    pub const MOE_GATE_FULL: i32 = 3;
+
     #[repr(C)]
     #[derive(Clone, Copy, Debug, Default)]
     pub struct MoeConfigC {
@@ -151,6 +164,159 @@ pub mod ffi {
         pub fn moe_plan_set_shared_overlap(plan: *mut MoePlan, on: i32) -> MoeStatus;
         pub fn moe_plan_stage_times(plan: *mut MoePlan, ms: *mut f32, calls: *mut i32,
                                     reset: i32) -> MoeStatus;
+        pub fn moe_sort_workspace_bytes(
+            num_tokens: i64,
+            experts_per_tok: i32,
+            num_experts: i32,
+        ) -> usize;
+        pub fn moe_sort_tokens(
+            device: i32,
+            stream: *mut c_void,
+            num_tokens: i64,
+            experts_per_tok: i32,
+            num_experts: i32,
+            index_bytes: i32,
+            topk_idx: *const c_void,
+            counts: *mut i32,
+            offsets: *mut i32,
+            perm: *mut i32,
+            inv_perm: *mut i32,
+            workspace: *mut c_void,
+        ) -> MoeStatus;
+        pub fn moe_permute(
+            device: i32,
+            stream: *mut c_void,
+            dtype: i32,
+            num_tokens: i64,
+            experts_per_tok: i32,
+            hidden: i32,
+            inv_perm: *const i32,
+            num_kept: *const i32,
+            x: *const c_void,
+            x_perm: *mut c_void,
+        ) -> MoeStatus;
+        pub fn moe_unpermute(
+            device: i32,
+            stream: *mut c_void,
+            dtype: i32,
+            num_tokens: i64,
+            experts_per_tok: i32,
+            hidden: i32,
+            inv_perm: *const i32,
+            num_kept: *const i32,
+            y: *const c_void,
+            weights: *const f32,
+            out: *mut c_void,
+        ) -> MoeStatus;
+        pub fn moe_unpermute_backward(
+            device: i32,
+            stream: *mut c_void,
+            dtype: i32,
+            num_tokens: i64,
+            experts_per_tok: i32,
+            hidden: i32,
+            inv_perm: *const i32,
+            num_kept: *const i32,
+            d_out: *const c_void,
+            y: *const c_void,
+            weights: *const f32,
+            d_y: *mut c_void,
+            d_weights: *mut f32,
+        ) -> MoeStatus;
+        pub fn moe_linear_workspace_bytes(
+            dtype: i32,
+            num_rows: i64,
+            in_features: i32,
+            out_features: i32,
+            num_groups: i32,
+            grouped: i32,
+            activation: i32,
+            backward: i32,
+        ) -> usize;
+        pub fn moe_linear_forward(
+            device: i32,
+            stream: *mut c_void,
+            dtype: i32,
+            num_rows: i64,
+            in_features: i32,
+            out_features: i32,
+            num_groups: i32,
+            offsets: *const i32,
+            x: *const c_void,
+            weight: *const c_void,
+            bias: *const c_void,
+            residual: *const c_void,
+            activation: i32,
+            y: *mut c_void,
+            pre_act: *mut c_void,
+            workspace: *mut c_void,
+        ) -> MoeStatus;
+        pub fn moe_linear_backward(
+            device: i32,
+            stream: *mut c_void,
+            dtype: i32,
+            num_rows: i64,
+            in_features: i32,
+            out_features: i32,
+            num_groups: i32,
+            offsets: *const i32,
+            d_y: *const c_void,
+            x: *const c_void,
+            weight: *const c_void,
+            pre_act: *const c_void,
+            activation: i32,
+            dx: *mut c_void,
+            d_weight: *mut c_void,
+            d_bias: *mut c_void,
+            workspace: *mut c_void,
+        ) -> MoeStatus;
+        pub fn moe_residual_norm(
+            device: i32,
+            stream: *mut c_void,
+            dtype: i32,
+            num_tokens: i64,
+            hidden: i32,
+            h: *const c_void,
+            y: *const c_void,
+            post_weight: *const c_void,
+            gate: *const c_void,
+            gate_kind: i32,
+            next_weight: *const c_void,
+            residual_scale: f32,
+            eps: f32,
+            h_out: *mut c_void,
+            n_out: *mut c_void,
+            rstd_post: *mut f32,
+            rstd_next: *mut f32,
+        ) -> MoeStatus;
+        pub fn moe_residual_norm_workspace_bytes(
+            num_tokens: i64,
+            hidden: i32,
+        ) -> usize;
+        pub fn moe_residual_norm_backward(
+            device: i32,
+            stream: *mut c_void,
+            dtype: i32,
+            num_tokens: i64,
+            hidden: i32,
+            d_h_out: *const c_void,
+            d_n_out: *const c_void,
+            h_out: *const c_void,
+            y: *const c_void,
+            post_weight: *const c_void,
+            gate: *const c_void,
+            gate_kind: i32,
+            next_weight: *const c_void,
+            residual_scale: f32,
+            rstd_post: *const f32,
+            rstd_next: *const f32,
+            d_h: *mut c_void,
+            d_y: *mut c_void,
+            d_post_weight: *mut c_void,
+            d_gate: *mut c_void,
+            d_next_weight: *mut c_void,
+            workspace: *mut c_void,
+        ) -> MoeStatus;
         pub fn moe_last_error() -> *const c_char;
         pub fn moe_version() -> *const c_char;
     }

@@ -1,0 +1,525 @@
+"""oxidizr_amd.ops on the GPU against plain float64 forms (tests/ops_ref.py), at the sizes, masks and
+layouts where they can go wrong, with bounds from arithmetic."""
+import pytest
+import torch
+
+from oxidizr_amd import ops
+from tests import ops_ref as ref
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.float32, torch.bfloat16]
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def normal(g, *shape, dtype=torch.float32, std=1.0, mean=0.0):
+    return torch.empty(shape, dtype=dtype, device="cuda").normal_(mean, std, generator=g)
+
+
+def routing(g, T, k, E, pad=0.0, skew=0.0):
+    logits = torch.randn(T, E, device="cuda", generator=g)
+    logits += skew * torch.randn(E, device="cuda", generator=g)
+    idx = torch.topk(logits, min(k, E), dim=1).indices.to(torch.int32)
+    if pad:
+        idx[torch.rand(T, device="cuda", generator=g) < pad] = -1
+    return idx
+
+
+def check_order(got, idx, E):
+    for name, a, b in zip(got._fields, got, ref.order(idx.cpu(), E)):
+        assert torch.equal(a.cpu(), b), name
+
+
+# ---------------------------------------------------------------- sorting
+
+@pytest.mark.parametrize("T,k,E", [(1, 1, 1), (1, 16, 16), (7, 3, 5), (64, 8, 128), (255, 2, 1024),
+                                   (257, 8, 64), (1023, 2, 7), (1025, 2, 300), (5000, 6, 64),
+                                   (3001, 16, 1023), (40000, 2, 16)])
+def test_sort_matches_brute_force(T, k, E):
+    g = gen(T + E)
+    idx = torch.randint(-1, E + 1, (T, k), device="cuda", generator=g, dtype=torch.int32)
+    check_order(ops.sort_tokens(idx, E), idx, E)
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_sort_index_types_and_what_has_no_expert(dtype):
+    far = 2 ** 31 - 1 if dtype == torch.int32 else 2 ** 32 + 3  # 3 in its low half
+    idx = torch.tensor([[3, 3], [-1, 0], [4, far], [-far, 1], [3, 0]], dtype=dtype, device="cuda")
+    check_order(ops.sort_tokens(idx, 4), idx, 4)
+
+
+def test_sort_edges():
+    for idx, E in [(torch.full((33, 4), -1), 8), (torch.full((3000, 2), 5), 8), (torch.zeros(0, 2), 3),
+                   (torch.arange(4096).view(2048, 2) % 1024, 1024)]:
+        idx = idx.to(torch.int32).cuda()
+        check_order(ops.sort_tokens(idx, E), idx, E)
+
+
+def test_sort_of_a_strided_index():
+    idx = routing(gen(3), 300, 5, 16)
+    part = idx[1:, 1:4]
+    check_order(ops.sort_tokens(part, 16), part, 16)
+
+
+def test_sort_beyond_one_chunk_per_block():
+    # more entries than the blocks take in one tile each: longer chunks
+    T, k, E = 200000, 6, 33
+    idx = torch.randint(-1, E, (T, k), device="cuda", generator=gen(8), dtype=torch.int32)
+    got = ops.sort_tokens(idx, E)
+    key = torch.where(idx.flatten() < 0, E, idx.flatten())
+    perm = torch.argsort(key, stable=True)
+    assert torch.equal(got.perm.long(), perm)
+    assert torch.equal(got.inv_perm.flatten().long()[perm], torch.arange(T * k, device="cuda"))
+    assert torch.equal(got.counts.long(), torch.bincount(key, minlength=E + 1)[:E])
+    assert int(got.offsets[-1]) == int((key < E).sum())
+
+
+# ---------------------------------------------------------------- rows to experts and back
+
+ROWS = [(1, 8, 1, 1, 0.0), (1, 2048, 16, 16, 0.0), (5, 384, 7, 2, 0.0), (33, 520, 12, 3, 0.3),
+        (64, 4096, 128, 8, 0.0), (130, 1032, 9, 5, 0.1), (259, 776, 64, 6, 0.5), (40, 7168, 256, 8, 0.2),
+        (17, 64, 8, 16, 0.0)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,H,E,k,pad", ROWS)
+def test_permute_and_its_gradient(T, H, E, k, pad, dtype):
+    g = gen(T * H)
+    idx = torch.randint(0, E, (T, k), device="cuda", generator=g, dtype=torch.int32)
+    idx[torch.rand(T, k, device="cuda", generator=g) < pad] = -1
+    order = ops.sort_tokens(idx, E)
+    x = normal(g, T, H, dtype=dtype).requires_grad_()
+    out = ops.permute_tokens(x, order)
+    kept = int(order.offsets[-1])
+    want = x.detach()[(order.perm // k).long()]
+    want[kept:] = 0
+    assert torch.equal(out.detach(), want)
+    d = normal(g, T * k, H, dtype=dtype)
+    d[kept:] = float("nan")  # rows without an expert are not read
+    dx, = torch.autograd.grad(out, x, d)
+    rows = torch.where((order.inv_perm < kept).flatten()[:, None],
+                       d.double()[order.inv_perm.flatten().long()], 0.0).view(T, k, H)
+    ref.assert_close(dx, rows.sum(1), k * ref.U32 * rows.abs().sum(1), "dx")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("weighted", [True, False])
+@pytest.mark.parametrize("T,H,E,k,pad", ROWS)
+def test_unpermute_and_its_gradients(T, H, E, k, pad, weighted, dtype):
+    g = gen(T * H + 1)
+    idx = torch.randint(0, E, (T, k), device="cuda", generator=g, dtype=torch.int32)
+    idx[torch.rand(T, k, device="cuda", generator=g) < pad] = -1
+    order = ops.sort_tokens(idx, E)
+    kept = int(order.offsets[-1])
+    y = normal(g, T * k, H, dtype=dtype)
+    y[kept:] = float("nan")
+    w = torch.rand(T, k, device="cuda", generator=g)
+    y.requires_grad_()
+    w.requires_grad_()
+    out = ops.unpermute_tokens(y, order, w if weighted else None)
+    at = order.inv_perm.long()
+    real = (at < kept)[..., None]
+    rows = torch.where(real, y.detach().double()[at.flatten()].view(T, k, H), 0.0)
+    w64 = w.detach().double() if weighted else torch.ones(T, k, device="cuda", dtype=torch.float64)
+    terms = w64[..., None] * rows
+    ref.assert_close(out.detach(), terms.sum(1), (k + 1) * ref.U32 * terms.abs().sum(1), "out")
+    dout = normal(g, T, H, dtype=dtype)
+    got = torch.autograd.grad(out, [y, w] if weighted else [y], dout)
+    d64 = dout.double()[:, None, :]
+    dy = torch.where(real, w64[..., None] * d64, 0.0).view(T * k, H)[order.perm.long()]
+    ref.assert_close(got[0], dy, ref.U32 * dy.abs(), "dy")
+    assert bool((got[0][kept:] == 0).all())
+    if weighted:
+        prod = d64 * rows
+        ref.assert_close(got[1], prod.sum(2), (H + 8) * ref.U32 * prod.abs().sum(2), "dw")
+
+
+def test_gradient_of_the_rows_alone():
+    # weights that need no gradient: the rows are not kept
+    g = gen(5)
+    order = ops.sort_tokens(routing(g, 50, 4, 8), 8)
+    y = normal(g, 200, 64).requires_grad_()
+    w = torch.rand(50, 4, device="cuda", generator=g)
+    out = ops.unpermute_tokens(y, order, w)
+    dy, = torch.autograd.grad(out, y, torch.ones_like(out))
+    assert torch.equal(dy, w.flatten()[order.perm.long()][:, None].expand(200, 64))
+
+
+# ---------------------------------------------------------------- expert products
+
+def linear_case(g, sizes, K, N, act, dtype, bias, res, tail=0, grouped=True):
+    """Runs expert_linear forward and backward over groups of the given sizes against the reference."""
+    E = len(sizes)
+    offsets = torch.tensor([0] + list(torch.tensor(sizes).cumsum(0)), dtype=torch.int32, device="cuda")
+    M = sum(sizes) + tail
+    t = {"x": normal(g, M, K, dtype=dtype),
+         "w": normal(g, *((E, N, K) if grouped else (N, K)), dtype=dtype, std=K ** -0.5)}
+    if bias:
+        t["b"] = normal(g, *((E, N) if grouped else (N,)), dtype=dtype, std=0.3)
+    if res:
+        t["r"] = normal(g, M, N, dtype=dtype)
+    dy = normal(g, M, N, dtype=dtype)
+    for v in t.values():
+        v.requires_grad_()
+    y = ops.expert_linear(t["x"], t["w"], t.get("b"), offsets=offsets if grouped else None, activation=act,
+                          residual=t.get("r"))
+    got = dict(zip(t, torch.autograd.grad(y, list(t.values()), dy)))
+    d = {n: v.detach().double() for n, v in t.items()}
+    want = ref.linear(d["x"], d["w"], d.get("b"), offsets if grouped else None, act, d.get("r"), dy.double(),
+                      dtype)
+    ref.assert_close(y.detach(), *want["y"], "y")
+    for n, v in got.items():
+        ref.assert_close(v, *want["d" + n], "d" + n)
+    with torch.no_grad():  # the forward that keeps nothing gives the same bits
+        again = ops.expert_linear(t["x"], t["w"], t.get("b"), offsets=offsets if grouped else None,
+                                  activation=act, residual=t.get("r"))
+    assert torch.equal(again, y)
+
+
+LINEAR = [  # group sizes, K, N, rows behind the last group
+    ([1], 8, 8, 0),
+    ([0, 3, 0, 1], 64, 40, 0),
+    ([5, 0, 17, 64, 65, 0], 136, 72, 3),
+    ([0, 0, 0], 64, 64, 9),
+    ([130, 7, 257], 264, 328, 0),
+    ([63, 320, 384, 31], 200, 776, 40),
+    ([1] * 40, 512, 264, 2),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ops.ACTIVATIONS)
+@pytest.mark.parametrize("sizes,K,N,tail", LINEAR)
+def test_grouped_linear(sizes, K, N, tail, act, dtype):
+    linear_case(gen(K + N), sizes, K, N, act, dtype, bias=True, res=False, tail=tail)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["none", "silu"])
+@pytest.mark.parametrize("bias", [True, False])
+@pytest.mark.parametrize("sizes,K,N,tail", LINEAR[1:6])
+def test_grouped_linear_with_a_residual(sizes, K, N, tail, bias, act, dtype):
+    linear_case(gen(K + N + 1), sizes, K, N, act, dtype, bias=bias, res=True, tail=tail)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act,bias,res", [("none", False, False), ("gelu", True, True), ("relu", True, False)])
+@pytest.mark.parametrize("M,K,N", [(1, 256, 48), (16, 1032, 40), (17, 64, 520), (64, 2048, 136),
+                                   (65, 136, 264), (300, 520, 392), (700, 264, 1032)])
+def test_dense_linear(M, K, N, act, bias, res, dtype):
+    linear_case(gen(M + K), [M], K, N, act, dtype, bias, res, grouped=False)
+
+
+@pytest.mark.parametrize("T,E,k", [(900, 4, 2), (2100, 3, 2), (1500, 24, 4)])
+def test_grouped_linear_over_the_tilings(T, E, k):
+    # row counts that reach the 256- and 384-row tiles, their tails and the shorter tilings
+    sizes = torch.bincount(routing(gen(T), T, k, E, skew=0.7).flatten(), minlength=E).tolist()
+    linear_case(gen(T + 1), sizes, 320, 520, "silu", torch.bfloat16, bias=True, res=True, tail=5)
+
+
+def test_linear_gradients_one_at_a_time():
+    g = gen(4)
+    x, w, b = normal(g, 100, 64), normal(g, 3, 40, 64, std=0.1), normal(g, 3, 40)
+    off = torch.tensor([0, 30, 30, 95], dtype=torch.int32, device="cuda")
+    dy = normal(g, 100, 40)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    want = torch.autograd.grad(ops.expert_linear(*leaves, offsets=off, activation="gelu"), leaves, dy)
+    for i in range(3):
+        one = [t.clone().requires_grad_(i == j) for j, t in enumerate((x, w, b))]
+        got, = torch.autograd.grad(ops.expert_linear(*one, offsets=off, activation="gelu"), one[i], dy)
+        assert torch.equal(got, want[i]), i
+    assert bool((want[0][95:] == 0).all()) and bool((want[1][1] == 0).all()) and bool((want[2][1] == 0).all())
+
+
+def test_linear_without_rows():
+    w = torch.ones(2, 16, 8, device="cuda", requires_grad=True)
+    b = torch.ones(2, 16, device="cuda", requires_grad=True)
+    x = torch.zeros(0, 8, device="cuda", requires_grad=True)
+    off = torch.zeros(3, dtype=torch.int32, device="cuda")
+    y = ops.expert_linear(x, w, b, offsets=off)
+    assert y.shape == (0, 16)
+    dx, dw, db = torch.autograd.grad(y, [x, w, b], torch.zeros_like(y))
+    assert dx.shape == x.shape and not bool(dw.any()) and not bool(db.any())
+
+
+def test_linear_rows_behind_the_last_group_do_not_reach_the_gradients():
+    g = gen(14)
+    x = normal(g, 90, 64)
+    x[70:] = float("nan")
+    dy = normal(g, 90, 32)
+    dy[70:] = float("inf")
+    x.requires_grad_()
+    w, b = normal(g, 2, 32, 64).requires_grad_(), normal(g, 2, 32).requires_grad_()
+    off = torch.tensor([0, 33, 70], dtype=torch.int32, device="cuda")
+    for act in ("none", "silu"):
+        y = ops.expert_linear(x, w, b, offsets=off, activation=act)
+        assert bool((y[70:] == 0).all()) and bool(torch.isfinite(y).all())
+        for t in torch.autograd.grad(y, [x, w, b], dy):
+            assert bool(torch.isfinite(t).all())
+
+
+@pytest.mark.parametrize("rows", [20, 3000])
+def test_offsets_that_are_none_stay_inside_the_buffers(rows):
+    # clamped to the running maximum and to the number of rows
+    g = gen(rows)
+    x, w = normal(g, rows, 64, dtype=torch.bfloat16), normal(g, 4, 32, 64, dtype=torch.bfloat16)
+    bad = torch.tensor([0, rows // 2, -7, rows // 4, 10 ** 9], dtype=torch.int32, device="cuda")
+    y = ops.expert_linear(x, w, offsets=bad)
+    assert y.shape == (rows, 32) and bool(torch.isfinite(y.float()).all())
+
+
+# ---------------------------------------------------------------- norms around a block
+
+NORMS = [(1, 8), (1, 2048), (3, 64), (9, 512), (33, 520), (130, 776), (66, 2048), (21, 2056), (17, 4104),
+         (600, 1032), (70, 7168), (5, 8200), (3, 16392), (1100, 384)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gate", [None, "channel", "token", "full"])
+@pytest.mark.parametrize("T,H", NORMS)
+def test_residual_norm(T, H, gate, dtype):
+    for post, nxt in ((True, True), (True, False), (False, True), (False, False)):
+        norm_case(gen(T + H), T, H, gate, dtype, post, nxt, 0.75)
+
+
+def norm_case(g, T, H, gate, dtype, post, nxt, scale, eps=1e-5):
+    t = {"h": normal(g, T, H, dtype=dtype, std=2.0), "y": normal(g, T, H, dtype=dtype)}
+    if post:
+        t["w2"] = normal(g, H, dtype=dtype, std=0.2, mean=1.0)
+    if gate:
+        t["gate"] = normal(g, *{"channel": (H,), "token": (T, 1), "full": (T, H)}[gate], dtype=dtype)
+    if nxt:
+        t["w3"] = normal(g, H, dtype=dtype, std=0.2, mean=1.0)
+    for v in t.values():
+        v.requires_grad_()
+    d_out = normal(g, T, H, dtype=dtype)
+    d_n = normal(g, T, H, dtype=dtype) if nxt else None
+    out = ops.residual_norm(t["h"], t["y"], t.get("w2"), gate=t.get("gate"), next_weight=t.get("w3"),
+                            residual_scale=scale, eps=eps)
+    outs = out if nxt else (out,)
+    got = dict(zip(t, torch.autograd.grad(outs, list(t.values()), (d_out, d_n) if nxt else (d_out,))))
+    d = {n: v.detach().double() for n, v in t.items()}
+    want = ref.norm(d["h"], d["y"], d.get("w2"), d.get("gate"), d.get("w3"), scale, eps, d_out.double(),
+                    d_n.double() if nxt else None, dtype)
+    for name, v in zip(("h", "n"), outs):
+        ref.assert_close(v.detach(), *want[name], name)
+    for n, v in got.items():
+        ref.assert_close(v, *want["d" + n], f"d{n} post={post} next={nxt}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,H", NORMS)
+def test_rms_norm(T, H, dtype):
+    g = gen(H)
+    x, w = normal(g, T, H, dtype=dtype, std=3.0), normal(g, H, dtype=dtype)
+    x.requires_grad_()
+    w.requires_grad_()
+    n = ops.rms_norm(x, w, eps=1e-5)
+    d = normal(g, T, H, dtype=dtype)
+    dx, dw = torch.autograd.grad(n, [x, w], d)
+    want = ref.norm(x.detach().double(), None, None, None, w.detach().double(), 1.0, 1e-5, None, d.double(), dtype)
+    ref.assert_close(n.detach(), *want["n"], "n")
+    ref.assert_close(dx, *want["dh"], "dx")
+    ref.assert_close(dw, *want["dw3"], "dw")
+
+
+def test_residual_norm_when_one_output_has_no_gradient():
+    g = gen(77)
+    leaves = [normal(g, 40, 264).requires_grad_(), normal(g, 40, 264).requires_grad_(),
+              normal(g, 264).requires_grad_(), normal(g, 264).requires_grad_()]
+    h, n = ops.residual_norm(leaves[0], leaves[1], leaves[2], next_weight=leaves[3])
+    d = normal(g, 40, 264)
+    z = torch.zeros_like(d)
+    for only, full in (((h, d), (d, z)), ((n, d), (z, d))):
+        got = torch.autograd.grad(only[0], leaves, only[1], retain_graph=True, allow_unused=True)
+        want = torch.autograd.grad((h, n), leaves, full, retain_graph=True)
+        for a, b in zip(got, want):
+            assert torch.allclose(a if a is not None else torch.zeros_like(b), b, rtol=1e-6, atol=1e-6)
+
+
+def test_rows_of_zeros_and_large_values():
+    # a row of zeros has rstd 1 / sqrt(eps); squares of 1e18 still fit fp32's range
+    h = torch.zeros(3, 64, device="cuda")
+    y = torch.zeros(3, 64, device="cuda")
+    y[1] = 1e18
+    w = torch.ones(64, device="cuda")
+    out, n = ops.residual_norm(h, y, w, next_weight=w, eps=1e-6)
+    assert torch.equal(out[0], h[0]) and torch.equal(n[2], h[0])
+    assert torch.allclose(out[1], torch.ones(64, device="cuda"), rtol=1e-6)
+
+
+def test_shapes_with_a_batch_and_broadcast_gradients():
+    g = gen(6)
+    h, y = normal(g, 2, 5, 64).requires_grad_(), normal(g, 2, 5, 64)
+    gate = normal(g, 2, 5, 1).requires_grad_()
+    out, n = ops.residual_norm(h, y, gate=gate, next_weight=torch.ones(64, device="cuda"))
+    assert out.shape == n.shape == h.shape
+    # sum()'s gradient is a broadcast view with stride 0
+    dh, dg = torch.autograd.grad(out.sum(), [h, gate])
+    assert torch.equal(dh, torch.ones_like(h)) and torch.allclose(dg, y.sum(2, keepdim=True), atol=1e-5)
+
+
+# ---------------------------------------------------------------- as a user runs them
+
+def chain(x, idx, w, p, E):
+    """Tokens to biased experts of two products and back, then the norms around the block."""
+    n = ops.rms_norm(x, p["pre"])
+    order = ops.sort_tokens(idx, E)
+    a = ops.expert_linear(ops.permute_tokens(n, order), p["w1"], p["b1"], offsets=order.offsets, activation="gelu")
+    b = ops.expert_linear(a, p["w2"], p["b2"], offsets=order.offsets)
+    return ops.residual_norm(x, ops.unpermute_tokens(b, order, w), p["post"], gate=p["gate"], next_weight=p["next"])
+
+
+def chain_inputs(g, T, H, I, E, k, dtype):
+    p = {"pre": normal(g, H, dtype=dtype, std=0.1, mean=1.0), "post": normal(g, H, dtype=dtype, std=0.1, mean=1.0),
+         "next": normal(g, H, dtype=dtype, std=0.1, mean=1.0), "gate": normal(g, H, dtype=dtype, std=0.5),
+         "w1": normal(g, E, I, H, dtype=dtype, std=H ** -0.5), "b1": normal(g, E, I, dtype=dtype, std=0.1),
+         "w2": normal(g, E, H, I, dtype=dtype, std=I ** -0.5), "b2": normal(g, E, H, dtype=dtype, std=0.1)}
+    return p, normal(g, T, H, dtype=dtype), routing(g, T, k, E, pad=0.1), torch.rand(T, k, device="cuda", generator=g)
+
+
+def chain_plain(x, idx, w, p, E):
+    """The same in torch, every expert on every token."""
+    def rms(t, weight):
+        return t * torch.rsqrt(t.square().mean(1, keepdim=True) + 1e-6) * weight
+    n = rms(x, p["pre"])
+    y = torch.zeros_like(x)
+    for e in range(E):
+        out = torch.nn.functional.gelu(n @ p["w1"][e].t() + p["b1"][e]) @ p["w2"][e].t() + p["b2"][e]
+        y = y + (w * (idx == e)).sum(1, keepdim=True) * out
+    h = x + p["gate"] * rms(y, p["post"])
+    return h, rms(h, p["next"])
+
+
+def test_a_run_of_them_with_its_gradients():
+    T, H, I, E, k = 150, 136, 200, 6, 2
+    p, x, idx, w = chain_inputs(gen(21), T, H, I, E, k, torch.float32)
+    leaves = [x, w] + list(p.values())
+    for t in leaves:
+        t.requires_grad_()
+    h, n = chain(x, idx, w, p, E)
+    dh, dn = normal(gen(22), T, H), normal(gen(23), T, H)
+    got = torch.autograd.grad((h, n), leaves, (dh, dn))
+    d = [t.detach().double().requires_grad_() for t in leaves]
+    q = dict(zip(p, d[2:]))
+    h64, n64 = chain_plain(d[0], idx, d[1], q, E)
+    want = torch.autograd.grad((h64, n64), d, (dh.double(), dn.double()))
+    # sums of up to T k I = 60000 fp32 terms, whose roundings add up like their root: 2^-24 sqrt(60000)
+    # = 1.5e-5 of the magnitudes
+    for name, a, b in zip(["h", "n", "x", "w"] + list(p), (h, n) + got, (h64, n64) + want):
+        err = float((a.double() - b).norm() / b.norm())
+        assert err < 1.5e-5, (name, err)
+
+
+def test_gradients_against_differences():
+    T, H, I, E, k = 12, 16, 24, 3, 2
+    p, x, idx, w = chain_inputs(gen(31), T, H, I, E, k, torch.float32)
+    leaves = {"x": x, "w": w, **p}
+    for t in leaves.values():
+        t.requires_grad_()
+    up = [normal(gen(32), T, H), normal(gen(33), T, H)]
+
+    def loss():
+        h, n = chain(x, idx, w, p, E)
+        return (h.double() * up[0]).sum() + (n.double() * up[1]).sum()
+    grads = dict(zip(leaves, torch.autograd.grad(loss(), list(leaves.values()))))
+    step = 2.0 ** -7
+    for name, t in leaves.items():
+        way = normal(gen(len(name)), *t.shape)
+        slope = float((grads[name].double() * way.double()).sum())
+        with torch.no_grad():
+            keep = t.clone()
+            values = []
+            for s in (-2, -1, 1, 2):
+                t.copy_(keep + s * step * way)
+                values.append(float(loss()))
+            t.copy_(keep)
+        # five points: off by step^4 of the fifth derivative; the loss is a sum of 2 T H = 384 fp32
+        # outputs of size about 1, each off by some 2^-22: 384^(1/2) 2^-22 / step = 6e-4 at most here
+        diff = (values[0] - 8 * values[1] + 8 * values[2] - values[3]) / (12 * step)
+        assert abs(diff - slope) < 2e-3 * max(1.0, float(grads[name].norm()) * float(way.norm()) ** 0.5), \
+            (name, diff, slope)
+
+
+@pytest.mark.parametrize("T", [3, 500])
+def test_replayed_graph_gives_the_eager_results(T):
+    H, I, E, k = 264, 136, 9, 3
+    p, x, idx, w = chain_inputs(gen(T), T, H, I, E, k, torch.bfloat16)
+    leaves = [x, w] + list(p.values())
+    for t in leaves:
+        t.requires_grad_()
+    dh, dn = normal(gen(1), T, H, dtype=torch.bfloat16), normal(gen(2), T, H, dtype=torch.bfloat16)
+
+    def step():
+        h, n = chain(x, idx, w, p, E)
+        return (h.detach(), n.detach()) + torch.autograd.grad((h, n), leaves, (dh, dn))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in range(4):
+        q, x2, idx2, w2 = chain_inputs(gen(100 + seed), T, H, I, E, k, torch.bfloat16)
+        with torch.no_grad():
+            for a, b in zip(leaves, [x2, w2] + list(q.values())):
+                a.copy_(b)
+            idx.copy_(idx2)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in captured]
+        want = step()
+        torch.cuda.synchronize()
+        for i, (a, b) in enumerate(zip(got, want)):
+            assert torch.equal(a, b), (seed, i)
+
+
+def test_calls_on_two_streams_at_once():
+    H, I, E, k = 520, 264, 8, 2
+    sets = [chain_inputs(gen(s), 400, H, I, E, k, torch.bfloat16) for s in (1, 2)]
+    want = [chain(x, idx, w, p, E) for p, x, idx, w in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(5):
+        for i, (p, x, idx, w) in enumerate(sets):
+            with torch.cuda.stream(streams[i]):
+                got[i] = chain(x, idx, w, p, E)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_strided_and_misaligned_inputs():
+    g = gen(9)
+    base = normal(g, 64, 3 * 64)
+    x = base[:, 64:128]
+    w = normal(g, 64, 48).t()                              # [48, 64], columns first
+    flat = normal(g, 64 * 48 + 1)[1:].view(64, 48)         # 4 bytes off a 16-byte boundary
+    want = ops.expert_linear(x.contiguous(), w.contiguous(), residual=flat.clone())
+    assert torch.equal(ops.expert_linear(x, w, residual=flat), want)
+    n = ops.rms_norm(x, base[0, :64])
+    assert torch.equal(n, ops.rms_norm(x.contiguous(), base[0, :64].clone()))
+    order = ops.sort_tokens(routing(g, 64, 2, 4), 4)
+    assert torch.equal(ops.permute_tokens(x, order), ops.permute_tokens(x.contiguous(), order))
+
+
+def test_results_are_the_same_bits_every_time():
+    p, x, idx, w = chain_inputs(gen(41), 300, 264, 392, 7, 3, torch.bfloat16)
+    leaves = [x, w] + list(p.values())
+    for t in leaves:
+        t.requires_grad_()
+
+    def step():
+        h, n = chain(x, idx, w, p, 7)
+        return (h, n) + torch.autograd.grad((h, n), leaves, (torch.ones_like(h), torch.ones_like(n)))
+    first = step()
+    for _ in range(3):
+        for a, b in zip(first, step()):
+            assert torch.equal(a, b)
