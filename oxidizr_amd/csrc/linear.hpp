@@ -43,6 +43,34 @@ MOE_DEV float act_slope(float z, int act) {
   }
 }
 
+// Eight at once: one branch on the activation, which is the same for the launch.
+MOE_DEV void act_value8(const float (&z)[8], float (&y)[8], int act) {
+  auto all = [&](auto a) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = act_value(z[i], decltype(a)::value);
+  };
+  switch (act) {
+    case kActRelu: return all(std::integral_constant<int, kActRelu>());
+    case kActSilu: return all(std::integral_constant<int, kActSilu>());
+    case kActGelu: return all(std::integral_constant<int, kActGelu>());
+    case kActGeluTanh: return all(std::integral_constant<int, kActGeluTanh>());
+    default: return all(std::integral_constant<int, kActNone>());
+  }
+}
+// d *= act'(z)
+MOE_DEV void act_slope8(const float (&z)[8], float (&d)[8], int act) {
+  auto all = [&](auto a) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) d[i] *= act_slope(z[i], decltype(a)::value);
+  };
+  switch (act) {
+    case kActRelu: return all(std::integral_constant<int, kActRelu>());
+    case kActSilu: return all(std::integral_constant<int, kActSilu>());
+    case kActGelu: return all(std::integral_constant<int, kActGelu>());
+    default: return all(std::integral_constant<int, kActGeluTanh>());
+  }
+}
+
 // What the epilogue of a forward needs.  bias: [G, N] (or [N]) or null; res, pre: row r
 // at r N, or null.
 template <typename T>
@@ -55,17 +83,21 @@ struct LinearEpi {
 // Eight outputs of row r from column n on.  The pre-activation is kept in the
 // dtype: a bf16 z is off by at most 2^-9 of itself, which moves act'(z) by less than
 // the rounding of dz behind it.
-template <typename T>
-MOE_DEV void linear_store8(const LinearEpi<T>& e, int64_t r, int n, const float* acc,
-                           const float* bias, const float* res) {
+template <typename T, bool RES>
+MOE_DEV void linear_store8(const LinearEpi<T>& e, int64_t r, int n, const float (&acc)[8],
+                           const T* bias, const float (&res)[8]) {
   const int64_t o = r * e.N + n;
   float z[8], y[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) z[i] = bias ? acc[i] + bias[i] : acc[i];
-  if (e.pre) store8(e.pre + o, z);
+  for (int i = 0; i < 8; ++i) z[i] = acc[i];
+  if (bias) {
+    load8(bias, y);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = act_value(z[i], e.act);
-  if (res) {
+    for (int i = 0; i < 8; ++i) z[i] += y[i];
+  }
+  if (e.pre) store8(e.pre + o, z);
+  act_value8(z, y, e.act);
+  if constexpr (RES) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] += res[i];
   }
@@ -142,13 +174,13 @@ template <typename T, class C>
 __global__ __launch_bounds__(C::THREADS) void k_linear_fwd(const T* __restrict__ X, RowGroups groups,
                                                            const T* const* w_tab, const T* w_one,
                                                            int K, LinearEpi<T> epi) {
-  __shared__ __align__(16) T smem[rowgroup_smem_elems<T, C, 1, 1, 1>()];
+  __shared__ __align__(16) T smem[rowcol_smem_elems<T, C, 1, 1, 1>()];
   int grp, row0, mv, n0;
   const int N = epi.N;
   if (!resolve_rows(groups, N, C::AR, C::BN, grp, row0, mv, n0)) return;
   const T* w = pick(w_tab, w_one, grp);
   const T* bias = epi.bias ? epi.bias + (int64_t)grp * N + n0 : nullptr;
-  with_tile_rows<T, C, 1>(mv, [&](auto ct) {
+  with_tile_shape<T, C>(mv, N - n0, [&](auto ct) {
     using CT = decltype(ct);
     OpDesc<T> a[1] = {{X + (int64_t)row0 * K, K, mv, K}};
     OpDesc<T> b[1] = {{w + (int64_t)n0 * K, K, N - n0, K}};
@@ -156,12 +188,6 @@ __global__ __launch_bounds__(C::THREADS) void k_linear_fwd(const T* __restrict__
     zero_acc<CT, 1>(acc, xacc);
     mainloop_x<CT, T, false, false, 1, 1>(acc, xacc, a, b, K, smem);
     static_assert(epi_lds_floats<CT, 1>() * 4 <= (int)sizeof(smem), "epilogue LDS");
-    auto visit = [&](int m, int n, const float* v, const float* res) {
-      if (m >= mv || n0 + n >= N) return;
-      float bv[8];
-      if (bias) load8(bias + n, bv);
-      linear_store8(epi, (int64_t)row0 + m, n0 + n, v, bias ? bv : nullptr, res);
-    };
     if (epi.res) {
       constexpr int V = Vec16<T>::N;
       struct Pre { u32x4 r[8 / V]; };
@@ -172,14 +198,18 @@ __global__ __launch_bounds__(C::THREADS) void k_linear_fwd(const T* __restrict__
 #pragma unroll
         for (int i = 0; i < 8 / V; ++i) q.r[i] = *gptr(reinterpret_cast<const u32x4*>(p + i * V));
       }, [&](int m, int n, auto& v, const Pre& q) {
+        if (m >= mv || n0 + n >= N) return;
         float r[8];
 #pragma unroll
         for (int i = 0; i < 8 / V; ++i) unpack16(q.r[i], r + i * V, T());
-        visit(m, n, v[0], r);
+        linear_store8<T, true>(epi, (int64_t)row0 + m, n0 + n, v[0], bias ? bias + n : nullptr, r);
       });
     } else {
       for_each_row8_x<CT, 1>(acc, xacc, reinterpret_cast<float*>(smem),
-                             [&](int m, int n, auto& v) { visit(m, n, v[0], nullptr); });
+                             [&](int m, int n, auto& v) {
+        if (m >= mv || n0 + n >= N) return;
+        linear_store8<T, false>(epi, (int64_t)row0 + m, n0 + n, v[0], bias ? bias + n : nullptr, v[0]);
+      });
     }
   });
 }
@@ -190,11 +220,11 @@ __global__ __launch_bounds__(C::THREADS) void k_linear_dgrad(const T* __restrict
                                                              RowGroups groups,
                                                              const T* const* w_tab, const T* w_one,
                                                              int N, int K, T* __restrict__ dX) {
-  __shared__ __align__(16) T smem[rowgroup_smem_elems<T, C, 1, 1, 1>()];
+  __shared__ __align__(16) T smem[rowcol_smem_elems<T, C, 1, 1, 1>()];
   int grp, row0, mv, k0;
   if (!resolve_rows(groups, K, C::AR, C::BN, grp, row0, mv, k0)) return;
   const T* w = pick(w_tab, w_one, grp);  // element (k, n) of the operand at w + n K + k
-  with_tile_rows<T, C, 1>(mv, [&](auto ct) {
+  with_tile_shape<T, C>(mv, K - k0, [&](auto ct) {
     using CT = decltype(ct);
     OpDesc<T> a[1] = {{dZ + (int64_t)row0 * N, N, mv, N}};
     OpDesc<T> b[1] = {{w + k0, K, K - k0, N}};
@@ -403,8 +433,7 @@ __global__ __launch_bounds__(256) void k_linear_dz(const T* __restrict__ dY,
       if (act != kActNone) {
         float z[8];
         load8(pre + o, z);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] *= act_slope(z[i], act);
+        act_slope8(z, d, act);
         store8(dZ + o, d);
       }
 #pragma unroll

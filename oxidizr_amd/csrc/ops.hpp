@@ -446,6 +446,21 @@ struct NormBwdArgs {
   int need_a, need_b;
 };
 
+// Eight elements as they lie in memory.
+template <typename T>
+struct Raw8 {
+  static constexpr int N = 8 / Vec16<T>::N;
+  u32x4 v[N];
+  MOE_DEV void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = *gptr(reinterpret_cast<const u32x4*>(p + i * Vec16<T>::N));
+  }
+  MOE_DEV void get(float (&f)[8]) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) unpack16(v[i], f + i * Vec16<T>::N, T());
+  }
+};
+
 template <typename T, int WPR, int NCH>
 __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_bwd(NormBwdArgs<T> a) {
   constexpr int NW = WPR > 4 ? WPR : 4, RPB = NW / WPR, TR = 64 * WPR;
@@ -454,22 +469,50 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_bwd(NormBwdAr
   const int i0 = threadIdx.x % TR;
   const int nch = a.H / 8;
   const float inv_h = 1.0f / (float)a.H;
+  const bool chan = a.gate_kind == kGateChannel, full = a.gate_kind == kGateFull;
+  // the row vectors of a thread's columns, and the next row's tensors
+  Raw8<T> w2[NCH], w3[NCH], gc[NCH], nd[NCH], nn[NCH], nh[NCH], ny[NCH], ng[NCH];
   float ca[NCH][8], cb[NCH][8];
 #pragma unroll
-  for (int c = 0; c < NCH; ++c)
+  for (int c = 0; c < NCH; ++c) {
+    const int ch = i0 + c * TR;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ca[c][i] = cb[c][i] = 0.0f;
-  const bool gated_sum = a.gate_kind == kGateChannel || a.gate_kind == kGateFull;
+    if (ch < nch) {
+      if (a.w2) w2[c].load(a.w2 + ch * 8);
+      if (a.w3) w3[c].load(a.w3 + ch * 8);
+      if (chan) gc[c].load(a.gate + ch * 8);
+    }
+  }
+  auto load_row = [&](int64_t t) {
+    if (t >= a.Tn) return;
+    const int64_t row = t * a.H;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const int ch = i0 + c * TR;
+      if (ch >= nch) continue;
+      if (a.dhn) nd[c].load(a.dhn + row + ch * 8);
+      if (a.w3) {
+        nn[c].load(a.dn + row + ch * 8);
+        nh[c].load(a.hn + row + ch * 8);
+      }
+      if (a.y) ny[c].load(a.y + row + ch * 8);
+      if (full) ng[c].load(a.gate + row + ch * 8);
+    }
+  };
   int set = 0;
   const int64_t stride = (int64_t)gridDim.x * RPB;
-  for (int64_t tb = (int64_t)blockIdx.x * RPB; tb < a.Tn; tb += stride, set ^= 1) {
+  const int64_t t0 = (int64_t)blockIdx.x * RPB;
+  load_row(t0 + wave / WPR);
+  for (int64_t tb = t0; tb < a.Tn; tb += stride, set ^= 1) {
     const int64_t t = tb + wave / WPR;
     const bool live = t < a.Tn;
     const int64_t row = t * a.H;
     const float r3 = live && a.w3 ? a.r3[t] : 0.0f;
-    const float r2 = live && a.y && a.w2 ? a.r2[t] : 1.0f;
+    const float r2 = live && a.w2 ? a.r2[t] : 1.0f;
     const float gt = live && a.gate_kind == kGateToken ? to_f<T>(a.gate[t]) : 1.0f;
     float p[NCH][8], hh[NCH][8], yh[NCH][8];
+    Raw8<T> g[NCH];
     float s3 = 0.0f, sp = 0.0f, sh = 0.0f;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
@@ -478,12 +521,12 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_bwd(NormBwdAr
       for (int i = 0; i < 8; ++i) p[c][i] = hh[c][i] = yh[c][i] = 0.0f;
       if (!live || ch >= nch) continue;
       float v[8];
-      if (a.dhn) load8(a.dhn + row + ch * 8, p[c]);
+      if (a.dhn) nd[c].get(p[c]);
       if (a.w3) {
         float d[8];
-        load8(a.dn + row + ch * 8, d);
-        load8(a.hn + row + ch * 8, hh[c]);
-        load8(a.w3 + ch * 8, v);
+        nn[c].get(d);
+        nh[c].get(hh[c]);
+        w3[c].get(v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           hh[c][i] *= r3;
@@ -495,16 +538,17 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_bwd(NormBwdAr
       }
       if (a.y) {
         float u[8];
-        load8(a.y + row + ch * 8, yh[c]);
+        ny[c].get(yh[c]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) u[i] = yh[c][i] *= r2;
         if (a.w2) {
-          load8(a.w2 + ch * 8, v);
+          w2[c].get(v);
 #pragma unroll
           for (int i = 0; i < 8; ++i) u[i] *= v[i];
         }
-        if (gated_sum) {
-          load8(a.gate + (a.gate_kind == kGateFull ? row : 0) + ch * 8, v);
+        if (chan || full) {
+          g[c] = full ? ng[c] : gc[c];
+          g[c].get(v);
 #pragma unroll
           for (int i = 0; i < 8; ++i) u[i] *= v[i];
         }
@@ -515,6 +559,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_bwd(NormBwdAr
         }
       }
     }
+    load_row(t + stride);  // in flight over this row's reduction and stores
     s3 = wave_sum(s3);
     sp = wave_sum(sp);
     sh = wave_sum(sh);
@@ -525,7 +570,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_bwd(NormBwdAr
         r[1][wave] = sp;
         r[2][wave] = sh;
       }
-      __syncthreads();
+      lds_barrier();  // not the row loads in flight
       const int w0 = wave / WPR * WPR;
       s3 = r[0][w0]; sp = r[1][w0]; sh = r[2][w0];
 #pragma unroll
@@ -552,15 +597,15 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_bwd(NormBwdAr
       }
       store8(a.dh + row + ch * 8, o);
       if (!a.y) continue;
-      float g[8], wv[8];
+      float gv[8], wv[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        g[i] = gt;
+        gv[i] = gt;
         wv[i] = 1.0f;
       }
-      if (gated_sum) load8(a.gate + (a.gate_kind == kGateFull ? row : 0) + ch * 8, g);
-      if (a.w2) load8(a.w2 + ch * 8, wv);
-      if (a.gate_kind == kGateFull) {
+      if (chan || full) g[c].get(gv);
+      if (a.w2) w2[c].get(wv);
+      if (full) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = p[c][i] * yh[c][i] * wv[i];
         store8(a.dgate + row + ch * 8, v);
@@ -568,7 +613,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_bwd(NormBwdAr
       const bool colg = a.gate_kind >= kGateToken;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float d = g[i] * p[c][i];
+        const float d = gv[i] * p[c][i];
         ca[c][i] += (colg ? d : p[c][i]) * yh[c][i];
         o[i] = r2 * (wv[i] * d - yh[c][i] * m2);
       }

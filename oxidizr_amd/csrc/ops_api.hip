@@ -173,36 +173,43 @@ moe_status check_norm(int dtype, int64_t T, int H, int gate_kind, bool y, bool p
   return MOE_OK;
 }
 
-// Calls f(waves to a row, chunks to a thread) with 64 * 8 * WPR * NCH >= H.
-template <class F>
+// Calls f(waves to a row, chunks to a thread) with 64 * 8 * WPR * NCH >= H. The backward
+// holds more to a column, so it takes one chunk to a thread as long as a workgroup has
+// the waves (H = 7168, T = 8192: 8 waves of two chunks 137 us, 16 of one 136; without
+// the next row's loads in flight 270 and 183).
+template <bool BWD, class F>
 void with_norm_shape(int H, F&& f) {
   using std::integral_constant;
   if (H <= 512) f(integral_constant<int, 1>(), integral_constant<int, 1>());
   else if (H <= 2048) f(integral_constant<int, 4>(), integral_constant<int, 1>());
   else if (H <= 4096) f(integral_constant<int, 8>(), integral_constant<int, 1>());
-  else if (H <= 8192) f(integral_constant<int, 8>(), integral_constant<int, 2>());
+  else if (H <= 8192) f(integral_constant<int, BWD ? 16 : 8>(), integral_constant<int, BWD ? 1 : 2>());
   else if (H <= 16384) f(integral_constant<int, 16>(), integral_constant<int, 2>());
   else f(integral_constant<int, 16>(), integral_constant<int, 4>());
 }
-constexpr int norm_threads(int wpr) { return wpr > 4 ? 64 * wpr : 256; }
-constexpr int norm_rows(int wpr) { return wpr > 4 ? 1 : 4 / wpr; }
+constexpr int norm_waves(int wpr) { return wpr > 4 ? wpr : 4; }
+constexpr int norm_rows(int wpr) { return norm_waves(wpr) / wpr; }
 
-// Blocks of the backward: enough to fill the CUs twice; each adds its rows' column
-// sums in registers and writes one partial row.
-constexpr int kNormBwdBlocks = 512;
+// Blocks of the backward: 16 waves to a CU, all running at once, each adding its rows'
+// column sums in registers. More blocks write more partial rows and gain nothing (H =
+// 7168, T = 8192: 256 blocks 136 us, 512 143, 1024 153; H = 2048: 1024 43, 4096 47).
+constexpr int kNormBwdWaves = 16 * 256;
 int norm_bwd_blocks(int64_t T, int H) {
-  int rows = 1;
-  with_norm_shape(H, [&](auto wpr, auto) { rows = norm_rows(decltype(wpr)::value); });
-  return (int)std::min<int64_t>(kNormBwdBlocks, (T + rows - 1) / rows);
+  int64_t blocks = 1;
+  with_norm_shape<true>(H, [&](auto wpr, auto) {
+    constexpr int W = decltype(wpr)::value;
+    blocks = std::min<int64_t>(kNormBwdWaves / norm_waves(W), (T + norm_rows(W) - 1) / norm_rows(W));
+  });
+  return (int)blocks;
 }
 
 template <typename D>
 moe_status launch_norm_fwd(hipStream_t s, const NormArgs<D>& a) {
-  with_norm_shape(a.H, [&](auto wpr, auto nch) {
+  with_norm_shape<false>(a.H, [&](auto wpr, auto nch) {
     constexpr int W = decltype(wpr)::value;
     const int64_t grid = (a.Tn + norm_rows(W) - 1) / norm_rows(W);
     hipLaunchKernelGGL((k_norm_fwd<D, W, decltype(nch)::value>), dim3((unsigned)grid),
-                       dim3(norm_threads(W)), 0, s, a);
+                       dim3(64 * norm_waves(W)), 0, s, a);
   });
   LAUNCH_CHECK();
   return MOE_OK;
@@ -211,9 +218,9 @@ moe_status launch_norm_fwd(hipStream_t s, const NormArgs<D>& a) {
 template <typename D>
 moe_status launch_norm_bwd(hipStream_t s, const NormBwdArgs<D>& a, D* dw2, D* dgate_chan, D* dw3) {
   const int nb = norm_bwd_blocks(a.Tn, a.H);
-  with_norm_shape(a.H, [&](auto wpr, auto nch) {
+  with_norm_shape<true>(a.H, [&](auto wpr, auto nch) {
     constexpr int W = decltype(wpr)::value;
-    hipLaunchKernelGGL((k_norm_bwd<D, W, decltype(nch)::value>), dim3(nb), dim3(norm_threads(W)), 0,
+    hipLaunchKernelGGL((k_norm_bwd<D, W, decltype(nch)::value>), dim3(nb), dim3(64 * norm_waves(W)), 0,
                        s, a);
   });
   if (a.need_a + a.need_b > 0)

@@ -36,11 +36,6 @@ class TokenOrder(NamedTuple):
     inv_perm: torch.Tensor  # [T, k] t * k + j -> position
 
 
-def _require(ok, message):
-    if not ok:
-        raise ModelError(message)
-
-
 def _ready(t):
     """t as the library reads it: contiguous and 16-byte aligned."""
     t = t.contiguous()
@@ -53,15 +48,18 @@ def _ptr(t):
 
 def _on_device(first, *others):
     """The device index of a call's tensors (the first is always there)."""
-    _require(first.is_cuda, f"expected CUDA tensors, got one on {first.device}")
+    dev = first.get_device()
+    if dev < 0:
+        raise ModelError(f"expected CUDA tensors, got one on {first.device}")
     for t in others:
-        _require(t is None or t.device == first.device,
-                 f"tensors on different devices: {first.device} and {t.device if t is not None else None}")
-    return first.device.index
+        if t is not None and t.get_device() != dev:
+            raise ModelError(f"tensors on different devices: {first.device} and {t.device}")
+    return dev
 
 
 def _call(fn, device, *args):
-    _lib.check(fn(device, torch.cuda.current_stream(device).cuda_stream, *args))
+    # the current stream's handle without the Stream object around it (1.5 us of a call)
+    _lib.check(fn(device, torch._C._cuda_getCurrentRawStream(device), *args))
 
 
 def _workspace(nbytes, like):
@@ -79,12 +77,15 @@ def _tracked(*tensors):
 def sort_tokens(topk_idx, num_experts: int) -> TokenOrder:
     """Stable sort of topk_idx [T, k] (int32 or int64) by expert, then by t * k + j. An index outside
     [0, num_experts) has no expert (a padding token) and comes behind every expert."""
-    _require(topk_idx.dim() == 2, f"topk_idx must be [T, k], got {list(topk_idx.shape)}")
-    _require(topk_idx.dtype in (torch.int32, torch.int64),
-             f"topk_idx must be int32 or int64, got {topk_idx.dtype}")
+    if topk_idx.dim() != 2:
+        raise ModelError(f"topk_idx must be [T, k], got {list(topk_idx.shape)}")
+    if topk_idx.dtype not in (torch.int32, torch.int64):
+        raise ModelError(f"topk_idx must be int32 or int64, got {topk_idx.dtype}")
     T, k = topk_idx.shape
-    _require(1 <= k <= MAX_EXPERTS_PER_TOK, f"experts per token must be 1..{MAX_EXPERTS_PER_TOK}, got {k}")
-    _require(1 <= num_experts <= MAX_EXPERTS, f"num_experts must be 1..{MAX_EXPERTS}, got {num_experts}")
+    if not 1 <= k <= MAX_EXPERTS_PER_TOK:
+        raise ModelError(f"experts per token must be 1..{MAX_EXPERTS_PER_TOK}, got {k}")
+    if not 1 <= num_experts <= MAX_EXPERTS:
+        raise ModelError(f"num_experts must be 1..{MAX_EXPERTS}, got {num_experts}")
     dev = _on_device(topk_idx)
     idx = _ready(topk_idx)
     L = _lib.load()
@@ -99,18 +100,23 @@ def sort_tokens(topk_idx, num_experts: int) -> TokenOrder:
 
 
 def _check_order(order):
-    _require(isinstance(order, TokenOrder), "order must be a TokenOrder (sort_tokens)")
-    _require(order.inv_perm.dim() == 2, "order.inv_perm must be [T, k]")
+    if not isinstance(order, TokenOrder):
+        raise ModelError("order must be a TokenOrder (sort_tokens)")
+    if order.inv_perm.dim() != 2:
+        raise ModelError("order.inv_perm must be [T, k]")
     for t in (order.offsets, order.inv_perm):
-        _require(t.dtype == torch.int32, f"a TokenOrder holds int32 tensors, got {t.dtype}")
-    _require(1 <= order.inv_perm.shape[1] <= MAX_EXPERTS_PER_TOK,
-             f"experts per token must be 1..{MAX_EXPERTS_PER_TOK}, got {order.inv_perm.shape[1]}")
-    _require(order.offsets.dim() == 1 and order.offsets.numel() >= 2, "order.offsets must be [E + 1]")
+        if t.dtype != torch.int32:
+            raise ModelError(f"a TokenOrder holds int32 tensors, got {t.dtype}")
+    if not 1 <= order.inv_perm.shape[1] <= MAX_EXPERTS_PER_TOK:
+        raise ModelError(f"experts per token must be 1..{MAX_EXPERTS_PER_TOK}, got {order.inv_perm.shape[1]}")
+    if not (order.offsets.dim() == 1 and order.offsets.numel() >= 2):
+        raise ModelError("order.offsets must be [E + 1]")
     return order.inv_perm.shape
 
 
 def _check_hidden(H):
-    _require(H >= 8 and H % 8 == 0, f"the hidden size must be a positive multiple of 8, got {H}")
+    if H < 8 or H % 8:
+        raise ModelError(f"the hidden size must be a positive multiple of 8, got {H}")
 
 
 class _Slots:
@@ -152,7 +158,8 @@ def permute_tokens(x, order: TokenOrder):
     """Rows of x [T, H] in the order's positions: out[inv_perm[t, j]] = x[t] [T k, H]; the rows behind
     the last expert's (assignments without one) are zeros."""
     T, k = _check_order(order)
-    _require(x.dim() == 2 and x.shape[0] == T, f"x must be [{T}, H], got {list(x.shape)}")
+    if not (x.dim() == 2 and x.shape[0] == T):
+        raise ModelError(f"x must be [{T}, H], got {list(x.shape)}")
     _check_hidden(x.shape[1])
     _dtype_code(x.dtype)
     _on_device(x, order.inv_perm, order.offsets)
@@ -190,12 +197,13 @@ def unpermute_tokens(y, order: TokenOrder, weights: Optional[torch.Tensor] = Non
     """out[t] = sum_j weights[t, j] * y[inv_perm[t, j]] [T, H] over the assignments that have an expert,
     j ascending; weights [T, k] float32, or None for a plain sum."""
     T, k = _check_order(order)
-    _require(y.dim() == 2 and y.shape[0] == T * k, f"y must be [{T * k}, H], got {list(y.shape)}")
+    if not (y.dim() == 2 and y.shape[0] == T * k):
+        raise ModelError(f"y must be [{T * k}, H], got {list(y.shape)}")
     _check_hidden(y.shape[1])
     _dtype_code(y.dtype)
     if weights is not None:
-        _require(weights.dtype == torch.float32 and weights.shape == (T, k),
-                 f"weights must be float32 [{T}, {k}], got {weights.dtype} {list(weights.shape)}")
+        if not (weights.dtype == torch.float32 and weights.shape == (T, k)):
+            raise ModelError(f"weights must be float32 [{T}, {k}], got {weights.dtype} {list(weights.shape)}")
     _on_device(y, order.inv_perm, order.offsets, weights)
     slots = _Slots(order)
     if _tracked(y, weights):
@@ -265,27 +273,33 @@ def expert_linear(x, weight, bias=None, *, offsets=None, activation: str = "none
     take weight[e] of weight [E, N, K] and bias[e] of bias [E, N]; rows behind the last expert's are the
     residual's, or zeros. Without offsets weight is [N, K] and bias [N]. K and N are multiples of 8.
     activation: one of ACTIVATIONS ("gelu" with the error function, "gelu_tanh" approximated)."""
-    _require(activation in ACTIVATIONS, f"activation must be one of {ACTIVATIONS}, got {activation!r}")
-    _require(x.dim() == 2, f"x must be [M, K], got {list(x.shape)}")
+    if activation not in ACTIVATIONS:
+        raise ModelError(f"activation must be one of {ACTIVATIONS}, got {activation!r}")
+    if x.dim() != 2:
+        raise ModelError(f"x must be [M, K], got {list(x.shape)}")
     M, K = x.shape
     grouped = offsets is not None
-    _require(weight.dim() == (3 if grouped else 2) and weight.shape[-1] == K,
-             f"weight must be {'[E, N' if grouped else '[N'}, {K}], got {list(weight.shape)}")
+    if not (weight.dim() == (3 if grouped else 2) and weight.shape[-1] == K):
+        raise ModelError(f"weight must be {'[E, N' if grouped else '[N'}, {K}], got {list(weight.shape)}")
     groups, N = (weight.shape[0], weight.shape[1]) if grouped else (1, weight.shape[0])
-    _require(K >= 8 and K % 8 == 0 and N >= 8 and N % 8 == 0,
-             f"input and output widths must be positive multiples of 8, got {K} and {N}")
+    if not (K >= 8 and K % 8 == 0 and N >= 8 and N % 8 == 0):
+        raise ModelError(f"input and output widths must be positive multiples of 8, got {K} and {N}")
     if grouped:
-        _require(1 <= groups <= MAX_EXPERTS, f"num_experts must be 1..{MAX_EXPERTS}, got {groups}")
-        _require(offsets.dtype == torch.int32 and offsets.shape == (groups + 1,),
-                 f"offsets must be int32 [{groups + 1}], got {offsets.dtype} {list(offsets.shape)}")
+        if not 1 <= groups <= MAX_EXPERTS:
+            raise ModelError(f"num_experts must be 1..{MAX_EXPERTS}, got {groups}")
+        if not (offsets.dtype == torch.int32 and offsets.shape == (groups + 1,)):
+            raise ModelError(f"offsets must be int32 [{groups + 1}], got {offsets.dtype} {list(offsets.shape)}")
     if bias is not None:
         want = (groups, N) if grouped else (N,)
-        _require(bias.shape == want, f"bias must be {list(want)}, got {list(bias.shape)}")
+        if bias.shape != want:
+            raise ModelError(f"bias must be {list(want)}, got {list(bias.shape)}")
     if residual is not None:
-        _require(residual.shape == (M, N), f"residual must be [{M}, {N}], got {list(residual.shape)}")
+        if not (residual.shape == (M, N)):
+            raise ModelError(f"residual must be [{M}, {N}], got {list(residual.shape)}")
     _dtype_code(x.dtype)
     for t in (weight, bias, residual):
-        _require(t is None or t.dtype == x.dtype, "x, weight, bias and residual must have one dtype")
+        if not (t is None or t.dtype == x.dtype):
+            raise ModelError("x, weight, bias and residual must have one dtype")
     _on_device(x, weight, bias, residual, offsets)
     s = _LinearShape(M, K, N, groups, grouped, ACTIVATIONS.index(activation))
     offsets = _ready(offsets) if grouped else None
@@ -366,20 +380,23 @@ def _gate_kind(gate, h):
         return _GATE_FULL
     if gate.shape == h.shape[-1:]:
         return _GATE_CHANNEL
-    _require(gate.shape == h.shape[:-1] + (1,),
-             f"gate must be {list(h.shape[-1:])}, {list(h.shape[:-1]) + [1]} or {list(h.shape)}, "
-             f"got {list(gate.shape)}")
+    if not (gate.shape == h.shape[:-1] + (1,)):
+        raise ModelError(
+            f"gate must be {list(h.shape[-1:])}, {list(h.shape[:-1]) + [1]} or {list(h.shape)}, " f"got {list(gate.shape)}")
     return _GATE_TOKEN
 
 
 def _check_norm(h, *weights):
-    _require(h.dim() >= 2, f"expected [..., T, H], got {list(h.shape)}")
+    if h.dim() < 2:
+        raise ModelError(f"expected [..., T, H], got {list(h.shape)}")
     H = h.shape[-1]
     _check_hidden(H)
     _dtype_code(h.dtype)
     for w in weights:
-        _require(w is None or w.shape == (H,), f"a norm's weight must be [{H}]")
-        _require(w is None or w.dtype == h.dtype, "activations and norm weights must have one dtype")
+        if not (w is None or w.shape == (H,)):
+            raise ModelError(f"a norm's weight must be [{H}]")
+        if not (w is None or w.dtype == h.dtype):
+            raise ModelError("activations and norm weights must have one dtype")
     return H
 
 
@@ -403,9 +420,10 @@ def residual_norm(h, y, post_weight=None, *, gate=None, next_weight=None, residu
     h, y [..., H]; post_weight, next_weight [H]; gate [H], [..., 1] or [..., H]. Returns h_out, or
     (h_out, n) with a next_weight."""
     H = _check_norm(h, post_weight, next_weight)
-    _require(y.shape == h.shape, f"y must be {list(h.shape)}, got {list(y.shape)}")
-    _require(y.dtype == h.dtype and (gate is None or gate.dtype == h.dtype),
-             "h, y and gate must have one dtype")
+    if y.shape != h.shape:
+        raise ModelError(f"y must be {list(h.shape)}, got {list(y.shape)}")
+    if not (y.dtype == h.dtype and (gate is None or gate.dtype == h.dtype)):
+        raise ModelError("h, y and gate must have one dtype")
     kind = _gate_kind(gate, h)
     _on_device(h, y, post_weight, gate, next_weight)
     s = _NormShape(h.numel() // H, H, kind, float(residual_scale), eps)

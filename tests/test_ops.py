@@ -164,7 +164,7 @@ def test_workspace_sizes():
     assert act - none == 4096 * 256 * 2                            # dz of an activation
     assert none >= (4096 // 64 + 8) * 256 * 4                      # the bias gradient's parts
     assert L.moe_linear_workspace_bytes(BF16, 4096, 500, 256, 8, 1, 0, 1) == 0
-    assert L.moe_residual_norm_workspace_bytes(10 ** 6, 2048) == 512 * 2 * 2048 * 4
+    assert L.moe_residual_norm_workspace_bytes(10 ** 6, 2048) == 1024 * 2 * 2048 * 4
     assert L.moe_residual_norm_workspace_bytes(3, 2048) == 3 * 2 * 2048 * 4
 
 
