@@ -274,8 +274,9 @@ moe_status moe_plan_stage_times(moe_plan* plan, float* ms, int32_t* calls, int32
  * norms on both sides of the block), as calls of their own: no plan, no state.
  * `device` is the device of every pointer and of `stream`; the caller's current
  * device is left as it was.  dtype: a moe_dtype of the activations, weights and
- * gradients.  Alignment, ownership, streams, errors and reproducibility as above;
- * a workspace is used only while the call's kernels run. */
+ * gradients.  Alignment, ownership, streams, errors and reproducibility as above,
+ * but integer arrays need only their own alignment (they may be slices); a workspace is
+ * used only while the call's kernels run. */
 
 /* Stable counting sort of the T k assignments by expert: expert ascending, then
  * t k + j ascending.  topk_idx [T, k]: int32 (index_bytes 4) or int64 (8); an index

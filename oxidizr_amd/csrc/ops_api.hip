@@ -44,6 +44,16 @@ moe_status check_dtype(int dtype) {
   return MOE_OK;
 }
 
+// Integer arrays (indices, orders, offsets) need their own alignment only: they may be
+// slices of one allocation.
+moe_status check_ints(std::initializer_list<const void*> needed, size_t bytes = 4) {
+  for (const void* p : needed) {
+    if (!p) return fail(MOE_ERR_INVALID, "a required pointer is NULL");
+    if ((uintptr_t)p % bytes) return fail(MOE_ERR_INVALID, "an integer array is not aligned");
+  }
+  return MOE_OK;
+}
+
 // Blocks of a launch of `waves` waves, four to a block; 0 when the grid would not
 // hold them.
 unsigned wave_grid(int64_t waves) {
@@ -444,9 +454,11 @@ moe_status moe_sort_tokens(int32_t device, void* stream, int64_t T, int32_t k, i
   if (st != MOE_OK) return st;
   if (index_bytes != 4 && index_bytes != 8)
     return fail(MOE_ERR_INVALID, "index_bytes %d is neither 4 nor 8", index_bytes);
-  if ((st = check_pointers({counts, offsets})) != MOE_OK) return st;
+  if ((st = check_ints({counts, offsets})) != MOE_OK) return st;
   const SortPlan p = sort_plan(T, k, E);
-  if (T > 0 && (st = check_pointers({topk_idx, perm, inv_perm})) != MOE_OK) return st;
+  if (T > 0 && ((st = check_ints({perm, inv_perm})) != MOE_OK ||
+                (st = check_ints({topk_idx}, index_bytes)) != MOE_OK))
+    return st;
   if (p.bytes && (st = check_pointers({workspace})) != MOE_OK) return st;
   DeviceScope dev(device);
   HIP_TRY(dev.enter());
@@ -463,8 +475,8 @@ moe_status moe_permute(int32_t device, void* stream, int32_t dtype, int64_t T, i
                        void* x_perm) {
   moe_status st = check_rows(dtype, T, k, H);
   if (st != MOE_OK || T == 0) return st;
-  if ((st = check_pointers({inv_perm, x, x_perm})) != MOE_OK) return st;
-  if (!num_kept) return fail(MOE_ERR_INVALID, "a required pointer is NULL");
+  if ((st = check_pointers({x, x_perm})) != MOE_OK) return st;
+  if ((st = check_ints({inv_perm, num_kept})) != MOE_OK) return st;
   DeviceScope dev(device);
   HIP_TRY(dev.enter());
   if (dtype == MOE_DTYPE_BF16)
@@ -479,8 +491,8 @@ moe_status moe_unpermute(int32_t device, void* stream, int32_t dtype, int64_t T,
                          const void* y, const float* weights, void* out) {
   moe_status st = check_rows(dtype, T, k, H);
   if (st != MOE_OK || T == 0) return st;
-  if ((st = check_pointers({inv_perm, y, out}, {weights})) != MOE_OK) return st;
-  if (!num_kept) return fail(MOE_ERR_INVALID, "a required pointer is NULL");
+  if ((st = check_pointers({y, out}, {weights})) != MOE_OK) return st;
+  if ((st = check_ints({inv_perm, num_kept})) != MOE_OK) return st;
   DeviceScope dev(device);
   HIP_TRY(dev.enter());
   if (dtype == MOE_DTYPE_BF16)
@@ -496,8 +508,8 @@ moe_status moe_unpermute_backward(int32_t device, void* stream, int32_t dtype, i
                                   const float* weights, void* d_y, float* d_weights) {
   moe_status st = check_rows(dtype, T, k, H);
   if (st != MOE_OK || T == 0) return st;
-  if ((st = check_pointers({inv_perm, d_out, d_y}, {y, weights, d_weights})) != MOE_OK) return st;
-  if (!num_kept) return fail(MOE_ERR_INVALID, "a required pointer is NULL");
+  if ((st = check_pointers({d_out, d_y}, {y, weights, d_weights})) != MOE_OK) return st;
+  if ((st = check_ints({inv_perm, num_kept})) != MOE_OK) return st;
   if (d_weights && !y) return fail(MOE_ERR_INVALID, "d_weights needs y");
   DeviceScope dev(device);
   HIP_TRY(dev.enter());
@@ -523,7 +535,9 @@ moe_status moe_linear_forward(int32_t device, void* stream, int32_t dtype, int64
   moe_status st = check_linear(dtype, M, K, N, E, offsets != nullptr, activation);
   if (st != MOE_OK || M == 0) return st;
   if ((st = check_pointers({x, weight, y}, {bias, residual, pre_act})) != MOE_OK) return st;
-  if (offsets && (st = check_pointers({offsets, workspace})) != MOE_OK) return st;
+  if (offsets && ((st = check_ints({offsets})) != MOE_OK ||
+                  (st = check_pointers({workspace})) != MOE_OK))
+    return st;
   DeviceScope dev(device);
   HIP_TRY(dev.enter());
   hipStream_t s = (hipStream_t)stream;
@@ -560,7 +574,7 @@ moe_status moe_linear_backward(int32_t device, void* stream, int32_t dtype, int6
   if ((st = check_pointers({d_y, x, weight}, {pre_act})) != MOE_OK) return st;
   if (activation != kActNone && !pre_act)
     return fail(MOE_ERR_INVALID, "the activation's backward needs pre_act");
-  if (offsets && (st = check_pointers({offsets})) != MOE_OK) return st;
+  if (offsets && (st = check_ints({offsets})) != MOE_OK) return st;
   if (linear_ws(dtype, M, K, N, E, offsets != nullptr, activation, true).total && !workspace)
     return fail(MOE_ERR_INVALID, "a required pointer is NULL");
   if (dtype == MOE_DTYPE_BF16)

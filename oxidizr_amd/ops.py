@@ -37,13 +37,24 @@ class TokenOrder(NamedTuple):
 
 
 def _ready(t):
-    """t as the library reads it: contiguous and 16-byte aligned."""
+    """t (or None) as the library reads it: contiguous and 16-byte aligned."""
+    if t is None:
+        return None
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def _once(backward):
+    """once_differentiable, at no cost where no second derivative can follow."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 def _on_device(first, *others):
@@ -69,7 +80,11 @@ def _workspace(nbytes, like):
 
 
 def _tracked(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 # ---------------------------------------------------------------- tokens sorted by expert and back
@@ -87,31 +102,15 @@ def sort_tokens(topk_idx, num_experts: int) -> TokenOrder:
     if not 1 <= num_experts <= MAX_EXPERTS:
         raise ModelError(f"num_experts must be 1..{MAX_EXPERTS}, got {num_experts}")
     dev = _on_device(topk_idx)
-    idx = _ready(topk_idx)
+    idx = topk_idx.contiguous()
     L = _lib.load()
-
-    def ints(*shape):
-        return torch.empty(shape, dtype=torch.int32, device=idx.device)
-    order = TokenOrder(ints(num_experts), ints(num_experts + 1), ints(T * k), ints(T, k))
+    # one allocation for all four
+    out = torch.empty(2 * num_experts + 1 + 2 * T * k, dtype=torch.int32, device=idx.device)
+    perm, inv, offsets, counts = out.split((T * k, T * k, num_experts + 1, num_experts))
     ws = _workspace(L.moe_sort_workspace_bytes(T, k, num_experts), idx)
-    _call(L.moe_sort_tokens, dev, T, k, num_experts, idx.element_size(), _ptr(idx), _ptr(order.counts),
-          _ptr(order.offsets), _ptr(order.perm), _ptr(order.inv_perm), _ptr(ws))
-    return order
-
-
-def _check_order(order):
-    if not isinstance(order, TokenOrder):
-        raise ModelError("order must be a TokenOrder (sort_tokens)")
-    if order.inv_perm.dim() != 2:
-        raise ModelError("order.inv_perm must be [T, k]")
-    for t in (order.offsets, order.inv_perm):
-        if t.dtype != torch.int32:
-            raise ModelError(f"a TokenOrder holds int32 tensors, got {t.dtype}")
-    if not 1 <= order.inv_perm.shape[1] <= MAX_EXPERTS_PER_TOK:
-        raise ModelError(f"experts per token must be 1..{MAX_EXPERTS_PER_TOK}, got {order.inv_perm.shape[1]}")
-    if not (order.offsets.dim() == 1 and order.offsets.numel() >= 2):
-        raise ModelError("order.offsets must be [E + 1]")
-    return order.inv_perm.shape
+    _call(L.moe_sort_tokens, dev, T, k, num_experts, idx.element_size(), idx.data_ptr(), counts.data_ptr(),
+          offsets.data_ptr(), perm.data_ptr(), inv.data_ptr(), _ptr(ws))
+    return TokenOrder(counts, offsets, perm, inv.view(T, k))
 
 
 def _check_hidden(H):
@@ -121,24 +120,39 @@ def _check_hidden(H):
 
 class _Slots:
     """What the row kernels read of a TokenOrder."""
+    __slots__ = ("inv", "offsets", "T", "k", "kept")
 
     def __init__(self, order):
-        self.inv, self.offsets = _ready(order.inv_perm), _ready(order.offsets)
-        self.T, self.k = order.inv_perm.shape
-        self.kept = self.offsets.data_ptr() + 4 * (self.offsets.numel() - 1)
+        if not isinstance(order, TokenOrder):
+            raise ModelError("order must be a TokenOrder (sort_tokens)")
+        offsets, inv = order.offsets, order.inv_perm
+        if inv.dim() != 2:
+            raise ModelError("order.inv_perm must be [T, k]")
+        if inv.dtype != torch.int32 or offsets.dtype != torch.int32:
+            raise ModelError(f"a TokenOrder holds int32 tensors, got {inv.dtype} and {offsets.dtype}")
+        self.T, self.k = inv.shape
+        if not 1 <= self.k <= MAX_EXPERTS_PER_TOK:
+            raise ModelError(f"experts per token must be 1..{MAX_EXPERTS_PER_TOK}, got {self.k}")
+        E = offsets.numel() - 1
+        if offsets.dim() != 1 or E < 1:
+            raise ModelError("order.offsets must be [E + 1]")
+        self.inv, self.offsets = inv.contiguous(), offsets.contiguous()
+        self.kept = self.offsets.data_ptr() + 4 * E
 
 
 def _permute(x, slots):
-    out = x.new_empty(slots.T * slots.k, x.shape[1])
-    _call(_lib.load().moe_permute, x.device.index, _dtype_code(x.dtype), slots.T, slots.k, x.shape[1],
-          _ptr(slots.inv), slots.kept, _ptr(x), _ptr(out))
+    H = x.shape[1]
+    out = x.new_empty(slots.T * slots.k, H)
+    _call(_lib.load().moe_permute, x.get_device(), _dtype_code(x.dtype), slots.T, slots.k, H,
+          slots.inv.data_ptr(), slots.kept, x.data_ptr(), out.data_ptr())
     return out
 
 
 def _unpermute(y, slots, weights):
-    out = y.new_empty(slots.T, y.shape[1])
-    _call(_lib.load().moe_unpermute, y.device.index, _dtype_code(y.dtype), slots.T, slots.k, y.shape[1],
-          _ptr(slots.inv), slots.kept, _ptr(y), _ptr(weights), _ptr(out))
+    H = y.shape[1]
+    out = y.new_empty(slots.T, H)
+    _call(_lib.load().moe_unpermute, y.get_device(), _dtype_code(y.dtype), slots.T, slots.k, H,
+          slots.inv.data_ptr(), slots.kept, y.data_ptr(), _ptr(weights), out.data_ptr())
     return out
 
 
@@ -149,7 +163,7 @@ class _Permute(torch.autograd.Function):
         return _permute(_ready(x), slots)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dxp):
         return _unpermute(_ready(dxp), ctx.slots, None), None
 
@@ -157,13 +171,12 @@ class _Permute(torch.autograd.Function):
 def permute_tokens(x, order: TokenOrder):
     """Rows of x [T, H] in the order's positions: out[inv_perm[t, j]] = x[t] [T k, H]; the rows behind
     the last expert's (assignments without one) are zeros."""
-    T, k = _check_order(order)
-    if not (x.dim() == 2 and x.shape[0] == T):
-        raise ModelError(f"x must be [{T}, H], got {list(x.shape)}")
+    slots = _Slots(order)
+    if x.dim() != 2 or x.shape[0] != slots.T:
+        raise ModelError(f"x must be [{slots.T}, H], got {list(x.shape)}")
     _check_hidden(x.shape[1])
     _dtype_code(x.dtype)
-    _on_device(x, order.inv_perm, order.offsets)
-    slots = _Slots(order)
+    _on_device(x, slots.inv, slots.offsets)
     if _tracked(x):
         return _Permute.apply(x, slots)
     return _permute(_ready(x), slots)
@@ -173,7 +186,7 @@ class _Unpermute(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, slots):
         y = _ready(y)
-        weights = None if weights is None else _ready(weights)
+        weights = _ready(weights)
         need_dw = weights is not None and ctx.needs_input_grad[1]
         # the rows are read again only for the gradient of the weights
         ctx.save_for_backward(y if need_dw else None, weights)
@@ -181,13 +194,13 @@ class _Unpermute(torch.autograd.Function):
         return _unpermute(y, slots, weights)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout):
         y, weights = ctx.saved_tensors
         slots, dout = ctx.slots, _ready(dout)
         dy = dout.new_empty(slots.T * slots.k, dout.shape[1])
         dw = torch.empty_like(weights) if y is not None else None
-        _call(_lib.load().moe_unpermute_backward, dout.device.index, _dtype_code(dout.dtype), slots.T,
+        _call(_lib.load().moe_unpermute_backward, dout.get_device(), _dtype_code(dout.dtype), slots.T,
               slots.k, dout.shape[1], _ptr(slots.inv), slots.kept, _ptr(dout), _ptr(y), _ptr(weights),
               _ptr(dy), _ptr(dw))
         return dy, dw, None
@@ -196,19 +209,18 @@ class _Unpermute(torch.autograd.Function):
 def unpermute_tokens(y, order: TokenOrder, weights: Optional[torch.Tensor] = None):
     """out[t] = sum_j weights[t, j] * y[inv_perm[t, j]] [T, H] over the assignments that have an expert,
     j ascending; weights [T, k] float32, or None for a plain sum."""
-    T, k = _check_order(order)
-    if not (y.dim() == 2 and y.shape[0] == T * k):
+    slots = _Slots(order)
+    T, k = slots.T, slots.k
+    if y.dim() != 2 or y.shape[0] != T * k:
         raise ModelError(f"y must be [{T * k}, H], got {list(y.shape)}")
     _check_hidden(y.shape[1])
     _dtype_code(y.dtype)
-    if weights is not None:
-        if not (weights.dtype == torch.float32 and weights.shape == (T, k)):
-            raise ModelError(f"weights must be float32 [{T}, {k}], got {weights.dtype} {list(weights.shape)}")
-    _on_device(y, order.inv_perm, order.offsets, weights)
-    slots = _Slots(order)
+    if weights is not None and (weights.dtype != torch.float32 or weights.shape != (T, k)):
+        raise ModelError(f"weights must be float32 [{T}, {k}], got {weights.dtype} {list(weights.shape)}")
+    _on_device(y, slots.inv, slots.offsets, weights)
     if _tracked(y, weights):
         return _Unpermute.apply(y, weights, slots)
-    return _unpermute(_ready(y), slots, None if weights is None else _ready(weights))
+    return _unpermute(_ready(y), slots, _ready(weights))
 
 
 # ---------------------------------------------------------------- expert products
@@ -228,7 +240,7 @@ def _linear(x, weight, bias, offsets, residual, s, keep):
     y = x.new_empty(s.M, s.N)
     pre = torch.empty_like(y) if keep else None
     ws = _workspace(L.moe_linear_workspace_bytes(code, s.M, s.K, s.N, s.groups, s.grouped, s.act, 0), x)
-    _call(L.moe_linear_forward, x.device.index, code, s.M, s.K, s.N, s.groups, _ptr(offsets), _ptr(x),
+    _call(L.moe_linear_forward, x.get_device(), code, s.M, s.K, s.N, s.groups, _ptr(offsets), _ptr(x),
           _ptr(weight), _ptr(bias), _ptr(residual), s.act, _ptr(y), _ptr(pre), _ptr(ws))
     return y, pre
 
@@ -237,8 +249,8 @@ class _ExpertLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, offsets, s):
         x, weight = _ready(x), _ready(weight)
-        bias = None if bias is None else _ready(bias)
-        residual = None if residual is None else _ready(residual)
+        bias = _ready(bias)
+        residual = _ready(residual)
         products = any(ctx.needs_input_grad[:3])  # any gradient that reads the pre-activation
         y, pre = _linear(x, weight, bias, offsets, residual, s, products and s.act != 0)
         ctx.save_for_backward(x, weight, pre, offsets)
@@ -246,7 +258,7 @@ class _ExpertLinear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         x, weight, pre, offsets = ctx.saved_tensors
         s, (need_x, need_w, need_b, need_r) = ctx.s, ctx.needs_input_grad[:4]
@@ -260,7 +272,7 @@ class _ExpertLinear(torch.autograd.Function):
             db = up.new_empty((s.groups, s.N) if s.grouped else (s.N,)) if need_b else None
             ws = _workspace(L.moe_linear_workspace_bytes(code, s.M, s.K, s.N, s.groups, s.grouped,
                                                          s.act, 1), up)
-            _call(L.moe_linear_backward, up.device.index, code, s.M, s.K, s.N, s.groups, _ptr(offsets),
+            _call(L.moe_linear_backward, up.get_device(), code, s.M, s.K, s.N, s.groups, _ptr(offsets),
                   _ptr(up), _ptr(x), _ptr(weight), _ptr(pre), s.act, _ptr(dx), _ptr(dw), _ptr(db),
                   _ptr(ws))
         return dx, dw, db, dy if need_r else None, None, None
@@ -302,11 +314,11 @@ def expert_linear(x, weight, bias=None, *, offsets=None, activation: str = "none
             raise ModelError("x, weight, bias and residual must have one dtype")
     _on_device(x, weight, bias, residual, offsets)
     s = _LinearShape(M, K, N, groups, grouped, ACTIVATIONS.index(activation))
-    offsets = _ready(offsets) if grouped else None
+    offsets = offsets.contiguous() if grouped else None
     if _tracked(x, weight, bias, residual):
         return _ExpertLinear.apply(x, weight, bias, residual, offsets, s)
-    return _linear(_ready(x), _ready(weight), None if bias is None else _ready(bias), offsets,
-                   None if residual is None else _ready(residual), s, False)[0]
+    return _linear(_ready(x), _ready(weight), _ready(bias), offsets,
+                   _ready(residual), s, False)[0]
 
 
 # ---------------------------------------------------------------- norms around a block
@@ -324,7 +336,7 @@ def _norm(h, y, post_weight, gate, next_weight, s, keep):
     n = torch.empty_like(h) if next_weight is not None else None
     r2 = h.new_empty(s.T, dtype=torch.float32) if keep and post_weight is not None else None
     r3 = h.new_empty(s.T, dtype=torch.float32) if keep and next_weight is not None else None
-    _call(_lib.load().moe_residual_norm, h.device.index, _dtype_code(h.dtype), s.T, s.H, _ptr(h), _ptr(y),
+    _call(_lib.load().moe_residual_norm, h.get_device(), _dtype_code(h.dtype), s.T, s.H, _ptr(h), _ptr(y),
           _ptr(post_weight), _ptr(gate), s.gate_kind, _ptr(next_weight), s.scale, s.eps, _ptr(out), _ptr(n),
           _ptr(r2), _ptr(r3))
     return out, n, r2, r3
@@ -336,8 +348,8 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, y, post_weight, gate, next_weight, s):
         ctx.set_materialize_grads(False)
-        h, y, post_weight, gate, next_weight = (None if t is None else _ready(t)
-                                                for t in (h, y, post_weight, gate, next_weight))
+        h, y, gate = _ready(h), _ready(y), _ready(gate)
+        post_weight, next_weight = _ready(post_weight), _ready(next_weight)
         out, n, r2, r3 = _norm(h, y, post_weight, gate, next_weight, s, True)
         after = h if y is None else out  # what the second norm is taken of
         ctx.save_for_backward(after if n is not None else None, y, post_weight, gate, next_weight, r2, r3)
@@ -345,13 +357,13 @@ class _ResidualNorm(torch.autograd.Function):
         return (out, n) if y is not None and n is not None else out if n is None else n
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, *up):
         after, y, post_weight, gate, next_weight, r2, r3 = ctx.saved_tensors
         s = ctx.s
         d_out = up[0] if y is not None else None
         d_n = up[-1] if next_weight is not None else None
-        d_out, d_n = (None if t is None else _ready(t) for t in (d_out, d_n))
+        d_out, d_n = _ready(d_out), _ready(d_n)
         like = d_out if d_out is not None else d_n
         if like is None:
             return (None,) * 6
@@ -366,7 +378,7 @@ class _ResidualNorm(torch.autograd.Function):
         d_gate = None if gate is None else torch.empty_like(gate)
         L = _lib.load()
         ws = _workspace(L.moe_residual_norm_workspace_bytes(s.T, s.H), like)
-        _call(L.moe_residual_norm_backward, like.device.index, _dtype_code(like.dtype), s.T, s.H,
+        _call(L.moe_residual_norm_backward, like.get_device(), _dtype_code(like.dtype), s.T, s.H,
               _ptr(d_out), _ptr(d_n), _ptr(after), _ptr(y), _ptr(post_weight), _ptr(gate), s.gate_kind,
               _ptr(used), s.scale, _ptr(r2), _ptr(r3), _ptr(d_h), _ptr(d_y), _ptr(d_post), _ptr(d_gate),
               _ptr(d_next) if used is not None else None, _ptr(ws))
@@ -380,9 +392,10 @@ def _gate_kind(gate, h):
         return _GATE_FULL
     if gate.shape == h.shape[-1:]:
         return _GATE_CHANNEL
-    if not (gate.shape == h.shape[:-1] + (1,)):
+    if gate.shape != h.shape[:-1] + (1,):
         raise ModelError(
-            f"gate must be {list(h.shape[-1:])}, {list(h.shape[:-1]) + [1]} or {list(h.shape)}, " f"got {list(gate.shape)}")
+            f"gate must be {list(h.shape[-1:])}, {list(h.shape[:-1]) + [1]} or {list(h.shape)}, "
+            f"got {list(gate.shape)}")
     return _GATE_TOKEN
 
 
@@ -429,6 +442,5 @@ def residual_norm(h, y, post_weight=None, *, gate=None, next_weight=None, residu
     s = _NormShape(h.numel() // H, H, kind, float(residual_scale), eps)
     if _tracked(h, y, post_weight, gate, next_weight):
         return _ResidualNorm.apply(h, y, post_weight, gate, next_weight, s)
-    out, n, _, _ = _norm(*(None if t is None else _ready(t) for t in (h, y, post_weight, gate, next_weight)),
-                         s, False)
+    out, n, _, _ = _norm(_ready(h), _ready(y), _ready(post_weight), _ready(gate), _ready(next_weight), s, False)
     return out if n is None else (out, n)

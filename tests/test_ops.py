@@ -98,7 +98,9 @@ def test_c_entries_refuse_before_any_device_call():
     assert status(sort(T=2 ** 30), "2^31") == 4
     assert status(sort(nbytes=2), "index_bytes") == 1
     assert status(sort(idx=None), "NULL") == 1
-    assert status(sort(counts=P + 4), "16-byte") == 1
+    assert status(sort(counts=P + 2), "aligned") == 1
+    assert status(sort(nbytes=8, idx=P + 4), "aligned") == 1
+    assert status(sort(T=10 ** 6, ws=P + 8), "16-byte") == 1
     assert status(sort(T=10 ** 6, ws=None), "NULL") == 1
 
     def rows(fn, T=4, k=2, H=16, dtype=F32, x=P, kept=P, extra=(P,)):
