@@ -633,9 +633,10 @@ constexpr int kernel_smem_elems() {
 // for every row of a block before any row of it is visited: it issues the
 // loads the visit needs into q (a QT), so a block's loads are all in flight
 // together instead of being waited for row group by row group, and the next
-// block's loads are issued before this block's rows are visited.
+// block's loads are issued before this block's rows are visited (AHEAD: every
+// block's loads before the first block, in registers the main loop has left).
 struct NoPre {};
-template <class C, int NACC, class QT, class PRE, class F>
+template <class C, int NACC, class QT, bool AHEAD = false, class PRE, class F>
 MOE_DEV void for_each_row8_pre(const f32x16 (&acc)[NACC][C::TN][C::TM], float* lds, PRE&& pre,
                                F&& f) {
   static_assert(C::WM % 16 == 0, "rows are visited 16 at a time");
@@ -651,19 +652,23 @@ MOE_DEV void for_each_row8_pre(const f32x16 (&acc)[NACC][C::TN][C::TM], float* l
   float* reg = lds + wave * NACC * SR * P;
   // the loads of pass b + 1 are issued before the rows of pass b are visited
   // (two register sets), so their latency overlaps one pass of work
-  QT q[2][RG];
+  constexpr int SETS = AHEAD ? NPASS : 2;
+  QT q[SETS][RG];
   auto prefetch = [&](int b, int set) {
     const int r0 = wm * C::WM + (b % NSP) * SR;
 #pragma unroll
     for (int g = 0; g < RG; ++g)
       pre(r0 + g * 16 + (lane >> 2), wn * C::WN + (b / NSP) * 32 + (lane & 3) * 8, q[set][g]);
   };
-  if constexpr (HAS_PRE) prefetch(0, 0);
+  if constexpr (HAS_PRE) {
+#pragma unroll
+    for (int b = 0; b < (AHEAD ? NPASS : 1); ++b) prefetch(b, b);
+  }
 #pragma unroll
   for (int b = 0; b < NPASS; ++b) {  // unrolled: acc is indexed by constants only
-    const int tn = b / NSP, sp = b % NSP, set = b & 1;
+    const int tn = b / NSP, sp = b % NSP, set = AHEAD ? b : b & 1;
     const int r0 = wm * C::WM + sp * SR;  // first row of this pass
-    if constexpr (HAS_PRE) {
+    if constexpr (HAS_PRE && !AHEAD) {
       if (b + 1 < NPASS) prefetch(b + 1, set ^ 1);
     }
 #pragma unroll
@@ -713,7 +718,7 @@ MOE_DEV void for_each_row8(const f32x16 (&acc)[NACC][C::TN][C::TM], float* lds, 
 // for_each_row8_pre over a tile that may be tall: the main blocks, then the
 // wave's extra blocks (C::XR > 0: rows BM + 32 (wm & 1) .., columns of half
 // wm >> 1 of its WN), staged the same way, 32 rows at a time.
-template <class C, int NACC, class QT, class PRE, class F>
+template <class C, int NACC, class QT, bool AHEAD = false, class PRE, class F>
 MOE_DEV void for_each_row8_xpre(const f32x16 (&acc)[NACC][C::TN][C::TM],
                                 const f32x16 (&xacc)[NACC][C::XTN], float* lds, PRE&& pre,
                                 F&& f) {
@@ -765,9 +770,9 @@ MOE_DEV void for_each_row8_xpre(const f32x16 (&acc)[NACC][C::TN][C::TM],
     // the extra blocks first: their 64 accumulators are then dead during the
     // main passes (config 3 gate/up input gradient 1.20 -> 1.19 ms)
     extra();
-    for_each_row8_pre<C, NACC, QT>(acc, lds, pre, f);
+    for_each_row8_pre<C, NACC, QT, AHEAD>(acc, lds, pre, f);
   } else {
-    for_each_row8_pre<C, NACC, QT>(acc, lds, pre, f);
+    for_each_row8_pre<C, NACC, QT, AHEAD>(acc, lds, pre, f);
     if constexpr (C::XR > 0) extra();
   }
 }

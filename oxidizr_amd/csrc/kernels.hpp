@@ -174,12 +174,12 @@ MOE_DEV void group_tile(const int* prefix, int G, int nN, int id, int& grp, int&
 // Row-grouped launches need a grid of at least 8 * ceil(tiles / 8) blocks
 // (xcd_slot2); dense ones at least the tile count.
 MOE_DEV bool resolve_rows(const RowGroups& g, int N, int BM, int BN, int& grp, int& row0,
-                          int& mv, int& n0) {
+                          int& mv, int& n0, int blk) {
   const int nN = (N + BN - 1) / BN;
   int id, mt, nt;
   if (g.offsets == nullptr) {
     const int nM = (g.M + BM - 1) / BM;
-    if (!xcd_slot(blockIdx.x, nM * nN, id) || !tile_order(id, nM, nN, mt, nt)) return false;
+    if (!xcd_slot(blk, nM * nN, id) || !tile_order(id, nM, nN, mt, nt)) return false;
     n0 = nt * BN;
     grp = 0;
     row0 = mt * BM;
@@ -190,7 +190,7 @@ MOE_DEV bool resolve_rows(const RowGroups& g, int N, int BM, int BN, int& grp, i
   if (g.half_last) {
     const int nB = g.big_prefix[g.G], nH = g.half_prefix[g.G];
     int cls;
-    if (!xcd_slot2(blockIdx.x, nB * nN, nH * nN, cls, id)) return false;
+    if (!xcd_slot2(blk, nB * nN, nH * nN, cls, id)) return false;
     if (cls) {  // one half tile per group at most: pairs down a column
       if (!tile_order(id, nH, nN, mt, nt)) return false;
       grp = uni(find_group(g.half_prefix, g.G, mt));
@@ -200,7 +200,7 @@ MOE_DEV bool resolve_rows(const RowGroups& g, int N, int BM, int BN, int& grp, i
     }
   } else {  // group by group
     const int nM = g.tile_prefix[g.G];
-    if (!xcd_slot(blockIdx.x, nM * nN, id)) return false;
+    if (!xcd_slot(blk, nM * nN, id)) return false;
     group_tile(g.tile_prefix, g.G, nN, id, grp, local, nt);
   }
   n0 = nt * BN;
@@ -224,6 +224,10 @@ MOE_DEV bool resolve_rows(const RowGroups& g, int N, int BM, int BN, int& grp, i
   const int left = rows - local;
   mv = uni(left > BM + g.tall ? BM : left);
   return mv > 0;
+}
+MOE_DEV bool resolve_rows(const RowGroups& g, int N, int BM, int BN, int& grp, int& row0,
+                          int& mv, int& n0) {
+  return resolve_rows(g, N, BM, BN, grp, row0, mv, n0, (int)blockIdx.x);
 }
 
 // K-grouped problems (weight gradients): groups split the reduction over

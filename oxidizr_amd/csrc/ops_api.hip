@@ -399,7 +399,7 @@ moe_status linear_backward(hipStream_t s, int64_t M, int K, int N, int E, const 
   const D** w_tab = grouped ? (const D**)(ws + L.w_tab) : nullptr;
   D** dw_tab = grouped ? (D**)(ws + L.dw_tab) : nullptr;
   if (grouped)
-    hipLaunchKernelGGL(k_linear_prep<D>, dim3(dx ? kPrepBlocks : 1), dim3(1024), 0, s, offsets, E,
+    hipLaunchKernelGGL(k_linear_prep<D>, dim3(kPrepBlocks), dim3(1024), 0, s, offsets, E,
                        (int)M, offs, prefixes, w, dw, (int64_t)N * K, w_tab, dw_tab,
                        (const D*)nullptr, dx, (D*)nullptr, K);
   const RowGroups chunks{offs, prefixes, nullptr, nullptr, E, (int)M, 0, 0};
@@ -416,25 +416,43 @@ moe_status linear_backward(hipStream_t s, int64_t M, int K, int N, int E, const 
                          db);
   }
   LAUNCH_CHECK();
+  using CW = WgradTiling<D, 1>;
+  const SplitPlan sp = grouped ? SplitPlan{1, 0} : plan_dense_wgrad<D, 1>(N, K, (int)M);
+  const KGroups kg{offs, E, (int)M, sp.nsplit, sp.kchunk, 1, nullptr};
+  const int wgrid = kgrouped_grid(grouped ? E : sp.nsplit, N, K, CW::BM, CW::BN);
+  float* partial = (float*)(ws + L.splitk);
+  auto wgrad = [&](auto g) {
+    hipLaunchKernelGGL((k_wgrad<D, 1, decltype(g)::value>), dim3(wgrid), dim3(CW::THREADS), 0, s, dz,
+                       (const D*)nullptr, (int64_t)N, x, (int64_t)K, kg, N, K, 1.0f,
+                       (D* const*)dw_tab, dw, (D* const*)nullptr, (D*)nullptr, partial, wgrid, 0);
+  };
+  bool done = false;  // the weight gradient rides with the input gradient
   if (dx)
     with_linear_tiling<D>(offs, prefixes, E, M, K, [&](auto c, const RowGroups& r, int grid) {
       using C = decltype(c);
+      if constexpr (C::THREADS == CW::THREADS && sizeof(D) == 2) {
+        if (dw) {
+          auto both = [&](auto g) {
+            hipLaunchKernelGGL((k_linear_bwd<D, C, decltype(g)::value>), dim3(wgrid + grid),
+                               dim3(C::THREADS), 0, s, dz, x, r, (const D* const*)w_tab, w, N, K,
+                               dx, kg, wgrid, (D* const*)dw_tab, dw, partial);
+          };
+          if (grouped) both(std::true_type());
+          else both(std::false_type());
+          done = true;
+          return;
+        }
+      }
       hipLaunchKernelGGL((k_linear_dgrad<D, C>), dim3(grid), dim3(C::THREADS), 0, s, dz, r,
                          (const D* const*)w_tab, w, N, K, dx);
     });
-  LAUNCH_CHECK();
-  if (!dw) return MOE_OK;
-  if (!grouped)
-    return launch_dense_wgrad<D, 1>(s, dz, nullptr, N, x, K, (int)M, N, K, 1.0f, dw, nullptr,
-                                    (float*)(ws + L.splitk), L.splitk_bytes);
-  using C = WgradTiling<D, 1>;
-  hipLaunchKernelGGL(k_linear_zero_dw<D>, dim3(8, E), dim3(256), 0, s, offs, (int64_t)N * K, dw);
-  const KGroups kg{offs, E, (int)M, 1, 0, 1, nullptr};
-  const int grid = kgrouped_grid(E, N, K, C::BM, C::BN);
-  hipLaunchKernelGGL((k_wgrad<D, 1, true>), dim3(grid), dim3(C::THREADS), 0, s, dz,
-                     (const D*)nullptr, (int64_t)N, x, (int64_t)K, kg, N, K, 1.0f,
-                     (D* const*)dw_tab, (D*)nullptr, (D* const*)nullptr, (D*)nullptr,
-                     (float*)nullptr, grid, 0);
+  if (dw && !done) {
+    if (grouped) wgrad(std::true_type());
+    else wgrad(std::false_type());
+  }
+  if (dw && sp.nsplit > 1)
+    hipLaunchKernelGGL(k_splitk_reduce<D>, dim3(ceil_div((int64_t)N * K, 2048), 1), dim3(256), 0, s,
+                       partial, sp.nsplit, (int64_t)N * K, 1.0f, dw, (D*)nullptr);
   LAUNCH_CHECK();
   return MOE_OK;
 }
