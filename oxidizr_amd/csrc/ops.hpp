@@ -144,6 +144,27 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(
   }
 }
 
+// Streamed accesses. Outputs of these operators are written once and read by a later
+// kernel, on any XCD, so keeping them in the writer's L2 until the kernel ends only
+// delays them: stores with the nontemporal hint measured faster at every size (norm
+// forward 8192 x 7168 89 -> 83 us and 1999 x 776 fp32 6.3 -> 5.5, its backward 8192 x
+// 2048 44.5 -> 37.9, permute 16384 x 2048, k = 6 94 -> 77, k = 2 of 8192 22 -> 13.5 with one
+// slice to a wave). Loads only where the rows outgrow the caches (kStreamBytes).
+template <typename T>
+MOE_DEV void st16_stream(T* p, u32x4 v) {
+  __builtin_nontemporal_store(v, gptr(reinterpret_cast<u32x4*>(p)));
+}
+template <bool STREAM, typename T>
+MOE_DEV u32x4 ld16_maybe_stream(const T* p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load(gptr(reinterpret_cast<const u32x4*>(p)));
+  return *gptr(reinterpret_cast<const u32x4*>(p));
+}
+MOE_DEV void store8_stream(bf16_t* p, const float* v) { st16_stream(p, pack16(v, bf16_t())); }
+MOE_DEV void store8_stream(float* p, const float* v) {
+  st16_stream(p, pack16(v, float()));
+  st16_stream(p + 4, pack16(v + 4, float()));
+}
+
 // ------------------------------------------------------------------ rows to experts and back
 // inv_perm[t k + j] says which row of the sorted order holds assignment (t, j);
 // rows at or beyond *kept belong to no expert.  A position outside [0, T k) (no
@@ -151,44 +172,41 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(
 constexpr int kMaxPerTok = 16;
 
 // xp[inv[t, j]] = x[t], or zeros for an assignment without an expert.  One wave
-// per (token, slice of 4 x 64 16-byte vectors): it reads its part of the row once
-// and writes it k times.
-constexpr int kPermuteVecs = 4;
+// per (token, 64 16-byte vectors): it reads its part of the row once and writes it k
+// times.  Bound by the writes: 8192 tokens, H = 7168, k = 8: PERM_US.
 template <typename T>
 __global__ __launch_bounds__(256) void k_permute(const T* __restrict__ x,
                                                  const int* __restrict__ inv,
                                                  const int* __restrict__ kept, int64_t Tn, int k,
                                                  int H, T* __restrict__ xp) {
   constexpr int V = Vec16<T>::N;
-  const int nv = H / V, nsl = (nv + 64 * kPermuteVecs - 1) / (64 * kPermuteVecs);
+  const int nv = H / V, nsl = (nv + 63) / 64;
   const int64_t wid = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (wid >= Tn * nsl) return;
   const int64_t t = wid / nsl;
   const int lane = threadIdx.x & 63;
-  const int c0 = (int)(wid - t * nsl) * 64 * kPermuteVecs + lane;
+  const int c = (int)(wid - t * nsl) * 64 + lane;
+  const bool in = c < nv;  // no early exit: lane j holds slot j's row
   const int64_t N = Tn * k;
   const int rows = *kept;
   const int at = lane < k ? inv[t * k + lane] : -1;
-  u32x4 v[kPermuteVecs];
-#pragma unroll
-  for (int u = 0; u < kPermuteVecs; ++u)
-    if (c0 + 64 * u < nv) v[u] = ld16(x + t * H + (int64_t)(c0 + 64 * u) * V);
+  const u32x4 v = in ? ld16(x + t * H + (int64_t)c * V) : u32x4{0, 0, 0, 0};
   for (int j = 0; j < k; ++j) {
     const int p = __builtin_amdgcn_readlane(at, j);
-    if (p < 0 || p >= N) continue;
-    const bool real = p < rows;
-    T* dst = xp + (int64_t)p * H;
-#pragma unroll
-    for (int u = 0; u < kPermuteVecs; ++u)
-      if (c0 + 64 * u < nv) st16(dst + (c0 + 64 * u) * V, real ? v[u] : u32x4{0, 0, 0, 0});
+    if (in && p >= 0 && p < N)
+      st16_stream(xp + (int64_t)p * H + c * V, p < rows ? v : u32x4{0, 0, 0, 0});
   }
 }
 
 // out[t] = sum_j w[t, j] y[inv[t, j]] over the assignments that have an expert, j
 // ascending, in fp32, rounded once (w null: every weight is 1).  One wave per
 // (token, 64 vectors); a slice's k rows are all requested before the first is added.
-template <typename T, int KMAX>
-__global__ __launch_bounds__(256) void k_unpermute(const T* __restrict__ y,
+// STREAM: rows of more than kStreamBytes, which the caches would not hold anyway, are
+// loaded with the nontemporal hint (939 MB, k = 8, H = 7168: 190 -> 176 us; 403 MB, k = 6:
+// 86 -> 78; but 67 MB just written, k = 2: 14.8 -> 18.2).
+constexpr int64_t kStreamBytes = int64_t(256) << 20;
+template <typename T, int KMAX, bool STREAM>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void k_unpermute(const T* __restrict__ y,
                                                    const int* __restrict__ inv,
                                                    const int* __restrict__ kept,
                                                    const float* __restrict__ w, int64_t Tn, int k,
@@ -206,26 +224,24 @@ __global__ __launch_bounds__(256) void k_unpermute(const T* __restrict__ y,
   const bool in = c < nv;  // no early exit: lane j holds slot j's row and weight
   u32x4 v[KMAX];
 #pragma unroll
-  for (int j = 0; j < KMAX; ++j)
-    if (j < k) {
-      const int p = __builtin_amdgcn_readlane(at, j);
-      if (in && p >= 0 && p < rows) v[j] = ld16(y + (int64_t)p * H + c * V);
-    }
+  for (int j = 0; j < KMAX; ++j) {  // slots past k are -1
+    const int p = __builtin_amdgcn_readlane(at, j);
+    if (in && p >= 0 && p < rows) v[j] = ld16_maybe_stream<STREAM>(y + (int64_t)p * H + c * V);
+  }
   float acc[V], f[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[i] = 0.0f;
 #pragma unroll
-  for (int j = 0; j < KMAX; ++j)
-    if (j < k) {
-      const int p = __builtin_amdgcn_readlane(at, j);
-      const float wj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wt), j));
-      if (in && p >= 0 && p < rows) {
-        unpack16(v[j], f, T());
+  for (int j = 0; j < KMAX; ++j) {
+    const int p = __builtin_amdgcn_readlane(at, j);
+    const float wj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wt), j));
+    if (in && p >= 0 && p < rows) {
+      unpack16(v[j], f, T());
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] += wj * f[i];
-      }
+      for (int i = 0; i < V; ++i) acc[i] += wj * f[i];
     }
-  if (in) st16(out + t * H + c * V, pack16(acc, T()));
+  }
+  if (in) st16_stream(out + t * H + c * V, pack16(acc, T()));
 }
 
 // dy[inv[t, j]] = w[t, j] dout[t] (zeros without an expert) and, with y,
@@ -280,7 +296,7 @@ __global__ __launch_bounds__(256) void k_unpermute_bwd(
             float o[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) o[i] = real ? wj * d[i] : 0.0f;
-            st16(dy + (int64_t)p * H + c * V, pack16(o, T()));
+            st16_stream(dy + (int64_t)p * H + c * V, pack16(o, T()));
           }
         }
     }
@@ -394,7 +410,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_fwd(NormArgs<
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[c][i] = a.scale * o[c][i] + gt * u[c][i];
-        store8(a.hn + row + ch * 8, o[c]);
+        store8_stream(a.hn + row + ch * 8, o[c]);
       }
     }
   }
@@ -414,7 +430,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_fwd(NormArgs<
       load8(a.w3 + ch * 8, v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = o[c][i] * s * v[i];
-      store8(a.n + row + ch * 8, v);
+      store8_stream(a.n + row + ch * 8, v);
     }
   }
 }
@@ -595,7 +611,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_bwd(NormBwdAr
         p[c][i] -= m3 * hh[c][i];
         o[i] = a.scale * p[c][i];
       }
-      store8(a.dh + row + ch * 8, o);
+      store8_stream(a.dh + row + ch * 8, o);
       if (!a.y) continue;
       float gv[8], wv[8];
 #pragma unroll
@@ -608,7 +624,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_bwd(NormBwdAr
       if (full) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = p[c][i] * yh[c][i] * wv[i];
-        store8(a.dgate + row + ch * 8, v);
+        store8_stream(a.dgate + row + ch * 8, v);
       }
       const bool colg = a.gate_kind >= kGateToken;
 #pragma unroll
@@ -617,7 +633,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_bwd(NormBwdAr
         ca[c][i] += (colg ? d : p[c][i]) * yh[c][i];
         o[i] = r2 * (wv[i] * d - yh[c][i] * m2);
       }
-      store8(a.dy + row + ch * 8, o);
+      store8_stream(a.dy + row + ch * 8, o);
     }
   }
   // the block's column sums: its rows' waves in order

@@ -121,8 +121,7 @@ void with_k(int k, F&& f) {
 template <typename D>
 moe_status launch_permute(hipStream_t s, int64_t T, int k, int H, const int* inv, const int* kept,
                           const D* x, D* xp) {
-  const int per = 64 * kPermuteVecs * Vec16<D>::N;
-  const unsigned grid = wave_grid(T * ceil_div(H, per));
+  const unsigned grid = wave_grid(T * ceil_div(H, 64 * Vec16<D>::N));
   if (!grid) return fail(MOE_ERR_UNSUPPORTED, "too many tokens for one launch");
   hipLaunchKernelGGL(k_permute<D>, dim3(grid), dim3(256), 0, s, x, inv, kept, T, k, H, xp);
   LAUNCH_CHECK();
@@ -134,9 +133,15 @@ moe_status launch_unpermute(hipStream_t s, int64_t T, int k, int H, const int* i
                             const int* kept, const D* y, const float* w, D* out) {
   const unsigned grid = wave_grid(T * ceil_div(H, 64 * Vec16<D>::N));
   if (!grid) return fail(MOE_ERR_UNSUPPORTED, "too many tokens for one launch");
+  const bool stream = T * k * H * (int64_t)sizeof(D) > kStreamBytes;
   with_k(k, [&](auto kc) {
-    hipLaunchKernelGGL((k_unpermute<D, decltype(kc)::value>), dim3(grid), dim3(256), 0, s, y, inv,
-                       kept, w, T, k, H, out);
+    constexpr int KM = decltype(kc)::value;
+    if (stream)
+      hipLaunchKernelGGL((k_unpermute<D, KM, true>), dim3(grid), dim3(256), 0, s, y, inv, kept, w, T,
+                         k, H, out);
+    else
+      hipLaunchKernelGGL((k_unpermute<D, KM, false>), dim3(grid), dim3(256), 0, s, y, inv, kept, w, T,
+                         k, H, out);
   });
   LAUNCH_CHECK();
   return MOE_OK;
@@ -261,6 +266,133 @@ moe_status check_linear(int dtype, int64_t M, int K, int N, int E, bool grouped,
   return MOE_OK;
 }
 
+// Whether a forward runs as the stream of its weights (k_linear_skinny): few rows to
+// an expert.  Rows are counted as evenly spread over the experts that can have any.
+constexpr int kSkinnyRowsPerGroup = 16;
+bool linear_skinny(int64_t M, int E, bool grouped) {
+  const int64_t groups = grouped ? std::min<int64_t>(E, M) : 1;
+  return grouped ? M <= kSkinnyRowsPerGroup * groups : M <= kLinearSkinnyRows;
+}
+
+// Row tilings of a product alone on the GPU, in tenths of a round of 256-row tiles (one
+// to a CU). Measured on dense products of random bf16 rows (zeros run at higher
+// clocks), us, 256-row / 384-row / 128 x 128 / 64 x 128 tiles: M = 16384, N = 2048, K = 1408
+// 82 / 106 / 95 / 125; 16384, 1408, 2048 107 / 140 / 97 / -; 8192, 2816, 2048 98 / 82 / 98 /
+// 125; 8192, 2048, 2816 76 / 98 / 90 / 122; 4096, 2048, 2816 63 / 87 / 47 / 64; 4096, 1408,
+// 2048 45 / 63 / 31 / 34; 1000, 2048, 2816 53 / 82 / 33 / 21; 300, 7168, 2048 41 / 51 / 25 / 23.
+constexpr TileCosts kLinearCosts{10.0, {4.8, 6.3}, {2.9, 4.3}};
+constexpr double kTallCost = 1.55;  // a 384-row tile against a 256-row one
+
+enum class RowTiles { kBig, kTall, kMid, kSmall };
+template <typename D>
+double tile_count(bool grouped, int E, int64_t M, int N, int bm, int bn) {
+  const int groups = grouped ? (int)std::min<int64_t>(E, M) : 1;
+  return (grouped ? group_row_tiles(groups, (double)M / groups, bm) : (double)ceil_div(M, bm)) *
+         ceil_div(N, bn);
+}
+// The row tiles of a product of M rows in E groups (or dense) with N output columns.
+template <typename D>
+RowTiles pick_tiles(bool grouped, int E, int64_t M, int N) {
+  using C = typename Tilings<D>::Big;
+  if constexpr (has_half_rows<D, C>()) {
+    using CM = typename LowTilings<C>::Mid;
+    using CS = typename LowTilings<C>::Small;
+    auto tiles = [&](int bm, int bn) { return tile_count<D>(grouped, E, M, N, bm, bn); };
+    const double big = big_cost(tiles(C::BM, C::BN), kLinearCosts.big);
+    const double mid = round_cost(tiles(CM::BM, CM::BN), kLinearCosts.mid);
+    const double small = round_cost(tiles(CS::BM, CS::BN), kLinearCosts.small);
+    // groups of fewer rows would run most of their 384-row tiles as shorter ones
+    const bool tall_ok = !grouped || M >= 2 * (int64_t)Rows384<C>::AR * E;
+    const double tall =
+        tall_ok ? big_cost(tiles(Rows384<C>::AR, C::BN), kLinearCosts.big * kTallCost) : 1e30;
+    if (std::min(mid, small) < std::min(big, tall))
+      return mid <= small ? RowTiles::kMid : RowTiles::kSmall;
+    if (tall < big) return RowTiles::kTall;
+  }
+  return RowTiles::kBig;
+}
+
+// Calls f(tiling, row groups, grid) for a launch of M rows in E groups (offsets and
+// prefixes of k_linear_prep), or dense (offsets null), with N output columns.
+template <typename D, class F>
+void with_row_tiles(RowTiles kind, const int* offsets, const int* prefixes, int E, int64_t M, int N,
+                    F&& f) {
+  using C = typename Tilings<D>::Big;
+  const bool grouped = offsets != nullptr;
+  auto go = [&](auto c, int half_last, int tall) {
+    using CC = decltype(c);
+    const int rows = CC::XR == 128 ? CC::AR : CC::BM;
+    if (!grouped) {
+      f(c, RowGroups{nullptr, nullptr, nullptr, nullptr, 1, (int)M, 0, 0},
+        (int)((int64_t)ceil_div(M, CC::AR) * ceil_div(N, CC::BN)));
+      return;
+    }
+    const int* tp = prefixes + prefix_slot(rows) * (E + 1);
+    const int64_t mt = ceil_div(M, rows) + E;
+    f(c, RowGroups{offsets, tp, tp + (E + 1), tp + 2 * (E + 1), E, (int)M, half_last, tall},
+      8 * ceil_div(mt * ceil_div(N, CC::BN), 8));
+  };
+  if constexpr (has_half_rows<D, C>()) {
+    if (kind == RowTiles::kTall) return go(Rows384<C>{}, 1, 0);
+    if (kind == RowTiles::kMid) return go(typename LowTilings<C>::Mid{}, 0, 0);
+    if (kind == RowTiles::kSmall) return go(typename LowTilings<C>::Small{}, 0, 0);
+    return go(C{}, grouped && M >= 2 * (int64_t)C::BM * E, tall_rows_for(C::BM));
+  }
+  go(C{}, 0, 0);
+}
+
+// Both products of a backward as one launch (k_linear_bwd): its estimated time, in
+// 64-deep k-tiles of a 256 x 256 tile. The weight gradient's tiles start first; work
+// that is left when they end is dealt tile by tile, so the last tiles end half a tile
+// apart on average. An epilogue costs about seven k-tiles.
+constexpr double kEpilogueTiles = 7.0;
+double bwd_cost(double wtiles, double wdepth, double dtiles, double ddepth) {
+  const double w = wdepth + kEpilogueTiles, d = ddepth + kEpilogueTiles;
+  return std::max(w, (wtiles * w + dtiles * d) / 256.0 + 0.5 * d);
+}
+struct BwdPlan {
+  SplitPlan split;  // chunks of the weight gradient's rows (dense only)
+  RowTiles tiles;   // of the input gradient
+  bool fused;
+};
+template <typename D>
+BwdPlan plan_bwd(bool grouped, int E, int64_t M, int K, int N) {
+  using C = typename Tilings<D>::Big;
+  BwdPlan p;
+  p.split = grouped ? SplitPlan{1, 0} : plan_dense_wgrad<D, 1>(N, K, (int)M);
+  p.tiles = pick_tiles<D>(grouped, E, M, K);
+  p.fused = false;
+  if constexpr (has_half_rows<D, C>()) {
+    if (p.tiles != RowTiles::kBig && p.tiles != RowTiles::kTall) return p;
+    p.fused = true;
+    const int groups = grouped ? (int)std::min<int64_t>(E, M) : 1;
+    const double wtiles = (double)groups * ceil_div(N, C::BM) * ceil_div(K, C::BN);
+    const double red = 3.1 * (double)N * K / ((double)C::BM * C::BN * C::BK);  // see plan_split
+    const int nkt = ceil_div((M + groups - 1) / groups, C::BK);
+    const int most = grouped ? 1 : std::max(1, std::min(64, nkt / 4));
+    const double dtiles = tile_count<D>(grouped, E, M, K, C::BM, C::BN);
+    const double ttiles = tile_count<D>(grouped, E, M, K, Rows384<C>::AR, C::BN);
+    const double depth = ceil_div(N, C::BK);
+    const bool tall_ok = p.tiles == RowTiles::kTall;
+    double best = 0;
+    for (int ns = 1; ns <= most; ++ns) {
+      const double d = ceil_div(nkt, ns), extra = ns > 1 ? red * ns : 0.0;
+      const double big = bwd_cost(wtiles * ns, d, dtiles, depth) + extra;
+      const double tall = tall_ok ? bwd_cost(wtiles * ns, d, ttiles, depth * kTallCost) + extra : 1e30;
+      const double cost = std::min(big, tall);
+      if (ns == 1 || cost < best) {
+        best = cost;
+        if (!grouped) {
+          const int chunk = ceil_div(ceil_div(M, ns), C::BK) * C::BK;
+          p.split = {ceil_div(M, chunk), chunk};
+        }
+        p.tiles = big <= tall ? RowTiles::kBig : RowTiles::kTall;
+      }
+    }
+  }
+  return p;
+}
+
 struct LinearWs {
   size_t offs, prefixes, w_tab, dw_tab, dz, part, splitk, splitk_bytes, total;
 };
@@ -281,69 +413,14 @@ LinearWs linear_ws(int dtype, int64_t M, int K, int N, int E, bool grouped, int 
     if (act != kActNone) w.dz = c.take((size_t)M * N * b);
     w.part = c.take((size_t)dz_chunks(M, E, grouped) * N * 4);
     if (!grouped) {
-      w.splitk_bytes = dtype == MOE_DTYPE_BF16
-                           ? dense_wgrad_partial_bytes<bf16_t, 1>(N, K, (int)M)
-                           : dense_wgrad_partial_bytes<float, 1>(N, K, (int)M);
+      const SplitPlan sp = dtype == MOE_DTYPE_BF16 ? plan_bwd<bf16_t>(false, 1, M, K, N).split
+                                                   : plan_bwd<float>(false, 1, M, K, N).split;
+      w.splitk_bytes = sp.nsplit > 1 ? (size_t)sp.nsplit * N * K * 4 : 0;
       w.splitk = c.take(w.splitk_bytes);
     }
   }
   w.total = c.off;
   return w;
-}
-
-// Whether a forward runs as the stream of its weights (k_linear_skinny): few rows to
-// an expert.  Rows are counted as evenly spread over the experts that can have any.
-constexpr int kSkinnyRowsPerGroup = 16;
-bool linear_skinny(int64_t M, int E, bool grouped) {
-  const int64_t groups = grouped ? std::min<int64_t>(E, M) : 1;
-  return grouped ? M <= kSkinnyRowsPerGroup * groups : M <= kLinearSkinnyRows;
-}
-
-// Row tilings of a product alone on the GPU, in tenths of a round of 256-row tiles
-// (measured on dense launches, see with_dense_tiling's table): 128 x 128 and 64 x 128
-// tiles where those leave CUs idle, 384-row tiles where they fill more rounds.
-constexpr TileCosts kLinearCosts{10.0, {6.8, 8.2}, {4.4, 5.7}};
-constexpr double kTallCost = 1.4;  // a 384-row tile against a 256-row one
-
-// Calls f(tiling, row groups, grid) for a launch of M rows in E groups (offsets and
-// prefixes of k_linear_prep), or dense (offsets null), with N output columns.
-template <typename D, class F>
-void with_linear_tiling(const int* offsets, const int* prefixes, int E, int64_t M, int N, F&& f) {
-  using C = typename Tilings<D>::Big;
-  const bool grouped = offsets != nullptr;
-  auto go = [&](auto c, int half_last, int tall) {
-    using CC = decltype(c);
-    const int rows = CC::XR == 128 ? CC::AR : CC::BM;
-    if (!grouped) {
-      f(c, RowGroups{nullptr, nullptr, nullptr, nullptr, 1, (int)M, 0, 0},
-        (int)((int64_t)ceil_div(M, CC::AR) * ceil_div(N, CC::BN)));
-      return;
-    }
-    const int* tp = prefixes + prefix_slot(rows) * (E + 1);
-    const int64_t mt = ceil_div(M, rows) + E;
-    f(c, RowGroups{offsets, tp, tp + (E + 1), tp + 2 * (E + 1), E, (int)M, half_last, tall},
-      8 * ceil_div(mt * ceil_div(N, CC::BN), 8));
-  };
-  if constexpr (has_half_rows<D, C>()) {
-    using C3 = Rows384<C>;
-    using CM = typename LowTilings<C>::Mid;
-    using CS = typename LowTilings<C>::Small;
-    const int groups = grouped ? (int)std::min<int64_t>(E, M) : 1;
-    const double r = (double)M / groups;
-    auto tiles = [&](int bm, int bn) {
-      return (grouped ? group_row_tiles(groups, r, bm) : (double)ceil_div(M, bm)) * ceil_div(N, bn);
-    };
-    const double big = big_cost(tiles(C::BM, C::BN), kLinearCosts.big) / (grouped ? 1.15 : 1.0);
-    const double mid = round_cost(tiles(CM::BM, CM::BN), kLinearCosts.mid);
-    const double small = round_cost(tiles(CS::BM, CS::BN), kLinearCosts.small);
-    const bool tall_ok = !grouped || M >= 2 * (int64_t)C3::AR * E;
-    const double tall = tall_ok ? big_cost(tiles(C3::AR, C3::BN), kLinearCosts.big * kTallCost) : 1e30;
-    if (std::min(mid, small) < std::min(big, tall))
-      return mid <= small ? go(CM{}, 0, 0) : go(CS{}, 0, 0);
-    if (tall < big) return go(C3{}, 1, 0);
-    return go(C{}, grouped && M >= 2 * (int64_t)C::BM * E, tall_rows_for(C::BM));
-  }
-  go(C{}, 0, 0);
 }
 
 // Blocks of k_linear_prep: one for the prefixes, the others for the rows behind the
@@ -378,7 +455,8 @@ moe_status linear_forward(hipStream_t s, int64_t M, int K, int N, int E, const i
     hipLaunchKernelGGL(k_linear_prep<D>, dim3(kPrepBlocks), dim3(1024), 0, s, offsets, E, (int)M,
                        offs, prefixes, w, (D*)nullptr, (int64_t)N * K, w_tab, (D**)nullptr, epi.res,
                        epi.y, epi.pre, N);
-  with_linear_tiling<D>(offs, prefixes, E, M, N, [&](auto c, const RowGroups& r, int grid) {
+  with_row_tiles<D>(pick_tiles<D>(grouped, E, M, N), offs, prefixes, E, M, N,
+                    [&](auto c, const RowGroups& r, int grid) {
     using C = decltype(c);
     hipLaunchKernelGGL((k_linear_fwd<D, C>), dim3(grid), dim3(C::THREADS), 0, s, x, r,
                        (const D* const*)w_tab, w, K, epi);
@@ -417,7 +495,8 @@ moe_status linear_backward(hipStream_t s, int64_t M, int K, int N, int E, const 
   }
   LAUNCH_CHECK();
   using CW = WgradTiling<D, 1>;
-  const SplitPlan sp = grouped ? SplitPlan{1, 0} : plan_dense_wgrad<D, 1>(N, K, (int)M);
+  const BwdPlan bp = plan_bwd<D>(grouped, E, M, K, N);
+  const SplitPlan& sp = bp.split;
   const KGroups kg{offs, E, (int)M, sp.nsplit, sp.kchunk, 1, nullptr};
   const int wgrid = kgrouped_grid(grouped ? E : sp.nsplit, N, K, CW::BM, CW::BN);
   float* partial = (float*)(ws + L.splitk);
@@ -428,10 +507,10 @@ moe_status linear_backward(hipStream_t s, int64_t M, int K, int N, int E, const 
   };
   bool done = false;  // the weight gradient rides with the input gradient
   if (dx)
-    with_linear_tiling<D>(offs, prefixes, E, M, K, [&](auto c, const RowGroups& r, int grid) {
+    with_row_tiles<D>(bp.tiles, offs, prefixes, E, M, K, [&](auto c, const RowGroups& r, int grid) {
       using C = decltype(c);
       if constexpr (C::THREADS == CW::THREADS && sizeof(D) == 2) {
-        if (dw) {
+        if (dw && bp.fused) {
           auto both = [&](auto g) {
             hipLaunchKernelGGL((k_linear_bwd<D, C, decltype(g)::value>), dim3(wgrid + grid),
                                dim3(C::THREADS), 0, s, dz, x, r, (const D* const*)w_tab, w, N, K,

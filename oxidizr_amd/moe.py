@@ -59,6 +59,16 @@ class MoeConfig:
     # default_rms_norm_eps is not pinned by the reference; 1e-6 is the default.
     fused_block: bool = False
     rms_norm_eps: float = 1e-6
+    # MoeBlock only: a norm of the layer's output (post_norm), a trained gate [hidden]
+    # on it (residual_gate) and a factor on the residual, by ops.residual_norm:
+    #   h_out = residual_scale * h + gate * RMSNorm(MoE(RMSNorm(h)))
+    post_norm: bool = False
+    residual_gate: bool = False
+    residual_scale: float = 1.0
+
+    def plain_residual(self) -> bool:
+        """Whether the block's residual is h + MoE(RMSNorm(h)), which a fused_block plan runs."""
+        return not self.post_norm and not self.residual_gate and self.residual_scale == 1.0
 
     def has_shared_expert(self) -> bool:
         return True if self.shared_expert_enabled is None else bool(self.shared_expert_enabled)
@@ -542,24 +552,49 @@ class _MoeBlockFunction(torch.autograd.Function):
 class MoeBlock(torch.nn.Module):
     """The MoE sub-block of a decoder block (src/model.rs:2792-2800):
     forward(h [B, S, H]) -> (MoE(post_attention_layernorm(h)) + h, aux, z),
-    run as one fused_block plan."""
+    run as one fused_block plan. With cfg.post_norm, residual_gate or
+    residual_scale the output is residual_scale * h + gate * post_norm(MoE(..)),
+    run as ops.rms_norm, the layer's plan and ops.residual_norm."""
 
     def __init__(self, cfg: MoeConfig, dtype=torch.bfloat16, device="cuda"):
         super().__init__()
-        cfg = dataclasses.replace(cfg, fused_block=True)
+        cfg = dataclasses.replace(cfg, fused_block=cfg.plain_residual())
+        kw = dict(dtype=dtype, device=device)
         self.post_attention_layernorm = torch.nn.Module()
-        self.post_attention_layernorm.weight = torch.nn.Parameter(
-            torch.ones(cfg.hidden_size, dtype=dtype, device=device))
+        self.post_attention_layernorm.weight = torch.nn.Parameter(torch.ones(cfg.hidden_size, **kw))
         self.ffn = MoeLayer(cfg, dtype=dtype, device=device)
+        self.post_ffn_layernorm = None
+        if cfg.post_norm:
+            self.post_ffn_layernorm = torch.nn.Module()
+            self.post_ffn_layernorm.weight = torch.nn.Parameter(torch.ones(cfg.hidden_size, **kw))
+        self.residual_gate = (torch.nn.Parameter(torch.ones(cfg.hidden_size, **kw))
+                              if cfg.residual_gate else None)
 
     def trainable_parameters(self):
-        return ([("post_attention_layernorm.weight", self.post_attention_layernorm.weight)] +
-                self.ffn.trainable_parameters())
+        out = ([("post_attention_layernorm.weight", self.post_attention_layernorm.weight)] +
+               self.ffn.trainable_parameters())
+        if self.post_ffn_layernorm is not None:
+            out.append(("post_ffn_layernorm.weight", self.post_ffn_layernorm.weight))
+        if self.residual_gate is not None:
+            out.append(("residual_gate", self.residual_gate))
+        return out
+
+    def _forward_residual_norm(self, h):
+        from . import ops
+        cfg = self.ffn.cfg
+        x = ops.rms_norm(h, self.post_attention_layernorm.weight, cfg.rms_norm_eps)
+        y, aux, z = self.ffn(x)
+        post = self.post_ffn_layernorm.weight if self.post_ffn_layernorm is not None else None
+        out = ops.residual_norm(h, y, post, gate=self.residual_gate,
+                                residual_scale=cfg.residual_scale, eps=cfg.rms_norm_eps)
+        return out, aux, z
 
     def forward(self, h):
         if h.dim() != 3:
             raise ModelError(f"MoE expects [B, Seq, Hidden], got {list(h.shape)}")
         B, S, H = h.shape
+        if not self.ffn.cfg.plain_residual():
+            return self._forward_residual_norm(h)
         h2d = h.reshape(B * S, H).contiguous()
         layer = self.ffn
         params = ([e.gate_proj.weight for e in layer.experts] +

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from oxidizr_amd import ops
+from oxidizr_amd.moe import MoeBlock, MoeConfig
 from tests import ops_ref as ref
 
 pytestmark = pytest.mark.gpu
@@ -214,11 +215,30 @@ def test_dense_linear(M, K, N, act, bias, res, dtype):
     linear_case(gen(M + K), [M], K, N, act, dtype, bias, res, grouped=False)
 
 
-@pytest.mark.parametrize("T,E,k", [(900, 4, 2), (2100, 3, 2), (1500, 24, 4)])
-def test_grouped_linear_over_the_tilings(T, E, k):
-    # row counts that reach the 256- and 384-row tiles, their tails and the shorter tilings
-    sizes = torch.bincount(routing(gen(T), T, k, E, skew=0.7).flatten(), minlength=E).tolist()
-    linear_case(gen(T + 1), sizes, 320, 520, "silu", torch.bfloat16, bias=True, res=True, tail=5)
+# Row counts around the edges of 64- to 384-row tiles and of their tails
+EDGES = [256, 257, 319, 320, 321, 383, 384, 385, 64, 65, 128, 129, 192, 193, 0, 1, 511, 512, 513, 576, 577, 640,
+         300, 440]
+# group sizes, and a pair of widths: the wider output takes the tiles named, the other way about the input
+# gradient does (together with the weight gradient's tiles)
+TILINGS = {"256 rows, group by group": (EDGES, 136, 1400),
+           "256 rows, short tiles last": ([997, 640, 575, 1088, 832, 321, 1150, 797], 136, 2000),
+           "384 rows": ([1152, 1217, 1534, 385, 1712], 136, 2704),
+           "128 rows": ([225] * 40, 200, 520)}
+
+
+@pytest.mark.parametrize("swap", [False, True])
+@pytest.mark.parametrize("tiles", TILINGS)
+def test_grouped_linear_over_the_tilings(tiles, swap):
+    sizes, K, N = TILINGS[tiles]
+    if swap:
+        K, N = N, K
+    linear_case(gen(len(sizes)), sizes, K, N, "silu", torch.bfloat16, bias=True, res=swap, tail=5)
+
+
+@pytest.mark.parametrize("M,K,N", [(8192, 136, 2048), (8192, 2048, 136), (6144, 136, 2816), (6100, 2816, 136),
+                                   (3000, 2048, 200)])
+def test_dense_linear_over_the_tilings(M, K, N):
+    linear_case(gen(M), [M], K, N, "gelu_tanh", torch.bfloat16, bias=True, res=True, grouped=False)
 
 
 def test_linear_gradients_one_at_a_time():
@@ -411,7 +431,7 @@ def test_a_run_of_them_with_its_gradients():
     # sums of up to T k I = 60000 fp32 terms, whose roundings add up like their root: 2^-24 sqrt(60000)
     # = 1.5e-5 of the magnitudes
     for name, a, b in zip(["h", "n", "x", "w"] + list(p), (h, n) + got, (h64, n64) + want):
-        err = float((a.double() - b).norm() / b.norm())
+        err = float(((a.double() - b).norm() / b.norm()).detach())
         assert err < 1.5e-5, (name, err)
 
 
@@ -443,6 +463,45 @@ def test_gradients_against_differences():
         diff = (values[0] - 8 * values[1] + 8 * values[2] - values[3]) / (12 * step)
         assert abs(diff - slope) < 2e-3 * max(1.0, float(grads[name].norm()) * float(way.norm()) ** 0.5), \
             (name, diff, slope)
+
+
+@pytest.mark.parametrize("post,gate,scale", [(True, False, 1.0), (False, True, 1.0), (True, True, 0.5),
+                                             (False, False, 0.75)])
+def test_block_with_norms_on_both_sides(post, gate, scale):
+    cfg = MoeConfig(hidden_size=64, num_experts=6, experts_per_tok=2, intermediate_size=48, post_norm=post,
+                    residual_gate=gate, residual_scale=scale)
+    block = MoeBlock(cfg, torch.float32)
+    g = gen(17)
+    with torch.no_grad():
+        for name, p in block.trainable_parameters():
+            p.normal_(1.0 if "layernorm" in name or name == "residual_gate" else 0.0, 0.1, generator=g)
+    names = [n for n, _ in block.trainable_parameters()]
+    assert ("post_ffn_layernorm.weight" in names) == post and ("residual_gate" in names) == gate
+    h = normal(g, 2, 35, 64).requires_grad_()
+    out, aux, z = block(h)
+    # the same from the layer's own forward and torch, in float64 around it
+    def rms(t, w):
+        return t * torch.rsqrt(t.square().mean(-1, keepdim=True) + cfg.rms_norm_eps) * w
+    h2 = h.detach().double().requires_grad_()
+    leaves = {n: p for n, p in block.named_parameters() if not n.startswith("ffn.")}
+    d = {n: p.detach().double().requires_grad_() for n, p in leaves.items()}
+    x = rms(h2, d["post_attention_layernorm.weight"])
+    y, aux2, z2 = block.ffn(x.float())
+    y = y.double()
+    u = rms(y, d["post_ffn_layernorm.weight"]) if post else y
+    want = scale * h2 + (d["residual_gate"] if gate else 1.0) * u
+    up = normal(gen(18), 2, 35, 64)
+    got = torch.autograd.grad(out, [h] + list(leaves.values()), up)
+    ref64 = torch.autograd.grad(want, [h2] + list(d.values()), up.double())
+    # the layer runs in fp32 on both sides, on inputs that differ by an fp32 rounding: sums of 64 and 48
+    # terms there, 70 x 64 in the weights' gradients; 2^-24 sqrt(4480) = 4e-6 of the magnitudes
+    assert torch.allclose(aux, aux2, rtol=1e-5) and torch.allclose(z, z2, rtol=1e-5)
+    for name, a, b in zip(["out", "h"] + list(leaves), (out,) + got, (want,) + ref64):
+        err = float(((a.double() - b).norm() / b.norm()).detach())
+        assert err < 4e-6, (name, err)
+    plain = MoeBlock(MoeConfig(hidden_size=64, num_experts=6, experts_per_tok=2, intermediate_size=48),
+                     torch.float32)
+    assert plain.ffn.cfg.fused_block and not block.ffn.cfg.fused_block
 
 
 @pytest.mark.parametrize("T", [3, 500])
