@@ -97,7 +97,7 @@ MOE_DEV void linear_store8(const LinearEpi<T>& e, int64_t r, int n, const float 
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] += res[i];
   }
-  store8(e.y + o, y);
+  store8_stream(e.y + o, y);
 }
 
 // ------------------------------------------------------------------ preparation
@@ -263,7 +263,7 @@ MOE_DEV void dgrad_tile(T* smem, int blk, const T* __restrict__ dZ, const RowGro
     mainloop_x<CT, T, false, true, 1, 1>(acc, xacc, a, b, N, smem);
     for_each_row8_x<CT, 1>(acc, xacc, reinterpret_cast<float*>(smem), [&](int m, int n, auto& v) {
       if (m >= mv || k0 + n >= K) return;
-      store8(dX + ((int64_t)row0 + m) * K + k0 + n, v[0]);
+      store8_stream(dX + ((int64_t)row0 + m) * K + k0 + n, v[0]);
     });
   });
 }

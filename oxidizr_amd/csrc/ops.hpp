@@ -144,27 +144,6 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(
   }
 }
 
-// Streamed accesses. Outputs of these operators are written once and read by a later
-// kernel, on any XCD, so keeping them in the writer's L2 until the kernel ends only
-// delays them: stores with the nontemporal hint measured faster at every size (norm
-// forward 8192 x 7168 89 -> 83 us and 1999 x 776 fp32 6.3 -> 5.5, its backward 8192 x
-// 2048 44.5 -> 37.9, permute 16384 x 2048, k = 6 94 -> 77, k = 2 of 8192 22 -> 13.5 with one
-// slice to a wave). Loads only where the rows outgrow the caches (kStreamBytes).
-template <typename T>
-MOE_DEV void st16_stream(T* p, u32x4 v) {
-  __builtin_nontemporal_store(v, gptr(reinterpret_cast<u32x4*>(p)));
-}
-template <bool STREAM, typename T>
-MOE_DEV u32x4 ld16_maybe_stream(const T* p) {
-  if constexpr (STREAM) return __builtin_nontemporal_load(gptr(reinterpret_cast<const u32x4*>(p)));
-  return *gptr(reinterpret_cast<const u32x4*>(p));
-}
-MOE_DEV void store8_stream(bf16_t* p, const float* v) { st16_stream(p, pack16(v, bf16_t())); }
-MOE_DEV void store8_stream(float* p, const float* v) {
-  st16_stream(p, pack16(v, float()));
-  st16_stream(p + 4, pack16(v + 4, float()));
-}
-
 // ------------------------------------------------------------------ rows to experts and back
 // inv_perm[t k + j] says which row of the sorted order holds assignment (t, j);
 // rows at or beyond *kept belong to no expert.  A position outside [0, T k) (no
