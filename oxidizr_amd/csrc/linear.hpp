@@ -309,6 +309,7 @@ __global__ __launch_bounds__(C::THREADS) void k_linear_bwd(const T* __restrict__
 // a workgroup share a block of 16 weight rows and take every KS-th k-chunk of 8
 // steps; their sums are added through LDS in wave order.
 constexpr int kLinearSkinnyRows = 64;  // rows of an expert that one workgroup takes
+constexpr int kSkinnyChunkBytes = 512;  // of a weight row, in one k-chunk
 // Slot s of a launch: the s-th (expert, 64 rows of it) pair with rows, experts
 // ascending.  Every wave finds its own from the offsets: lane l counts the chunks of
 // experts l E/64 .., a prefix sum over the lanes finds the lane that holds slot s.
@@ -356,8 +357,9 @@ __global__ __launch_bounds__(256) void k_linear_skinny(const T* __restrict__ X,
                                                        const int* __restrict__ offsets, int E,
                                                        int M, int nslot, const T* __restrict__ W,
                                                        int K, LinearEpi<T> epi) {
-  constexpr int RB = 4 / KS, V = Vec16<T>::N, KC = 32 * V;
-  __shared__ f32x4 red[KS > 1 ? (KS - 1) * RB * NC * 64 : 1];
+  constexpr int RB = 4 / KS, V = Vec16<T>::N, KC = kSkinnyChunkBytes / sizeof(T);
+  static_assert(KC == 32 * V, "eight steps of four vectors");
+  __shared__ f32x4 red[(KS - 1) * RB * NC * 64];
   const int N = epi.N;
   const int nNb = (N + 16 * RB - 1) / (16 * RB);
   const int slot = uni(blockIdx.x / nNb), nb = uni(blockIdx.x % nNb);
@@ -399,7 +401,7 @@ __global__ __launch_bounds__(256) void k_linear_skinny(const T* __restrict__ X,
     for (int c = 0; c < NC; ++c)
       vx[c] = c * 16 + rl < rows ? (uint32_t)(((c * 16 + rl) * K + V * g) * (int)sizeof(T)) : kOobOffset;
     for (int kc = ks; kc * KC < K; kc += KS) {
-      const uint32_t soff = (uint32_t)kc * 512;
+      const uint32_t soff = (uint32_t)kc * kSkinnyChunkBytes;
       u32x4 wa[8];
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
@@ -421,20 +423,18 @@ __global__ __launch_bounds__(256) void k_linear_skinny(const T* __restrict__ X,
       }
     }
   }
-  if constexpr (KS > 1) {
-    if (ks > 0) {
+  if (ks > 0) {
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
-        if (c < nch) red[((ks - 1) * RB + rb) * NC * 64 + c * 64 + lane] = acc[c];
-    }
-    __syncthreads();
-    if (ks > 0) return;
-#pragma unroll
-    for (int q = 1; q < KS; ++q)
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-        if (c < nch) acc[c] += red[((q - 1) * RB + rb) * NC * 64 + c * 64 + lane];
+    for (int c = 0; c < NC; ++c)
+      if (c < nch) red[((ks - 1) * RB + rb) * NC * 64 + c * 64 + lane] = acc[c];
   }
+  __syncthreads();
+  if (ks > 0) return;
+#pragma unroll
+  for (int q = 1; q < KS; ++q)
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      if (c < nch) acc[c] += red[((q - 1) * RB + rb) * NC * 64 + c * 64 + lane];
   // lane holds row 16 c + 4 g + r, column n0 + rl
   if (rl >= nrows) return;
   const int n = n0 + rl;

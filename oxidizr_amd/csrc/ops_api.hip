@@ -267,11 +267,20 @@ moe_status check_linear(int dtype, int64_t M, int K, int N, int E, bool grouped,
 }
 
 // Whether a forward runs as the stream of its weights (k_linear_skinny): few rows to
-// an expert.  Rows are counted as evenly spread over the experts that can have any.
-constexpr int kSkinnyRowsPerGroup = 16;
-bool linear_skinny(int64_t M, int E, bool grouped) {
+// an expert (rows counted as evenly spread over the experts that can have any), or
+// somewhat more where the row tiles would leave half of the CUs idle. us, tiles / this,
+// at 1, 4, 8, 16 rows an expert: bf16 128 experts of 4096 x 1536 181 / 168, 267 / 258, 276 /
+// 302, 288 / 404; 64 of 1408 x 2048 43 / 40, 68 / 70, 73 / 81, 74 / 104; 8 of 1024 x 512 14 /
+// 4.4, 15 / 5.7, 15 / 5.7, 15 / 7.7; fp32 448 / 337, 756 / 537, 780 / 636, 809 / 802. One weight of
+// 4096 x 4096 at 1, 16, 32, 64 rows: 24 / 7.6, 24 / 10.6, 25 / 16, 27 / 26; 1408 x 7168 11 / 5.7, 10
+// / 8.3, 11 / 12, 13 / 19; fp32 81 / 18, 81 / 20, 82 / 29, 82 / 45 and 30 / 10, 30 / 14, 32 / 21, 32 / 33.
+template <typename D>
+bool linear_skinny(int64_t M, int N, int E, bool grouped) {
   const int64_t groups = grouped ? std::min<int64_t>(E, M) : 1;
-  return grouped ? M <= kSkinnyRowsPerGroup * groups : M <= kLinearSkinnyRows;
+  const bool idle = groups * ceil_div(N, 128) <= (grouped ? 128 : 32);
+  if (sizeof(D) == 4) return M <= (grouped ? 16 * groups : kLinearSkinnyRows);
+  if (grouped) return M <= (idle ? 16 : 4) * groups;
+  return M <= (idle ? kLinearSkinnyRows : 24);
 }
 
 // Row tilings of a product alone on the GPU, in tenths of a round of 256-row tiles (one
@@ -431,18 +440,24 @@ template <typename D>
 moe_status linear_forward(hipStream_t s, int64_t M, int K, int N, int E, const int* offsets,
                           const D* x, const D* w, const LinearEpi<D>& epi, char* ws) {
   const bool grouped = offsets != nullptr;
-  if (linear_skinny(M, E, grouped)) {
+  if (linear_skinny<D>(M, N, E, grouped)) {
     const int64_t nslot = grouped ? std::min<int64_t>(E, M) + M / kLinearSkinnyRows
                                   : ceil_div(M, kLinearSkinnyRows);
-    constexpr int KS = 2, RB = 4 / KS;
-    const int nNb = ceil_div(N, 16 * RB);
-    const unsigned grid = (unsigned)(nslot * nNb + (grouped ? 64 : 0));
-    auto go = [&](auto nc) {
-      hipLaunchKernelGGL((k_linear_skinny<D, decltype(nc)::value, KS>), dim3(grid), dim3(256), 0, s,
-                         x, offsets, E, (int)M, (int)nslot, w, K, epi);
+    auto go = [&](auto nc, auto ks) {
+      constexpr int KS = decltype(ks)::value;
+      const unsigned grid = (unsigned)(nslot * ceil_div(N, 64 / KS) + (grouped ? 64 : 0));
+      hipLaunchKernelGGL((k_linear_skinny<D, decltype(nc)::value, KS>), dim3(grid), dim3(256), 0,
+                         s, x, offsets, E, (int)M, (int)nslot, w, K, epi);
     };
-    if (M <= 16) go(std::integral_constant<int, 1>());
-    else go(std::integral_constant<int, 4>());
+    // four waves to a block of 16 weight rows, each with two k-chunks at least; two
+    // where K holds fewer (4096 x 4096, one row: 12.0 -> 7.6 us; 64 experts of 1408 x 2048,
+    // one row each, six chunks: 40 -> 46; eight waves: 7.5 and 60)
+    auto split = [&](auto nc) {
+      if (K >= 8 * kSkinnyChunkBytes / (int)sizeof(D)) go(nc, std::integral_constant<int, 4>());
+      else go(nc, std::integral_constant<int, 2>());
+    };
+    if (M <= 16) split(std::integral_constant<int, 1>());
+    else split(std::integral_constant<int, 4>());
     LAUNCH_CHECK();
     return MOE_OK;
   }
