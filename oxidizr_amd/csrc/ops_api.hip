@@ -501,7 +501,7 @@ moe_status linear_backward(hipStream_t s, int64_t M, int K, int N, int E, const 
   if (act != kActNone || db) {
     D* out = (D*)(ws + L.dz);
     float* part = db ? (float*)(ws + L.part) : nullptr;
-    hipLaunchKernelGGL(k_linear_dz<D>, dim3((unsigned)dz_chunks(M, E, grouped), ceil_div(N, 256)),
+    hipLaunchKernelGGL(k_linear_dz<D>, dim3((unsigned)dz_chunks(M, E, grouped), ceil_div(N, kDzCols)),
                        dim3(256), 0, s, dy, pre, act, chunks, N, out, part);
     if (act != kActNone) dz = out;
     if (db)
