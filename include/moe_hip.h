@@ -281,7 +281,7 @@ moe_status moe_plan_stage_times(moe_plan* plan, float* ms, int32_t* calls, int32
 /* Stable counting sort of the T k assignments by expert: expert ascending, then
  * t k + j ascending.  topk_idx [T, k]: int32 (index_bytes 4) or int64 (8); an index
  * outside [0, E) is an assignment without an expert (padding) and is sorted behind
- * every expert.  The same expert may occur several times in a token.  counts [E],
+ * every expert, in t k + j's order.  The same expert may occur several times in a token.  counts [E],
  * offsets [E + 1] (offsets[E] = assignments that have an expert), perm [T k]
  * (position -> t k + j), inv_perm [T k] (t k + j -> position).  1 <= E <= 1024, 1 <= k
  * <= 16, T k < 2^31.  The workspace may be NULL where
@@ -325,9 +325,10 @@ typedef enum {
  * NULL, y [M, N]; K = in_features and N = out_features are multiples of 8.  Rows behind
  * the last group's get y = residual (or 0).  offsets NULL: one weight [N, K] for every
  * row (num_groups 1).  pre_act [M, N] (or NULL) receives the pre-activation for a
- * backward.  Offsets that descend or leave [0, M] read as clamped to the running
- * maximum.  Refused with MOE_ERR_UNSUPPORTED: a weight matrix of 2^31 bytes, more than
- * 2^26 rows or operands of 2^34 bytes (2^31 in the backward). */
+ * backward.  Offsets ascend from 0 to at most M; with others no access leaves the
+ * tensors, but which rows a group has, and whether every row of y is written, is not
+ * defined.  Refused with MOE_ERR_UNSUPPORTED: a width above 2^20, a weight matrix of 2^31
+ * bytes, more than 2^26 rows, operands of 2^34 bytes (2^31 in the backward). */
 size_t moe_linear_workspace_bytes(int32_t dtype, int64_t num_rows, int32_t in_features,
                                   int32_t out_features, int32_t num_groups, int32_t grouped,
                                   int32_t activation, int32_t backward);

@@ -147,7 +147,9 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(
 // ------------------------------------------------------------------ rows to experts and back
 // inv_perm[t k + j] says which row of the sorted order holds assignment (t, j);
 // rows at or beyond *kept belong to no expert.  A position outside [0, T k) (no
-// sort makes one) counts as such and is not written.
+// sort makes one) counts as such, and neither it nor a *kept beyond T k makes a kernel
+// leave its buffers.
+MOE_DEV int kept_rows(const int* kept, int64_t N) { return (int)min((int64_t)*kept, N); }
 constexpr int kMaxPerTok = 16;
 
 // xp[inv[t, j]] = x[t], or zeros for an assignment without an expert.  One wave
@@ -167,7 +169,7 @@ __global__ __launch_bounds__(256) void k_permute(const T* __restrict__ x,
   const int c = (int)(wid - t * nsl) * 64 + lane;
   const bool in = c < nv;  // no early exit: lane j holds slot j's row
   const int64_t N = Tn * k;
-  const int rows = *kept;
+  const int rows = kept_rows(kept, N);
   const int at = lane < k ? inv[t * k + lane] : -1;
   const u32x4 v = in ? ld16(x + t * H + (int64_t)c * V) : u32x4{0, 0, 0, 0};
   for (int j = 0; j < k; ++j) {
@@ -197,7 +199,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void k
   const int64_t t = wid / nsl;
   const int lane = threadIdx.x & 63;
   const int c = (int)(wid - t * nsl) * 64 + lane;
-  const int rows = *kept;
+  const int rows = kept_rows(kept, Tn * k);
   const int at = lane < k ? inv[t * k + lane] : -1;
   const float wt = lane < k ? (w ? w[t * k + lane] : 1.0f) : 0.0f;
   const bool in = c < nv;  // no early exit: lane j holds slot j's row and weight
@@ -239,7 +241,7 @@ __global__ __launch_bounds__(256) void k_unpermute_bwd(
   const int64_t t = (int64_t)blockIdx.x * TPB + wave / WPT, N = Tn * k;
   const bool live = t < Tn;
   const int nv = H / V;
-  const int rows = *kept;
+  const int rows = kept_rows(kept, Tn * k);
   const int at = live && lane < k ? inv[t * k + lane] : -1;
   const float wt = live && lane < k ? (w ? w[t * k + lane] : 1.0f) : 0.0f;
   float dot[KMAX];

@@ -54,11 +54,12 @@ moe_status check_ints(std::initializer_list<const void*> needed, size_t bytes = 
   return MOE_OK;
 }
 
-// Blocks of a launch of `waves` waves, four to a block; 0 when the grid would not
-// hold them.
-unsigned wave_grid(int64_t waves) {
-  const int64_t g = (waves + 3) / 4;
-  return g <= INT32_MAX ? (unsigned)g : 0u;
+// Whether a launch of `blocks` workgroups of `threads` fits a grid, which holds fewer
+// than 2^32 threads.
+moe_status check_grid(int64_t blocks, int threads) {
+  if (blocks * threads >= int64_t(1) << 32)
+    return fail(MOE_ERR_UNSUPPORTED, "too many rows for one launch: split the batch");
+  return MOE_OK;
 }
 
 // ---- sort by expert
@@ -121,9 +122,10 @@ void with_k(int k, F&& f) {
 template <typename D>
 moe_status launch_permute(hipStream_t s, int64_t T, int k, int H, const int* inv, const int* kept,
                           const D* x, D* xp) {
-  const unsigned grid = wave_grid(T * ceil_div(H, 64 * Vec16<D>::N));
-  if (!grid) return fail(MOE_ERR_UNSUPPORTED, "too many tokens for one launch");
-  hipLaunchKernelGGL(k_permute<D>, dim3(grid), dim3(256), 0, s, x, inv, kept, T, k, H, xp);
+  const int64_t grid = (T * ceil_div(H, 64 * Vec16<D>::N) + 3) / 4;
+  moe_status st = check_grid(grid, 256);
+  if (st != MOE_OK) return st;
+  hipLaunchKernelGGL(k_permute<D>, dim3((unsigned)grid), dim3(256), 0, s, x, inv, kept, T, k, H, xp);
   LAUNCH_CHECK();
   return MOE_OK;
 }
@@ -131,16 +133,17 @@ moe_status launch_permute(hipStream_t s, int64_t T, int k, int H, const int* inv
 template <typename D>
 moe_status launch_unpermute(hipStream_t s, int64_t T, int k, int H, const int* inv,
                             const int* kept, const D* y, const float* w, D* out) {
-  const unsigned grid = wave_grid(T * ceil_div(H, 64 * Vec16<D>::N));
-  if (!grid) return fail(MOE_ERR_UNSUPPORTED, "too many tokens for one launch");
+  const int64_t grid = (T * ceil_div(H, 64 * Vec16<D>::N) + 3) / 4;
+  moe_status st = check_grid(grid, 256);
+  if (st != MOE_OK) return st;
   const bool stream = T * k * H * (int64_t)sizeof(D) > kStreamBytes;
   with_k(k, [&](auto kc) {
     constexpr int KM = decltype(kc)::value;
     if (stream)
-      hipLaunchKernelGGL((k_unpermute<D, KM, true>), dim3(grid), dim3(256), 0, s, y, inv, kept, w, T,
+      hipLaunchKernelGGL((k_unpermute<D, KM, true>), dim3((unsigned)grid), dim3(256), 0, s, y, inv, kept, w, T,
                          k, H, out);
     else
-      hipLaunchKernelGGL((k_unpermute<D, KM, false>), dim3(grid), dim3(256), 0, s, y, inv, kept, w, T,
+      hipLaunchKernelGGL((k_unpermute<D, KM, false>), dim3((unsigned)grid), dim3(256), 0, s, y, inv, kept, w, T,
                          k, H, out);
   });
   LAUNCH_CHECK();
@@ -152,6 +155,8 @@ moe_status launch_unpermute_bwd(hipStream_t s, int64_t T, int k, int H, const in
                                 const int* kept, const D* dout, const D* y, const float* w, D* dy,
                                 float* dw) {
   const int slices = ceil_div(H, 64 * Vec16<D>::N);
+  moe_status st = check_grid(T, 256);  // one token to a block at most
+  if (st != MOE_OK) return st;
   with_k(k, [&](auto kc) {
     constexpr int KM = decltype(kc)::value;
     auto go = [&](auto wpt) {
@@ -179,6 +184,7 @@ moe_status check_norm(int dtype, int64_t T, int H, int gate_kind, bool y, bool p
     return fail(MOE_ERR_UNSUPPORTED, "hidden %d is above %d", H, kNormMaxHidden);
   if (gate_kind < kGateNone || gate_kind > kGateFull)
     return fail(MOE_ERR_INVALID, "unknown gate kind %d", gate_kind);
+  if (T == 0) return MOE_OK;  // no rows: their tensors may have no address
   if ((gate_kind != kGateNone) != gate)
     return fail(MOE_ERR_INVALID, "gate and gate_kind do not go together");
   if (!y && (post || gate))
@@ -220,6 +226,8 @@ int norm_bwd_blocks(int64_t T, int H) {
 
 template <typename D>
 moe_status launch_norm_fwd(hipStream_t s, const NormArgs<D>& a) {
+  moe_status st = check_grid(a.Tn, a.H <= 2048 ? 256 : a.H <= 8192 ? 512 : 1024);
+  if (st != MOE_OK) return st;
   with_norm_shape<false>(a.H, [&](auto wpr, auto nch) {
     constexpr int W = decltype(wpr)::value;
     const int64_t grid = (a.Tn + norm_rows(W) - 1) / norm_rows(W);
@@ -247,6 +255,7 @@ moe_status launch_norm_bwd(hipStream_t s, const NormBwdArgs<D>& a, D* dw2, D* dg
 }
 
 // ---- expert products
+constexpr int kLinearMaxWidth = 1 << 20;
 moe_status check_linear(int dtype, int64_t M, int K, int N, int E, bool grouped, int act) {
   moe_status st = check_dtype(dtype);
   if (st != MOE_OK) return st;
@@ -258,6 +267,9 @@ moe_status check_linear(int dtype, int64_t M, int K, int N, int E, bool grouped,
     return fail(MOE_ERR_INVALID, grouped ? "num_groups %d is outside 1..1024"
                                          : "num_groups %d without offsets is not 1", E);
   if (act < 0 || act >= kNumActs) return fail(MOE_ERR_INVALID, "unknown activation %d", act);
+  if (K > kLinearMaxWidth || N > kLinearMaxWidth)
+    return fail(MOE_ERR_UNSUPPORTED, "in_features %d or out_features %d is above %d", K, N,
+                kLinearMaxWidth);
   const int64_t b = elt_size(dtype);
   if ((int64_t)K * N * b >= kMaxExtentBytes)
     return fail(MOE_ERR_UNSUPPORTED, "a weight matrix reaches 2^31 bytes");
@@ -744,20 +756,20 @@ moe_status moe_residual_norm_backward(int32_t device, void* stream, int32_t dtyp
                                 rstd_post, rstd_next, d_h, d_y, d_post_weight, d_gate,
                                 d_next_weight, workspace})) != MOE_OK)
     return st;
-  if ((post_weight && !d_post_weight) || (gate && !d_gate) || (next_weight && !d_next_weight))
-    return fail(MOE_ERR_INVALID, "a required pointer is NULL");
   const size_t b = elt_size(dtype);
   DeviceScope dev(device);
-  HIP_TRY(dev.enter());
   hipStream_t s = (hipStream_t)stream;
   if (T == 0) {  // sums over no row
+    HIP_TRY(dev.enter());
     if ((st = zero_async(s, d_post_weight, H * b)) != MOE_OK) return st;
     if ((st = zero_async(s, gate_kind == kGateChannel ? d_gate : nullptr, H * b)) != MOE_OK) return st;
     return zero_async(s, d_next_weight, H * b);
   }
-  if (!d_h || (y && !d_y) || !workspace || (post_weight && !rstd_post) ||
+  if (!d_h || (y && !d_y) || !workspace || (post_weight && (!d_post_weight || !rstd_post)) ||
+      (gate && !d_gate) || (next_weight && !d_next_weight) ||
       (next_weight && (!rstd_next || !h_out || !d_n_out)) || (!next_weight && !d_h_out))
     return fail(MOE_ERR_INVALID, "a required pointer is NULL");
+  HIP_TRY(dev.enter());
   const bool chan = gate_kind == kGateChannel;
   auto go = [&](auto d) {
     using D = decltype(d);

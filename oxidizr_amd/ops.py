@@ -281,9 +281,9 @@ class _ExpertLinear(torch.autograd.Function):
 def expert_linear(x, weight, bias=None, *, offsets=None, activation: str = "none", residual=None):
     """activation(x W^T + bias) + residual, [M, N].
 
-    With offsets (int32 [E + 1], as sort_tokens gives them) rows offsets[e] .. offsets[e + 1] of x [M, K]
-    take weight[e] of weight [E, N, K] and bias[e] of bias [E, N]; rows behind the last expert's are the
-    residual's, or zeros. Without offsets weight is [N, K] and bias [N]. K and N are multiples of 8.
+    With offsets (int32 [E + 1], ascending from 0, as sort_tokens gives them) rows offsets[e] ..
+    offsets[e + 1] of x [M, K] take weight[e] of weight [E, N, K] and bias[e] of bias [E, N]; rows behind
+    the last expert's are the residual's, or zeros. Without offsets weight is [N, K] and bias [N]. K and N are multiples of 8.
     activation: one of ACTIVATIONS ("gelu" with the error function, "gelu_tanh" approximated)."""
     if activation not in ACTIVATIONS:
         raise ModelError(f"activation must be one of {ACTIVATIONS}, got {activation!r}")

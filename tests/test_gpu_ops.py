@@ -139,6 +139,24 @@ def test_unpermute_and_its_gradients(T, H, E, k, pad, weighted, dtype):
         ref.assert_close(got[1], prod.sum(2), (H + 8) * ref.U32 * prod.abs().sum(2), "dw")
 
 
+def test_an_order_that_no_sort_made_stays_inside_the_buffers():
+    # positions and a count of kept rows beyond T k
+    g = gen(2)
+    good = ops.sort_tokens(routing(g, 40, 3, 8), 8)
+    inv = good.inv_perm.clone()
+    inv[3, 1], inv[4, 2] = 10 ** 9, -5
+    offsets = good.offsets.clone()
+    offsets[-1] = 2 ** 31 - 1
+    bad = ops.TokenOrder(good.counts, offsets, good.perm, inv)
+    x, y = normal(g, 40, 64).requires_grad_(), normal(g, 120, 64).requires_grad_()
+    w = torch.rand(40, 3, device="cuda", generator=g).requires_grad_()
+    out = ops.unpermute_tokens(y, bad, w)
+    rows = torch.where(((inv >= 0) & (inv < 120))[..., None], y.detach()[inv.long().clamp(0, 119)], 0.0)
+    assert torch.allclose(out, (w[..., None] * rows).sum(1), atol=1e-5)
+    torch.autograd.grad(out, [y, w], torch.ones_like(out))
+    torch.autograd.grad(ops.permute_tokens(x, bad), x, torch.ones(120, 64, device="cuda"))
+
+
 def test_gradient_of_the_rows_alone():
     # weights that need no gradient: the rows are not kept
     g = gen(5)
@@ -359,6 +377,24 @@ def test_residual_norm_when_one_output_has_no_gradient():
         want = torch.autograd.grad((h, n), leaves, full, retain_graph=True)
         for a, b in zip(got, want):
             assert torch.allclose(a if a is not None else torch.zeros_like(b), b, rtol=1e-6, atol=1e-6)
+
+
+def test_norms_without_rows():
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    gate = torch.ones(64, device="cuda", requires_grad=True)
+    h = torch.zeros(0, 64, device="cuda", requires_grad=True)
+    out, n = ops.residual_norm(h, h, w, gate=gate, next_weight=w)
+    assert out.shape == n.shape == (0, 64)
+    for t in torch.autograd.grad((out, n), [h, w, gate], (torch.zeros_like(out), torch.zeros_like(n))):
+        assert not bool(t.any())
+
+
+def test_a_second_derivative_is_refused():
+    x = torch.ones(4, 64, device="cuda", requires_grad=True)
+    n = ops.rms_norm(x, torch.ones(64, device="cuda"))
+    dx, = torch.autograd.grad(n.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
 
 
 def test_rows_of_zeros_and_large_values():

@@ -130,6 +130,7 @@ def test_c_entries_refuse_before_any_device_call():
         assert status(fn(off=None), "num_groups") == 1  # three groups without offsets
         assert status(fn(act=5), "activation") == 1
         assert status(fn(K=2 ** 15, N=2 ** 15), "weight matrix") == 4
+        assert status(fn(K=8, N=2 ** 20 + 8), "above 1048576") == 4
         assert status(fn(M=2 ** 27), "rows") == 4
         assert status(fn(ws=P + 8), "16-byte") == 1
     assert status(bwd(M=2 ** 21, K=1024, dtype=BF16), "2^31") == 4
