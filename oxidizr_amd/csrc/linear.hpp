@@ -216,7 +216,11 @@ MOE_DEV void add_bias(f32x16 (&acc)[1][C::TN][C::TM], f32x16 (&xacc)[1][C::XTN],
   }
 }
 
-// y tile by tile.  The residual of the whole tile is requested when the main loop has
+// y tile by tile.  Bound by the matrix cores and, one 256-row tile to a CU, by its
+// epilogue, which nothing overlaps: 8192 x 2048, K = 2816 with bias and residual 85-90 us
+// (1050-1110 TFLOP/s; the library's product alone 69), of which the k-loop is some 70;
+// 16 experts of 1024 rows, 1408 x 2048, silu, two outputs, 128-row tiles 115-125 us.
+// The residual of the whole tile is requested when the main loop has
 // ended (in the fragments' registers; a 384-row tile has none left and takes it a pass
 // ahead).
 template <typename T, class C>
@@ -296,7 +300,8 @@ __global__ __launch_bounds__(C::THREADS) void k_linear_dgrad(const T* __restrict
 // Both products of a backward in one launch: the wblocks (a multiple of 8) weight
 // gradient tiles, then the input gradient's.  One workgroup fills a CU, so a launch of
 // its own ends with a partial round; here the second product's tiles start as the
-// first's end, and one partial round is left.
+// first's end, and one partial round is left: 16 experts of 1024 rows, 1408 x 2048, 248 ->
+// 209 us; 8192 rows of 2816 x 2048 205 -> 161-181.
 template <typename T, class C, bool GROUPED>
 __global__ __launch_bounds__(C::THREADS) void k_linear_bwd(const T* __restrict__ dZ,
                                                            const T* __restrict__ X,
@@ -324,7 +329,8 @@ __global__ __launch_bounds__(C::THREADS) void k_linear_bwd(const T* __restrict__
 // from memory: lane l supplies 16-byte vector l / 16 + 4 q of weight row l % 16 and
 // of token row l % 16 in step q, so four lanes read 64 contiguous bytes.  KS waves of
 // a workgroup share a block of 16 weight rows and take every KS-th k-chunk of 8
-// steps; their sums are added through LDS in wave order.
+// steps; their sums are added through LDS in wave order.  Bound by the weights: 128
+// experts of 4096 x 1536 bf16, 512 rows (1.61 GB) 231-240 us, 6.7-7.0 TB/s.
 constexpr int kLinearSkinnyRows = 64;  // rows of an expert that one workgroup takes
 constexpr int kSkinnyChunkBytes = 512;  // of a weight row, in one k-chunk
 // Slot s of a launch: the s-th (expert, 64 rows of it) pair with rows, experts
@@ -477,7 +483,7 @@ __global__ __launch_bounds__(256) void k_linear_skinny(const T* __restrict__ X,
 // the column sums of dz for the bias gradient, from the unrounded products.  Block
 // (chunk, 64 columns): thread (r, c) takes rows r and r + 32 of 8 columns, so that a
 // few rows fill the CUs as well; the 32 row lanes are added in order.  Bound by its
-// reads and writes (16384 x 1408 bf16: DZ_US).
+// reads and writes (16384 x 1408 bf16, 138 MB: 26 us, 5.2 TB/s).
 constexpr int kDzRows = kF32RowTile;  // rows of a chunk: the prefix of 64-row tiles counts them
 constexpr int kDzCols = 64;
 template <typename T>
