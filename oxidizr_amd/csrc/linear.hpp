@@ -33,7 +33,7 @@ MOE_DEV float normal_cdf(float z, float& e) {
 }
 MOE_DEV float act_value(float z, int act) {
   switch (act) {
-    case kActRelu: return z > 0.0f ? z : 0.0f;
+    case kActRelu: return z <= 0.0f ? 0.0f : z;  // a NaN stays one
     case kActSilu: return z * logistic(z);
     case kActGelu: {
       float e;
@@ -45,7 +45,7 @@ MOE_DEV float act_value(float z, int act) {
 }
 MOE_DEV float act_slope(float z, int act) {
   switch (act) {
-    case kActRelu: return z > 0.0f ? 1.0f : 0.0f;
+    case kActRelu: return z <= 0.0f ? 0.0f : 1.0f;
     case kActSilu: {
       const float s = logistic(z);
       return s * (1.0f + z * (1.0f - s));
@@ -57,7 +57,9 @@ MOE_DEV float act_slope(float z, int act) {
     }
     case kActGeluTanh: {
       const float s = logistic(2.0f * kGeluC * (z + 0.044715f * z * z * z));
-      return s + 2.0f * z * s * (1.0f - s) * kGeluC * (1.0f + 3.0f * 0.044715f * z * z);
+      // s (1 - s) is 0 from |z| = 10 on: squares beyond 1e6 would only make 0 inf a NaN
+      const float zz = fminf(z * z, 1e6f);
+      return s + s * (1.0f - s) * z * (2.0f * kGeluC * (1.0f + 3.0f * 0.044715f * zz));
     }
     default: return 1.0f;
   }

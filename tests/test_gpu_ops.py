@@ -259,6 +259,34 @@ def test_dense_linear_over_the_tilings(M, K, N):
     linear_case(gen(M), [M], K, N, "gelu_tanh", torch.bfloat16, bias=True, res=True, grouped=False)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ops.ACTIVATIONS)
+@pytest.mark.parametrize("M", [1, 200])
+def test_activations_far_from_zero(M, act, dtype):
+    # from |z| = 30 on value and slope are z and 1, or within 1e-10 of 0, up to the type's range
+    lim = torch.finfo(dtype).max
+    v = [30.0, 100.0, 1e4, 1e13, 1e20, lim]
+    z = torch.tensor(v + [-a for a in v] + [float("inf"), float("nan"), 0.0, -0.0], dtype=dtype, device="cuda")
+    x = torch.zeros(M, 64, dtype=dtype, device="cuda")
+    w = torch.zeros(16, 64, dtype=dtype, device="cuda")
+    b = z.clone().requires_grad_()
+    y = ops.expert_linear(x, w, b, activation=act)
+    dy = torch.zeros_like(y)
+    dy[0] = 1.0
+    db, = torch.autograd.grad(y, b, dy)
+    keep = act == "none"
+    z64 = z[:12].double()
+    value = z64 if keep else z64.clamp(min=0)
+    slope = torch.ones_like(z64) if keep else (z64 > 0).double()
+    tol = ref.u(dtype) + 2.0 ** -20
+    for r in (0, M - 1):
+        err = (y[r, :12].detach().double() - value).abs()
+        assert bool((err <= tol * value.abs() + 1e-10).all()), err
+    assert bool(((db[:12].double() - slope).abs() <= tol * slope + 1e-10).all()), db
+    assert bool((y[:, 12] == float("inf")).all()) and bool(y[:, 13].isnan().all())
+    assert bool((y[:, 14:] == 0).all())
+
+
 def test_linear_gradients_one_at_a_time():
     g = gen(4)
     x, w, b = normal(g, 100, 64), normal(g, 3, 40, 64, std=0.1), normal(g, 3, 40)
