@@ -322,10 +322,11 @@ typedef enum {
 
 /* y[r] = act(x[r] W_g^T + b_g) + residual[r] for the rows offsets[g] <= r < offsets[g + 1]
  * of each group g.  x [M, K], weight [G, N, K], bias [G, N] or NULL, residual [M, N] or
- * NULL, y [M, N]; K = in_features and N = out_features are multiples of 8.  Rows behind
- * the last group's get y = residual (or 0).  offsets NULL: one weight [N, K] for every
+ * NULL, y [M, N]; K = in_features and N = out_features are multiples of 8.  Rows before
+ * the first group's and behind the last one's get y = residual (or 0).  offsets NULL: one weight [N, K] for every
  * row (num_groups 1).  pre_act [M, N] (or NULL) receives the pre-activation for a
- * backward.  Offsets ascend from 0 to at most M; with others no access leaves the
+ * backward.  Offsets ascend within 0..M (a range of a longer array will do, for
+ * a range of its groups); with others no access leaves the
  * tensors, but which rows a group has, and whether every row of y is written, is not
  * defined.  Refused with MOE_ERR_UNSUPPORTED: a width above 2^20, a weight matrix of 2^31
  * bytes, more than 2^26 rows, operands of 2^34 bytes (2^31 in the backward). */
@@ -337,7 +338,7 @@ moe_status moe_linear_forward(int32_t device, void* stream, int32_t dtype, int64
                               const int32_t* offsets, const void* x, const void* weight,
                               const void* bias, const void* residual, int32_t activation, void* y,
                               void* pre_act, void* workspace);
-/* dx [M, K] (0 behind the last group's rows), d_weight [G, N, K] and d_bias [G, N] (0 for a
+/* dx [M, K] (0 for rows of no group), d_weight [G, N, K] and d_bias [G, N] (0 for a
  * group without rows), each written unless NULL.  The residual's gradient is d_y. */
 moe_status moe_linear_backward(int32_t device, void* stream, int32_t dtype, int64_t num_rows,
                                int32_t in_features, int32_t out_features, int32_t num_groups,

@@ -3,8 +3,8 @@
 // weight for all rows.
 //   z[r] = x[r] W_e^T + b_e,  y[r] = act(z[r]) + res[r]   for r in expert e's rows,
 //   dz = dy act'(z),  dx = dz W_e,  dW_e = dz^T x,  db_e = sum_r dz[r],  dres = dy.
-// W_e is [N, K] row-major (out, in).  Rows behind the last expert's have y = res (or
-// 0), dx = 0 and no part in dW and db.  The GEMM main loop is gemm.hpp's.
+// W_e is [N, K] row-major (out, in).  Rows of no expert (before the first one's or
+// behind the last one's) have y = res (or 0), dx = 0 and no part in dW and db.  The GEMM main loop is gemm.hpp's.
 #pragma once
 #include "kernels.hpp"
 
@@ -123,8 +123,8 @@ MOE_DEV void linear_store8(const LinearEpi<T>& e, int64_t r, int n, const float 
 // Before the tiled launches of a grouped call.  Block 0: a clean copy of the offsets
 // (clamped to [0, M] and made ascending, so that no offsets make a launch leave its
 // buffers), the tile prefixes, and the experts' weight (and weight gradient)
-// addresses.  The blocks after it: rows behind the last expert's, which are out =
-// res (or zeros), `cols` wide, and out2 = 0; and zeros for the weight gradient of an
+// addresses.  The blocks after it: rows of no expert, which are out = res (or
+// zeros), `cols` wide, and out2 = 0; and zeros for the weight gradient of an
 // expert without rows.
 template <typename T>
 __global__ __launch_bounds__(1024) void k_linear_prep(const int* __restrict__ offsets, int E, int M,
@@ -157,9 +157,12 @@ __global__ __launch_bounds__(1024) void k_linear_prep(const int* __restrict__ of
     const int64_t first = (int64_t)(blockIdx.x - 1) * 1024 + tid;
     const int64_t step = (int64_t)(gridDim.x - 1) * 1024;
     const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    const int64_t v0 = (int64_t)offs[E - 1] * cols / 8, v1 = (int64_t)M * cols / 8;
+    // vectors [0, head) and [tail, M cols / 8)
+    const int64_t head = (int64_t)o0 * cols / 8, tail = (int64_t)offs[E - 1] * cols / 8;
+    const int64_t none = head + (int64_t)M * cols / 8 - tail;
     if (out)
-      for (int64_t i = v0 + first; i < v1; i += step) {
+      for (int64_t j = first; j < none; j += step) {
+        const int64_t i = j < head ? j : j - head + tail;
         float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         if (res) load8(res + i * 8, f);
         store8(out + i * 8, f);
@@ -175,7 +178,7 @@ __global__ __launch_bounds__(1024) void k_linear_prep(const int* __restrict__ of
     w_tab[tid] = w + tid * stride;
     if (dw) dw_tab[tid] = dw + tid * stride;
   }
-  // the scan writes offsets from zero; rows before the first offset are none's
+  // the scan writes offsets from zero; rows before the first offset are no expert's
   scan_counts(cnt, E, offs_out, prefixes, offs, wsum);
   if (tid < E) offs_out[tid] += o0;
   if (tid == 1023) offs_out[E] += o0;  // the thread that wrote it
@@ -375,8 +378,8 @@ MOE_DEV bool skinny_slot(const int* __restrict__ offsets, int E, int M, int s, i
 }
 
 // NC: chunks of 16 rows (1 for calls of at most 16 rows, else 4).  Blocks below
-// nslot x nNb are (slot, row blocks) pairs; the others write the rows behind the
-// last expert's.  offsets null: one weight, rows s 64 .. .
+// nslot x nNb are (slot, row blocks) pairs; the others write the rows of no
+// expert.  offsets null: one weight, rows s 64 .. .
 template <typename T, int NC, int KS>
 __global__ __launch_bounds__(256) void k_linear_skinny(const T* __restrict__ X,
                                                        const int* __restrict__ offsets, int E,
@@ -392,10 +395,12 @@ __global__ __launch_bounds__(256) void k_linear_skinny(const T* __restrict__ X,
     int m = 0;
     for (int e = threadIdx.x & 63; e <= E; e += 64) m = max(m, offsets[e]);
     m = min(wave_max(m), M);
-    const int64_t v0 = (int64_t)m * N / 8, v1 = (int64_t)M * N / 8;
+    const int64_t head = (int64_t)min(max(offsets[0], 0), M) * N / 8, tail = (int64_t)m * N / 8;
+    const int64_t none = head + (int64_t)M * N / 8 - tail;
     const int64_t step = ((int64_t)gridDim.x - (int64_t)nslot * nNb) * 256;
-    for (int64_t v = v0 + ((int64_t)blockIdx.x - (int64_t)nslot * nNb) * 256 + threadIdx.x; v < v1;
-         v += step) {
+    for (int64_t j = ((int64_t)blockIdx.x - (int64_t)nslot * nNb) * 256 + threadIdx.x; j < none;
+         j += step) {
+      const int64_t v = j < head ? j : j - head + tail;
       float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
       const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
       if (epi.res) load8(epi.res + v * 8, f);

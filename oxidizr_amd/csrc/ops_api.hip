@@ -54,10 +54,10 @@ moe_status check_ints(std::initializer_list<const void*> needed, size_t bytes = 
   return MOE_OK;
 }
 
-// Whether a launch of `blocks` workgroups of `threads` fits a grid, which holds fewer
-// than 2^32 threads.
+// Whether a launch of `blocks` workgroups of `threads` fits a grid.
+constexpr int64_t kMaxGridThreads = int64_t(1) << 32;
 moe_status check_grid(int64_t blocks, int threads) {
-  if (blocks * threads >= int64_t(1) << 32)
+  if (blocks * threads >= kMaxGridThreads)
     return fail(MOE_ERR_UNSUPPORTED, "too many rows for one launch: split the batch");
   return MOE_OK;
 }
@@ -278,6 +278,20 @@ moe_status check_linear(int dtype, int64_t M, int K, int N, int E, bool grouped,
   return MOE_OK;
 }
 
+// Waves of k_linear_skinny to a block of 16 weight rows: four with two k-chunks each at
+// least, two where K holds fewer (4096 x 4096, one row: 12.0 -> 7.6 us; 64 experts of 1408 x
+// 2048, one row each, six chunks: 40 -> 46; eight waves: 7.5 and 60).
+template <typename D>
+int skinny_split(int K) {
+  return K >= 8 * kSkinnyChunkBytes / (int)sizeof(D) ? 4 : 2;
+}
+int64_t skinny_slots(int64_t M, int E, bool grouped) {
+  return grouped ? std::min<int64_t>(E, M) + M / kLinearSkinnyRows : ceil_div(M, kLinearSkinnyRows);
+}
+int64_t skinny_blocks(int64_t M, int N, int E, bool grouped, int split) {
+  return skinny_slots(M, E, grouped) * ceil_div(N, 64 / split) + (grouped ? 64 : 0);
+}
+
 // Whether a forward runs as the stream of its weights (k_linear_skinny): few rows to
 // an expert (rows counted as evenly spread over the experts that can have any), or
 // somewhat more where the row tiles would leave half of the CUs idle. us, tiles / this,
@@ -287,8 +301,10 @@ moe_status check_linear(int dtype, int64_t M, int K, int N, int E, bool grouped,
 // 4096 x 4096 at 1, 16, 32, 64 rows: 24 / 7.6, 24 / 10.6, 25 / 16, 27 / 26; 1408 x 7168 11 / 5.7, 10
 // / 8.3, 11 / 12, 13 / 19; fp32 81 / 18, 81 / 20, 82 / 29, 82 / 45 and 30 / 10, 30 / 14, 32 / 21, 32 / 33.
 template <typename D>
-bool linear_skinny(int64_t M, int N, int E, bool grouped) {
+bool linear_skinny(int64_t M, int K, int N, int E, bool grouped) {
   const int64_t groups = grouped ? std::min<int64_t>(E, M) : 1;
+  // a thousand experts a million columns wide are more workgroups than a launch holds
+  if (skinny_blocks(M, N, E, grouped, skinny_split<D>(K)) * 256 >= kMaxGridThreads) return false;
   const bool idle = groups * ceil_div(N, 128) <= (grouped ? 128 : 32);
   if (sizeof(D) == 4) return M <= (grouped ? 16 * groups : kLinearSkinnyRows);
   if (grouped) return M <= (idle ? 16 : 4) * groups;
@@ -444,28 +460,23 @@ LinearWs linear_ws(int dtype, int64_t M, int K, int N, int E, bool grouped, int 
   return w;
 }
 
-// Blocks of k_linear_prep: one for the prefixes, the others for the rows behind the
-// last expert's.
+// Blocks of k_linear_prep: one for the prefixes, the others for the rows of no expert.
 constexpr int kPrepBlocks = 1 + 128;
 
 template <typename D>
 moe_status linear_forward(hipStream_t s, int64_t M, int K, int N, int E, const int* offsets,
                           const D* x, const D* w, const LinearEpi<D>& epi, char* ws) {
   const bool grouped = offsets != nullptr;
-  if (linear_skinny<D>(M, N, E, grouped)) {
-    const int64_t nslot = grouped ? std::min<int64_t>(E, M) + M / kLinearSkinnyRows
-                                  : ceil_div(M, kLinearSkinnyRows);
+  if (linear_skinny<D>(M, K, N, E, grouped)) {
+    const int64_t nslot = skinny_slots(M, E, grouped);
     auto go = [&](auto nc, auto ks) {
       constexpr int KS = decltype(ks)::value;
-      const unsigned grid = (unsigned)(nslot * ceil_div(N, 64 / KS) + (grouped ? 64 : 0));
+      const unsigned grid = (unsigned)skinny_blocks(M, N, E, grouped, KS);
       hipLaunchKernelGGL((k_linear_skinny<D, decltype(nc)::value, KS>), dim3(grid), dim3(256), 0,
                          s, x, offsets, E, (int)M, (int)nslot, w, K, epi);
     };
-    // four waves to a block of 16 weight rows, each with two k-chunks at least; two
-    // where K holds fewer (4096 x 4096, one row: 12.0 -> 7.6 us; 64 experts of 1408 x 2048,
-    // one row each, six chunks: 40 -> 46; eight waves: 7.5 and 60)
     auto split = [&](auto nc) {
-      if (K >= 8 * kSkinnyChunkBytes / (int)sizeof(D)) go(nc, std::integral_constant<int, 4>());
+      if (skinny_split<D>(K) == 4) go(nc, std::integral_constant<int, 4>());
       else go(nc, std::integral_constant<int, 2>());
     };
     if (M <= 16) split(std::integral_constant<int, 1>());

@@ -119,13 +119,11 @@ def _check_hidden(H):
 
 
 class _Slots:
-    """What the row kernels read of a TokenOrder."""
+    """What the row kernels read of a TokenOrder. A backward makes its own from the tensors that its
+    forward saved, so that autograd sees whether they were written to in between."""
     __slots__ = ("inv", "offsets", "T", "k", "kept")
 
-    def __init__(self, order):
-        if not isinstance(order, TokenOrder):
-            raise ModelError("order must be a TokenOrder (sort_tokens)")
-        offsets, inv = order.offsets, order.inv_perm
+    def __init__(self, offsets, inv):
         if inv.dim() != 2:
             raise ModelError("order.inv_perm must be [T, k]")
         if inv.dtype != torch.int32 or offsets.dtype != torch.int32:
@@ -138,6 +136,12 @@ class _Slots:
             raise ModelError("order.offsets must be [E + 1]")
         self.inv, self.offsets = inv.contiguous(), offsets.contiguous()
         self.kept = self.offsets.data_ptr() + 4 * E
+
+
+def _slots(order):
+    if not isinstance(order, TokenOrder):
+        raise ModelError("order must be a TokenOrder (sort_tokens)")
+    return _Slots(order.offsets, order.inv_perm)
 
 
 def _permute(x, slots):
@@ -159,19 +163,19 @@ def _unpermute(y, slots, weights):
 class _Permute(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, slots):
-        ctx.slots = slots
+        ctx.save_for_backward(slots.offsets, slots.inv)
         return _permute(_ready(x), slots)
 
     @staticmethod
     @_once
     def backward(ctx, dxp):
-        return _unpermute(_ready(dxp), ctx.slots, None), None
+        return _unpermute(_ready(dxp), _Slots(*ctx.saved_tensors), None), None
 
 
 def permute_tokens(x, order: TokenOrder):
     """Rows of x [T, H] in the order's positions: out[inv_perm[t, j]] = x[t] [T k, H]; the rows behind
     the last expert's (assignments without one) are zeros."""
-    slots = _Slots(order)
+    slots = _slots(order)
     if x.dim() != 2 or x.shape[0] != slots.T:
         raise ModelError(f"x must be [{slots.T}, H], got {list(x.shape)}")
     _check_hidden(x.shape[1])
@@ -189,15 +193,14 @@ class _Unpermute(torch.autograd.Function):
         weights = _ready(weights)
         need_dw = weights is not None and ctx.needs_input_grad[1]
         # the rows are read again only for the gradient of the weights
-        ctx.save_for_backward(y if need_dw else None, weights)
-        ctx.slots = slots
+        ctx.save_for_backward(y if need_dw else None, weights, slots.offsets, slots.inv)
         return _unpermute(y, slots, weights)
 
     @staticmethod
     @_once
     def backward(ctx, dout):
-        y, weights = ctx.saved_tensors
-        slots, dout = ctx.slots, _ready(dout)
+        y, weights, offsets, inv = ctx.saved_tensors
+        slots, dout = _Slots(offsets, inv), _ready(dout)
         dy = dout.new_empty(slots.T * slots.k, dout.shape[1])
         dw = torch.empty_like(weights) if y is not None else None
         _call(_lib.load().moe_unpermute_backward, dout.get_device(), _dtype_code(dout.dtype), slots.T,
@@ -209,7 +212,7 @@ class _Unpermute(torch.autograd.Function):
 def unpermute_tokens(y, order: TokenOrder, weights: Optional[torch.Tensor] = None):
     """out[t] = sum_j weights[t, j] * y[inv_perm[t, j]] [T, H] over the assignments that have an expert,
     j ascending; weights [T, k] float32, or None for a plain sum."""
-    slots = _Slots(order)
+    slots = _slots(order)
     T, k = slots.T, slots.k
     if y.dim() != 2 or y.shape[0] != T * k:
         raise ModelError(f"y must be [{T * k}, H], got {list(y.shape)}")
@@ -281,9 +284,11 @@ class _ExpertLinear(torch.autograd.Function):
 def expert_linear(x, weight, bias=None, *, offsets=None, activation: str = "none", residual=None):
     """activation(x W^T + bias) + residual, [M, N].
 
-    With offsets (int32 [E + 1], ascending from 0, as sort_tokens gives them) rows offsets[e] ..
-    offsets[e + 1] of x [M, K] take weight[e] of weight [E, N, K] and bias[e] of bias [E, N]; rows behind
-    the last expert's are the residual's, or zeros. Without offsets weight is [N, K] and bias [N]. K and N are multiples of 8.
+    With offsets (int32 [E + 1], ascending, as sort_tokens gives them, or a range of those with as
+    many weights) rows offsets[e] .. offsets[e + 1] of x [M, K] take weight[e] of weight [E, N, K] and
+    bias[e] of bias [E, N]; rows of no expert are the residual's, or zeros. Without offsets weight is
+    [N, K] and bias [N]. K and N are multiples of 8. A call that a backward follows takes x and y of less
+    than 2^31 bytes.
     activation: one of ACTIVATIONS ("gelu" with the error function, "gelu_tanh" approximated)."""
     if activation not in ACTIVATIONS:
         raise ModelError(f"activation must be one of {ACTIVATIONS}, got {activation!r}")
@@ -312,10 +317,13 @@ def expert_linear(x, weight, bias=None, *, offsets=None, activation: str = "none
     for t in (weight, bias, residual):
         if not (t is None or t.dtype == x.dtype):
             raise ModelError("x, weight, bias and residual must have one dtype")
+    tracked = _tracked(x, weight, bias, residual)
+    if tracked and M * max(K, N) * x.element_size() >= 1 << 31:
+        raise ModelError(f"{M} rows of {max(K, N)} reach 2^31 bytes, more than a backward takes: split the batch")
     _on_device(x, weight, bias, residual, offsets)
     s = _LinearShape(M, K, N, groups, grouped, ACTIVATIONS.index(activation))
     offsets = offsets.contiguous() if grouped else None
-    if _tracked(x, weight, bias, residual):
+    if tracked:
         return _ExpertLinear.apply(x, weight, bias, residual, offsets, s)
     return _linear(_ready(x), _ready(weight), _ready(bias), offsets,
                    _ready(residual), s, False)[0]
@@ -415,6 +423,8 @@ def _check_norm(h, *weights):
 
 def rms_norm(x, weight, eps: float = 1e-6):
     """x / sqrt(mean(x^2) + eps) * weight over the last dimension."""
+    if weight is None:
+        raise ModelError("rms_norm needs a weight")
     H = _check_norm(x, weight)
     _on_device(x, weight)
     s = _NormShape(x.numel() // H, H, _GATE_NONE, 1.0, eps)

@@ -157,6 +157,17 @@ def test_an_order_that_no_sort_made_stays_inside_the_buffers():
     torch.autograd.grad(ops.permute_tokens(x, bad), x, torch.ones(120, 64, device="cuda"))
 
 
+def test_an_order_written_to_before_the_backward_is_refused():
+    g = gen(8)
+    for weights in (None, torch.rand(20, 2, device="cuda", generator=g)):
+        order = ops.sort_tokens(routing(g, 20, 2, 4), 4)
+        x = normal(g, 20, 64).requires_grad_()
+        out = ops.unpermute_tokens(ops.permute_tokens(x, order), order, weights)
+        order.inv_perm.zero_()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.sum().backward()
+
+
 def test_gradient_of_the_rows_alone():
     # weights that need no gradient: the rows are not kept
     g = gen(5)
@@ -326,6 +337,58 @@ def test_linear_rows_behind_the_last_group_do_not_reach_the_gradients():
         assert bool((y[70:] == 0).all()) and bool(torch.isfinite(y).all())
         for t in torch.autograd.grad(y, [x, w, b], dy):
             assert bool(torch.isfinite(t).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act,res", [("none", True), ("gelu", False)])
+@pytest.mark.parametrize("each", [1, 40, 300])
+def test_a_range_of_the_experts(each, act, res, dtype):
+    # offsets 3 .. 7 of nine experts' with four weights: the other experts' rows are no expert's
+    g = gen(each)
+    sizes = torch.full((9,), each, dtype=torch.int64)
+    sizes[4] = 0
+    off = torch.cat([torch.zeros(1, dtype=torch.int64), sizes.cumsum(0)]).int().cuda()
+    M = int(off[-1])
+    x, r, dy = normal(g, M, 64, dtype=dtype), normal(g, M, 72, dtype=dtype), normal(g, M, 72, dtype=dtype)
+    w, b = normal(g, 9, 72, 64, dtype=dtype, std=0.125), normal(g, 9, 72, dtype=dtype)
+    a, z = int(off[3]), int(off[7])
+    x[:a], x[z:] = float("nan"), float("nan")
+    part = [t.clone().requires_grad_() for t in (x, w[3:7].contiguous(), b[3:7].contiguous())]
+    y = ops.expert_linear(*part, offsets=off[3:8], activation=act, residual=r if res else None)
+    got = torch.autograd.grad(y, part, dy)
+    only = [t.clone().requires_grad_() for t in (x[a:z].contiguous(), w[3:7].contiguous(), b[3:7].contiguous())]
+    yo = ops.expert_linear(*only, offsets=off[3:8] - off[3], activation=act,
+                           residual=r[a:z].contiguous() if res else None)
+    want = torch.autograd.grad(yo, only, dy[a:z].contiguous())
+    # the tilings may add the products of a sum of n terms in different orders (n 2^-24 S each, S the
+    # sum of the terms' sizes, less than the figures below), which may round dz the other way (a step,
+    # 2 u, of each term) and the result too
+    def close(u, v, n, S, rounded):
+        off = 2 * n * 2.0 ** -24 * S + (2 * ref.u(dtype) * S if rounded else 0.0)
+        err = (u.double() - v.double()).abs()
+        assert bool((err <= off + 2 * ref.u(dtype) * (v.double().abs() + off)).all()), float(err.max())
+    close(y[a:z].detach(), yo.detach(), 65, 16.0, False)
+    dz = act != "none"
+    close(got[0][a:z], want[0], 72, 24.0, dz)
+    close(got[1], want[1], each, 2.0 * each + 16.0, dz)
+    close(got[2], want[2], each, 2.0 * each + 16.0, dz)
+    rest = r if res else torch.zeros_like(r)
+    assert torch.equal(y[:a], rest[:a]) and torch.equal(y[z:], rest[z:])
+    assert not bool(got[0][:a].any()) and not bool(got[0][z:].any())
+
+
+def test_more_columns_than_a_launch_of_few_rows_holds():
+    # 600 rows of as many experts, 2^20 columns: above 2^32 threads of the few-row kernel
+    E, K, N = 600, 8, 1 << 20
+    x = torch.ones(E, K, dtype=torch.bfloat16, device="cuda")
+    w = torch.zeros(E, N, K, dtype=torch.bfloat16, device="cuda")
+    ids = torch.arange(E, device="cuda")
+    w[:, :, 0] = (ids % 120).to(torch.bfloat16)[:, None]
+    w[:, -1, 1] = 0.5
+    off = torch.arange(E + 1, dtype=torch.int32, device="cuda")
+    y = ops.expert_linear(x, w, offsets=off)
+    want = (ids % 120).to(torch.bfloat16)
+    assert bool((y[:, :-1] == want[:, None]).all()) and torch.equal(y[:, -1], want + 0.5)
 
 
 @pytest.mark.parametrize("rows", [20, 3000])

@@ -204,3 +204,15 @@ def test_a_bound_that_is_passed_is_seen():
     ref.assert_close(a, a.double() * (1 + 2.0 ** -25), torch.zeros(4), "a")
     with pytest.raises(AssertionError):
         ref.assert_close(a, a.double() * (1 + 2.0 ** -22), torch.zeros(4, dtype=torch.float64), "a")
+
+
+def test_a_linear_whose_backward_would_be_refused_is_refused_at_once():
+    x = torch.zeros(1, 1024).expand(1 << 19, 1024)
+    w = torch.zeros(8, 1024, requires_grad=True)
+    fails("reach 2\\^31 bytes", ops.expert_linear, x, w)
+    with torch.no_grad():
+        fails("CUDA", ops.expert_linear, x, w)  # a forward alone takes them
+
+
+def test_rms_norm_needs_a_weight():
+    fails("needs a weight", ops.rms_norm, torch.zeros(2, 64), None)
