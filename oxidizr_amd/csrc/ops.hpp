@@ -439,7 +439,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_fwd(NormArgs<
 // A block takes rows b, b + grid, ..; its column sums stay in registers and go to
 // part[b] = (colA | colB), which k_norm_colsum adds in order.  The next row's loads are
 // in flight over a row's reduction and stores.  Bound by memory: 8192 x 7168 bf16 (705 MB)
-// 130 us, 5.4 TB/s (without the loads ahead 270), and 5.5 for the column sums.
+// 130 us, 5.4 TB/s (without the loads ahead 270).
 template <typename T>
 struct NormBwdArgs {
   const T *dhn, *dn;  // either may be null (zero)
@@ -671,8 +671,11 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_bwd(NormBwdAr
 
 // Column sums of the nb partial rows of k_norm_bwd, and the weight gradients
 // from them: dw2 = colA (g of a channel gate), dgate = colA w2 (channel gate), dw3 =
-// colB.  A block owns 64 columns of one sum; its thread (r, c) adds rows r, r + 32,
-// .. of 8 columns, and the 32 parts are added in order.
+// colB.  A block owns kColsumCols columns of one sum; its thread (r, c) adds rows r, r +
+// 128, .. of 8 columns, then eight threads' sums, then the sixteen that are left, each in
+// order.  Bound by its chain of loads: 1024 rows of 776 7 us, 256 of 7168 5 (16 columns to a
+// block 5 and 7, 64 columns 12 and 6).
+constexpr int kColsumCols = 32;
 template <typename T>
 __global__ __launch_bounds__(256) void k_norm_colsum(const float* __restrict__ part, int nb, int H,
                                                      int need_a, int need_b,
@@ -680,16 +683,17 @@ __global__ __launch_bounds__(256) void k_norm_colsum(const float* __restrict__ p
                                                      const T* __restrict__ chan_gate,
                                                      T* __restrict__ dw2, T* __restrict__ dgate,
                                                      T* __restrict__ dw3) {
-  __shared__ float col[32][64];
+  constexpr int C = kColsumCols, R = 256 / (C / 8), G = 256 / C;  // row lanes, and their groups
+  __shared__ float col[R][C], grp[G][C];
   const int which = blockIdx.y;
-  const int r0 = threadIdx.x >> 3, c8 = (threadIdx.x & 7) * 8;
-  const int c = blockIdx.x * 64 + c8;
+  const int r0 = threadIdx.x / (C / 8), c8 = threadIdx.x % (C / 8) * 8;
+  const int c = blockIdx.x * C + c8;
   const int64_t ld = (int64_t)(need_a + need_b) * H;
   float s[8], v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) s[i] = 0.0f;
   if (c < H)
-    for (int r = r0; r < nb; r += 32) {
+    for (int r = r0; r < nb; r += R) {
       load8(part + r * ld + (int64_t)which * H + c, v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) s[i] += v[i];
@@ -697,11 +701,17 @@ __global__ __launch_bounds__(256) void k_norm_colsum(const float* __restrict__ p
 #pragma unroll
   for (int i = 0; i < 8; ++i) col[r0][c8 + i] = s[i];
   __syncthreads();
-  const int cc = blockIdx.x * 64 + threadIdx.x;
-  if (threadIdx.x >= 64 || cc >= H) return;
+  const int g = threadIdx.x / C, n = threadIdx.x % C;
   float t = 0.0f;
 #pragma unroll
-  for (int r = 0; r < 32; ++r) t += col[r][threadIdx.x];
+  for (int r = 0; r < R / G; ++r) t += col[g * (R / G) + r][n];
+  grp[g][n] = t;
+  __syncthreads();
+  const int cc = blockIdx.x * C + n;
+  if (g > 0 || cc >= H) return;
+  t = 0.0f;
+#pragma unroll
+  for (int r = 0; r < G; ++r) t += grp[r][n];
   if (which == need_a) {
     dw3[cc] = from_f<T>(t);
     return;

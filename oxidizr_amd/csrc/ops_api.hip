@@ -247,7 +247,7 @@ moe_status launch_norm_bwd(hipStream_t s, const NormBwdArgs<D>& a, D* dw2, D* dg
                        s, a);
   });
   if (a.need_a + a.need_b > 0)
-    hipLaunchKernelGGL(k_norm_colsum<D>, dim3(ceil_div(a.H, 64), a.need_a + a.need_b), dim3(256), 0,
+    hipLaunchKernelGGL(k_norm_colsum<D>, dim3(ceil_div(a.H, kColsumCols), a.need_a + a.need_b), dim3(256), 0,
                        s, a.part, nb, a.H, a.need_a, a.need_b, a.w2,
                        a.gate_kind == kGateChannel ? a.gate : nullptr, dw2, dgate_chan, dw3);
   LAUNCH_CHECK();
