@@ -672,7 +672,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_bwd(NormBwdAr
 // Column sums of the nb partial rows of k_norm_bwd, and the weight gradients
 // from them: dw2 = colA (g of a channel gate), dgate = colA w2 (channel gate), dw3 =
 // colB.  A block owns kColsumCols columns of one sum; its thread (r, c) adds rows r, r +
-// 128, .. of 8 columns, then eight threads' sums, then the sixteen that are left, each in
+// 64, .. of 8 columns, then eight threads' sums, then the eight that are left, each in
 // order.  Bound by its chain of loads: 1024 rows of 776 7 us, 256 of 7168 5 (16 columns to a
 // block 5 and 7, 64 columns 12 and 6).
 constexpr int kColsumCols = 32;
