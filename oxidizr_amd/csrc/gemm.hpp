@@ -106,6 +106,23 @@ MOE_DEV void mfma_frag(f32x16& acc, u32x4 bt, u32x4 at, float) {
   acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(bt.w), __uint_as_float(at.w), acc, 0, 0, 0);
 }
 
+// KW vectors of each operand (fp32 with two: element by element, so a 16-deep step adds k in
+// the order 0, 4, 8, 12, 1, 5, ..).
+template <int KW, typename T>
+MOE_DEV void mfma_frags(f32x16& acc, const u32x4 (&bt)[KW], const u32x4 (&at)[KW], T t) {
+  if constexpr (KW == 1) {
+    mfma_frag(acc, bt[0], at[0], t);
+  } else {
+    static_assert(sizeof(T) == 4, "k order of fp32 sums");
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int w = 0; w < KW; ++w)
+        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(bt[w][e]), __uint_as_float(at[w][e]), acc,
+                                                   0, 0, 0);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Direct-to-LDS path.  Buffer loads with the LDS modifier stream 16-byte
 // vectors from global memory straight into LDS (no staging registers, no
@@ -328,7 +345,8 @@ using KMajorStager = typename std::conditional<sizeof(T) == 4, DmaStagerT32<C, R
 // than two stages at each k-tile.
 MOE_DEV void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-template <class C, typename T, bool A_T, bool B_T, int NA, int NB, bool AG = false>
+// KW: 16-byte vectors of k in one step (1, or 2 for fp32: see mfma_frags).
+template <class C, typename T, bool A_T, bool B_T, int NA, int NB, bool AG = false, int KW = 1>
 MOE_DEV void mainloop_dma(f32x16 (&acc)[NA * NB][C::TN][C::TM],
                           f32x16 (&xacc)[NA * NB][C::XTN], const OpDesc<T> (&a)[NA],
                           const OpDesc<T> (&b)[NB], int K, T* smem, const OpDesc<T>* a2,
@@ -376,31 +394,35 @@ MOE_DEV void mainloop_dma(f32x16 (&acc)[NA * NB][C::TN][C::TM],
   for (int kt = 0; kt < pro; ++kt) issue(kt);
   const int frag_row = lane & 31;
   const int frag_kv = lane >> 5;
-  constexpr int KSTEPS = C::BK / (2 * C::V);
+  constexpr int KSTEPS = C::BK / (2 * C::V * KW);
+  static_assert(KW == 1 || (!A_T && !B_T && !TALL && !C::FB1), "wide steps: K-contiguous operands");
   static_assert(KSTEPS % 2 == 0, "the next tile's first fragments go to register set 0");
   constexpr int NSET = C::FB1 ? 1 : 2;
-  u32x4 af[NSET][NA][C::TM], bfr[NSET][NB][C::TN], afx[NSET][NA];
+  u32x4 af[NSET][NA][C::TM][KW], bfr[NSET][NB][C::TN][KW], afx[NSET][NA];
   // tall tiles: the wave's extra row block and column half (wave-uniform)
   const int xrow = C::BM + 32 * (C::XR == 128 ? wm : (wm & 1)) + frag_row;
   const bool xhi = __builtin_amdgcn_readfirstlane(wm >> 1) != 0;
   auto read_frags = [&](const T* sA, const T* sB, int ks, int set) {
-    const int kv = ks * 2 + frag_kv;
+    const int kv = ks * 2 * KW + frag_kv;
 #pragma unroll
-    for (int i = 0; i < NA; ++i) {
+    for (int w = 0; w < KW; ++w) {
 #pragma unroll
-      for (int tm = 0; tm < C::TM; ++tm) {
-        if constexpr (A_T) af[set][i][tm] = SA::frag(sA + i * TILE_A, wm * C::WM + tm * 32, ks * 2 * C::V);
-        else af[set][i][tm] = SA::frag(sA + i * TILE_A, wm * C::WM + tm * 32 + frag_row, kv);
+      for (int i = 0; i < NA; ++i) {
+#pragma unroll
+        for (int tm = 0; tm < C::TM; ++tm) {
+          if constexpr (A_T) af[set][i][tm][w] = SA::frag(sA + i * TILE_A, wm * C::WM + tm * 32, ks * 2 * C::V);
+          else af[set][i][tm][w] = SA::frag(sA + i * TILE_A, wm * C::WM + tm * 32 + frag_row, kv + 2 * w);
+        }
+        if constexpr (TALL) afx[set][i] = SA::frag(sA + i * TILE_A, xrow, kv);
       }
-      if constexpr (TALL) afx[set][i] = SA::frag(sA + i * TILE_A, xrow, kv);
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int tn = 0; tn < C::TN; ++tn) {
+          if constexpr (B_T) bfr[set][i][tn][w] = SB::frag(sB + i * TILE_B, wn * C::WN + tn * 32, ks * 2 * C::V);
+          else bfr[set][i][tn][w] = SB::frag(sB + i * TILE_B, wn * C::WN + tn * 32 + frag_row, kv + 2 * w);
+        }
     }
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-#pragma unroll
-      for (int tn = 0; tn < C::TN; ++tn) {
-        if constexpr (B_T) bfr[set][i][tn] = SB::frag(sB + i * TILE_B, wn * C::WN + tn * 32, ks * 2 * C::V);
-        else bfr[set][i][tn] = SB::frag(sB + i * TILE_B, wn * C::WN + tn * 32 + frag_row, kv);
-      }
   };
   // wait until k-tile kt has landed when k-tiles up to `last` were issued
   auto wait_tile = [&](int kt, int last) {
@@ -484,15 +506,15 @@ MOE_DEV void mainloop_dma(f32x16 (&acc)[NA * NB][C::TN][C::TM],
           for (int tn = 0; tn < C::TN; ++tn)
 #pragma unroll
             for (int tm = 0; tm < C::TM; ++tm)
-              mfma_frag(acc[ia * NB + ib][tn][tm], bfr[cur][ib][tn], af[cur][ia][tm], T());
+              mfma_frags<KW>(acc[ia * NB + ib][tn][tm], bfr[cur][ib][tn], af[cur][ia][tm], T());
           if constexpr (C::XR == 128) {
 #pragma unroll
             for (int j = 0; j < C::XTN; ++j)
-              mfma_frag(xacc[ia * NB + ib][j], bfr[cur][ib][j], afx[cur][ia], T());
+              mfma_frag(xacc[ia * NB + ib][j], bfr[cur][ib][j][0], afx[cur][ia], T());
           } else if constexpr (TALL) {
 #pragma unroll
             for (int j = 0; j < C::XTN; ++j) {
-              const u32x4 bx = xhi ? bfr[cur][ib][C::XTN + j] : bfr[cur][ib][j];
+              const u32x4 bx = xhi ? bfr[cur][ib][C::XTN + j][0] : bfr[cur][ib][j][0];
               mfma_frag(xacc[ia * NB + ib][j], bx, afx[cur][ia], T());
             }
           }
@@ -505,7 +527,7 @@ MOE_DEV void mainloop_dma(f32x16 (&acc)[NA * NB][C::TN][C::TM],
           // per fragment of a transposed operand), then one DMA instruction
           // after each MFMA while they last
           if constexpr (!C::FB1)
-            __builtin_amdgcn_sched_group_barrier(0x100, (NA * (C::TM + (TALL ? 1 : 0)) * (A_T ? 2 : 1)) + (NB * C::TN * (B_T ? 2 : 1)), 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, KW * ((NA * (C::TM + (TALL ? 1 : 0)) * (A_T ? 2 : 1)) + (NB * C::TN * (B_T ? 2 : 1))), 0);
 #pragma unroll
           for (int i = 0; i < NM; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
@@ -531,26 +553,26 @@ constexpr int smem_elems() { return C::NST * (NA * C::AR + NB * C::BN) * C::BK; 
 // acc[a * NB + b][tn][tm] += B_b-tile x A_a-tile over k in [0, K).  An optional
 // second K segment (a2, b2, K2: same ld and rows as a and b) continues the same
 // pipeline, so sum_k A1 B1 + sum_k A2 B2 runs as one loop.
-template <class C, typename T, bool A_T, bool B_T, int NA, int NB, bool AG = false>
+template <class C, typename T, bool A_T, bool B_T, int NA, int NB, bool AG = false, int KW = 1>
 MOE_DEV void mainloop(f32x16 (&acc)[NA * NB][C::TN][C::TM], const OpDesc<T> (&a)[NA],
                       const OpDesc<T> (&b)[NB], int K, T* smem, const OpDesc<T>* a2 = nullptr,
                       const OpDesc<T>* b2 = nullptr, int K2 = 0) {
   static_assert(C::XR == 0, "tall tiles run mainloop_x");
   f32x16 unused[NA * NB][C::XTN];
-  mainloop_dma<C, T, A_T, B_T, NA, NB, AG>(acc, unused, a, b, K, smem, a2, b2, K2);
+  mainloop_dma<C, T, A_T, B_T, NA, NB, AG, KW>(acc, unused, a, b, K, smem, a2, b2, K2);
 }
 
 // mainloop for a row tile that may be tall (C::XR > 0, bf16): xacc holds the
 // wave's extra blocks (unused when C::XR == 0).
-template <class C, typename T, bool A_T, bool B_T, int NA, int NB, bool AG = false>
+template <class C, typename T, bool A_T, bool B_T, int NA, int NB, bool AG = false, int KW = 1>
 MOE_DEV void mainloop_x(f32x16 (&acc)[NA * NB][C::TN][C::TM], f32x16 (&xacc)[NA * NB][C::XTN],
                         const OpDesc<T> (&a)[NA], const OpDesc<T> (&b)[NB], int K, T* smem,
                         const OpDesc<T>* a2 = nullptr, const OpDesc<T>* b2 = nullptr,
                         int K2 = 0) {
   if constexpr (C::XR > 0)
-    mainloop_dma<C, T, A_T, B_T, NA, NB, AG>(acc, xacc, a, b, K, smem, a2, b2, K2);
+    mainloop_dma<C, T, A_T, B_T, NA, NB, AG, KW>(acc, xacc, a, b, K, smem, a2, b2, K2);
   else
-    mainloop<C, T, A_T, B_T, NA, NB, AG>(acc, a, b, K, smem, a2, b2, K2);
+    mainloop<C, T, A_T, B_T, NA, NB, AG, KW>(acc, a, b, K, smem, a2, b2, K2);
 }
 
 template <class C, int NACC>
