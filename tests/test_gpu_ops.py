@@ -709,3 +709,67 @@ def test_results_are_the_same_bits_every_time():
     for _ in range(3):
         for a, b in zip(first, step()):
             assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------- offsets past 32 bits
+
+def test_rows_past_2_31_elements():
+    T, k, H, E = 70000, 8, 4104, 16  # 2.3e9 elements of rows
+    g = gen(3)
+    order = ops.sort_tokens(routing(g, T, k, E, pad=0.05), E)
+    x = normal(g, T, H, dtype=torch.bfloat16).requires_grad_()
+    rows = ops.permute_tokens(x, order)
+    kept = int(order.offsets[-1])
+    assert kept * H > 2 ** 31
+    at = torch.cat([torch.arange(64), torch.arange(kept - 64, kept + 64), torch.arange(T * k - 64, T * k)]).cuda()
+    assert torch.equal(rows[at], torch.where((at < kept)[:, None], x.detach()[order.perm[at].long() // k], 0.0))
+    w = torch.rand(T, k, device="cuda", generator=g).requires_grad_()
+    y = rows.detach().requires_grad_()
+    out = ops.unpermute_tokens(y, order, w)
+    dout = normal(g, T, H, dtype=torch.bfloat16)
+    dy, dw = torch.autograd.grad(out, [y, w], dout)
+    few = torch.cat([torch.arange(32), torch.arange(T - 32, T)]).cuda()
+    pos = order.inv_perm[few].long()
+    real = (pos < kept).double()
+    v, d, w64 = y.detach()[pos].double(), dout[few].double(), w.detach()[few].double() * real
+    ref.assert_close(out.detach()[few], (w64[:, :, None] * v).sum(1),
+                     k * ref.U32 * (w64[:, :, None] * v.abs()).sum(1), "out")
+    ref.assert_close(dy[pos.flatten()], (w64[:, :, None] * d[:, None]).flatten(0, 1), 0.0, "dy")
+    ref.assert_close(dw[few], (d[:, None] * v).sum(2) * real, H * ref.U32 * (d[:, None] * v).abs().sum(2), "dw")
+    del v
+    dx, = torch.autograd.grad(rows, x, dy)
+    ref.assert_close(dx[few], (dy[pos].double() * real[:, :, None]).sum(1),
+                     k * ref.U32 * dy[pos].double().abs().sum(1), "dx")
+
+
+def test_norm_past_2_31_elements():
+    T, H = 300000, 7176
+    g = gen(4)
+    w = [normal(g, H, dtype=torch.bfloat16).requires_grad_() for _ in range(3)]
+    h, y = (normal(g, T, H, dtype=torch.bfloat16).requires_grad_() for _ in range(2))
+    dh, dn = normal(g, T, H, dtype=torch.bfloat16), normal(g, T, H, dtype=torch.bfloat16)
+
+    def step(a, b):
+        p, q = (t.detach()[a:b].requires_grad_() for t in (h, y))
+        out, n = ops.residual_norm(p, q, w[0], gate=w[1], next_weight=w[2])
+        return (out.detach(), n.detach()) + torch.autograd.grad((out, n), [p, q], (dh[a:b], dn[a:b]))
+    for big, small in zip(step(0, T), step(T - 40, T)):  # a row's results are its own
+        assert torch.equal(big[-40:], small)
+
+
+@pytest.mark.parametrize("grouped", [True, False])
+def test_linear_past_2_31_elements(grouped):
+    M, K, N = 1050003, 64, 2056
+    g = gen(5)
+    x = normal(g, M, K, dtype=torch.bfloat16)
+    w = normal(g, *((3, N, K) if grouped else (N, K)), dtype=torch.bfloat16, std=0.125)
+    off = torch.tensor([0, 500000, 500000, M - 3], dtype=torch.int32, device="cuda") if grouped else None
+    res = normal(g, M, N, dtype=torch.bfloat16)
+    y = ops.expert_linear(x, w, offsets=off, residual=res)
+    at = torch.cat([torch.arange(40), torch.arange(M - 300, M - 3)]).cuda()
+    for part, e in ((at[:40], 0), (at[40:], 2)):
+        a, b = x[part].double(), (w[e] if grouped else w).double()
+        ref.assert_close(y[part], a @ b.t() + res[part].double(),
+                         (K + 1) * ref.U32 * (a.abs() @ b.abs().t() + res[part].double().abs()), "y")
+    if grouped:
+        assert torch.equal(y[-3:], res[-3:])
