@@ -118,12 +118,19 @@ def _check_hidden(H):
         raise ModelError(f"the hidden size must be a positive multiple of 8, got {H}")
 
 
+def _kept(offsets):
+    """Address of the number of assignments that have an expert."""
+    return offsets.data_ptr() + 4 * (offsets.numel() - 1)
+
+
 class _Slots:
-    """What the row kernels read of a TokenOrder. A backward makes its own from the tensors that its
-    forward saved, so that autograd sees whether they were written to in between."""
+    """What the row kernels read of a TokenOrder."""
     __slots__ = ("inv", "offsets", "T", "k", "kept")
 
-    def __init__(self, offsets, inv):
+    def __init__(self, order):
+        if not isinstance(order, TokenOrder):
+            raise ModelError("order must be a TokenOrder (sort_tokens)")
+        offsets, inv = order.offsets, order.inv_perm
         if inv.dim() != 2:
             raise ModelError("order.inv_perm must be [T, k]")
         if inv.dtype != torch.int32 or offsets.dtype != torch.int32:
@@ -135,13 +142,7 @@ class _Slots:
         if offsets.dim() != 1 or E < 1:
             raise ModelError("order.offsets must be [E + 1]")
         self.inv, self.offsets = inv.contiguous(), offsets.contiguous()
-        self.kept = self.offsets.data_ptr() + 4 * E
-
-
-def _slots(order):
-    if not isinstance(order, TokenOrder):
-        raise ModelError("order must be a TokenOrder (sort_tokens)")
-    return _Slots(order.offsets, order.inv_perm)
+        self.kept = _kept(self.offsets)
 
 
 def _permute(x, slots):
@@ -163,19 +164,26 @@ def _unpermute(y, slots, weights):
 class _Permute(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, slots):
+        # saved, so that autograd sees whether the order was written to before the backward
         ctx.save_for_backward(slots.offsets, slots.inv)
         return _permute(_ready(x), slots)
 
     @staticmethod
     @_once
     def backward(ctx, dxp):
-        return _unpermute(_ready(dxp), _Slots(*ctx.saved_tensors), None), None
+        offsets, inv = ctx.saved_tensors
+        dxp = _ready(dxp)
+        (T, k), H = inv.shape, dxp.shape[1]
+        dx = dxp.new_empty(T, H)
+        _call(_lib.load().moe_unpermute, dxp.get_device(), _dtype_code(dxp.dtype), T, k, H, inv.data_ptr(),
+              _kept(offsets), dxp.data_ptr(), None, dx.data_ptr())
+        return dx, None
 
 
 def permute_tokens(x, order: TokenOrder):
     """Rows of x [T, H] in the order's positions: out[inv_perm[t, j]] = x[t] [T k, H]; the rows behind
     the last expert's (assignments without one) are zeros."""
-    slots = _slots(order)
+    slots = _Slots(order)
     if x.dim() != 2 or x.shape[0] != slots.T:
         raise ModelError(f"x must be [{slots.T}, H], got {list(x.shape)}")
     _check_hidden(x.shape[1])
@@ -200,19 +208,20 @@ class _Unpermute(torch.autograd.Function):
     @_once
     def backward(ctx, dout):
         y, weights, offsets, inv = ctx.saved_tensors
-        slots, dout = _Slots(offsets, inv), _ready(dout)
-        dy = dout.new_empty(slots.T * slots.k, dout.shape[1])
+        dout = _ready(dout)
+        (T, k), H = inv.shape, dout.shape[1]
+        dy = dout.new_empty(T * k, H)
         dw = torch.empty_like(weights) if y is not None else None
-        _call(_lib.load().moe_unpermute_backward, dout.get_device(), _dtype_code(dout.dtype), slots.T,
-              slots.k, dout.shape[1], _ptr(slots.inv), slots.kept, _ptr(dout), _ptr(y), _ptr(weights),
-              _ptr(dy), _ptr(dw))
+        _call(_lib.load().moe_unpermute_backward, dout.get_device(), _dtype_code(dout.dtype), T, k, H,
+              inv.data_ptr(), _kept(offsets), dout.data_ptr(), _ptr(y), _ptr(weights), dy.data_ptr(),
+              _ptr(dw))
         return dy, dw, None
 
 
 def unpermute_tokens(y, order: TokenOrder, weights: Optional[torch.Tensor] = None):
     """out[t] = sum_j weights[t, j] * y[inv_perm[t, j]] [T, H] over the assignments that have an expert,
     j ascending; weights [T, k] float32, or None for a plain sum."""
-    slots = _slots(order)
+    slots = _Slots(order)
     T, k = slots.T, slots.k
     if y.dim() != 2 or y.shape[0] != T * k:
         raise ModelError(f"y must be [{T * k}, H], got {list(y.shape)}")
@@ -362,6 +371,8 @@ class _ResidualNorm(torch.autograd.Function):
         after = h if y is None else out  # what the second norm is taken of
         ctx.save_for_backward(after if n is not None else None, y, post_weight, gate, next_weight, r2, r3)
         ctx.s = s
+        # the backward runs in autograd's thread, where every call costs several times as much
+        ctx.ws_bytes = _lib.load().moe_residual_norm_workspace_bytes(s.T, s.H)
         return (out, n) if y is not None and n is not None else out if n is None else n
 
     @staticmethod
@@ -384,9 +395,8 @@ class _ResidualNorm(torch.autograd.Function):
         d_y = None if y is None else torch.empty_like(like)
         d_post = None if post_weight is None else torch.empty_like(post_weight)
         d_gate = None if gate is None else torch.empty_like(gate)
-        L = _lib.load()
-        ws = _workspace(L.moe_residual_norm_workspace_bytes(s.T, s.H), like)
-        _call(L.moe_residual_norm_backward, like.get_device(), _dtype_code(like.dtype), s.T, s.H,
+        ws = _workspace(ctx.ws_bytes, like)
+        _call(_lib.load().moe_residual_norm_backward, like.get_device(), _dtype_code(like.dtype), s.T, s.H,
               _ptr(d_out), _ptr(d_n), _ptr(after), _ptr(y), _ptr(post_weight), _ptr(gate), s.gate_kind,
               _ptr(used), s.scale, _ptr(r2), _ptr(r3), _ptr(d_h), _ptr(d_y), _ptr(d_post), _ptr(d_gate),
               _ptr(d_next) if used is not None else None, _ptr(ws))
