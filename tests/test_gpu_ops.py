@@ -1,7 +1,10 @@
 """oxidizr_amd.ops on the GPU against plain float64 forms (tests/ops_ref.py), at the sizes, masks and
 layouts where they can go wrong, with bounds from arithmetic."""
+import threading
+
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from oxidizr_amd import ops
 from oxidizr_amd.moe import MoeBlock, MoeConfig
@@ -678,6 +681,46 @@ def test_calls_on_two_streams_at_once():
             with torch.cuda.stream(streams[i]):
                 got[i] = chain(x, idx, w, p, E)
     torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_kept_tensors_may_move_or_be_made_again():
+    # saved tensors offloaded to the host and back, and a forward run again in the backward
+    p, x, idx, w = chain_inputs(gen(8), 120, 264, 136, 5, 2, torch.bfloat16)
+    leaves = [x, w] + list(p.values())
+    for t in leaves:
+        t.requires_grad_()
+    d = normal(gen(9), 2, 120, 264, dtype=torch.bfloat16)
+
+    def grads(h, n):
+        return torch.autograd.grad((h, n), leaves, (d[0], d[1]))
+    want = grads(*chain(x, idx, w, p, 5))
+    with torch.autograd.graph.save_on_cpu():
+        out = chain(x, idx, w, p, 5)
+    again = torch.utils.checkpoint.checkpoint(lambda a: chain(a, idx, w, p, 5), x, use_reentrant=False)
+    for got in (grads(*out), grads(*again)):
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+def test_threads_with_streams_of_their_own():
+    sets = [chain_inputs(gen(s), 300, 264, 136, 6, 2, torch.bfloat16) for s in range(3)]
+    want = [chain(x, idx, w, p, 6) for p, x, idx, w in sets]
+    torch.cuda.synchronize()
+    got = [None] * 3
+
+    def work(i):
+        p, x, idx, w = sets[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i] = chain(x, idx, w, p, 6)
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
     for a, b in zip(got, want):
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
