@@ -405,24 +405,31 @@ MOE_DEV void mainloop_dma(f32x16 (&acc)[NA * NB][C::TN][C::TM],
   auto read_frags = [&](const T* sA, const T* sB, int ks, int set) {
     const int kv = ks * 2 * KW + frag_kv;
 #pragma unroll
-    for (int w = 0; w < KW; ++w) {
+    for (int i = 0; i < NA; ++i) {
 #pragma unroll
-      for (int i = 0; i < NA; ++i) {
+      for (int tm = 0; tm < C::TM; ++tm) {
+        if constexpr (A_T) {
+          af[set][i][tm][0] = SA::frag(sA + i * TILE_A, wm * C::WM + tm * 32, ks * 2 * C::V);
+        } else {
 #pragma unroll
-        for (int tm = 0; tm < C::TM; ++tm) {
-          if constexpr (A_T) af[set][i][tm][w] = SA::frag(sA + i * TILE_A, wm * C::WM + tm * 32, ks * 2 * C::V);
-          else af[set][i][tm][w] = SA::frag(sA + i * TILE_A, wm * C::WM + tm * 32 + frag_row, kv + 2 * w);
+          for (int w = 0; w < KW; ++w)
+            af[set][i][tm][w] = SA::frag(sA + i * TILE_A, wm * C::WM + tm * 32 + frag_row, kv + 2 * w);
         }
-        if constexpr (TALL) afx[set][i] = SA::frag(sA + i * TILE_A, xrow, kv);
       }
-#pragma unroll
-      for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int tn = 0; tn < C::TN; ++tn) {
-          if constexpr (B_T) bfr[set][i][tn][w] = SB::frag(sB + i * TILE_B, wn * C::WN + tn * 32, ks * 2 * C::V);
-          else bfr[set][i][tn][w] = SB::frag(sB + i * TILE_B, wn * C::WN + tn * 32 + frag_row, kv + 2 * w);
-        }
+      if constexpr (TALL) afx[set][i] = SA::frag(sA + i * TILE_A, xrow, kv);
     }
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int tn = 0; tn < C::TN; ++tn) {
+        if constexpr (B_T) {
+          bfr[set][i][tn][0] = SB::frag(sB + i * TILE_B, wn * C::WN + tn * 32, ks * 2 * C::V);
+        } else {
+#pragma unroll
+          for (int w = 0; w < KW; ++w)
+            bfr[set][i][tn][w] = SB::frag(sB + i * TILE_B, wn * C::WN + tn * 32 + frag_row, kv + 2 * w);
+        }
+      }
   };
   // wait until k-tile kt has landed when k-tiles up to `last` were issued
   auto wait_tile = [&](int kt, int last) {
