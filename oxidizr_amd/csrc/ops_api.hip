@@ -399,6 +399,7 @@ BwdPlan plan_bwd(bool grouped, int E, int64_t M, int K, int N) {
   p.split = grouped ? SplitPlan{1, 0} : plan_dense_wgrad<D, 1>(N, K, (int)M);
   p.tiles = pick_tiles<D>(grouped, E, M, K);
   p.fused = false;
+  if (M == 0) return p;  // no rows to plan for: nothing is launched
   if constexpr (has_half_rows<D, C>()) {
     if (p.tiles != RowTiles::kBig && p.tiles != RowTiles::kTall) return p;
     p.fused = true;

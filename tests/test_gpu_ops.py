@@ -816,3 +816,21 @@ def test_linear_past_2_31_elements(grouped):
                          (K + 1) * ref.U32 * (a.abs() @ b.abs().t() + res[part].double().abs()), "y")
     if grouped:
         assert torch.equal(y[-3:], res[-3:])
+
+
+# ---------------------------------------------------------------- empty batches
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["none", "silu"])
+@pytest.mark.parametrize("grouped", [True, False])
+def test_linear_gradients_without_rows(grouped, act, dtype):
+    w = torch.ones(*((2, 64, 128) if grouped else (64, 128)), dtype=dtype, device="cuda", requires_grad=True)
+    b = torch.ones(*((2, 64) if grouped else (64,)), dtype=dtype, device="cuda", requires_grad=True)
+    x = torch.zeros(0, 128, dtype=dtype, device="cuda", requires_grad=True)
+    r = torch.zeros(0, 64, dtype=dtype, device="cuda", requires_grad=True)
+    off = torch.zeros(3, dtype=torch.int32, device="cuda") if grouped else None
+    y = ops.expert_linear(x, w, b, offsets=off, activation=act, residual=r)
+    assert y.shape == (0, 64)
+    dx, dw, db, dr = torch.autograd.grad(y, [x, w, b, r], torch.zeros_like(y))
+    assert dx.shape == x.shape and dr.shape == r.shape
+    assert dw.shape == w.shape and not bool(dw.any()) and db.shape == b.shape and not bool(db.any())

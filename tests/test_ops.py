@@ -1,6 +1,9 @@
 """Refusals of oxidizr_amd.ops and of their C entries, workspace sizes, and the reference forms
 themselves, without a GPU."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -216,3 +219,24 @@ def test_a_linear_whose_backward_would_be_refused_is_refused_at_once():
 
 def test_rms_norm_needs_a_weight():
     fails("needs a weight", ops.rms_norm, torch.zeros(2, 64), None)
+
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def test_workspace_of_a_linear_without_rows():
+    # in a process of its own: a division by zero would end it
+    code = """
+from oxidizr_amd import _lib
+L = _lib.load()
+for dtype in (_lib.MOE_DTYPE_F32, _lib.MOE_DTYPE_BF16):
+    for K, N in ((8, 8), (64, 64), (2048, 1408), (8, 1 << 20)):
+        for act in range(5):
+            for backward in (0, 1):
+                assert L.moe_linear_workspace_bytes(dtype, 0, K, N, 1, 0, act, backward) == 0
+                for E in (1, 3, 1024):
+                    assert L.moe_linear_workspace_bytes(dtype, 0, K, N, E, 1, act, backward) > 0
+print("done")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "done" in r.stdout, (r.returncode, r.stderr[-500:])
