@@ -365,11 +365,22 @@ moe_status moe_residual_norm(int32_t device, void* stream, int32_t dtype, int64_
                              void* h_out, void* n_out, float* rstd_post, float* rstd_next);
 /* Backward: d_h, d_y [T, H] and the gradients of post_weight, gate and next_weight, each in
  * its tensor's shape, for what the forward was given.  d_h_out may be NULL (0) where
- * d_n_out is given.  h_out is the forward's (without y: h). */
+ * d_n_out is given.  h_out is the forward's (without y: h).  _from_input takes the forward's h
+ * instead and forms h_out from it again as it was before its rounding (from which the forward
+ * formed n_out): the gradients are then those of the values that the forward used. */
 size_t moe_residual_norm_workspace_bytes(int64_t num_tokens, int32_t hidden);
 moe_status moe_residual_norm_backward(int32_t device, void* stream, int32_t dtype,
                                       int64_t num_tokens, int32_t hidden, const void* d_h_out,
                                       const void* d_n_out, const void* h_out, const void* y,
+                                      const void* post_weight, const void* gate,
+                                      int32_t gate_kind, const void* next_weight,
+                                      float residual_scale, const float* rstd_post,
+                                      const float* rstd_next, void* d_h, void* d_y,
+                                      void* d_post_weight, void* d_gate, void* d_next_weight,
+                                      void* workspace);
+moe_status moe_residual_norm_backward_from_input(int32_t device, void* stream, int32_t dtype,
+                                      int64_t num_tokens, int32_t hidden, const void* d_h_out,
+                                      const void* d_n_out, const void* h, const void* y,
                                       const void* post_weight, const void* gate,
                                       int32_t gate_kind, const void* next_weight,
                                       float residual_scale, const float* rstd_post,

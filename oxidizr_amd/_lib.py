@@ -26,6 +26,7 @@ EXPORTED = [
     "moe_unpermute", "moe_unpermute_backward", "moe_linear_workspace_bytes",
     "moe_linear_forward", "moe_linear_backward", "moe_residual_norm",
     "moe_residual_norm_workspace_bytes", "moe_residual_norm_backward",
+    "moe_residual_norm_backward_from_input",
 ]
 NUM_STAGES = 20
 
@@ -142,6 +143,8 @@ def load():
     L.moe_residual_norm_backward.argtypes = [i32, _vp, i32, i64, i32, _vp, _vp, _vp, _vp, _vp, _vp,
                                              i32, _vp, f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]
     L.moe_residual_norm_backward.restype = i32
+    L.moe_residual_norm_backward_from_input.argtypes = L.moe_residual_norm_backward.argtypes
+    L.moe_residual_norm_backward_from_input.restype = i32
     L.moe_last_error.argtypes = []
     L.moe_last_error.restype = ctypes.c_char_p
     L.moe_version.argtypes = []

@@ -425,7 +425,8 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_fwd(NormArgs<
   }
 }
 
-// Backward, with hh = hn r3, yh = y r2, u = yh w2 (u = y without w2):
+// Backward, with hh = hn r3, yh = y r2, u = yh w2 (u = y without w2); hn is formed again
+// from h and u, as the forward had it before its rounding (hn_given: read as the forward stored it):
 //   D = dhn + r3 (w3 dn - hh mean(hh w3 dn)),  dh = scale D,
 //   dgate = D u,  dy = r2 (g w2 D - yh mean(yh g w2 D))  (g D without w2),
 //   dw3 = sum_t dn hh,  dw2 = sum_t g D yh.
@@ -439,12 +440,13 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_fwd(NormArgs<
 // A block takes rows b, b + grid, ..; its column sums stay in registers and go to
 // part[b] = (colA | colB), which k_norm_colsum adds in order.  The next row's loads are
 // in flight over a row's reduction and stores.  Bound by memory: 8192 x 7168 bf16 (705 MB)
-// 130 us, 5.4 TB/s (without the loads ahead 270).
+// 135 us, 5.2 TB/s (without the loads ahead 270).  Forming hn costs some 5 us of them; with the
+// rounded hn the gradients were 2.5e-3 off a 64-bit form, now 1.7e-3 (relative L2).
 template <typename T>
 struct NormBwdArgs {
   const T *dhn, *dn;  // either may be null (zero)
-  const T *hn, *y, *w2, *gate, *w3;
-  int gate_kind;
+  const T *h, *y, *w2, *gate, *w3;  // h: hn in its place when hn_given
+  int gate_kind, hn_given;
   float scale;
   int64_t Tn;
   int H;
@@ -478,6 +480,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_bwd(NormBwdAr
   const int nch = a.H / 8;
   const float inv_h = 1.0f / (float)a.H;
   const bool chan = a.gate_kind == kGateChannel, full = a.gate_kind == kGateFull;
+  const bool form = a.y && !a.hn_given;
   // the row vectors of a thread's columns, and the next row's tensors
   Raw8<T> w2[NCH], w3[NCH], gc[NCH], nd[NCH], nn[NCH], nh[NCH], ny[NCH], ng[NCH];
   float ca[NCH][8], cb[NCH][8];
@@ -502,7 +505,7 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_bwd(NormBwdAr
       if (a.dhn) nd[c].load(a.dhn + row + ch * 8);
       if (a.w3) {
         nn[c].load(a.dn + row + ch * 8);
-        nh[c].load(a.hn + row + ch * 8);
+        nh[c].load(a.h + row + ch * 8);
       }
       if (a.y) ny[c].load(a.y + row + ch * 8);
       if (full) ng[c].load(a.gate + row + ch * 8);
@@ -528,24 +531,9 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_bwd(NormBwdAr
 #pragma unroll
       for (int i = 0; i < 8; ++i) p[c][i] = hh[c][i] = yh[c][i] = 0.0f;
       if (!live || ch >= nch) continue;
-      float v[8];
+      float v[8], u[8];
       if (a.dhn) nd[c].get(p[c]);
-      if (a.w3) {
-        float d[8];
-        nn[c].get(d);
-        nh[c].get(hh[c]);
-        w3[c].get(v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          hh[c][i] *= r3;
-          cb[c][i] += d[i] * hh[c][i];
-          d[i] *= v[i];
-          s3 += hh[c][i] * d[i];
-          p[c][i] += r3 * d[i];
-        }
-      }
       if (a.y) {
-        float u[8];
         ny[c].get(yh[c]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) u[i] = yh[c][i] *= r2;
@@ -560,6 +548,26 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_bwd(NormBwdAr
 #pragma unroll
           for (int i = 0; i < 8; ++i) u[i] *= v[i];
         }
+      }
+      if (a.w3) {
+        float d[8];
+        nn[c].get(d);
+        nh[c].get(hh[c]);
+        w3[c].get(v);
+        if (form) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) hh[c][i] = a.scale * hh[c][i] + gt * u[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          hh[c][i] *= r3;
+          cb[c][i] += d[i] * hh[c][i];
+          d[i] *= v[i];
+          s3 += hh[c][i] * d[i];
+          p[c][i] += r3 * d[i];
+        }
+      }
+      if (a.y) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           sp += u[i] * p[c][i];

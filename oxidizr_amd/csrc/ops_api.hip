@@ -254,6 +254,48 @@ moe_status launch_norm_bwd(hipStream_t s, const NormBwdArgs<D>& a, D* dw2, D* dg
   return MOE_OK;
 }
 
+// hn_given: h is the forward's h_out in place of its h.
+moe_status norm_backward(int device, void* stream, int dtype, int64_t T, int H, bool hn_given,
+                         const void* d_h_out, const void* d_n_out, const void* h, const void* y,
+                         const void* post_weight, const void* gate, int gate_kind,
+                         const void* next_weight, float residual_scale, const float* rstd_post,
+                         const float* rstd_next, void* d_h, void* d_y, void* d_post_weight,
+                         void* d_gate, void* d_next_weight, void* workspace) {
+  moe_status st = check_norm(dtype, T, H, gate_kind, y, post_weight, gate, next_weight,
+                             residual_scale);
+  if (st != MOE_OK) return st;
+  if ((st = check_pointers({}, {d_h_out, d_n_out, h, y, post_weight, gate, next_weight,
+                                rstd_post, rstd_next, d_h, d_y, d_post_weight, d_gate,
+                                d_next_weight, workspace})) != MOE_OK)
+    return st;
+  const size_t b = elt_size(dtype);
+  DeviceScope dev(device);
+  hipStream_t s = (hipStream_t)stream;
+  if (T == 0) {  // sums over no row
+    HIP_TRY(dev.enter());
+    if ((st = zero_async(s, d_post_weight, H * b)) != MOE_OK) return st;
+    if ((st = zero_async(s, gate_kind == kGateChannel ? d_gate : nullptr, H * b)) != MOE_OK) return st;
+    return zero_async(s, d_next_weight, H * b);
+  }
+  if (!d_h || (y && !d_y) || !workspace || (post_weight && (!d_post_weight || !rstd_post)) ||
+      (gate && !d_gate) || (next_weight && !d_next_weight) ||
+      (next_weight && (!rstd_next || !h || !d_n_out)) || (!next_weight && !d_h_out))
+    return fail(MOE_ERR_INVALID, "a required pointer is NULL");
+  HIP_TRY(dev.enter());
+  const bool chan = gate_kind == kGateChannel;
+  auto go = [&](auto d) {
+    using D = decltype(d);
+    const NormBwdArgs<D> a{(const D*)d_h_out, (const D*)d_n_out, (const D*)h, (const D*)y,
+                           (const D*)post_weight, (const D*)gate, (const D*)next_weight, gate_kind,
+                           hn_given ? 1 : 0, residual_scale, T, H, rstd_post, rstd_next, (D*)d_h, (D*)d_y,
+                           chan ? nullptr : (D*)d_gate, (float*)workspace,
+                           post_weight || chan ? 1 : 0, next_weight ? 1 : 0};
+    return launch_norm_bwd<D>(s, a, (D*)d_post_weight, chan ? (D*)d_gate : nullptr,
+                              (D*)d_next_weight);
+  };
+  return dtype == MOE_DTYPE_BF16 ? go(bf16_t()) : go(float());
+}
+
 // ---- expert products
 constexpr int kLinearMaxWidth = 1 << 20;
 moe_status check_linear(int dtype, int64_t M, int K, int N, int E, bool grouped, int act) {
@@ -761,39 +803,22 @@ moe_status moe_residual_norm_backward(int32_t device, void* stream, int32_t dtyp
                                       const float* rstd_next, void* d_h, void* d_y,
                                       void* d_post_weight, void* d_gate, void* d_next_weight,
                                       void* workspace) {
-  moe_status st = check_norm(dtype, T, H, gate_kind, y, post_weight, gate, next_weight,
-                             residual_scale);
-  if (st != MOE_OK) return st;
-  if ((st = check_pointers({}, {d_h_out, d_n_out, h_out, y, post_weight, gate, next_weight,
-                                rstd_post, rstd_next, d_h, d_y, d_post_weight, d_gate,
-                                d_next_weight, workspace})) != MOE_OK)
-    return st;
-  const size_t b = elt_size(dtype);
-  DeviceScope dev(device);
-  hipStream_t s = (hipStream_t)stream;
-  if (T == 0) {  // sums over no row
-    HIP_TRY(dev.enter());
-    if ((st = zero_async(s, d_post_weight, H * b)) != MOE_OK) return st;
-    if ((st = zero_async(s, gate_kind == kGateChannel ? d_gate : nullptr, H * b)) != MOE_OK) return st;
-    return zero_async(s, d_next_weight, H * b);
-  }
-  if (!d_h || (y && !d_y) || !workspace || (post_weight && (!d_post_weight || !rstd_post)) ||
-      (gate && !d_gate) || (next_weight && !d_next_weight) ||
-      (next_weight && (!rstd_next || !h_out || !d_n_out)) || (!next_weight && !d_h_out))
-    return fail(MOE_ERR_INVALID, "a required pointer is NULL");
-  HIP_TRY(dev.enter());
-  const bool chan = gate_kind == kGateChannel;
-  auto go = [&](auto d) {
-    using D = decltype(d);
-    const NormBwdArgs<D> a{(const D*)d_h_out, (const D*)d_n_out, (const D*)h_out, (const D*)y,
-                           (const D*)post_weight, (const D*)gate, (const D*)next_weight, gate_kind,
-                           residual_scale, T, H, rstd_post, rstd_next, (D*)d_h, (D*)d_y,
-                           chan ? nullptr : (D*)d_gate, (float*)workspace,
-                           post_weight || chan ? 1 : 0, next_weight ? 1 : 0};
-    return launch_norm_bwd<D>(s, a, (D*)d_post_weight, chan ? (D*)d_gate : nullptr,
-                              (D*)d_next_weight);
-  };
-  return dtype == MOE_DTYPE_BF16 ? go(bf16_t()) : go(float());
+  return norm_backward(device, stream, dtype, T, H, true, d_h_out, d_n_out, h_out, y, post_weight, gate,
+                       gate_kind, next_weight, residual_scale, rstd_post, rstd_next, d_h, d_y,
+                       d_post_weight, d_gate, d_next_weight, workspace);
+}
+
+moe_status moe_residual_norm_backward_from_input(int32_t device, void* stream, int32_t dtype, int64_t T,
+                                      int32_t H, const void* d_h_out, const void* d_n_out,
+                                      const void* h, const void* y, const void* post_weight,
+                                      const void* gate, int32_t gate_kind, const void* next_weight,
+                                      float residual_scale, const float* rstd_post,
+                                      const float* rstd_next, void* d_h, void* d_y,
+                                      void* d_post_weight, void* d_gate, void* d_next_weight,
+                                      void* workspace) {
+  return norm_backward(device, stream, dtype, T, H, false, d_h_out, d_n_out, h, y, post_weight, gate,
+                       gate_kind, next_weight, residual_scale, rstd_post, rstd_next, d_h, d_y,
+                       d_post_weight, d_gate, d_next_weight, workspace);
 }
 
 }  // extern "C"

@@ -368,8 +368,8 @@ class _ResidualNorm(torch.autograd.Function):
         h, y, gate = _ready(h), _ready(y), _ready(gate)
         post_weight, next_weight = _ready(post_weight), _ready(next_weight)
         out, n, r2, r3 = _norm(h, y, post_weight, gate, next_weight, s, True)
-        after = h if y is None else out  # what the second norm is taken of
-        ctx.save_for_backward(after if n is not None else None, y, post_weight, gate, next_weight, r2, r3)
+        # h alone: what the second norm is taken of is formed from it again, unrounded
+        ctx.save_for_backward(h if n is not None else None, y, post_weight, gate, next_weight, r2, r3)
         ctx.s = s
         # the backward runs in autograd's thread, where every call costs several times as much
         ctx.ws_bytes = _lib.load().moe_residual_norm_workspace_bytes(s.T, s.H)
@@ -378,7 +378,7 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     @_once
     def backward(ctx, *up):
-        after, y, post_weight, gate, next_weight, r2, r3 = ctx.saved_tensors
+        h, y, post_weight, gate, next_weight, r2, r3 = ctx.saved_tensors
         s = ctx.s
         d_out = up[0] if y is not None else None
         d_n = up[-1] if next_weight is not None else None
@@ -396,8 +396,8 @@ class _ResidualNorm(torch.autograd.Function):
         d_post = None if post_weight is None else torch.empty_like(post_weight)
         d_gate = None if gate is None else torch.empty_like(gate)
         ws = _workspace(ctx.ws_bytes, like)
-        _call(_lib.load().moe_residual_norm_backward, like.get_device(), _dtype_code(like.dtype), s.T, s.H,
-              _ptr(d_out), _ptr(d_n), _ptr(after), _ptr(y), _ptr(post_weight), _ptr(gate), s.gate_kind,
+        _call(_lib.load().moe_residual_norm_backward_from_input, like.get_device(), _dtype_code(like.dtype),
+              s.T, s.H, _ptr(d_out), _ptr(d_n), _ptr(h), _ptr(y), _ptr(post_weight), _ptr(gate), s.gate_kind,
               _ptr(used), s.scale, _ptr(r2), _ptr(r3), _ptr(d_h), _ptr(d_y), _ptr(d_post), _ptr(d_gate),
               _ptr(d_next) if used is not None else None, _ptr(ws))
         return d_h, d_y, d_post, d_gate, d_next, None

@@ -317,6 +317,30 @@ pub mod ffi {
             d_next_weight: *mut c_void,
             workspace: *mut c_void,
         ) -> MoeStatus;
+        pub fn moe_residual_norm_backward_from_input(
+            device: i32,
+            stream: *mut c_void,
+            dtype: i32,
+            num_tokens: i64,
+            hidden: i32,
+            d_h_out: *const c_void,
+            d_n_out: *const c_void,
+            h: *const c_void,
+            y: *const c_void,
+            post_weight: *const c_void,
+            gate: *const c_void,
+            gate_kind: i32,
+            next_weight: *const c_void,
+            residual_scale: f32,
+            rstd_post: *const f32,
+            rstd_next: *const f32,
+            d_h: *mut c_void,
+            d_y: *mut c_void,
+            d_post_weight: *mut c_void,
+            d_gate: *mut c_void,
+            d_next_weight: *mut c_void,
+            workspace: *mut c_void,
+        ) -> MoeStatus;
         pub fn moe_last_error() -> *const c_char;
         pub fn moe_version() -> *const c_char;
     }

@@ -121,8 +121,9 @@ def linear(x, w, b, offsets, act, res, dy, dtype):
     return out
 
 
-def norm(h, y, w2, gate, w3, scale, eps, d_out, d_n, dtype):
-    """{name: (reference, error bound)} of residual_norm and its gradients. Inputs are float64."""
+def norm(h, y, w2, gate, w3, scale, eps, d_out, d_n, dtype, hn_rounded=True):
+    """{name: (reference, error bound)} of residual_norm and its gradients. Inputs are float64.
+    hn_rounded: the backward may have read h_out in dtype."""
     T, H = h.shape
     c = (H + 32) * U32
     ud = u(dtype)
@@ -146,8 +147,8 @@ def norm(h, y, w2, gate, w3, scale, eps, d_out, d_n, dtype):
     D = d_out if d_out is not None else torch.zeros_like(h)
     De = U32 * D.abs()
     if d_n is not None:
-        # the backward reads h_out again, rounded (without y the input itself)
-        hhe = hh.abs() * (c + (ud if y is not None else 0.0)) + oute * r3
+        # h_out as the backward reads it again (without y the input itself)
+        hhe = hh.abs() * (c + (ud if y is not None and hn_rounded else 0.0)) + oute * r3
         a = d_n * w3
         m = (hh * a).mean(1, keepdim=True)
         mm = (hh * a).abs().mean(1, keepdim=True)

@@ -6,7 +6,7 @@ import pytest
 import torch
 import torch.utils.checkpoint
 
-from oxidizr_amd import ops
+from oxidizr_amd import _lib, ops
 from oxidizr_amd.moe import MoeBlock, MoeConfig
 from tests import ops_ref as ref
 
@@ -834,3 +834,63 @@ def test_linear_gradients_without_rows(grouped, act, dtype):
     dx, dw, db, dr = torch.autograd.grad(y, [x, w, b, r], torch.zeros_like(y))
     assert dx.shape == x.shape and dr.shape == r.shape
     assert dw.shape == w.shape and not bool(dw.any()) and db.shape == b.shape and not bool(db.any())
+
+
+# ---------------------------------------------------------------- what the norm's backward is taken of
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gate", [None, "channel", "token", "full"])
+@pytest.mark.parametrize("T,H", [(1, 64), (130, 776), (66, 2048), (70, 7168), (5, 8200), (3, 16392)])
+def test_norm_gradients_are_those_of_the_unrounded_residual(T, H, gate, dtype):
+    # no rounding of h_out to the dtype between the forward and its gradients
+    for post in (True, False):
+        g = gen(T + H + 7)
+        t = {"h": normal(g, T, H, dtype=dtype, std=2.0), "y": normal(g, T, H, dtype=dtype)}
+        if post:
+            t["w2"] = normal(g, H, dtype=dtype, std=0.2, mean=1.0)
+        if gate:
+            t["gate"] = normal(g, *{"channel": (H,), "token": (T, 1), "full": (T, H)}[gate], dtype=dtype)
+        t["w3"] = normal(g, H, dtype=dtype, std=0.2, mean=1.0)
+        for v in t.values():
+            v.requires_grad_()
+        d_out, d_n = normal(g, T, H, dtype=dtype), normal(g, T, H, dtype=dtype)
+        out, n = ops.residual_norm(t["h"], t["y"], t.get("w2"), gate=t.get("gate"), next_weight=t["w3"],
+                                   residual_scale=1.25, eps=1e-5)
+        got = dict(zip(t, torch.autograd.grad((out, n), list(t.values()), (d_out, d_n))))
+        d = {name: v.detach().double() for name, v in t.items()}
+        want = ref.norm(d["h"], d["y"], d.get("w2"), d.get("gate"), d["w3"], 1.25, 1e-5, d_out.double(),
+                        d_n.double(), dtype, hn_rounded=False)
+        for name, v in got.items():
+            ref.assert_close(v, *want["d" + name], f"d{name} post={post}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", [0, 1, 2, 3])
+def test_the_c_entry_that_takes_the_rounded_residual(kind, dtype):
+    T, H, scale = 37, 520, 0.5
+    g = gen(kind)
+    h, y = normal(g, T, H, dtype=dtype, std=2.0), normal(g, T, H, dtype=dtype)
+    w2, w3 = normal(g, H, dtype=dtype, std=0.2, mean=1.0), normal(g, H, dtype=dtype, std=0.2, mean=1.0)
+    gate = [None, normal(g, H, dtype=dtype), normal(g, T, 1, dtype=dtype), normal(g, T, H, dtype=dtype)][kind]
+    d_out, d_n = normal(g, T, H, dtype=dtype), normal(g, T, H, dtype=dtype)
+    L, code = _lib.load(), _lib.MOE_DTYPE_F32 if dtype == torch.float32 else _lib.MOE_DTYPE_BF16
+    out, n = torch.empty_like(h), torch.empty_like(h)
+    r2, r3 = (torch.empty(T, device="cuda") for _ in range(2))
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def p(t):
+        return None if t is None else t.data_ptr()
+    _lib.check(L.moe_residual_norm(0, stream, code, T, H, p(h), p(y), p(w2), p(gate), kind, p(w3), scale, 1e-5,
+                                   p(out), p(n), p(r2), p(r3)))
+    ws = torch.empty(L.moe_residual_norm_workspace_bytes(T, H), dtype=torch.uint8, device="cuda")
+    d = [None if t is None else t.double() for t in (h, y, w2, gate, w3)]
+    for entry, kept, rounded in ((L.moe_residual_norm_backward, out, True),
+                                 (L.moe_residual_norm_backward_from_input, h, False)):
+        got = {"h": torch.empty_like(h), "y": torch.empty_like(y), "w2": torch.empty_like(w2),
+               "gate": None if gate is None else torch.empty_like(gate), "w3": torch.empty_like(w3)}
+        _lib.check(entry(0, stream, code, T, H, p(d_out), p(d_n), p(kept), p(y), p(w2), p(gate), kind, p(w3), scale,
+                         p(r2), p(r3), p(got["h"]), p(got["y"]), p(got["w2"]), p(got["gate"]), p(got["w3"]), p(ws)))
+        want = ref.norm(*d, scale, 1e-5, d_out.double(), d_n.double(), dtype, hn_rounded=rounded)
+        for name, t in got.items():
+            if t is not None:
+                ref.assert_close(t, *want["d" + name], "d" + name)

@@ -240,3 +240,19 @@ print("done")
 """
     r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and "done" in r.stdout, (r.returncode, r.stderr[-500:])
+
+
+def test_norm_backward_entries_refuse_before_any_device_call():
+    L = _lib.load()
+    for entry in (L.moe_residual_norm_backward, L.moe_residual_norm_backward_from_input):
+        def bwd(T=4, H=16, d_out=P, d_n=P, h=P, y=P, w2=P, gate=None, kind=0, w3=P, r2=P, r3=P, dw2=P, dgate=None,
+                dw3=P, ws=P, dtype=F32):
+            return entry(0, None, dtype, T, H, d_out, d_n, h, y, w2, gate, kind, w3, 1.0, r2, r3, P, P, dw2, dgate,
+                         dw3, ws)
+        assert status(bwd(H=12), "multiple of 8") == 1
+        assert status(bwd(dtype=7), "dtype") == 1
+        assert status(bwd(kind=2), "do not go together") == 1
+        assert status(bwd(kind=2, gate=P), "NULL") == 1
+        for missing in ("h", "r2", "r3", "d_n", "dw2", "dw3", "ws"):
+            assert status(bwd(**{missing: None}), "NULL") == 1
+        assert status(bwd(h=P + 8), "16-byte") == 1
