@@ -14,49 +14,62 @@ enum { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3, kActGeluTanh = 4,
 
 // Activations and their derivatives in fp32.  gelu: z Phi(z) with the error
 // function; gelu_tanh: 0.5 z (1 + tanh(c (z + 0.044715 z^3))), written with the
-// logistic function: 0.5 (1 + tanh(v)) = 1 / (1 + exp(-2 v)).
+// logistic function: 0.5 (1 + tanh(v)) = 1 / (1 + exp(-2 v)).  For float tensors by the device
+// library's expf, erfcf and a division; for bf16 ones, whose results keep 8 bits, by v_exp_f32,
+// v_rcp_f32 and a polynomial, all within 2^-18 of the value.
 constexpr float kGeluC = 0.7978845608028654f;  // sqrt(2 / pi)
-// 1 / (1 + exp(-z)) with v_rcp_f32 (one step) instead of a division (ten instructions):
+// 1 / (1 + exp(-z)); bf16 with v_rcp_f32 (one step) instead of a division (ten instructions):
 // an epilogue runs it 128 times a lane, alone (8192 x 2048 outputs, K = 2816) 9 us of 88.
-MOE_DEV float logistic(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
-// Phi(z) and exp(-z^2 / 2), which erfc(|z| / sqrt 2) = t P(t) exp(-z^2 / 2), t = 1 / (1 + p |z| /
-// sqrt 2), needs as well (Hastings' approximation, Abramowitz and Stegun 7.1.26: erf to
-// 1.5e-7, and the lower tail without 1 - erf's cancellation). With erff the slope of
-// 500 x 2816 outputs took 18.8 us.
-MOE_DEV float normal_cdf(float z, float& e) {
-  const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * 0.7071067811865476f * fabsf(z));
+MOE_DEV float logistic(float z, bf16_t) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
+MOE_DEV float logistic(float z, float) { return 1.0f / (1.0f + expf(-z)); }
+// Phi(z) and exp(-z^2 / 2).  No tail is formed as 1 - erf, which cancels: a value is off by a few
+// fp32 steps of itself, and by z^2 more for the rounding of the exponent's argument.
+MOE_DEV float normal_cdf(float z, float& e, float) {
+  e = expf(-0.5f * z * z);
+  return 0.5f * erfcf(-0.7071067811865476f * z);
+}
+// Phi(-|z|) exp(z^2 / 2) = t P(t), t = 1 / (1 + p |z|): p and P by linear programming for the
+// smallest largest relative error over |z| <= 14, 6.5e-7 (9e-7 in fp32 arithmetic); below -14 Phi is
+// under 2^-146.  With erff the slope of 500 x 2816 outputs took 18.8 us.
+MOE_DEV float normal_cdf(float z, float& e, bf16_t) {
+  const float t = __builtin_amdgcn_rcpf(1.0f + 0.265f * fabsf(z));
   e = __expf(-0.5f * z * z);
-  const float q = 0.5f * e * t *
-                  (0.254829592f +
-                   t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  const float q = e * t *
+                  (0.105599158f +
+                   t * (0.107845433f +
+                        t * (0.0829029307f +
+                             t * (0.142605081f +
+                                  t * (-0.066516608f + t * (0.195381135f + t * -0.0678174347f))))));
   return z < 0.0f ? q : 1.0f - q;
 }
+template <typename T>
 MOE_DEV float act_value(float z, int act) {
   switch (act) {
     case kActRelu: return z <= 0.0f ? 0.0f : z;  // a NaN stays one
-    case kActSilu: return z * logistic(z);
+    case kActSilu: return z * logistic(z, T());
     case kActGelu: {
       float e;
-      return z * normal_cdf(z, e);
+      return z * normal_cdf(z, e, T());
     }
-    case kActGeluTanh: return z * logistic(2.0f * kGeluC * (z + 0.044715f * z * z * z));
+    case kActGeluTanh: return z * logistic(2.0f * kGeluC * (z + 0.044715f * z * z * z), T());
     default: return z;
   }
 }
+template <typename T>
 MOE_DEV float act_slope(float z, int act) {
   switch (act) {
     case kActRelu: return z <= 0.0f ? 0.0f : 1.0f;
     case kActSilu: {
-      const float s = logistic(z);
+      const float s = logistic(z, T());
       return s * (1.0f + z * (1.0f - s));
     }
     case kActGelu: {
       float e;
-      const float cdf = normal_cdf(z, e);
+      const float cdf = normal_cdf(z, e, T());
       return cdf + z * 0.3989422804014327f * e;
     }
     case kActGeluTanh: {
-      const float s = logistic(2.0f * kGeluC * (z + 0.044715f * z * z * z));
+      const float s = logistic(2.0f * kGeluC * (z + 0.044715f * z * z * z), T());
       // s (1 - s) is 0 from |z| = 10 on: squares beyond 1e6 would only make 0 inf a NaN
       const float zz = fminf(z * z, 1e6f);
       return s + s * (1.0f - s) * z * (2.0f * kGeluC * (1.0f + 3.0f * 0.044715f * zz));
@@ -66,10 +79,11 @@ MOE_DEV float act_slope(float z, int act) {
 }
 
 // Eight at once: one branch on the activation, which is the same for the launch.
+template <typename T>
 MOE_DEV void act_value8(const float (&z)[8], float (&y)[8], int act) {
   auto all = [&](auto a) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = act_value(z[i], decltype(a)::value);
+    for (int i = 0; i < 8; ++i) y[i] = act_value<T>(z[i], decltype(a)::value);
   };
   switch (act) {
     case kActRelu: return all(std::integral_constant<int, kActRelu>());
@@ -80,10 +94,11 @@ MOE_DEV void act_value8(const float (&z)[8], float (&y)[8], int act) {
   }
 }
 // d *= act'(z)
+template <typename T>
 MOE_DEV void act_slope8(const float (&z)[8], float (&d)[8], int act) {
   auto all = [&](auto a) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) d[i] *= act_slope(z[i], decltype(a)::value);
+    for (int i = 0; i < 8; ++i) d[i] *= act_slope<T>(z[i], decltype(a)::value);
   };
   switch (act) {
     case kActRelu: return all(std::integral_constant<int, kActRelu>());
@@ -111,7 +126,7 @@ MOE_DEV void linear_store8(const LinearEpi<T>& e, int64_t r, int n, const float 
   const int64_t o = r * e.N + n;
   float y[8];
   if (e.pre) store8(e.pre + o, z);
-  act_value8(z, y, e.act);
+  act_value8<T>(z, y, e.act);
   if constexpr (RES) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] += res[i];
@@ -489,7 +504,7 @@ __global__ __launch_bounds__(256) void k_linear_skinny(const T* __restrict__ X,
       const int64_t o = ((int64_t)r0 + t) * N + n;
       const float z = acc[c][r] + bias;
       if (epi.pre) epi.pre[o] = from_f<T>(z);
-      const float y = act_value(z, epi.act);
+      const float y = act_value<T>(z, epi.act);
       epi.y[o] = from_f<T>(epi.res ? y + to_f<T>(epi.res[o]) : y);
     }
   }
@@ -536,7 +551,7 @@ __global__ __launch_bounds__(256) void k_linear_dz(const T* __restrict__ dY,
   if (act != kActNone) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      act_slope8(z[j], d[j], act);
+      act_slope8<T>(z[j], d[j], act);
       if (n < N && rl + 32 * j < rows) store8(dZ + ((int64_t)r0 + rl + 32 * j) * N + n, d[j]);
     }
   }

@@ -894,3 +894,51 @@ def test_the_c_entry_that_takes_the_rounded_residual(kind, dtype):
         for name, t in got.items():
             if t is not None:
                 ref.assert_close(t, *want["d" + name], "d" + name)
+
+
+# ---------------------------------------------------------------- activations relative to their value
+
+def activation_of(z, act, rows):
+    """act(z) and act'(z) of each z through expert_linear, by way of its bias."""
+    n = (z.numel() + 7) // 8 * 8
+    b = torch.cat([z, z.new_zeros(n - z.numel())]).requires_grad_()
+    y = ops.expert_linear(z.new_zeros(rows, 64), z.new_zeros(n, 64), b, activation=act)
+    dy = torch.zeros_like(y)
+    dy[rows - 1] = 1.0
+    slope, = torch.autograd.grad(y, b, dy)
+    return y.detach()[:, :z.numel()], slope[:z.numel()]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 200])
+def test_gelu_keeps_its_relative_error_in_the_tails(rows, dtype):
+    z = torch.linspace(-12.0, 12.0, 2401).to(dtype).cuda()
+    y, slope = activation_of(z, "gelu", rows)
+    z64 = z.double()
+    cdf = 0.5 * torch.special.erfc(-z64 * 0.5 ** 0.5)
+    pdf = torch.exp(-z64 * z64 / 2) / (2.0 * torch.pi) ** 0.5
+    # fp32: erfc to 16 steps (2^-20) of its value; its argument and exp's are off by 1.5 steps and one, which
+    # moves their values by up to z^2 2^-23 and less.  bf16: 2^-18 for the polynomial and the approximate exp
+    # and reciprocal; exp's argument, rounded twice, by z^2 2^-23
+    rel = (2.0 ** -20 if dtype == torch.float32 else 2.0 ** -18) + z64 * z64 * 2.0 ** -23
+    for r in (0, rows - 1):
+        ref.assert_close(y[r], z64 * cdf, (z64 * cdf).abs() * rel, "gelu")
+    ref.assert_close(slope, cdf + z64 * pdf, (cdf + (z64 * pdf).abs()) * rel, "gelu'")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 200])
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+def test_logistic_activations_keep_their_relative_error(act, rows, dtype):
+    z = torch.linspace(-9.0, 9.0, 2401).to(dtype).cuda()
+    if act == "silu":
+        z = z * 8
+    y, _ = activation_of(z, act, rows)
+    z64 = z.double()
+    # z logistic(a); a of gelu_tanh takes five roundings.  fp32: exp, sum, division and product to some eight
+    # steps together; bf16: v_exp_f32's argument rounded once more, a reciprocal of one step
+    a = z64 if act == "silu" else 2 * (2 / torch.pi) ** 0.5 * (z64 + 0.044715 * z64 ** 3)
+    steps = (0.0 if act == "silu" else 5.0) + (0.0 if dtype == torch.float32 else 2.0)
+    want = z64 * torch.sigmoid(a)
+    for r in (0, rows - 1):
+        ref.assert_close(y[r], want, want.abs() * (8 + steps * a.abs()) * 2.0 ** -24, act)
