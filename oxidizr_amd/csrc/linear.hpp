@@ -117,9 +117,12 @@ struct LinearEpi {
   int act, N;
 };
 
-// Eight outputs of row r from column n on.  The pre-activation is kept in the
-// dtype: a bf16 z is off by at most 2^-9 of itself, which moves act'(z) by less than
-// the rounding of dz behind it.
+// Eight outputs of row r from column n on.  The pre-activation is kept in the dtype.  A bf16 z is
+// off by up to 2^-8 of itself and act'(z) by up to |z act''(z)| 2^-8, which is more than dz's own
+// rounding where the slope is small: silu 5 times it at z = -1, gelu 3 at -2 and 20 at -5.  A choice:
+// kept in fp32 it takes twice the memory of a tensor that lives until the backward and a tenth more
+// traffic, and since dz is rounded to bf16 for the products in any case, gradients over N(0, 1)
+// data come to 2.42e-3 instead of 2.35e-3 (relative L2).
 template <typename T, bool RES>
 MOE_DEV void linear_store8(const LinearEpi<T>& e, int64_t r, int n, const float (&z)[8],
                            const float (&res)[8]) {
