@@ -19,6 +19,9 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
+from torch._C import _get_tracing_state, _len_torch_dispatch_stack
+from torch._ops import _len_torch_dispatch_stack_pre_dispatch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -100,6 +103,29 @@ def _dtype_code(dtype):
     if dtype == torch.float32:
         return _lib.MOE_DTYPE_F32
     raise ModelError(f"unsupported MoE dtype {dtype} (float32 or bfloat16)")
+
+
+def _derivable(*tensors):
+    """Whether a call has to go through its autograd function: a backward may follow, or a forward-mode
+    level is open, whose tensors carry derivatives without requires_grad (the function, which has no
+    forward mode, raises on those)."""
+    if forward_ad._current_level >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _refuse_trace():
+    """A trace records torch's operations, not what the library writes into their results."""
+    tracing = _get_tracing_state()
+    if tracing is None and (_len_torch_dispatch_stack() or _len_torch_dispatch_stack_pre_dispatch()):
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode  # here: its import takes long
+        tracing = get_proxy_mode()
+    if tracing is not None:
+        raise ModelError("this call can not be traced: it would record an uninitialised result")
 
 
 def _p(t):

@@ -10,7 +10,7 @@ experts (src/model.rs:1416-1446), biases, other activations, norms on both sides
 
 Every function takes float32 or bfloat16 CUDA tensors (one dtype to a call; routing weights are
 float32), runs on the current stream of their device, sums in fp32 in a fixed order and is
-differentiable once.  Tensors that are not contiguous or not 16-byte aligned are copied first.
+differentiable once, backward; a forward-mode derivative and a trace (torch.jit.trace, make_fx) are refused.  Tensors that are not contiguous or not 16-byte aligned are copied first.
 Wrong arguments raise ModelError, what the library refuses MoeError.  The arithmetic runs in
 libmoe_hip.so; PyTorch provides memory, streams and the autograd nodes.
 """
@@ -20,7 +20,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .moe import ModelError, _dtype_code
+from .moe import ModelError, _derivable, _dtype_code, _refuse_trace
 
 ACTIVATIONS = ("none", "relu", "silu", "gelu", "gelu_tanh")  # moe_activation's order
 _GATE_NONE, _GATE_CHANNEL, _GATE_TOKEN, _GATE_FULL = range(4)
@@ -59,6 +59,7 @@ def _once(backward):
 
 def _on_device(first, *others):
     """The device index of a call's tensors (the first is always there)."""
+    _refuse_trace()
     dev = first.get_device()
     if dev < 0:
         raise ModelError(f"expected CUDA tensors, got one on {first.device}")
@@ -77,14 +78,6 @@ def _workspace(nbytes, like):
     """Scratch of one call, from the caching allocator: its stream hands the memory out again only
     behind the call's kernels, and a captured call keeps its own in the graph's pool."""
     return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
-
-
-def _tracked(*tensors):
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                return True
-    return False
 
 
 # ---------------------------------------------------------------- tokens sorted by expert and back
@@ -189,7 +182,7 @@ def permute_tokens(x, order: TokenOrder):
     _check_hidden(x.shape[1])
     _dtype_code(x.dtype)
     _on_device(x, slots.inv, slots.offsets)
-    if _tracked(x):
+    if _derivable(x):
         return _Permute.apply(x, slots)
     return _permute(_ready(x), slots)
 
@@ -230,7 +223,7 @@ def unpermute_tokens(y, order: TokenOrder, weights: Optional[torch.Tensor] = Non
     if weights is not None and (weights.dtype != torch.float32 or weights.shape != (T, k)):
         raise ModelError(f"weights must be float32 [{T}, {k}], got {weights.dtype} {list(weights.shape)}")
     _on_device(y, slots.inv, slots.offsets, weights)
-    if _tracked(y, weights):
+    if _derivable(y, weights):
         return _Unpermute.apply(y, weights, slots)
     return _unpermute(_ready(y), slots, _ready(weights))
 
@@ -326,7 +319,7 @@ def expert_linear(x, weight, bias=None, *, offsets=None, activation: str = "none
     for t in (weight, bias, residual):
         if not (t is None or t.dtype == x.dtype):
             raise ModelError("x, weight, bias and residual must have one dtype")
-    tracked = _tracked(x, weight, bias, residual)
+    tracked = _derivable(x, weight, bias, residual)
     if tracked and M * max(K, N) * x.element_size() >= 1 << 31:
         raise ModelError(f"{M} rows of {max(K, N)} reach 2^31 bytes, more than a backward takes: split the batch")
     _on_device(x, weight, bias, residual, offsets)
@@ -438,7 +431,7 @@ def rms_norm(x, weight, eps: float = 1e-6):
     H = _check_norm(x, weight)
     _on_device(x, weight)
     s = _NormShape(x.numel() // H, H, _GATE_NONE, 1.0, eps)
-    if _tracked(x, weight):
+    if _derivable(x, weight):
         return _ResidualNorm.apply(x, None, None, None, weight, s)
     return _norm(_ready(x), None, None, None, _ready(weight), s, False)[1]
 
@@ -460,7 +453,7 @@ def residual_norm(h, y, post_weight=None, *, gate=None, next_weight=None, residu
     kind = _gate_kind(gate, h)
     _on_device(h, y, post_weight, gate, next_weight)
     s = _NormShape(h.numel() // H, H, kind, float(residual_scale), eps)
-    if _tracked(h, y, post_weight, gate, next_weight):
+    if _derivable(h, y, post_weight, gate, next_weight):
         return _ResidualNorm.apply(h, y, post_weight, gate, next_weight, s)
     out, n, _, _ = _norm(_ready(h), _ready(y), _ready(post_weight), _ready(gate), _ready(next_weight), s, False)
     return out if n is None else (out, n)

@@ -7,7 +7,7 @@ import torch
 import torch.utils.checkpoint
 
 from oxidizr_amd import _lib, ops
-from oxidizr_amd.moe import MoeBlock, MoeConfig
+from oxidizr_amd.moe import MoeBlock, MoeConfig, ModelError
 from tests import ops_ref as ref
 
 pytestmark = pytest.mark.gpu
@@ -942,3 +942,24 @@ def test_logistic_activations_keep_their_relative_error(act, rows, dtype):
     want = z64 * torch.sigmoid(a)
     for r in (0, rows - 1):
         ref.assert_close(y[r], want, want.abs() * (8 + steps * a.abs()) * 2.0 ** -24, act)
+
+
+# ---------------------------------------------------------------- derivatives that the operators do not have
+
+def test_forward_mode_and_traces_are_refused_on_the_device():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    g = gen(2)
+    x, w = normal(g, 40, 64), normal(g, 64)
+    order = ops.sort_tokens(routing(g, 40, 2, 4), 4)
+    calls = [lambda t: ops.rms_norm(t, w), lambda t: ops.permute_tokens(t, order),
+             lambda t: ops.unpermute_tokens(torch.cat([t, t]), order), lambda t: ops.expert_linear(t, w[None].repeat(8, 1)),
+             lambda t: ops.residual_norm(t, t)]
+    for call in calls:
+        want = call(x)
+        with torch.autograd.forward_ad.dual_level():
+            with pytest.raises(NotImplementedError, match="forward mode"):
+                call(torch.autograd.forward_ad.make_dual(x, x))
+            assert torch.equal(call(x), want)
+        with pytest.raises(ModelError, match="traced"):
+            make_fx(call)(x)
+        assert torch.equal(call(x), want)

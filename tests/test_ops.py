@@ -256,3 +256,66 @@ def test_norm_backward_entries_refuse_before_any_device_call():
         for missing in ("h", "r2", "r3", "d_n", "dw2", "dw3", "ws"):
             assert status(bwd(**{missing: None}), "NULL") == 1
         assert status(bwd(h=P + 8), "16-byte") == 1
+
+
+# ---- forward-mode derivatives and traces: nothing may come back without them
+
+def calls(t, order_=None):
+    """One call of each operator on tensors made by t(shape), by name."""
+    o = order_ or order()
+    return {
+        "permute": lambda x: ops.permute_tokens(x, o),
+        "unpermute": lambda x: ops.unpermute_tokens(torch.cat([x, x]), o, t(4, 2)),
+        "weights": lambda x: ops.unpermute_tokens(t(8, 16), o, x[:, :2].contiguous()),
+        "linear": lambda x: ops.expert_linear(x, t(8, 16)),
+        "residual": lambda x: ops.expert_linear(t(4, 16), t(16, 16), residual=x),
+        "rms_norm": lambda x: ops.rms_norm(x, t(16)),
+        "norm weight": lambda x: ops.rms_norm(t(4, 16), x[0].contiguous()),
+        "residual_norm": lambda x: ops.residual_norm(t(4, 16), x, t(16)),
+    }
+
+
+@pytest.mark.parametrize("name", sorted(calls(None)))
+def test_forward_mode_is_refused(name, monkeypatch):
+    monkeypatch.setattr(ops, "_on_device", lambda *a: 0)
+    monkeypatch.setattr(ops, "_call", lambda *a: None)  # the library is not reached
+    call = calls(torch.ones)[name]
+    with torch.autograd.forward_ad.dual_level():
+        x = torch.autograd.forward_ad.make_dual(torch.ones(4, 16), torch.ones(4, 16))
+        assert not x.requires_grad
+        with pytest.raises(NotImplementedError, match="forward mode"):
+            call(x)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="forward mode"):
+            call(x)
+        call(torch.ones(4, 16))  # without a derivative there is nothing to lose
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+@pytest.mark.parametrize("name", sorted(calls(None)))
+def test_traces_are_refused(name):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    call = calls(torch.ones)[name]
+    x = torch.ones(4, 16)
+    for leaf in (x, x.clone().requires_grad_()):
+        fails("traced", torch.jit.trace, call, leaf, check_trace=False)
+        for pre in (False, True):
+            fails("traced", make_fx(call, pre_dispatch=pre), leaf)
+    fails("CUDA", call, x)  # and outside a trace the call is looked at as before
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+def test_sorting_is_not_traced():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    idx = torch.zeros(4, 2, dtype=torch.int32)
+    fails("traced", torch.jit.trace, lambda i: ops.sort_tokens(i, 3).perm, idx, check_trace=False)
+    fails("traced", make_fx(lambda i: ops.sort_tokens(i, 3).perm), idx)
+
+
+def test_other_modes_are_no_trace():
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Count(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+    with Count():
+        fails("CUDA", ops.rms_norm, torch.ones(4, 16), torch.ones(16))
