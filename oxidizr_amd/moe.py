@@ -497,6 +497,7 @@ class MoeLayer(torch.nn.Module):
         return out
 
     def forward(self, x):
+        _refuse_trace()
         if x.dim() != 3:
             raise ModelError(f"MoE expects [B, Seq, Hidden], got {list(x.shape)}")
         B, S, H = x.shape
@@ -510,7 +511,7 @@ class MoeLayer(torch.nn.Module):
         tracked = [x2d, self.router.gate.weight] + params
         if self.router.bias is not None:
             tracked.append(self.router.bias)
-        if not (torch.is_grad_enabled() and any(t.requires_grad for t in tracked)):
+        if not _derivable(*tracked):
             # no backward can follow: forward-only call, no saved state
             plan = self.plan(x2d)
             shared = params[3 * self.num_experts:] if self.shared_expert is not None else None
@@ -616,6 +617,7 @@ class MoeBlock(torch.nn.Module):
         return out, aux, z
 
     def forward(self, h):
+        _refuse_trace()
         if h.dim() != 3:
             raise ModelError(f"MoE expects [B, Seq, Hidden], got {list(h.shape)}")
         B, S, H = h.shape
@@ -633,7 +635,7 @@ class MoeBlock(torch.nn.Module):
         tracked = [h2d, norm_w, layer.router.gate.weight] + params
         if layer.router.bias is not None:
             tracked.append(layer.router.bias)
-        if not (torch.is_grad_enabled() and any(t.requires_grad for t in tracked)):
+        if not _derivable(*tracked):
             plan = layer.plan(h2d)
             E = layer.num_experts
             shared = params[3 * E:] if layer.shared_expert is not None else None
