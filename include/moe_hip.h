@@ -329,7 +329,7 @@ typedef enum {
  * a range of its groups); with others no access leaves the
  * tensors, but which rows a group has, and whether every row of y is written, is not
  * defined.  Refused with MOE_ERR_UNSUPPORTED: a width above 2^20, a weight matrix of 2^31
- * bytes, more than 2^26 rows, operands of 2^34 bytes (2^31 in the backward). */
+ * bytes, more than 2^26 rows, operands of 2^34 bytes (2^31 where d_weight is asked for). */
 size_t moe_linear_workspace_bytes(int32_t dtype, int64_t num_rows, int32_t in_features,
                                   int32_t out_features, int32_t num_groups, int32_t grouped,
                                   int32_t activation, int32_t backward);

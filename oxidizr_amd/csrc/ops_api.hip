@@ -738,10 +738,18 @@ moe_status moe_linear_backward(int32_t device, void* stream, int32_t dtype, int6
   moe_status st = check_linear(dtype, M, K, N, E, offsets != nullptr, activation);
   if (st != MOE_OK) return st;
   const int64_t b = elt_size(dtype);
-  // the weight gradient's operands reach over all rows of a group
-  if (M * std::max(K, N) * b >= kMaxExtentBytes)
+  // the weight gradient's operands reach over all rows of a group; the others' over a tile's
+  if (d_weight && M * std::max(K, N) * b >= kMaxExtentBytes)
     return fail(MOE_ERR_UNSUPPORTED, "num_rows x max(in, out features) reaches 2^31 bytes");
   if ((st = check_pointers({}, {dx, d_weight, d_bias, workspace})) != MOE_OK) return st;
+  if (M > 0) {
+    if ((st = check_pointers({d_y, x, weight}, {pre_act})) != MOE_OK) return st;
+    if (activation != kActNone && !pre_act)
+      return fail(MOE_ERR_INVALID, "the activation's backward needs pre_act");
+    if (offsets && (st = check_ints({offsets})) != MOE_OK) return st;
+    if (linear_ws(dtype, M, K, N, E, offsets != nullptr, activation, true).total && !workspace)
+      return fail(MOE_ERR_INVALID, "a required pointer is NULL");
+  }
   DeviceScope dev(device);
   HIP_TRY(dev.enter());
   hipStream_t s = (hipStream_t)stream;
@@ -749,12 +757,6 @@ moe_status moe_linear_backward(int32_t device, void* stream, int32_t dtype, int6
     if ((st = zero_async(s, d_weight, (size_t)E * N * K * b)) != MOE_OK) return st;
     return zero_async(s, d_bias, (size_t)E * N * b);
   }
-  if ((st = check_pointers({d_y, x, weight}, {pre_act})) != MOE_OK) return st;
-  if (activation != kActNone && !pre_act)
-    return fail(MOE_ERR_INVALID, "the activation's backward needs pre_act");
-  if (offsets && (st = check_ints({offsets})) != MOE_OK) return st;
-  if (linear_ws(dtype, M, K, N, E, offsets != nullptr, activation, true).total && !workspace)
-    return fail(MOE_ERR_INVALID, "a required pointer is NULL");
   if (dtype == MOE_DTYPE_BF16)
     return linear_backward<bf16_t>(s, M, K, N, E, offsets, (const bf16_t*)d_y, (const bf16_t*)x,
                                    (const bf16_t*)weight, (const bf16_t*)pre_act, activation,

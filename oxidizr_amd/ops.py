@@ -289,8 +289,8 @@ def expert_linear(x, weight, bias=None, *, offsets=None, activation: str = "none
     With offsets (int32 [E + 1], ascending, as sort_tokens gives them, or a range of those with as
     many weights) rows offsets[e] .. offsets[e + 1] of x [M, K] take weight[e] of weight [E, N, K] and
     bias[e] of bias [E, N]; rows of no expert are the residual's, or zeros. Without offsets weight is
-    [N, K] and bias [N]. K and N are multiples of 8. A call that a backward follows takes x and y of less
-    than 2^31 bytes.
+    [N, K] and bias [N]. K and N are multiples of 8. Where weight requires a gradient, x and y hold less than
+    2^31 bytes.
     activation: one of ACTIVATIONS ("gelu" with the error function, "gelu_tanh" approximated)."""
     if activation not in ACTIVATIONS:
         raise ModelError(f"activation must be one of {ACTIVATIONS}, got {activation!r}")
@@ -319,13 +319,14 @@ def expert_linear(x, weight, bias=None, *, offsets=None, activation: str = "none
     for t in (weight, bias, residual):
         if not (t is None or t.dtype == x.dtype):
             raise ModelError("x, weight, bias and residual must have one dtype")
-    tracked = _derivable(x, weight, bias, residual)
-    if tracked and M * max(K, N) * x.element_size() >= 1 << 31:
-        raise ModelError(f"{M} rows of {max(K, N)} reach 2^31 bytes, more than a backward takes: split the batch")
+    # the operands of the weight's gradient reach over all rows
+    if M * max(K, N) * x.element_size() >= 1 << 31 and torch.is_grad_enabled() and weight.requires_grad:
+        raise ModelError(f"{M} rows of {max(K, N)} reach 2^31 bytes, more than the weight's gradient takes: "
+                         "split the batch")
     _on_device(x, weight, bias, residual, offsets)
     s = _LinearShape(M, K, N, groups, grouped, ACTIVATIONS.index(activation))
     offsets = offsets.contiguous() if grouped else None
-    if tracked:
+    if _derivable(x, weight, bias, residual):
         return _ExpertLinear.apply(x, weight, bias, residual, offsets, s)
     return _linear(_ready(x), _ready(weight), _ready(bias), offsets,
                    _ready(residual), s, False)[0]

@@ -963,3 +963,37 @@ def test_forward_mode_and_traces_are_refused_on_the_device():
         with pytest.raises(ModelError, match="traced"):
             make_fx(call)(x)
         assert torch.equal(call(x), want)
+
+
+# ---------------------------------------------------------------- gradients past 2^31 bytes, without the weight's
+
+@pytest.mark.parametrize("grouped", [True, False])
+@pytest.mark.parametrize("K,N", [(64, 4104), (4104, 64)])
+def test_gradients_of_rows_past_2_31_bytes_without_the_weights(K, N, grouped):
+    M, dt = 262151, torch.bfloat16
+    assert M * max(K, N) * 2 > 2 ** 31
+    g = gen(K)
+    x, r = normal(g, M, K, dtype=dt).requires_grad_(), normal(g, M, N, dtype=dt).requires_grad_()
+    w = normal(g, *((3, N, K) if grouped else (N, K)), dtype=dt, std=K ** -0.5)
+    b = normal(g, *((3, N) if grouped else (N,)), dtype=dt, std=0.3).requires_grad_()
+    edges = [0, 100000, 100000, M - 4]
+    off = torch.tensor(edges, dtype=torch.int32, device="cuda") if grouped else None
+    dy = normal(g, M, N, dtype=dt)
+    y = ops.expert_linear(x, w, b, offsets=off, activation="silu", residual=r)
+    dx, db, dr = torch.autograd.grad(y, [x, b, r], dy)
+    assert torch.equal(dr, dy)
+    for e, (lo, hi) in enumerate(zip(edges, edges[1:]) if grouped else [(0, M)]):
+        want, bound = torch.zeros(N, dtype=torch.float64, device="cuda"), 0.0
+        for i in range(lo, hi, 16384):
+            s = slice(i, min(i + 16384, hi))
+            part = ref.linear(x.detach()[s].double(), (w[e] if grouped else w).double(),
+                              (b.detach()[e] if grouped else b.detach()).double(), None, "silu",
+                              r.detach()[s].double(), dy[s].double(), dt)
+            ref.assert_close(y.detach()[s], *part["y"], "y")
+            ref.assert_close(dx[s], *part["dx"], "dx")
+            want += part["db"][0]
+            bound = bound + part["db"][1] + (hi - lo) / 64 * ref.U32 * part["db"][0].abs()
+        # the chunks' sums add up in fp32: at most (hi - lo) / 64 more terms, each smaller than their bounds' sums
+        ref.assert_close(db[e] if grouped else db, want, bound + (hi - lo) * ref.U32 * dy[lo:hi].double().abs().sum(0), "db")
+    if grouped:
+        assert not bool(dx[M - 4:].any()) and torch.equal(y[M - 4:], r[M - 4:])

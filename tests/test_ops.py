@@ -319,3 +319,15 @@ def test_other_modes_are_no_trace():
             return func(*args, **(kwargs or {}))
     with Count():
         fails("CUDA", ops.rms_norm, torch.ones(4, 16), torch.ones(16))
+
+
+def test_only_the_weights_gradient_is_refused_past_2_31_bytes():
+    x = torch.zeros(1, 1024).expand(1 << 19, 1024)
+    w, b = torch.zeros(8, 1024), torch.zeros(8, requires_grad=True)
+    r = torch.zeros(1 << 19, 8, requires_grad=True)
+    fails("reach 2\\^31 bytes", ops.expert_linear, x, w.clone().requires_grad_())
+    for kw in ({"bias": b}, {"residual": r}):
+        fails("CUDA", ops.expert_linear, x, w, **kw)  # taken, as far as the device
+    L, M, K = _lib.load(), 2 ** 21, 1024
+    assert status(L.moe_linear_backward(0, None, BF16, M, K, 8, 3, P, P, P, P, None, 0, P, P, P, P), "2^31") == 4
+    assert status(L.moe_linear_backward(0, None, BF16, M, K, 8, 3, P, None, P, P, None, 0, P, None, P, P), "NULL") == 1
