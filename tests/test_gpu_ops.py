@@ -997,3 +997,24 @@ def test_gradients_of_rows_past_2_31_bytes_without_the_weights(K, N, grouped):
         ref.assert_close(db[e] if grouped else db, want, bound + (hi - lo) * ref.U32 * dy[lo:hi].double().abs().sum(0), "db")
     if grouped:
         assert not bool(dx[M - 4:].any()) and torch.equal(y[M - 4:], r[M - 4:])
+
+
+# ---------------------------------------------------------------- what of an order a backward needs
+
+def test_counts_and_perm_may_be_written_before_a_backward():
+    g = gen(8)
+    idx = routing(g, 20, 2, 4, pad=0.2)
+    w = torch.rand(20, 2, device="cuda", generator=g)
+    x = normal(g, 20, 64).requires_grad_()
+
+    def run(write):
+        order = ops.sort_tokens(idx, 4)
+        check_order(order, idx, 4)
+        out = ops.unpermute_tokens(ops.permute_tokens(x, order), order, w)
+        write(order)
+        return torch.autograd.grad(out, x, torch.ones_like(out))[0]
+    want = run(lambda o: None)
+    assert torch.equal(run(lambda o: (o.counts.add_(1), o.perm.zero_())), want)
+    for field in ("inv_perm", "offsets"):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            run(lambda o: getattr(o, field).zero_())
