@@ -329,7 +329,9 @@ typedef enum {
  * a range of its groups); with others no access leaves the
  * tensors, but which rows a group has, and whether every row of y is written, is not
  * defined.  Refused with MOE_ERR_UNSUPPORTED: a width above 2^20, a weight matrix of 2^31
- * bytes, more than 2^26 rows, operands of 2^34 bytes (2^31 where d_weight is asked for). */
+ * bytes, more than 2^26 rows, operands of 2^34 bytes (2^31 where d_weight is asked for), and
+ * more tiles than a launch holds (a thousand groups of a million columns).  moe_linear_workspace_bytes
+ * is 0 for a refused call, backward: for one that asks for dx and d_weight. */
 size_t moe_linear_workspace_bytes(int32_t dtype, int64_t num_rows, int32_t in_features,
                                   int32_t out_features, int32_t num_groups, int32_t grouped,
                                   int32_t activation, int32_t backward);

@@ -11,6 +11,7 @@ LIB_PATH = os.path.join(_HERE, "libmoe_hip.so")
 
 MOE_DTYPE_F32 = 0
 MOE_DTYPE_BF16 = 1
+MOE_ERR_UNSUPPORTED = 4
 
 SAVED_FIELDS = ["logits", "probs", "lse", "topk_idx", "topk_w", "counts", "offsets", "perm",
                 "inv_perm", "mean_prob", "x_perm", "gate_act", "up_act", "swiglu", "expert_out",

@@ -53,10 +53,12 @@ inline bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 // Clears n bytes of device memory at q on stream s with a kernel (graph
 // capture records no memset node for it).
 static inline moe_status zero_async(hipStream_t s, void* q, size_t n) {
-  if (!q || n == 0) return MOE_OK;
-  const int64_t vecs = ((int64_t)n + 15) / 16;
-  hipLaunchKernelGGL(k_zero, dim3((unsigned)((vecs + 255) / 256)), dim3(256), 0, s, (uint8_t*)q,
-                     (int64_t)n);
+  if (!q) return MOE_OK;
+  constexpr size_t kMost = size_t(1) << 35;  // 2^31 threads of 16 bytes, half of what a launch takes
+  for (size_t at = 0; at < n; at += kMost) {
+    const int64_t part = (int64_t)std::min(kMost, n - at), vecs = (part + 15) / 16;
+    hipLaunchKernelGGL(k_zero, dim3((unsigned)((vecs + 255) / 256)), dim3(256), 0, s, (uint8_t*)q + at, part);
+  }
   LAUNCH_CHECK();
   return MOE_OK;
 }

@@ -58,7 +58,7 @@ moe_status check_ints(std::initializer_list<const void*> needed, size_t bytes = 
 constexpr int64_t kMaxGridThreads = int64_t(1) << 32;
 moe_status check_grid(int64_t blocks, int threads) {
   if (blocks * threads >= kMaxGridThreads)
-    return fail(MOE_ERR_UNSUPPORTED, "too many rows for one launch: split the batch");
+    return fail(MOE_ERR_UNSUPPORTED, "too many rows or tiles for one launch: split the batch");
   return MOE_OK;
 }
 
@@ -345,7 +345,7 @@ int64_t skinny_blocks(int64_t M, int N, int E, bool grouped, int split) {
 template <typename D>
 bool linear_skinny(int64_t M, int K, int N, int E, bool grouped) {
   const int64_t groups = grouped ? std::min<int64_t>(E, M) : 1;
-  // a thousand experts a million columns wide are more workgroups than a launch holds
+  // a thousand experts a million columns wide can be more workgroups than a launch holds
   if (skinny_blocks(M, N, E, grouped, skinny_split<D>(K)) * 256 >= kMaxGridThreads) return false;
   const bool idle = groups * ceil_div(N, 128) <= (grouped ? 128 : 32);
   if (sizeof(D) == 4) return M <= (grouped ? 16 * groups : kLinearSkinnyRows);
@@ -391,33 +391,54 @@ RowTiles pick_tiles(bool grouped, int E, int64_t M, int N) {
   return RowTiles::kBig;
 }
 
+// Blocks of a launch of C over M rows in E groups, or dense, with N output columns.
+template <class C>
+constexpr int prefix_rows() { return C::XR == 128 ? C::AR : C::BM; }
+template <class C>
+int64_t row_grid(bool grouped, int E, int64_t M, int N) {
+  if (!grouped) return (int64_t)ceil_div(M, C::AR) * ceil_div(N, C::BN);
+  const int64_t mt = ceil_div(M, prefix_rows<C>()) + E;
+  return (mt * ceil_div(N, C::BN) + 7) / 8 * 8;
+}
+
+// Calls f(tiling).
+template <typename D, class F>
+void with_tiling(RowTiles kind, F&& f) {
+  using C = typename Tilings<D>::Big;
+  if constexpr (has_half_rows<D, C>()) {
+    if (kind == RowTiles::kTall) return f(Rows384<C>{});
+    if (kind == RowTiles::kMid) return f(typename LowTilings<C>::Mid{});
+    if (kind == RowTiles::kSmall) return f(typename LowTilings<C>::Small{});
+  }
+  f(C{});
+}
+// Whether that launch, behind `before` other blocks, fits a grid.
+template <typename D>
+moe_status check_tiles(RowTiles kind, bool grouped, int E, int64_t M, int N, int64_t before = 0) {
+  moe_status st = MOE_OK;
+  with_tiling<D>(kind, [&](auto c) {
+    using C = decltype(c);
+    st = check_grid(before + row_grid<C>(grouped, E, M, N), C::THREADS);
+  });
+  return st;
+}
+
 // Calls f(tiling, row groups, grid) for a launch of M rows in E groups (offsets and
 // prefixes of k_linear_prep), or dense (offsets null), with N output columns.
 template <typename D, class F>
 void with_row_tiles(RowTiles kind, const int* offsets, const int* prefixes, int E, int64_t M, int N,
                     F&& f) {
-  using C = typename Tilings<D>::Big;
-  const bool grouped = offsets != nullptr;
-  auto go = [&](auto c, int half_last, int tall) {
-    using CC = decltype(c);
-    const int rows = CC::XR == 128 ? CC::AR : CC::BM;
-    if (!grouped) {
-      f(c, RowGroups{nullptr, nullptr, nullptr, nullptr, 1, (int)M, 0, 0},
-        (int)((int64_t)ceil_div(M, CC::AR) * ceil_div(N, CC::BN)));
-      return;
-    }
-    const int* tp = prefixes + prefix_slot(rows) * (E + 1);
-    const int64_t mt = ceil_div(M, rows) + E;
-    f(c, RowGroups{offsets, tp, tp + (E + 1), tp + 2 * (E + 1), E, (int)M, half_last, tall},
-      8 * ceil_div(mt * ceil_div(N, CC::BN), 8));
-  };
-  if constexpr (has_half_rows<D, C>()) {
-    if (kind == RowTiles::kTall) return go(Rows384<C>{}, 1, 0);
-    if (kind == RowTiles::kMid) return go(typename LowTilings<C>::Mid{}, 0, 0);
-    if (kind == RowTiles::kSmall) return go(typename LowTilings<C>::Small{}, 0, 0);
-    return go(C{}, grouped && M >= 2 * (int64_t)C::BM * E, tall_rows_for(C::BM));
-  }
-  go(C{}, 0, 0);
+  with_tiling<D>(kind, [&](auto c) {
+    using C = decltype(c);
+    const bool grouped = offsets != nullptr;
+    const int grid = (int)row_grid<C>(grouped, E, M, N);
+    if (!grouped) return f(c, RowGroups{nullptr, nullptr, nullptr, nullptr, 1, (int)M, 0, 0}, grid);
+    const int* tp = prefixes + prefix_slot(prefix_rows<C>()) * (E + 1);
+    constexpr bool tall = C::XR == 128, big = std::is_same<C, typename Tilings<D>::Big>::value && sizeof(D) == 2;
+    const int half_last = tall || (big && M >= 2 * (int64_t)C::BM * E);
+    f(c, RowGroups{offsets, tp, tp + (E + 1), tp + 2 * (E + 1), E, (int)M, half_last, big ? tall_rows_for(C::BM) : 0},
+      grid);
+  });
 }
 
 // Both products of a backward as one launch (k_linear_bwd): its estimated time, in
@@ -471,6 +492,28 @@ BwdPlan plan_bwd(bool grouped, int E, int64_t M, int K, int N) {
     }
   }
   return p;
+}
+
+template <typename D>
+int wgrad_blocks(const BwdPlan& p, bool grouped, int E, int K, int N) {
+  using CW = WgradTiling<D, 1>;
+  return kgrouped_grid(grouped ? E : p.split.nsplit, N, K, CW::BM, CW::BN);
+}
+// Whether the launches of a forward, or of a backward of dx and dw (as asked for), fit their grids.
+template <typename D>
+moe_status check_launches(bool backward, bool grouped, int E, int64_t M, int K, int N, bool dx, bool dw) {
+  if (!backward)
+    return linear_skinny<D>(M, K, N, E, grouped) ? MOE_OK
+                                                 : check_tiles<D>(pick_tiles<D>(grouped, E, M, N), grouped, E, M, N);
+  const BwdPlan p = plan_bwd<D>(grouped, E, M, K, N);
+  const int64_t wblocks = dw ? wgrad_blocks<D>(p, grouped, E, K, N) : 0;
+  moe_status st = check_grid(wblocks, WgradTiling<D, 1>::THREADS);
+  if (st == MOE_OK && dx) st = check_tiles<D>(p.tiles, grouped, E, M, K, p.fused ? wblocks : 0);
+  return st;
+}
+moe_status check_launches(int dtype, bool backward, bool grouped, int E, int64_t M, int K, int N, bool dx, bool dw) {
+  return dtype == MOE_DTYPE_BF16 ? check_launches<bf16_t>(backward, grouped, E, M, K, N, dx, dw)
+                                 : check_launches<float>(backward, grouped, E, M, K, N, dx, dw);
 }
 
 struct LinearWs {
@@ -579,7 +622,7 @@ moe_status linear_backward(hipStream_t s, int64_t M, int K, int N, int E, const 
   const BwdPlan bp = plan_bwd<D>(grouped, E, M, K, N);
   const SplitPlan& sp = bp.split;
   const KGroups kg{offs, E, (int)M, sp.nsplit, sp.kchunk, 1, nullptr};
-  const int wgrid = kgrouped_grid(grouped ? E : sp.nsplit, N, K, CW::BM, CW::BN);
+  const int wgrid = wgrad_blocks<D>(bp, grouped, E, K, N);
   float* partial = (float*)(ws + L.splitk);
   auto wgrad = [&](auto g) {
     hipLaunchKernelGGL((k_wgrad<D, 1, decltype(g)::value>), dim3(wgrid), dim3(CW::THREADS), 0, s, dz,
@@ -703,6 +746,7 @@ moe_status moe_unpermute_backward(int32_t device, void* stream, int32_t dtype, i
 size_t moe_linear_workspace_bytes(int32_t dtype, int64_t M, int32_t K, int32_t N, int32_t E,
                                   int32_t grouped, int32_t activation, int32_t backward) {
   if (check_linear(dtype, M, K, N, E, grouped != 0, activation) != MOE_OK) return 0;
+  if (M > 0 && check_launches(dtype, backward != 0, grouped != 0, E, M, K, N, true, true) != MOE_OK) return 0;
   return linear_ws(dtype, M, K, N, E, grouped != 0, activation, backward != 0).total;
 }
 
@@ -716,6 +760,7 @@ moe_status moe_linear_forward(int32_t device, void* stream, int32_t dtype, int64
   if (offsets && ((st = check_ints({offsets})) != MOE_OK ||
                   (st = check_pointers({workspace})) != MOE_OK))
     return st;
+  if ((st = check_launches(dtype, false, offsets != nullptr, E, M, K, N, false, false)) != MOE_OK) return st;
   DeviceScope dev(device);
   HIP_TRY(dev.enter());
   hipStream_t s = (hipStream_t)stream;
@@ -749,6 +794,7 @@ moe_status moe_linear_backward(int32_t device, void* stream, int32_t dtype, int6
     if (offsets && (st = check_ints({offsets})) != MOE_OK) return st;
     if (linear_ws(dtype, M, K, N, E, offsets != nullptr, activation, true).total && !workspace)
       return fail(MOE_ERR_INVALID, "a required pointer is NULL");
+    if ((st = check_launches(dtype, true, offsets != nullptr, E, M, K, N, dx, d_weight)) != MOE_OK) return st;
   }
   DeviceScope dev(device);
   HIP_TRY(dev.enter());

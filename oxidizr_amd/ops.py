@@ -259,6 +259,13 @@ class _ExpertLinear(torch.autograd.Function):
         bias = _ready(bias)
         residual = _ready(residual)
         products = any(ctx.needs_input_grad[:3])  # any gradient that reads the pre-activation
+        if products:
+            # here, where a refused backward can still be told (and calls cost less than in autograd's thread)
+            L = _lib.load()
+            ctx.ws_bytes = L.moe_linear_workspace_bytes(_dtype_code(x.dtype), s.M, s.K, s.N, s.groups, s.grouped,
+                                                        s.act, 1)
+            if ctx.ws_bytes == 0 and s.M > 0:
+                raise _lib.MoeError(_lib.MOE_ERR_UNSUPPORTED, L.moe_last_error().decode())
         y, pre = _linear(x, weight, bias, offsets, residual, s, products and s.act != 0)
         ctx.save_for_backward(x, weight, pre, offsets)
         ctx.s = s
@@ -277,8 +284,7 @@ class _ExpertLinear(torch.autograd.Function):
             dx = torch.empty_like(x) if need_x else None
             dw = torch.empty_like(weight) if need_w else None
             db = up.new_empty((s.groups, s.N) if s.grouped else (s.N,)) if need_b else None
-            ws = _workspace(L.moe_linear_workspace_bytes(code, s.M, s.K, s.N, s.groups, s.grouped,
-                                                         s.act, 1), up)
+            ws = _workspace(ctx.ws_bytes, up)
             _call(L.moe_linear_backward, up.get_device(), code, s.M, s.K, s.N, s.groups, _ptr(offsets),
                   _ptr(up), _ptr(x), _ptr(weight), _ptr(pre), s.act, _ptr(dx), _ptr(dw), _ptr(db),
                   _ptr(ws))

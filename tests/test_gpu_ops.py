@@ -1018,3 +1018,32 @@ def test_counts_and_perm_may_be_written_before_a_backward():
     for field in ("inv_perm", "offsets"):
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             run(lambda o: getattr(o, field).zero_())
+
+
+# ---------------------------------------------------------------- past what one launch holds
+
+def test_a_backward_of_too_many_tiles_is_refused_in_the_forward():
+    E, N = 1024, 1 << 20
+    w = torch.empty(E, N, 8, device="cuda", requires_grad=True)  # 32 GiB, not read
+    x = torch.zeros(100, 8, device="cuda")
+    off = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+    with pytest.raises(_lib.MoeError, match="too many rows or tiles"):
+        ops.expert_linear(x, w, offsets=off)
+    del w
+    torch.cuda.empty_cache()
+
+
+def test_the_gradient_of_no_rows_past_2_36_bytes():
+    # zeros over more bytes than one launch of 16-byte stores covers
+    shape = (33, 32768, 32760)
+    w = torch.empty(shape, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    assert w.numel() * 2 > 2 ** 36
+    block = torch.ones(shape, dtype=torch.bfloat16, device="cuda")
+    del block  # its memory is the gradient's next
+    off = torch.zeros(34, dtype=torch.int32, device="cuda")
+    y = ops.expert_linear(torch.zeros(0, 32760, dtype=torch.bfloat16, device="cuda"), w, offsets=off)
+    dw, = torch.autograd.grad(y, w, torch.zeros_like(y))
+    for part in dw:
+        assert not bool(part.any())
+    del w, dw, y
+    torch.cuda.empty_cache()

@@ -331,3 +331,21 @@ def test_only_the_weights_gradient_is_refused_past_2_31_bytes():
     L, M, K = _lib.load(), 2 ** 21, 1024
     assert status(L.moe_linear_backward(0, None, BF16, M, K, 8, 3, P, P, P, P, None, 0, P, P, P, P), "2^31") == 4
     assert status(L.moe_linear_backward(0, None, BF16, M, K, 8, 3, P, None, P, P, None, 0, P, None, P, P), "NULL") == 1
+
+
+def test_linears_of_more_tiles_than_a_launch_are_refused_at_once():
+    L, N = _lib.load(), 1 << 20
+    fwd, bwd = L.moe_linear_forward, L.moe_linear_backward
+
+    def forward(dtype, M, K, N, E):
+        return fwd(0, None, dtype, M, K, N, E, P, P, P, None, None, 0, P, None, P)
+
+    def backward(dtype, M, K, N, E, dx=P, dw=P):
+        return bwd(0, None, dtype, M, K, N, E, P, P, P, P, None, 0, dx, dw, None, P)
+    # fp32: 16384 column tiles of 64, and as many weight tiles to an expert
+    assert status(forward(F32, 2000, 8, N, 1024), "too many rows or tiles") == 4
+    assert L.moe_linear_workspace_bytes(F32, 2000, 8, N, 1024, 1, 0, 0) == 0
+    assert status(backward(F32, 100, 8, N, 1024), "too many rows or tiles") == 4
+    assert L.moe_linear_workspace_bytes(F32, 100, 8, N, 1024, 1, 0, 1) == 0
+    assert status(backward(F32, 2000, N, 8, 1024, dw=None), "too many rows or tiles") == 4
+    assert L.moe_linear_workspace_bytes(F32, 100, 8, N, 1000, 1, 0, 1) > 0  # just below
