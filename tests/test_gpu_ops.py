@@ -1047,3 +1047,41 @@ def test_the_gradient_of_no_rows_past_2_36_bytes():
         assert not bool(part.any())
     del w, dw, y
     torch.cuda.empty_cache()
+
+
+# ---------------------------------------------------------------- the block in bf16
+
+@pytest.mark.parametrize("post,gate,scale", [(True, False, 1.0), (False, True, 1.0), (True, True, 0.5),
+                                             (False, False, 0.75)])
+def test_block_with_norms_on_both_sides_in_bf16(post, gate, scale):
+    dt = torch.bfloat16
+    cfg = MoeConfig(hidden_size=136, num_experts=6, experts_per_tok=2, intermediate_size=48, post_norm=post,
+                    residual_gate=gate, residual_scale=scale)
+    block = MoeBlock(cfg, dt)
+    g = gen(27)
+    with torch.no_grad():
+        for name, p in block.trainable_parameters():
+            p.normal_(1.0 if "layernorm" in name or name == "residual_gate" else 0.0, 0.1, generator=g)
+    h, up = normal(g, 2, 65, 136, dtype=dt).requires_grad_(), normal(g, 2, 65, 136, dtype=dt)
+    norms = {n: p for n, p in block.named_parameters() if not n.startswith("ffn.")}
+    leaves = [h] + list(norms.values()) + [block.ffn.router.gate.weight]
+    out, aux, z = block(h)
+    got = torch.autograd.grad((out, aux, z), leaves, (up, torch.ones_like(aux), torch.ones_like(z)))
+    # the same calls one by one: the same bits
+    x = ops.rms_norm(h, block.post_attention_layernorm.weight, cfg.rms_norm_eps)
+    y, aux2, z2 = block.ffn(x)
+    w2 = block.post_ffn_layernorm.weight if post else None
+    out2 = ops.residual_norm(h, y, w2, gate=block.residual_gate, residual_scale=scale, eps=cfg.rms_norm_eps)
+    want = torch.autograd.grad((out2, aux2, z2), leaves, (up, torch.ones_like(aux), torch.ones_like(z)))
+    for a, b in zip((out, aux, z) + got, (out2, aux2, z2) + want):
+        assert torch.equal(a, b)
+    # and what is around the layer against float64
+    d = [None if t is None else t.detach().double() for t in (h.view(-1, 136), y.view(-1, 136), w2, block.residual_gate)]
+    ref64 = ref.norm(*d, None, scale, cfg.rms_norm_eps, up.view(-1, 136).double(), None, dt)
+    ref.assert_close(out.detach().view(-1, 136), *ref64["h"], "out")
+    pre = ref.norm(d[0], None, None, None, block.post_attention_layernorm.weight.detach().double(), 1.0,
+                   cfg.rms_norm_eps, None, None, dt)
+    ref.assert_close(x.detach().view(-1, 136), *pre["n"], "x")
+    for name, key in (("post_ffn_layernorm.weight", "dw2"), ("residual_gate", "dgate")):
+        if name in norms:
+            ref.assert_close(got[1 + list(norms).index(name)], *ref64[key], name)
