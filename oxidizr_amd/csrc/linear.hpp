@@ -253,8 +253,8 @@ constexpr int kF32StepVectors = 2;
 // (1050-1110 TFLOP/s; the library's product alone 69), of which the k-loop is some 70;
 // 16 experts of 1024 rows, 1408 x 2048, silu, two outputs, 128-row tiles 115-125 us.
 // The residual of the whole tile is requested when the main loop has
-// ended (in the fragments' registers; a 384-row tile has none left and takes it a pass
-// ahead).
+// ended (in the fragments' registers; a 384-row tile has none left, takes it a pass ahead and
+// spills 40 of its 256 registers, 84 bytes a lane).
 template <typename T, class C>
 __global__ __launch_bounds__(C::THREADS) void k_linear_fwd(const T* __restrict__ X, RowGroups groups,
                                                            const T* const* w_tab, const T* w_one,

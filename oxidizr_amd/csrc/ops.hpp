@@ -437,10 +437,14 @@ __global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void k_norm_fwd(NormArgs<
 // vector.  So a row costs one barrier, and there are at most two column sums:
 //   colA = sum_t D yh (channel or no gate; yh = y without w2) or sum_t g D yh,
 //   colB = sum_t dn hh.
-// A block takes rows b, b + grid, ..; its column sums stay in registers and go to
+// A block takes rows b, b + grid, ..; its column sums stay with their threads and go to
 // part[b] = (colA | colB), which k_norm_colsum adds in order.  The next row's loads are
 // in flight over a row's reduction and stores.  Bound by memory: 8192 x 7168 bf16 (705 MB)
-// 135 us, 5.2 TB/s (without the loads ahead 270).  Forming hn costs some 5 us of them; with the
+// 135 us, 5.2 TB/s (without the loads ahead 270); fp32 8192 x 4096 155 us, 5.2.  That holds up to H =
+// 8192 in bf16 and 4096 in fp32, where all of a thread's columns are in registers.  Wider rows have
+// 128 registers for more (16 waves to a block) and spill 57 (fp32 up to 8192) to 871 of them, 136 to
+// 1600 bytes a lane, and that traffic bounds them: fp32 8192 x 7168 354 us, 4.0 TB/s; 4096 x 16384 472
+// bf16 and 968 fp32, 1.7; 2048 x 32768 848 and 1531, 1.0.  Forming hn costs some 5 us of them; with the
 // rounded hn the gradients were 2.5e-3 off a 64-bit form, now 1.7e-3 (relative L2).
 template <typename T>
 struct NormBwdArgs {

@@ -211,9 +211,11 @@ void with_norm_shape(int H, F&& f) {
 constexpr int norm_waves(int wpr) { return wpr > 4 ? wpr : 4; }
 constexpr int norm_rows(int wpr) { return norm_waves(wpr) / wpr; }
 
-// Blocks of the backward: 16 waves to a CU, all running at once, each adding its rows'
-// column sums in registers. More blocks write more partial rows and gain nothing (H =
-// 7168, T = 8192: 256 blocks 136 us, 512 143, 1024 153; H = 2048: 1024 43, 4096 47).
+// Blocks of the backward: 16 waves to a CU, each adding its rows' column sums. bf16 ones all
+// run at once (four waves to a SIMD); fp32 ones up to H = 4096 take 150 to 168 registers, three waves
+// to a SIMD, so 768 of 1024 blocks (H <= 2048) or 256 of 512 run in the first round and the others
+// behind them. More blocks write more partial rows and gain nothing (bf16 H = 7168, T = 8192: 256
+// blocks 136 us, 512 143, 1024 153; H = 2048: 1024 43, 4096 47).
 constexpr int kNormBwdWaves = 16 * 256;
 int norm_bwd_blocks(int64_t T, int H) {
   int64_t blocks = 1;
@@ -360,7 +362,9 @@ bool linear_skinny(int64_t M, int K, int N, int E, bool grouped) {
 // 125; 8192, 2048, 2816 76 / 98 / 90 / 122; 4096, 2048, 2816 63 / 87 / 47 / 64; 4096, 1408,
 // 2048 45 / 63 / 31 / 34; 1000, 2048, 2816 53 / 82 / 33 / 21; 300, 7168, 2048 41 / 51 / 25 / 23.
 constexpr TileCosts kLinearCosts{10.0, {4.8, 6.3}, {2.9, 4.3}};
-constexpr double kTallCost = 1.55;  // a 384-row tile against a 256-row one
+// A 384-row tile against a 256-row one (its kernel spills 40 registers, 84 bytes a lane, around the
+// epilogue, and was measured so).
+constexpr double kTallCost = 1.55;
 
 enum class RowTiles { kBig, kTall, kMid, kSmall };
 template <typename D>
