@@ -155,19 +155,21 @@ moe_status launch_unpermute_bwd(hipStream_t s, int64_t T, int k, int H, const in
                                 const int* kept, const D* dout, const D* y, const float* w, D* dy,
                                 float* dw) {
   const int slices = ceil_div(H, 64 * Vec16<D>::N);
-  moe_status st = check_grid(T, 256);  // one token to a block at most
-  if (st != MOE_OK) return st;
+  moe_status st = MOE_OK;
   with_k(k, [&](auto kc) {
     constexpr int KM = decltype(kc)::value;
     auto go = [&](auto wpt) {
       constexpr int W = decltype(wpt)::value;
-      hipLaunchKernelGGL((k_unpermute_bwd<D, W, KM>), dim3((unsigned)((T + 4 / W - 1) / (4 / W))),
-                         dim3(256), 0, s, dout, y, inv, kept, w, T, k, H, dy, dw);
+      const int64_t grid = (T + 4 / W - 1) / (4 / W);
+      if ((st = check_grid(grid, 256)) != MOE_OK) return;
+      hipLaunchKernelGGL((k_unpermute_bwd<D, W, KM>), dim3((unsigned)grid), dim3(256), 0, s, dout, y, inv, kept, w, T,
+                         k, H, dy, dw);
     };
     if (slices == 1) go(std::integral_constant<int, 1>());
     else if (slices == 2) go(std::integral_constant<int, 2>());
     else go(std::integral_constant<int, 4>());
   });
+  if (st != MOE_OK) return st;
   LAUNCH_CHECK();
   return MOE_OK;
 }
@@ -228,14 +230,15 @@ int norm_bwd_blocks(int64_t T, int H) {
 
 template <typename D>
 moe_status launch_norm_fwd(hipStream_t s, const NormArgs<D>& a) {
-  moe_status st = check_grid(a.Tn, a.H <= 2048 ? 256 : a.H <= 8192 ? 512 : 1024);
-  if (st != MOE_OK) return st;
+  moe_status st = MOE_OK;
   with_norm_shape<false>(a.H, [&](auto wpr, auto nch) {
     constexpr int W = decltype(wpr)::value;
     const int64_t grid = (a.Tn + norm_rows(W) - 1) / norm_rows(W);
+    if ((st = check_grid(grid, 64 * norm_waves(W))) != MOE_OK) return;
     hipLaunchKernelGGL((k_norm_fwd<D, W, decltype(nch)::value>), dim3((unsigned)grid),
                        dim3(64 * norm_waves(W)), 0, s, a);
   });
+  if (st != MOE_OK) return st;
   LAUNCH_CHECK();
   return MOE_OK;
 }

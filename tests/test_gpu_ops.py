@@ -1085,3 +1085,25 @@ def test_block_with_norms_on_both_sides_in_bf16(post, gate, scale):
     for name, key in (("post_ffn_layernorm.weight", "dw2"), ("residual_gate", "dgate")):
         if name in norms:
             ref.assert_close(got[1 + list(norms).index(name)], *ref64[key], name)
+
+
+def test_rows_of_few_columns_past_2_24():
+    # four rows to a block: 2^24 rows are a quarter of what a launch takes
+    T, H = (1 << 24) + 5, 64
+    g = gen(6)
+    x = normal(g, T, H, dtype=torch.bfloat16)
+    w = normal(g, H, dtype=torch.bfloat16)
+    n = ops.rms_norm(x, w)
+    idx = torch.arange(T, device="cuda", dtype=torch.int32)[:, None] % 7
+    order = ops.sort_tokens(idx, 7)
+    weights = torch.rand(T, 1, device="cuda", generator=g).requires_grad_()
+    y = x.requires_grad_()
+    dy, dw = torch.autograd.grad(ops.unpermute_tokens(y, order, weights), [y, weights], n)
+    for at in (slice(0, 50), slice(T - 50, T)):
+        d = x.detach()[at].double()
+        want = ref.norm(d, None, None, None, w.double(), 1.0, 1e-6, None, None, torch.bfloat16)
+        ref.assert_close(n[at], *want["n"], "n")
+        pos = order.inv_perm[at, 0].long()
+        rows, up = x.detach()[pos].double(), n[at].double()
+        ref.assert_close(dy[pos], weights.detach()[at].double() * up, 0.0, "dy")
+        ref.assert_close(dw[at, 0], (rows * up).sum(1), (H + 8) * ref.U32 * (rows * up).abs().sum(1), "dw")
