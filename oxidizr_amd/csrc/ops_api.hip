@@ -763,11 +763,11 @@ moe_status moe_linear_forward(int32_t device, void* stream, int32_t dtype, int64
                               int32_t activation, void* y, void* pre_act, void* workspace) {
   moe_status st = check_linear(dtype, M, K, N, E, offsets != nullptr, activation);
   if (st != MOE_OK || M == 0) return st;
+  if ((st = check_launches(dtype, false, offsets != nullptr, E, M, K, N, false, false)) != MOE_OK) return st;
   if ((st = check_pointers({x, weight, y}, {bias, residual, pre_act})) != MOE_OK) return st;
   if (offsets && ((st = check_ints({offsets})) != MOE_OK ||
                   (st = check_pointers({workspace})) != MOE_OK))
     return st;
-  if ((st = check_launches(dtype, false, offsets != nullptr, E, M, K, N, false, false)) != MOE_OK) return st;
   DeviceScope dev(device);
   HIP_TRY(dev.enter());
   hipStream_t s = (hipStream_t)stream;
@@ -795,13 +795,13 @@ moe_status moe_linear_backward(int32_t device, void* stream, int32_t dtype, int6
     return fail(MOE_ERR_UNSUPPORTED, "num_rows x max(in, out features) reaches 2^31 bytes");
   if ((st = check_pointers({}, {dx, d_weight, d_bias, workspace})) != MOE_OK) return st;
   if (M > 0) {
+    if ((st = check_launches(dtype, true, offsets != nullptr, E, M, K, N, dx, d_weight)) != MOE_OK) return st;
     if ((st = check_pointers({d_y, x, weight}, {pre_act})) != MOE_OK) return st;
     if (activation != kActNone && !pre_act)
       return fail(MOE_ERR_INVALID, "the activation's backward needs pre_act");
     if (offsets && (st = check_ints({offsets})) != MOE_OK) return st;
     if (linear_ws(dtype, M, K, N, E, offsets != nullptr, activation, true).total && !workspace)
       return fail(MOE_ERR_INVALID, "a required pointer is NULL");
-    if ((st = check_launches(dtype, true, offsets != nullptr, E, M, K, N, dx, d_weight)) != MOE_OK) return st;
   }
   DeviceScope dev(device);
   HIP_TRY(dev.enter());

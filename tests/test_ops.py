@@ -345,6 +345,7 @@ def test_linears_of_more_tiles_than_a_launch_are_refused_at_once():
     # fp32: 16384 column tiles of 64, and as many weight tiles to an expert
     assert status(forward(F32, 2000, 8, N, 1024), "too many rows or tiles") == 4
     assert L.moe_linear_workspace_bytes(F32, 2000, 8, N, 1024, 1, 0, 0) == 0
+    assert status(fwd(0, None, F32, 2000, 8, N, 1024, P, P, P, None, None, 0, P, None, None), "too many") == 4
     assert status(backward(F32, 100, 8, N, 1024), "too many rows or tiles") == 4
     assert L.moe_linear_workspace_bytes(F32, 100, 8, N, 1024, 1, 0, 1) == 0
     assert status(backward(F32, 2000, N, 8, 1024, dw=None), "too many rows or tiles") == 4
