@@ -97,11 +97,11 @@ def sort_tokens(topk_idx, num_experts: int) -> TokenOrder:
     dev = _on_device(topk_idx)
     idx = topk_idx.contiguous()
     L = _lib.load()
-    # one allocation for all four; .data gives perm and counts a version counter apart from that of inv
-    # and offsets, which gradients read: writing to the former before a backward is no error
+    # one allocation for all four; .data gives perm and counts version counters of their own, apart from that
+    # of inv and offsets, which gradients read: writing to the former before a backward is no error
     out = torch.empty(2 * num_experts + 1 + 2 * T * k, dtype=torch.int32, device=idx.device)
-    inv, offsets, rest = out.split((T * k, num_experts + 1, T * k + num_experts))
-    perm, counts = rest.data.split((T * k, num_experts))
+    perm, inv, offsets, counts = out.split((T * k, T * k, num_experts + 1, num_experts))
+    perm, counts = perm.data, counts.data
     ws = _workspace(L.moe_sort_workspace_bytes(T, k, num_experts), idx)
     _call(L.moe_sort_tokens, dev, T, k, num_experts, idx.element_size(), idx.data_ptr(), counts.data_ptr(),
           offsets.data_ptr(), perm.data_ptr(), inv.data_ptr(), _ptr(ws))
