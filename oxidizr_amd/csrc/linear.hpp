@@ -16,7 +16,7 @@ enum { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3, kActGeluTanh = 4,
 // function; gelu_tanh: 0.5 z (1 + tanh(c (z + 0.044715 z^3))), written with the
 // logistic function: 0.5 (1 + tanh(v)) = 1 / (1 + exp(-2 v)).  For float tensors by the device
 // library's expf, erfcf and a division; for bf16 ones, whose results keep 8 bits, by v_exp_f32,
-// v_rcp_f32 and a polynomial, all within 2^-18 of the value.
+// v_rcp_f32 and a polynomial, within 2^-16 of the value.
 constexpr float kGeluC = 0.7978845608028654f;  // sqrt(2 / pi)
 // 1 / (1 + exp(-z)); bf16 with v_rcp_f32 (one step) instead of a division (ten instructions):
 // an epilogue runs it 128 times a lane, alone (8192 x 2048 outputs, K = 2816) 9 us of 88.
