@@ -76,6 +76,22 @@ def test_drawn_products(programs):
     run(programs["linear"], lines)
 
 
+def test_ranges_of_experts_and_offsets_that_are_none(programs):
+    # a range of a longer array, whose other rows are no group's; and offsets of any values, which may leave rows
+    # undefined but no buffer
+    r = random.Random(9)
+    lines = []
+    for i in range(60):
+        M, E = r.choice((7, 40, 300, 900)), r.choice((1, 2, 5, 40, 130))
+        top = r.choice((M, M, M // 2, 3 * M, 2 ** 31 - 1))
+        offsets = [r.randint(-5 if i % 3 else 0, top) for _ in range(E + 1)]
+        if i % 2:
+            offsets = sorted(min(max(o, 0), M) for o in offsets)
+        lines.append(f"?offsets{i} {i % 4 > 0:d} {i % 5} 1 {i % 2} 1 {r.choice((-1, -1, 0, 1, 2, 3, 4)) if i % 4 else -1} "
+                     f"{r.choice((24, 136))} {r.choice((40, 264))} {M} " + " ".join(map(str, offsets)))
+    run(programs["linear"], lines)
+
+
 def test_sorting_rows_and_norms(programs):
     lines = ["sort a 4 1 1 1 0", "sort b 8 300 5 33 4", "sort c 4 5000 6 64 9", "sort d 4 40 16 1024 3", "sort e 8 0 2 3 0",
              "rows f 0 33 3 12 520 5", "rows g 1 64 8 16 4096 0", "rows h 1 7 16 8 64 2", "rows i 1 5 2 7 1032 0",
