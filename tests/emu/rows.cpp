@@ -1,6 +1,7 @@
 // The sort, row and norm entries on the emulated device.  Each input line is one call:
 //   sort name index_bytes T k E pad            (against a stable sort; pad: every pad-th index has no expert)
-//   rows name dtype T k E H pad                (permute, unpermute with and without weights, their gradients)
+//   rows name dtype T k E H pad                (permute, unpermute with and without weights, their gradients;
+//                                               pad < 0: over an order that no sort made)
 //   norm name dtype T H gate post next given   (forward and backward; given: from h_out)
 // Buffers are of exactly their sizes: every access is checked, and that every output is written.
 #include <unistd.h>
@@ -98,8 +99,13 @@ int main() {
       int64_t T;
       in >> dtype >> T >> k >> E >> H >> pad;
       const size_t b = dtype == MOE_DTYPE_F32 ? 4 : 2;
-      Order o(T, k, E, 4, pad);
-      const int* inv = (int*)o.inv.p;
+      Order o(T, k, E, 4, std::max(pad, 0));
+      int* inv = (int*)o.inv.p;
+      if (pad < 0) {
+        const int any[] = {-1, INT_MAX, INT_MIN, (int)(T * k), (int)(T * k) - 1, 1000000007};
+        for (int64_t i = 0; i < T * k; i += 3) inv[i] = any[i / 3 % 6];
+        ((int*)o.offsets.p)[E] = pad == -1 ? INT_MAX : pad == -2 ? -7 : (int)(T * k) + 1;
+      }
       const int* kept = (int*)o.offsets.p + E;
       Buffer x(T * H * b), y(T * k * H * b), w(T * k * 4);
       Out xp(y.n), out(x.n), plain(x.n), dy(y.n), dy2(y.n), dw(w.n);
@@ -110,7 +116,8 @@ int main() {
                  MOE_OK, "backward");
       expect(moe_unpermute_backward(0, nullptr, dtype, T, k, H, inv, kept, x.p, nullptr, nullptr, dy2.p, nullptr) ==
                  MOE_OK, "backward");
-      xp.written("x_perm"), out.written("out"), plain.written("out"), dy.written("d_y"), dy2.written("d_y");
+      if (pad >= 0) xp.written("x_perm"), dy.written("d_y"), dy2.written("d_y");
+      out.written("out"), plain.written("out");
       dw.written("d_weights");
     } else {
       int dtype, H, gate, post, next, given;
