@@ -19,9 +19,9 @@ pytestmark = pytest.mark.skipif(not os.path.exists(emu.CLANG), reason="needs ROC
 
 @pytest.fixture(scope="module")
 def programs(tmp_path_factory):
+    to = {name: tmp_path_factory.mktemp(name) / "build" for name in ("linear", "rows")}
     with ThreadPoolExecutor(2) as pool:
-        return dict(zip(("linear", "rows"), pool.map(
-            lambda p: emu.build(tmp_path_factory.mktemp(p) / "build", p), ("linear", "rows"))))
+        return dict(zip(to, pool.map(emu.build, to.values(), to)))
 
 
 def run(program, lines):
