@@ -10,7 +10,8 @@ experts (src/model.rs:1416-1446), biases, other activations, norms on both sides
 
 Every function takes float32 or bfloat16 CUDA tensors (one dtype to a call; routing weights are
 float32), runs on the current stream of their device, sums in fp32 in a fixed order and is
-differentiable once, backward; a forward-mode derivative and a trace (torch.jit.trace, make_fx) are refused.  Tensors that are not contiguous or not 16-byte aligned are copied first.
+differentiable once, backward; a forward-mode derivative and a trace (torch.jit.trace, make_fx) are
+refused.  Tensors that are not contiguous or not 16-byte aligned are copied first.
 Wrong arguments raise ModelError, what the library refuses MoeError.  The arithmetic runs in
 libmoe_hip.so; PyTorch provides memory, streams and the autograd nodes.
 """
