@@ -19,8 +19,8 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
-from torch._C import _get_tracing_state, _len_torch_dispatch_stack
-from torch._ops import _len_torch_dispatch_stack_pre_dispatch
+from torch._C import _get_dispatch_mode, _get_tracing_state, _len_torch_dispatch_stack, _TorchDispatchModeKey
+from torch._ops import mode_stack_state_for_pre_dispatch
 from torch.autograd import forward_ad
 
 from . import _lib
@@ -118,13 +118,13 @@ def _derivable(*tensors):
     return False
 
 
+_pre_dispatch_modes = mode_stack_state_for_pre_dispatch()
+
+
 def _refuse_trace():
     """A trace records torch's operations, not what the library writes into their results."""
-    tracing = _get_tracing_state()
-    if tracing is None and (_len_torch_dispatch_stack() or _len_torch_dispatch_stack_pre_dispatch()):
-        from torch.fx.experimental.proxy_tensor import get_proxy_mode  # here: its import takes long
-        tracing = get_proxy_mode()
-    if tracing is not None:
+    if (_get_tracing_state() is not None or _pre_dispatch_modes.get(0) is not None or  # 0: make_fx's mode
+            (_len_torch_dispatch_stack() and _get_dispatch_mode(_TorchDispatchModeKey.PROXY) is not None)):
         raise ModelError("this call can not be traced: it would record an uninitialised result")
 
 
