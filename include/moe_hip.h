@@ -390,6 +390,67 @@ moe_status moe_residual_norm_backward_from_input(int32_t device, void* stream, i
                                       void* d_post_weight, void* d_gate, void* d_next_weight,
                                       void* workspace);
 
+/* Losses of a router over given logits [T, E] and chosen experts topk_idx [T, k] (int32 or int64 by
+ * index_bytes), and the experts' counts.  A token is real when one of its indices is in [0, E); rows of others are
+ * not read into any sum and have no gradient.  For each sequence s of offsets [S + 1] (rows offsets[s] ..
+ * offsets[s + 1]; NULL: one sequence of all rows, S = 1) with n real tokens and M_e assignments to expert e:
+ *   x = logits / temperature, q = softmax(x) or sigmoid(x) / sum sigmoid(x), P_e = sum q_te / n, f_e = M_e / (k n),
+ *   balance[s] = E sum_e (switch_coef f_e P_e + sqprob_coef P_e^2), z[s] = sum logsumexp(x_t)^2 / n
+ * (0 for n = 0), counts [S, E] = M_e.  1 <= E <= 1024, 1 <= k <= 16, T k < 2^31, S < 2^22.  slope [S, E] (of
+ * balance in q_te), inv_real [S] (1 / n, or 0) and lse [T]: kept for a backward, or NULL.  Offsets ascend within 0..T; with others no access
+ * leaves the tensors, but the results are not defined. */
+typedef enum { MOE_SCORE_SOFTMAX = 0, MOE_SCORE_SIGMOID } moe_score;
+size_t moe_router_losses_workspace_bytes(int64_t num_tokens, int32_t num_experts, int64_t num_sequences);
+moe_status moe_router_losses(int32_t device, void* stream, int32_t dtype, int64_t num_tokens,
+                             int32_t num_experts, int32_t experts_per_tok, int32_t index_bytes,
+                             const void* logits, const void* topk_idx, int32_t score, float temperature,
+                             float switch_coef, float sqprob_coef, const int32_t* offsets,
+                             int64_t num_sequences, float* balance, float* z, int32_t* counts,
+                             float* slope, float* inv_real, float* lse, void* workspace);
+/* d_logits [T, E] of d_balance and d_z [S] (either may be NULL: 0), for what the forward was given and kept. */
+moe_status moe_router_losses_backward(int32_t device, void* stream, int32_t dtype, int64_t num_tokens,
+                                      int32_t num_experts, int32_t experts_per_tok, int32_t index_bytes,
+                                      const void* logits, const void* topk_idx, int32_t score,
+                                      float temperature, const int32_t* offsets, int64_t num_sequences,
+                                      const float* slope, const float* inv_real, const float* lse,
+                                      const float* d_balance, const float* d_z, void* d_logits);
+
+/* Microscaled 4-bit numbers (OCP MXFP4).  32 elements share a scale 2^s, a byte s + 127 (255: NaN); an element
+ * is a sign (bit 3) and a code 0..7 of 0 0.5 1 1.5 2 3 4 6; element 2 i of a row is the low half of its byte i.  A
+ * tensor [.., K], K a multiple of 32, is codes [.., K / 2] and scales [.., K / 32].  Quantising num_blocks blocks of
+ * 32: s = floor(log2 of the largest magnitude) - 2, at least -127; to the nearest code, ties to the even one, what is
+ * above the largest becomes it; a block with an infinity or a NaN becomes NaN (scale 255).  Codes are 16-byte
+ * aligned, scales have any alignment.  num_blocks < 2^30. */
+moe_status moe_mx_quantize(int32_t device, void* stream, int32_t dtype, int64_t num_blocks, const void* x,
+                           uint8_t* codes, uint8_t* scales);
+/* The numbers that they stand for, in fp32 or bf16 (both hold them exactly but for 6 2^127 in bf16, which
+ * becomes infinite; no quantised block reaches it). */
+moe_status moe_mx_dequantize(int32_t device, void* stream, int32_t dtype, int64_t num_blocks,
+                             const uint8_t* codes, const uint8_t* scales, void* y);
+
+/* moe_linear_forward over 4-bit weights w_codes [G, N, K / 2], w_scales [G, N, K / 32].  x_format: bf16 rows x [M, K]
+ * (dtype bf16), or 4-bit rows x [M, K / 2] with x_scales [M, K / 32].  bias [G, N], residual, y and pre_act [M, N] are
+ * of dtype.  in_features K is a multiple of 32, out_features N of 8; products are summed in fp32.  Refused with
+ * MOE_ERR_UNSUPPORTED: a width above 2^20, a weight matrix of 2^30 elements, more than 2^26 rows, rows x max(K, N) of
+ * 2^34 bytes, and more tiles than a launch holds.  moe_mx_linear_workspace_bytes is 0 for a refused call. */
+typedef enum { MOE_MX_ROWS_BF16 = 0, MOE_MX_ROWS_FOUR_BIT } moe_mx_rows;
+size_t moe_mx_linear_workspace_bytes(int32_t x_format, int32_t dtype, int64_t num_rows,
+                                     int32_t in_features, int32_t out_features, int32_t num_groups,
+                                     int32_t grouped, int32_t activation, int32_t backward);
+moe_status moe_mx_linear_forward(int32_t device, void* stream, int32_t x_format, int32_t dtype,
+                                 int64_t num_rows, int32_t in_features, int32_t out_features,
+                                 int32_t num_groups, const int32_t* offsets, const void* x,
+                                 const uint8_t* x_scales, const uint8_t* w_codes,
+                                 const uint8_t* w_scales, const void* bias, const void* residual,
+                                 int32_t activation, void* y, void* pre_act, void* workspace);
+/* dx [M, K] (0 for rows of no group) and d_bias [G, N] (0 for a group without rows) in bf16, each written
+ * unless NULL, of a forward over bf16 rows.  The residual's gradient is d_y; the weights have none. */
+moe_status moe_mx_linear_backward(int32_t device, void* stream, int64_t num_rows, int32_t in_features,
+                                  int32_t out_features, int32_t num_groups, const int32_t* offsets,
+                                  const void* d_y, const uint8_t* w_codes, const uint8_t* w_scales,
+                                  const void* pre_act, int32_t activation, void* dx, void* d_bias,
+                                  void* workspace);
+
 const char* moe_last_error(void);
 const char* moe_version(void);
 

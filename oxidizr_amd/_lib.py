@@ -12,6 +12,8 @@ LIB_PATH = os.path.join(_HERE, "libmoe_hip.so")
 MOE_DTYPE_F32 = 0
 MOE_DTYPE_BF16 = 1
 MOE_ERR_UNSUPPORTED = 4
+MOE_MX_ROWS_BF16 = 0
+MOE_MX_ROWS_FOUR_BIT = 1
 
 SAVED_FIELDS = ["logits", "probs", "lse", "topk_idx", "topk_w", "counts", "offsets", "perm",
                 "inv_perm", "mean_prob", "x_perm", "gate_act", "up_act", "swiglu", "expert_out",
@@ -27,7 +29,9 @@ EXPORTED = [
     "moe_unpermute", "moe_unpermute_backward", "moe_linear_workspace_bytes",
     "moe_linear_forward", "moe_linear_backward", "moe_residual_norm",
     "moe_residual_norm_workspace_bytes", "moe_residual_norm_backward",
-    "moe_residual_norm_backward_from_input",
+    "moe_residual_norm_backward_from_input", "moe_router_losses_workspace_bytes",
+    "moe_router_losses", "moe_router_losses_backward", "moe_mx_quantize", "moe_mx_dequantize",
+    "moe_mx_linear_workspace_bytes", "moe_mx_linear_forward", "moe_mx_linear_backward",
 ]
 NUM_STAGES = 20
 
@@ -146,6 +150,26 @@ def load():
     L.moe_residual_norm_backward.restype = i32
     L.moe_residual_norm_backward_from_input.argtypes = L.moe_residual_norm_backward.argtypes
     L.moe_residual_norm_backward_from_input.restype = i32
+    L.moe_router_losses_workspace_bytes.argtypes = [i64, i32, i64]
+    L.moe_router_losses_workspace_bytes.restype = sz
+    L.moe_router_losses.argtypes = [i32, _vp, i32, i64, i32, i32, i32, _vp, _vp, i32, f32, f32, f32, _vp, i64,
+                                    _vp, _vp, _vp, _vp, _vp, _vp, _vp]
+    L.moe_router_losses.restype = i32
+    L.moe_router_losses_backward.argtypes = [i32, _vp, i32, i64, i32, i32, i32, _vp, _vp, i32, f32, _vp, i64,
+                                             _vp, _vp, _vp, _vp, _vp, _vp]
+    L.moe_router_losses_backward.restype = i32
+    L.moe_mx_quantize.argtypes = [i32, _vp, i32, i64, _vp, _vp, _vp]
+    L.moe_mx_quantize.restype = i32
+    L.moe_mx_dequantize.argtypes = L.moe_mx_quantize.argtypes
+    L.moe_mx_dequantize.restype = i32
+    L.moe_mx_linear_workspace_bytes.argtypes = [i32, i32, i64, i32, i32, i32, i32, i32, i32]
+    L.moe_mx_linear_workspace_bytes.restype = sz
+    L.moe_mx_linear_forward.argtypes = [i32, _vp, i32, i32, i64, i32, i32, i32, _vp, _vp, _vp, _vp, _vp, _vp,
+                                        _vp, i32, _vp, _vp, _vp]
+    L.moe_mx_linear_forward.restype = i32
+    L.moe_mx_linear_backward.argtypes = [i32, _vp, i64, i32, i32, i32, _vp, _vp, _vp, _vp, _vp, i32, _vp, _vp,
+                                         _vp]
+    L.moe_mx_linear_backward.restype = i32
     L.moe_last_error.argtypes = []
     L.moe_last_error.restype = ctypes.c_char_p
     L.moe_version.argtypes = []

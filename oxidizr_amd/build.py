@@ -5,7 +5,7 @@ import subprocess
 import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SRCS = [os.path.join(HERE, "csrc", n) for n in ("moe_api.hip", "ops_api.hip")]
+SRCS = [os.path.join(HERE, "csrc", n) for n in ("moe_api.hip", "ops_api.hip", "router_api.hip", "mx_api.hip")]
 OUT = os.path.join(HERE, "libmoe_hip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 

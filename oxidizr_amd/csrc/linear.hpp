@@ -239,6 +239,36 @@ MOE_DEV void add_bias(f32x16 (&acc)[1][C::TN][C::TM], f32x16 (&xacc)[1][C::XTN],
   }
 }
 
+// The epilogue of a row tile, of mv rows from row0 and the columns from n0 on; bias: that of the tile's
+// group, from column n0 on, or null.
+template <class C, typename T>
+MOE_DEV void linear_epilogue(f32x16 (&acc)[1][C::TN][C::TM], f32x16 (&xacc)[1][C::XTN], const LinearEpi<T>& epi,
+                             const T* bias, int row0, int mv, int n0, float* lds) {
+  const int N = epi.N;
+  if (bias) add_bias<C, T>(acc, xacc, bias, N - n0);
+  if (epi.res) {
+    constexpr int V = Vec16<T>::N;
+    struct Pre { u32x4 r[8 / V]; };
+    for_each_row8_xpre<C, 1, Pre, C::XR == 0 && sizeof(T) == 2>(acc, xacc, lds, [&](int m, int n, Pre& q) {
+      if (m >= mv || n0 + n >= N) return;
+      const T* p = epi.res + ((int64_t)row0 + m) * N + n0 + n;
+#pragma unroll
+      for (int i = 0; i < 8 / V; ++i) q.r[i] = *gptr(reinterpret_cast<const u32x4*>(p + i * V));
+    }, [&](int m, int n, auto& v, const Pre& q) {
+      if (m >= mv || n0 + n >= N) return;
+      float r[8];
+#pragma unroll
+      for (int i = 0; i < 8 / V; ++i) unpack16(q.r[i], r + i * V, T());
+      linear_store8<T, true>(epi, (int64_t)row0 + m, n0 + n, v[0], r);
+    });
+  } else {
+    for_each_row8_x<C, 1>(acc, xacc, lds, [&](int m, int n, auto& v) {
+      if (m >= mv || n0 + n >= N) return;
+      linear_store8<T, false>(epi, (int64_t)row0 + m, n0 + n, v[0], v[0]);
+    });
+  }
+}
+
 // fp32 sums run over k in the order 0, 4, 8, 12, 1, 5, .. of 16-deep steps, in which a 16 x 16
 // x 4 MFMA fed by 16-byte vectors takes it: that of a wave of k_linear_skinny, and, by
 // their bits, of torch's fp32 products in most shapes.  relu's slope jumps at 0, so a sum
@@ -274,30 +304,7 @@ __global__ __launch_bounds__(C::THREADS) void k_linear_fwd(const T* __restrict__
     constexpr int KW = sizeof(T) == 4 ? kF32StepVectors : 1;
     mainloop_x<CT, T, false, false, 1, 1, false, KW>(acc, xacc, a, b, K, smem);
     static_assert(epi_lds_floats<CT, 1>() * 4 <= (int)sizeof(smem), "epilogue LDS");
-    if (bias) add_bias<CT, T>(acc, xacc, bias, N - n0);
-    if (epi.res) {
-      constexpr int V = Vec16<T>::N;
-      struct Pre { u32x4 r[8 / V]; };
-      for_each_row8_xpre<CT, 1, Pre, CT::XR == 0 && sizeof(T) == 2>(acc, xacc, reinterpret_cast<float*>(smem),
-                                     [&](int m, int n, Pre& q) {
-        if (m >= mv || n0 + n >= N) return;
-        const T* p = epi.res + ((int64_t)row0 + m) * N + n0 + n;
-#pragma unroll
-        for (int i = 0; i < 8 / V; ++i) q.r[i] = *gptr(reinterpret_cast<const u32x4*>(p + i * V));
-      }, [&](int m, int n, auto& v, const Pre& q) {
-        if (m >= mv || n0 + n >= N) return;
-        float r[8];
-#pragma unroll
-        for (int i = 0; i < 8 / V; ++i) unpack16(q.r[i], r + i * V, T());
-        linear_store8<T, true>(epi, (int64_t)row0 + m, n0 + n, v[0], r);
-      });
-    } else {
-      for_each_row8_x<CT, 1>(acc, xacc, reinterpret_cast<float*>(smem),
-                             [&](int m, int n, auto& v) {
-        if (m >= mv || n0 + n >= N) return;
-        linear_store8<T, false>(epi, (int64_t)row0 + m, n0 + n, v[0], v[0]);
-      });
-    }
+    linear_epilogue<CT>(acc, xacc, epi, bias, row0, mv, n0, reinterpret_cast<float*>(smem));
   });
 }
 
@@ -405,6 +412,46 @@ MOE_DEV bool skinny_slot(const int* __restrict__ offsets, int E, int M, int s, i
   return false;
 }
 
+// Rows of no expert, as block `block` of `blocks`: the residual, or zeros.
+template <typename T>
+MOE_DEV void skinny_no_group(const int* __restrict__ offsets, int E, int M, int N, int64_t block, int64_t blocks,
+                             const LinearEpi<T>& epi) {
+  int m = 0;
+  for (int e = threadIdx.x & 63; e <= E; e += 64) m = max(m, offsets[e]);
+  m = min(wave_max(m), M);
+  const int64_t head = (int64_t)min(max(offsets[0], 0), M) * N / 8, tail = (int64_t)m * N / 8;
+  const int64_t none = head + (int64_t)M * N / 8 - tail;
+  const int64_t step = blocks * 256;
+  for (int64_t j = block * 256 + threadIdx.x; j < none; j += step) {
+    const int64_t v = j < head ? j : j - head + tail;
+    float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (epi.res) load8(epi.res + v * 8, f);
+    store8(epi.y + v * 8, f);
+    if (epi.pre) store8(epi.pre + v * 8, zero);
+  }
+}
+// Column n of the nch chunks of 16 rows that a wave has the sums of: lane 16 g + rl holds rows 16 c + 4 g + r of its column.
+template <typename T, int NC>
+MOE_DEV void skinny_store(const LinearEpi<T>& epi, const f32x4 (&acc)[NC], int nch, int r0, int rows, int n, int grp) {
+  const int g = (threadIdx.x & 63) >> 4;
+  const float bias = epi.bias ? to_f<T>(epi.bias[(int64_t)grp * epi.N + n]) : 0.0f;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    if (c >= nch) break;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int t = c * 16 + 4 * g + r;
+      if (t >= rows) continue;
+      const int64_t o = ((int64_t)r0 + t) * epi.N + n;
+      const float z = acc[c][r] + bias;
+      if (epi.pre) epi.pre[o] = from_f<T>(z);
+      const float y = act_value<T>(z, epi.act);
+      epi.y[o] = from_f<T>(epi.res ? y + to_f<T>(epi.res[o]) : y);
+    }
+  }
+}
+
 // NC: chunks of 16 rows (1 for calls of at most 16 rows, else 4).  Blocks below
 // nslot x nNb are (slot, row blocks) pairs; the others write the rows of no
 // expert.  offsets null: one weight, rows s 64 .. .
@@ -420,21 +467,8 @@ __global__ __launch_bounds__(256) void k_linear_skinny(const T* __restrict__ X,
   const int nNb = (N + 16 * RB - 1) / (16 * RB);
   const int slot = uni(blockIdx.x / nNb), nb = uni(blockIdx.x % nNb);
   if (slot >= nslot) {
-    int m = 0;
-    for (int e = threadIdx.x & 63; e <= E; e += 64) m = max(m, offsets[e]);
-    m = min(wave_max(m), M);
-    const int64_t head = (int64_t)min(max(offsets[0], 0), M) * N / 8, tail = (int64_t)m * N / 8;
-    const int64_t none = head + (int64_t)M * N / 8 - tail;
-    const int64_t step = ((int64_t)gridDim.x - (int64_t)nslot * nNb) * 256;
-    for (int64_t j = ((int64_t)blockIdx.x - (int64_t)nslot * nNb) * 256 + threadIdx.x; j < none;
-         j += step) {
-      const int64_t v = j < head ? j : j - head + tail;
-      float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (epi.res) load8(epi.res + v * 8, f);
-      store8(epi.y + v * 8, f);
-      if (epi.pre) store8(epi.pre + v * 8, zero);
-    }
+    skinny_no_group(offsets, E, M, N, (int64_t)blockIdx.x - (int64_t)nslot * nNb,
+                    (int64_t)gridDim.x - (int64_t)nslot * nNb, epi);
     return;
   }
   int grp = 0, r0 = slot * kLinearSkinnyRows, rows = min(kLinearSkinnyRows, M - r0);
@@ -493,24 +527,8 @@ __global__ __launch_bounds__(256) void k_linear_skinny(const T* __restrict__ X,
 #pragma unroll
     for (int c = 0; c < NC; ++c)
       if (c < nch) acc[c] += red[((q - 1) * RB + rb) * NC * 64 + c * 64 + lane];
-  // lane holds row 16 c + 4 g + r, column n0 + rl
   if (rl >= nrows) return;
-  const int n = n0 + rl;
-  const float bias = epi.bias ? to_f<T>(epi.bias[(int64_t)grp * N + n]) : 0.0f;
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    if (c >= nch) break;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int t = c * 16 + 4 * g + r;
-      if (t >= rows) continue;
-      const int64_t o = ((int64_t)r0 + t) * N + n;
-      const float z = acc[c][r] + bias;
-      if (epi.pre) epi.pre[o] = from_f<T>(z);
-      const float y = act_value<T>(z, epi.act);
-      epi.y[o] = from_f<T>(epi.res ? y + to_f<T>(epi.res[o]) : y);
-    }
-  }
+  skinny_store<T, NC>(epi, acc, nch, r0, rows, n0 + rl, grp);
 }
 
 // ------------------------------------------------------------------ backward, element-wise part

@@ -1,0 +1,609 @@
+// HIP kernels of microscaled 4-bit numbers (gfx950 / CDNA4): quantisation and back, and expert products
+// over 4-bit weights.
+//
+// The format is the OCP microscaling formats' MXFP4: 32 elements along a row share a scale 2^s, an E8M0 byte
+// s + 127 (255: NaN); an element is an E2M1 number, 0 0.5 1 1.5 2 3 4 6 with a sign in bit 3.  Element 2 i of a
+// row is the low half of its byte i.  A row of K elements (K a multiple of 32) is K / 2 bytes of codes and K / 32
+// bytes of scales, both row-major.
+//
+//   z[r] = x[r] W_e^T + b_e,  y[r] = act(z[r]) + res[r]   for r in expert e's rows,
+//   dz = dy act'(z),  dx = dz W_e,  db_e = sum_r dz[r],  dres = dy
+// with W_e [N, K] in 4 bits and x in bf16, or in 4 bits too (no gradients then: a rounding has none).
+#pragma once
+#include "linear.hpp"
+
+namespace moe {
+
+constexpr int kMxBlock = 32;  // elements under one scale
+
+// An E8M0 byte as the conversions take it: they read a float's exponent alone, for which 0 is 2^-127
+// and 255 a NaN (which makes every element one).
+MOE_DEV float mx_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// Eight elements (a dword of codes) as bf16: exact (2 bits of mantissa, and bf16 has E8M0's range; 6 2^127, above the
+// largest bf16, becomes infinite, but no quantisation makes a scale above 2^125).
+MOE_DEV u32x4 mx_bf16x8(uint32_t c, float s) {
+  u32x4 r;
+  r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0));
+  r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1));
+  r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2));
+  r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3));
+  return r;
+}
+
+// ------------------------------------------------------------------ quantisation
+// s = floor(log2 of the block's largest magnitude) - 2, so that it becomes 4 .. 8 2^s and what is above 6 2^s
+// becomes that; elements are rounded to the nearest code, ties to the even one (v_cvt_scalef32_pk_fp4).  A
+// block with an infinity or a NaN has scale 255: all of it is NaN.  A lane takes eight elements, four neighbouring
+// lanes a block.
+template <typename T>
+__global__ __launch_bounds__(256) void k_mx_quantize(const T* __restrict__ x, int64_t nvec,
+                                                     uint32_t* __restrict__ codes,
+                                                     uint8_t* __restrict__ scales) {
+  const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (v >= nvec) return;  // whole blocks of four lanes
+  float f[8];
+  load8(x + v * 8, f);
+  int m = 0;  // magnitudes order as integers, infinity and NaN above all numbers
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_int(f[i]) & 0x7fffffff);
+  m = max(m, lane_xor<1>(m));
+  m = max(m, lane_xor<2>(m));
+  const bool none = m >= 0x7f800000;
+  const int byte = none ? 255 : max((m >> 23) - 2, 0);
+  const float s = mx_scale(byte);
+  uint32_t c = 0;
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[0], f[1], s, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[2], f[3], s, 1);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[4], f[5], s, 2);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[6], f[7], s, 3);
+  codes[v] = none ? 0u : c;
+  if ((threadIdx.x & 3) == 0) scales[v >> 2] = (uint8_t)byte;
+}
+
+MOE_DEV void mx_store8(bf16_t* p, uint32_t c, float s) { st16_stream(p, mx_bf16x8(c, s)); }
+MOE_DEV void mx_store8(float* p, uint32_t c, float s) {
+  const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 0);
+  const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 1);
+  const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 2);
+  const f32x2 e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 3);
+  const float v[8] = {a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1]};
+  store8_stream(p, v);
+}
+template <typename T>
+__global__ __launch_bounds__(256) void k_mx_dequantize(const uint32_t* __restrict__ codes,
+                                                       const uint8_t* __restrict__ scales, int64_t nvec,
+                                                       T* __restrict__ y) {
+  const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (v >= nvec) return;
+  mx_store8(y + v * 8, codes[v], mx_scale(scales[v >> 2]));
+}
+
+// ------------------------------------------------------------------ tiled products
+// The weights of a launch: group g's matrix at codes + g N K / 2, scales + g N K / 32.
+struct MxWeights {
+  const uint8_t *codes, *scales;
+  int N, K;
+};
+
+// One operand tile of 4-bit weights, staged through registers: a piece is a block of 32 elements, 16 bytes of
+// codes and a scale; a thread loads its pieces of a k-tile one k-tile ahead, and writes them as 4 x 16 bytes of bf16
+// into the LDS tile, laid out as the direct loads of a bf16 operand would have left it (gemm.hpp), so the
+// fragments are read the same way.  Each weight is converted once a workgroup.
+// K-contiguous (KM false): R weight rows, two pieces of a 64-deep k-tile each.  K-major (KM true: the
+// contraction runs over weight rows): 64 weight rows of R columns.
+template <class C, int R, bool KM>
+struct MxStager {
+  static_assert(C::BK == 64 && (R % 32) == 0, "two blocks to a k-tile");
+  static constexpr int PIECES = R * C::BK / kMxBlock;
+  static constexpr int PER = (PIECES + C::THREADS - 1) / C::THREADS;
+  static constexpr int CB = KM ? R / kMxBlock : C::BK / kMxBlock;  // pieces side by side
+  rsrc_t rc, rs;
+  int rows, blocks;  // valid rows and pieces side by side, from the tile's first (KM: rows run along the contraction)
+  uint32_t ldc, lds_;  // bytes of a weight row
+  u32x4 code[PER];
+  uint32_t scale[PER];
+  // codes, scales: the tile's first row and block; rows_valid rows and cols_valid elements from there
+  MOE_DEV void init(const uint8_t* codes, const uint8_t* scales, int K, int rows_valid, int cols_valid) {
+    ldc = (uint32_t)(K / 2);
+    lds_ = (uint32_t)(K / kMxBlock);
+    rows = rows_valid;
+    blocks = cols_valid / kMxBlock;
+    rc = make_rsrc(codes, (uint32_t)(rows - 1) * ldc + (uint32_t)blocks * 16);
+    rs = make_rsrc(scales, (uint32_t)(rows - 1) * lds_ + (uint32_t)blocks);
+  }
+  MOE_DEV static void piece(int i, int& row, int& blk) {
+    const int p = threadIdx.x + i * C::THREADS;
+    row = p / CB;
+    blk = p % CB;
+  }
+  // the k-tile from contraction index k0 on
+  MOE_DEV void load(int k0) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      int row, blk;
+      piece(i, row, blk);
+      const int r = KM ? k0 + row : row, b = KM ? blk : k0 / kMxBlock + blk;
+      const bool in = r < rows && b < blocks && (PIECES % C::THREADS == 0 || threadIdx.x + i * C::THREADS < PIECES);
+      code[i] = buf_ld16(rc, in ? (uint32_t)r * ldc + (uint32_t)b * 16 : kOobOffset, 0);
+      scale[i] = __builtin_amdgcn_raw_buffer_load_b8(rs, in ? (uint32_t)r * lds_ + (uint32_t)b : kOobOffset, 0, 0);
+    }
+  }
+  MOE_DEV void write(bf16_t* tile) const {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (PIECES % C::THREADS != 0 && threadIdx.x + i * C::THREADS >= PIECES) break;
+      int row, blk;
+      piece(i, row, blk);
+      const float s = mx_scale(scale[i]);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int slot = 4 * blk + v;
+        bf16_t* to = KM ? tile + row * R + ((slot ^ tr_swz(row)) << 3)
+                        : tile + row * C::BK + ((slot ^ nt_swz(row)) << 3);
+        *reinterpret_cast<u32x4*>(to) = mx_bf16x8(code[i][v], s);
+      }
+    }
+  }
+};
+
+// acc += W-tile x A-tile over the contraction, A (bf16, K-contiguous) by direct-to-LDS loads as in
+// mainloop_dma, W through MxStager.  Per k-tile kt: the pieces of kt + 1, loaded during kt - 1, are written
+// to their stage (which was last read before the barrier that began kt), those of kt + 2 are requested, then
+// the k-steps run as in mainloop_dma.  The wait before the barrier leaves at most the direct loads of later k-tiles
+// outstanding, whatever the order in which the pieces' loads were issued among them.
+template <class C, bool KM>
+MOE_DEV void mainloop_mx(f32x16 (&acc)[1][C::TN][C::TM], f32x16 (&xacc)[1][C::XTN], const OpDesc<bf16_t>& a,
+                         MxStager<C, C::BN, KM>& sb, int K, bf16_t* smem) {
+  using T = bf16_t;
+  constexpr int TILE_A = C::AR * C::BK, TILE_B = C::BN * C::BK, STAGE = TILE_A + TILE_B;
+  constexpr int NST = C::NST;
+  constexpr bool TALL = C::XR > 0;
+  static_assert(C::XR == 0 || C::XR == 64, "no 384-row tiles");
+  using SA = DmaStager<C, T, C::AR>;
+  using SBN = DmaStager<C, T, C::BN>;
+  using SBT = DmaStagerT<C, T, C::BN>;
+  constexpr int IPT = SA::PER;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave / C::WGN, wn = wave % C::WGN;
+  const int nk = (K + C::BK - 1) / C::BK;
+  if (nk <= 0) return;
+  SA sa;
+  sa.init(a, threadIdx.x);
+  auto stage = [&](int kt) { return smem + (NST == 2 ? (kt & 1) : kt % NST) * STAGE; };
+  auto issue = [&](int kt) { sa.issue(stage(kt), kt * C::BK, 0); };
+  const int pro = min(NST - 1, nk);
+  for (int kt = 0; kt < pro; ++kt) issue(kt);
+  sb.load(0);
+  sb.write(stage(0) + TILE_A);
+  if (nk > 1) sb.load(C::BK);
+  constexpr int KSTEPS = C::BK / (2 * C::V);
+  const int frag_row = lane & 31, frag_kv = lane >> 5;
+  u32x4 af[2][C::TM], bfr[2][C::TN], afx[2];
+  const int xrow = C::BM + 32 * (wm & 1) + frag_row;
+  const bool xhi = __builtin_amdgcn_readfirstlane(wm >> 1) != 0;
+  auto read_frags = [&](const T* sA, int ks, int set) {
+    const T* sB = sA + TILE_A;
+    const int kv = ks * 2 + frag_kv;
+#pragma unroll
+    for (int tm = 0; tm < C::TM; ++tm) af[set][tm] = SA::frag(sA, wm * C::WM + tm * 32 + frag_row, kv);
+    if constexpr (TALL) afx[set] = SA::frag(sA, xrow, kv);
+#pragma unroll
+    for (int tn = 0; tn < C::TN; ++tn) {
+      if constexpr (KM) bfr[set][tn] = SBT::frag(sB, wn * C::WN + tn * 32, ks * 2 * C::V);
+      else bfr[set][tn] = SBN::frag(sB, wn * C::WN + tn * 32 + frag_row, kv);
+    }
+  };
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  lds_barrier();
+  if (NST - 1 < nk) issue(NST - 1);
+  read_frags(smem, 0, 0);
+  auto body = [&](int kt, auto phase_c) {
+    constexpr int phase = decltype(phase_c)::value;  // 0: refills a stage, 1: all issued, 2: the last
+    const T* sA = stage(kt);
+    if constexpr (phase < 2) {
+      sb.write(stage(kt + 1) + TILE_A);
+      if (kt + 2 < nk) sb.load((kt + 2) * C::BK);
+    }
+#pragma unroll
+    for (int ks = 0; ks < KSTEPS; ++ks) {
+      const int cur = ks & 1;
+      if (ks + 1 < KSTEPS) {
+        read_frags(sA, ks + 1, cur ^ 1);
+      } else if constexpr (phase < 2) {
+        if constexpr (phase == 0) {
+          asm volatile("s_waitcnt vmcnt(%0)" :: "n"((NST - 2) * IPT) : "memory");
+        } else {
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        lds_barrier();
+        read_frags(stage(kt + 1), 0, cur ^ 1);
+        if constexpr (phase == 0) issue(kt + NST);
+      }
+#pragma unroll
+      for (int tn = 0; tn < C::TN; ++tn)
+#pragma unroll
+        for (int tm = 0; tm < C::TM; ++tm) mfma_frag(acc[0][tn][tm], bfr[cur][tn], af[cur][tm], T());
+      if constexpr (TALL) {
+#pragma unroll
+        for (int j = 0; j < C::XTN; ++j) {
+          const u32x4 bx = xhi ? bfr[cur][C::XTN + j] : bfr[cur][j];
+          mfma_frag(xacc[0][j], bx, afx[cur], T());
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  int kt = 0;
+  for (; kt + NST < nk; ++kt) body(kt, std::integral_constant<int, 0>{});
+  for (; kt + 1 < nk; ++kt) body(kt, std::integral_constant<int, 1>{});
+  body(kt, std::integral_constant<int, 2>{});
+  __syncthreads();  // the caller's epilogue reuses the LDS
+}
+
+// y tile by tile, bf16 rows.
+template <class C>
+__global__ __launch_bounds__(C::THREADS) void k_mx_fwd(const bf16_t* __restrict__ X, RowGroups groups, MxWeights w,
+                                                       LinearEpi<bf16_t> epi) {
+  __shared__ __align__(16) bf16_t smem[rowcol_smem_elems<bf16_t, C, 1, 1, 1>()];
+  int grp, row0, mv, n0;
+  const int N = w.N, K = w.K;
+  if (!resolve_rows(groups, N, C::AR, C::BN, grp, row0, mv, n0)) return;
+  const int64_t first = (int64_t)grp * N + n0;  // weight row
+  with_tile_shape<bf16_t, C>(mv, N - n0, [&](auto ct) {
+    using CT = decltype(ct);
+    const OpDesc<bf16_t> a{X + (int64_t)row0 * K, K, mv, K};
+    MxStager<CT, CT::BN, false> sb;
+    sb.init(uni_ptr(w.codes + first * (K / 2)), uni_ptr(w.scales + first * (K / kMxBlock)), K, min(N - n0, CT::BN), K);
+    f32x16 acc[1][CT::TN][CT::TM], xacc[1][CT::XTN];
+    zero_acc<CT, 1>(acc, xacc);
+    mainloop_mx<CT, false>(acc, xacc, a, sb, K, smem);
+    static_assert(epi_lds_floats<CT, 1>() * 4 <= (int)sizeof(smem), "epilogue LDS");
+    linear_epilogue<CT>(acc, xacc, epi, epi.bias ? epi.bias + first : nullptr, row0, mv, n0,
+                        reinterpret_cast<float*>(smem));
+  });
+}
+
+// dx = dz W tile by tile: the contraction runs over the weight's rows.
+template <class C>
+__global__ __launch_bounds__(C::THREADS) void k_mx_dgrad(const bf16_t* __restrict__ dZ, RowGroups groups, MxWeights w,
+                                                         bf16_t* __restrict__ dX) {
+  __shared__ __align__(16) bf16_t smem[rowcol_smem_elems<bf16_t, C, 1, 1, 1>()];
+  int grp, row0, mv, k0;
+  const int N = w.N, K = w.K;
+  if (!resolve_rows(groups, K, C::AR, C::BN, grp, row0, mv, k0)) return;
+  const int64_t first = (int64_t)grp * N;
+  with_tile_shape<bf16_t, C>(mv, K - k0, [&](auto ct) {
+    using CT = decltype(ct);
+    const OpDesc<bf16_t> a{dZ + (int64_t)row0 * N, N, mv, N};
+    MxStager<CT, CT::BN, true> sb;
+    sb.init(uni_ptr(w.codes + first * (K / 2) + k0 / 2),
+            uni_ptr(w.scales + first * (K / kMxBlock) + k0 / kMxBlock), K, N, min(K - k0, CT::BN));
+    f32x16 acc[1][CT::TN][CT::TM], xacc[1][CT::XTN];
+    zero_acc<CT, 1>(acc, xacc);
+    mainloop_mx<CT, true>(acc, xacc, a, sb, N, smem);
+    for_each_row8_x<CT, 1>(acc, xacc, reinterpret_cast<float*>(smem), [&](int m, int n, auto& v) {
+      if (m >= mv || k0 + n >= K) return;
+      store8_stream(dX + ((int64_t)row0 + m) * K + k0 + n, v[0]);
+    });
+  });
+}
+
+// ------------------------------------------------------------------ tiled products, both sides in 4 bits
+// A 16-byte vector is 32 elements, so a k-tile of 64 bf16's bytes is 256 elements and the tilings, direct
+// loads, swizzles and fragments of gemm.hpp serve as they are, over rows of K / 4 two-byte units.
+// v_mfma_scale_f32_32x32x64_f8f6f4 takes such a vector of each operand and a scale for each.  Half h of a
+// wave reads vector 4 h + ks in k-step ks of a k-tile instead of 2 ks + h: its four scales of a row are then one dword,
+// of which step ks takes byte ks.
+MOE_DEV void mfma_mx(f32x16& acc, u32x4 bt, u32x4 at, uint32_t sb, uint32_t sa, int ks) {
+  typedef int i32x8 __attribute__((ext_vector_type(8)));
+  const i32x8 b = {(int)bt.x, (int)bt.y, (int)bt.z, (int)bt.w, 0, 0, 0, 0};
+  const i32x8 a = {(int)at.x, (int)at.y, (int)at.z, (int)at.w, 0, 0, 0, 0};
+  switch (ks) {  // a constant
+    case 0: acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b, a, acc, 4, 4, 0, (int)sb, 0, (int)sa); break;
+    case 1: acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b, a, acc, 4, 4, 1, (int)sb, 1, (int)sa); break;
+    case 2: acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b, a, acc, 4, 4, 2, (int)sb, 2, (int)sa); break;
+    default: acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b, a, acc, 4, 4, 3, (int)sb, 3, (int)sa); break;
+  }
+}
+
+// The scales of a tile's rows (AR of x, then BN of the weight), through registers: a thread loads the 16 of two
+// k-tiles at once from its rows (rows of K / 32 bytes have any alignment, and 8 bytes of a cache line a
+// k-tile would fetch each line many times) and writes 8 a k-tile to LDS.
+template <class C>
+struct MxScaleStager {
+  static constexpr int ROWS = C::AR + C::BN;
+  static constexpr int PER = (ROWS + C::THREADS - 1) / C::THREADS;
+  const uint8_t* row[PER];  // null past the valid rows
+  int bytes;                // of a row
+  u32x4 s[PER];
+  MOE_DEV void init(const uint8_t* xs, const uint8_t* ws, int mv, int nv, int K) {
+    bytes = K / kMxBlock;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int r = threadIdx.x + i * C::THREADS;
+      row[i] = r < C::AR ? (r < mv ? xs + (int64_t)r * bytes : nullptr)
+                         : (r - C::AR < nv ? ws + (int64_t)(r - C::AR) * bytes : nullptr);
+    }
+  }
+  // the 16 scales from byte `at` of each row on
+  MOE_DEV void load(int at) {
+    const int left = bytes - at;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      s[i] = u32x4{0, 0, 0, 0};
+      if (!row[i]) continue;
+      if (left >= 16) {
+        typedef u32x4 any_u32x4 __attribute__((aligned(1)));
+        s[i] = *(const __attribute__((address_space(1))) any_u32x4*)(row[i] + at);
+      } else {
+        for (int j = 0; j < left; ++j) {
+          const uint32_t b = gptr(row[i])[at + j];
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+            if (j >> 2 == d) s[i][d] |= b << (8 * (j & 3));
+        }
+      }
+    }
+  }
+  // 8 bytes a row: the first or (hi) second k-tile of a load
+  MOE_DEV void write(u32x2* tile, bool hi) const {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int r = threadIdx.x + i * C::THREADS;
+      if (ROWS % C::THREADS != 0 && r >= ROWS) break;
+      tile[r] = hi ? u32x2{s[i].z, s[i].w} : u32x2{s[i].x, s[i].y};
+    }
+  }
+};
+
+// As mainloop_dma, with scales.  OUT, the results' type, only sets the instantiations of two kernels apart: hipcc's host
+// pass takes the second use of one as an error.
+template <class C, typename OUT>
+MOE_DEV void mainloop_mxmx(f32x16 (&acc)[1][C::TN][C::TM], f32x16 (&xacc)[1][C::XTN], const OpDesc<bf16_t>& a,
+                           const OpDesc<bf16_t>& b, MxScaleStager<C>& ss, int K4, bf16_t* smem, u32x2* scales) {
+  using T = bf16_t;
+  constexpr int TILE_A = C::AR * C::BK, TILE_B = C::BN * C::BK, STAGE = TILE_A + TILE_B;
+  constexpr int NST = C::NST, ROWS = MxScaleStager<C>::ROWS;
+  constexpr bool TALL = C::XR > 0;
+  static_assert(C::XR == 0 || C::XR == 64, "no 384-row tiles");
+  using SA = DmaStager<C, T, C::AR>;
+  using SB = DmaStager<C, T, C::BN>;
+  constexpr int IPT = SA::PER + SB::PER;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave / C::WGN, wn = wave % C::WGN;
+  const int nk = (K4 + C::BK - 1) / C::BK;
+  if (nk <= 0) return;
+  SA sa;
+  SB sb;
+  sa.init(a, threadIdx.x);
+  sb.init(b, threadIdx.x);
+  auto stage = [&](int kt) { return smem + (NST == 2 ? (kt & 1) : kt % NST) * STAGE; };
+  auto scales_of = [&](int kt) { return scales + (kt & 1) * ROWS; };
+  auto issue = [&](int kt) {
+    sa.issue(stage(kt), kt * C::BK, 0);
+    sb.issue(stage(kt) + TILE_A, kt * C::BK, 0);
+  };
+  const int pro = min(NST - 1, nk);
+  for (int kt = 0; kt < pro; ++kt) issue(kt);
+  ss.load(0);
+  ss.write(scales_of(0), false);
+  constexpr int KSTEPS = C::BK / (2 * C::V);
+  static_assert(KSTEPS == 4, "four scales to a dword");
+  const int frag_row = lane & 31, half = lane >> 5;
+  u32x4 af[2][C::TM], bfr[2][C::TN], afx[2];
+  uint32_t as[2][C::TM], bs[2][C::TN], asx[2];  // of this k-tile and the next
+  const int xrow = C::BM + 32 * (wm & 1) + frag_row;
+  const bool xhi = __builtin_amdgcn_readfirstlane(wm >> 1) != 0;
+  auto read_scales = [&](int kt, int set) {
+    const uint32_t* t = reinterpret_cast<const uint32_t*>(scales_of(kt)) + half;
+#pragma unroll
+    for (int tm = 0; tm < C::TM; ++tm) as[set][tm] = t[2 * (wm * C::WM + tm * 32 + frag_row)];
+    if constexpr (TALL) asx[set] = t[2 * xrow];
+#pragma unroll
+    for (int tn = 0; tn < C::TN; ++tn) bs[set][tn] = t[2 * (C::AR + wn * C::WN + tn * 32 + frag_row)];
+  };
+  auto read_frags = [&](const T* sA, int ks, int set) {
+    const T* sB = sA + TILE_A;
+    const int kv = 4 * half + ks;
+#pragma unroll
+    for (int tm = 0; tm < C::TM; ++tm) af[set][tm] = SA::frag(sA, wm * C::WM + tm * 32 + frag_row, kv);
+    if constexpr (TALL) afx[set] = SA::frag(sA, xrow, kv);
+#pragma unroll
+    for (int tn = 0; tn < C::TN; ++tn) bfr[set][tn] = SB::frag(sB, wn * C::WN + tn * 32 + frag_row, kv);
+  };
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  lds_barrier();
+  if (NST - 1 < nk) issue(NST - 1);
+  read_frags(smem, 0, 0);
+  read_scales(0, 0);
+  // odd: which half of a load of scales, and register set, a k-tile has
+  auto body = [&](int kt, auto phase_c, auto odd_c) {
+    constexpr int phase = decltype(phase_c)::value;  // 0: refills a stage, 1: all issued, 2: the last
+    constexpr int odd = decltype(odd_c)::value;
+    const T* sA = stage(kt);
+    if constexpr (phase < 2) {
+      // the next k-tile's scales: the second half of a load, or the load that this k-tile's predecessor began
+      ss.write(scales_of(kt + 1), odd == 0);
+      if constexpr (odd == 0) {
+        if (kt + 2 < nk) ss.load((kt + 2) * 8);
+      }
+    }
+#pragma unroll
+    for (int ks = 0; ks < KSTEPS; ++ks) {
+      const int cur = ks & 1;
+      if (ks + 1 < KSTEPS) {
+        read_frags(sA, ks + 1, cur ^ 1);
+      } else if constexpr (phase < 2) {
+        if constexpr (phase == 0) {
+          asm volatile("s_waitcnt vmcnt(%0)" :: "n"((NST - 2) * IPT) : "memory");
+        } else {
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        lds_barrier();
+        read_frags(stage(kt + 1), 0, cur ^ 1);
+        read_scales(kt + 1, odd ^ 1);
+        if constexpr (phase == 0) issue(kt + NST);
+      }
+#pragma unroll
+      for (int tn = 0; tn < C::TN; ++tn)
+#pragma unroll
+        for (int tm = 0; tm < C::TM; ++tm)
+          mfma_mx(acc[0][tn][tm], bfr[cur][tn], af[cur][tm], bs[odd][tn], as[odd][tm], ks);
+      if constexpr (TALL) {
+#pragma unroll
+        for (int j = 0; j < C::XTN; ++j) {
+          const u32x4 bx = xhi ? bfr[cur][C::XTN + j] : bfr[cur][j];
+          const uint32_t sx = xhi ? bs[odd][C::XTN + j] : bs[odd][j];
+          mfma_mx(xacc[0][j], bx, afx[cur], sx, asx[odd], ks);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  using Even = std::integral_constant<int, 0>;
+  using Odd = std::integral_constant<int, 1>;
+  auto run = [&](int kt, auto phase) {
+    if (kt & 1) body(kt, phase, Odd{});
+    else body(kt, phase, Even{});
+  };
+  int kt = 0;
+  for (; kt + NST + 1 < nk; kt += 2) {
+    body(kt, std::integral_constant<int, 0>{}, Even{});
+    body(kt + 1, std::integral_constant<int, 0>{}, Odd{});
+  }
+  if (kt + NST < nk) {
+    body(kt, std::integral_constant<int, 0>{}, Even{});
+    ++kt;
+  }
+  for (; kt + 1 < nk; ++kt) run(kt, std::integral_constant<int, 1>{});
+  run(kt, std::integral_constant<int, 2>{});
+  __syncthreads();
+}
+
+// Rows of scales in LDS: the most that a tile shape of C has, twice.
+template <class C>
+constexpr int mx_scale_rows() { return 2 * (C::BM + (has_half_rows<bf16_t, C>() ? C::BM / 4 : 0) + C::BN); }
+
+template <class C, typename T>
+__global__ __launch_bounds__(C::THREADS) void k_mxmx_fwd(const uint8_t* __restrict__ X, const uint8_t* __restrict__ XS,
+                                                         RowGroups groups, MxWeights w, LinearEpi<T> epi) {
+  __shared__ __align__(16) bf16_t smem[rowcol_smem_elems<bf16_t, C, 1, 1, 1>()];
+  __shared__ u32x2 scales[mx_scale_rows<C>()];
+  int grp, row0, mv, n0;
+  const int N = w.N, K = w.K, K4 = K / 4;
+  if (!resolve_rows(groups, N, C::AR, C::BN, grp, row0, mv, n0)) return;
+  const int64_t first = (int64_t)grp * N + n0;
+  with_tile_shape<bf16_t, C>(mv, N - n0, [&](auto ct) {
+    using CT = decltype(ct);
+    static_assert(2 * MxScaleStager<CT>::ROWS <= mx_scale_rows<C>(), "scales' LDS");
+    const OpDesc<bf16_t> a{reinterpret_cast<const bf16_t*>(X + (int64_t)row0 * (K / 2)), K4, mv, K4};
+    const OpDesc<bf16_t> b{reinterpret_cast<const bf16_t*>(w.codes + first * (K / 2)), K4, N - n0, K4};
+    MxScaleStager<CT> ss;
+    ss.init(XS + (int64_t)row0 * (K / kMxBlock), w.scales + first * (K / kMxBlock), mv, N - n0, K);
+    f32x16 acc[1][CT::TN][CT::TM], xacc[1][CT::XTN];
+    zero_acc<CT, 1>(acc, xacc);
+    mainloop_mxmx<CT, T>(acc, xacc, a, b, ss, K4, smem, scales);
+    static_assert(epi_lds_floats<CT, 1>() * 4 <= (int)sizeof(smem), "epilogue LDS");
+    linear_epilogue<CT>(acc, xacc, epi, epi.bias ? epi.bias + first : nullptr, row0, mv, n0,
+                        reinterpret_cast<float*>(smem));
+  });
+}
+
+// ------------------------------------------------------------------ few rows
+// As in k_linear_skinny a launch with few rows to an expert is the stream of the weights that it touches: a wave
+// multiplies 16 weight rows with the rows of the expert (up to four chunks of 16) straight from memory,
+// KS waves of a workgroup share 16 weight rows and take every KS-th k-chunk of kMxChunk elements.  Lane l supplies block
+// l / 16 + 4 q of weight row l % 16 in load q, so four lanes read 64 contiguous bytes.
+// bf16 rows: the block becomes four 8-element vectors, multiplied with the four of the token row by 16 x 16 x 32 MFMAs.
+// 4-bit rows: one 16 x 16 x 128 scaled MFMA.
+constexpr int kMxChunk = 512;
+template <bool X4, typename T, int NC, int KS>
+__global__ __launch_bounds__(256) void k_mx_skinny(const void* __restrict__ X, const uint8_t* __restrict__ XS,
+                                                   const int* __restrict__ offsets, int E, int M, int nslot,
+                                                   MxWeights w, LinearEpi<T> epi) {
+  constexpr int RB = 4 / KS, Q = kMxChunk / 128;
+  __shared__ f32x4 red[(KS - 1) * RB * NC * 64];
+  const int N = w.N, K = w.K;
+  const int nNb = (N + 16 * RB - 1) / (16 * RB);
+  const int slot = uni(blockIdx.x / nNb), nb = uni(blockIdx.x % nNb);
+  if (slot >= nslot) {
+    skinny_no_group(offsets, E, M, N, (int64_t)blockIdx.x - (int64_t)nslot * nNb,
+                    (int64_t)gridDim.x - (int64_t)nslot * nNb, epi);
+    return;
+  }
+  int grp = 0, r0 = slot * kLinearSkinnyRows, rows = min(kLinearSkinnyRows, M - r0);
+  if (offsets && !skinny_slot(offsets, E, M, slot, grp, r0, rows)) return;  // workgroup-uniform
+  grp = uni(grp); r0 = uni(r0); rows = uni(rows);
+  const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int rb = wave / KS, ks = wave % KS;
+  const int n0 = (nb * RB + rb) * 16;
+  const int nrows = uni(min(16, N - n0));
+  const int g = lane >> 4, rl = lane & 15;
+  const int nch = (rows + 15) / 16;
+  const int bytes = K / 2, blocks = K / kMxBlock;
+  f32x4 acc[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) acc[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (nrows > 0) {
+    const int xb = X4 ? bytes : 2 * K;  // bytes of a token row
+    const rsrc_t rx = make_rsrc(uni_ptr((const uint8_t*)X + (int64_t)r0 * xb), (uint32_t)uni(rows * xb));
+    const rsrc_t rxs = make_rsrc(uni_ptr(X4 ? XS + (int64_t)r0 * blocks : w.scales), (uint32_t)uni(X4 ? rows * blocks : 0));
+    const int64_t first = (int64_t)grp * N + n0;
+    const rsrc_t rw = make_rsrc(uni_ptr(w.codes + first * bytes), (uint32_t)uni(nrows * bytes));
+    const rsrc_t rs = make_rsrc(uni_ptr(w.scales + first * blocks), (uint32_t)uni(nrows * blocks));
+    for (int kc = ks; kc * kMxChunk < K; kc += KS) {
+      u32x4 wa[Q];
+      uint32_t ws[Q];
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        const int b = kc * (kMxChunk / kMxBlock) + 4 * q + g;
+        const bool in = b < blocks;
+        wa[q] = buf_ld16(rw, in ? (uint32_t)(rl * bytes + 16 * b) : kOobOffset, 0);
+        ws[q] = __builtin_amdgcn_raw_buffer_load_b8(rs, in ? (uint32_t)(rl * blocks + b) : kOobOffset, 0, 0);
+      }
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        if (c >= nch) break;
+        const int t = c * 16 + rl;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+          const int b = kc * (kMxChunk / kMxBlock) + 4 * q + g;
+          const bool in = b < blocks && t < rows;
+          if constexpr (X4) {
+            typedef int i32x8 __attribute__((ext_vector_type(8)));
+            const u32x4 xa = buf_ld16(rx, in ? (uint32_t)(t * bytes + 16 * b) : kOobOffset, 0);
+            const uint32_t xs = __builtin_amdgcn_raw_buffer_load_b8(rxs, in ? (uint32_t)(t * blocks + b) : kOobOffset, 0, 0);
+            const i32x8 av = {(int)xa.x, (int)xa.y, (int)xa.z, (int)xa.w, 0, 0, 0, 0};
+            const i32x8 bv = {(int)wa[q].x, (int)wa[q].y, (int)wa[q].z, (int)wa[q].w, 0, 0, 0, 0};
+            acc[c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc[c], 4, 4, 0, (int)xs, 0, (int)ws[q]);
+          } else {
+            u32x4 xa[4];
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+              xa[v] = buf_ld16(rx, in ? (uint32_t)(t * xb + 64 * b + 16 * v) : kOobOffset, 0);
+            const float s = mx_scale(ws[q]);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) mfma16(acc[c], xa[v], mx_bf16x8(wa[q][v], s));
+          }
+        }
+      }
+    }
+  }
+  if (ks > 0) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      if (c < nch) red[((ks - 1) * RB + rb) * NC * 64 + c * 64 + lane] = acc[c];
+  }
+  __syncthreads();
+  if (ks > 0) return;
+#pragma unroll
+  for (int q = 1; q < KS; ++q)
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      if (c < nch) acc[c] += red[((q - 1) * RB + rb) * NC * 64 + c * 64 + lane];
+  if (rl >= nrows) return;
+  skinny_store<T, NC>(epi, acc, nch, r0, rows, n0 + rl, grp);
+}
+
+}  // namespace moe

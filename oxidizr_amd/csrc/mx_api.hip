@@ -1,0 +1,301 @@
+// C ABI of microscaled 4-bit numbers: quantisation and back, and expert products over 4-bit weights.
+// Declared in include/moe_hip.h.  The calls keep no state.
+#include "entry.hpp"
+#include "mx.hpp"
+
+using namespace moe;
+
+namespace {
+
+// ---- quantisation
+moe_status check_mx(int dtype, int64_t blocks) {
+  moe_status st = check_dtype(dtype);
+  if (st != MOE_OK) return st;
+  if (blocks < 0) return fail(MOE_ERR_INVALID, "num_blocks is negative");
+  // four lanes to a block
+  return blocks >= kMaxGridThreads / 4 ? fail(MOE_ERR_UNSUPPORTED, "num_blocks reaches 2^30: split the tensor") : MOE_OK;
+}
+
+// ---- products
+constexpr int kMxMaxWidth = 1 << 20;
+moe_status check_mx_linear(int x_format, int dtype, int64_t M, int K, int N, int E, bool grouped, int act) {
+  moe_status st = check_dtype(dtype);
+  if (st != MOE_OK) return st;
+  if (x_format != MOE_MX_ROWS_BF16 && x_format != MOE_MX_ROWS_FOUR_BIT)
+    return fail(MOE_ERR_INVALID, "unknown row format %d", x_format);
+  if (x_format == MOE_MX_ROWS_BF16 && dtype != MOE_DTYPE_BF16)
+    return fail(MOE_ERR_INVALID, "bf16 rows have bf16 results");
+  if (M < 0) return fail(MOE_ERR_INVALID, "num_rows is negative");
+  if (K < kMxBlock || K % kMxBlock != 0)
+    return fail(MOE_ERR_INVALID, "in_features %d is not a positive multiple of %d", K, kMxBlock);
+  if (N < 8 || N % 8 != 0) return fail(MOE_ERR_INVALID, "out_features %d is not a positive multiple of 8", N);
+  if (grouped ? (E < 1 || E > 1024) : E != 1)
+    return fail(MOE_ERR_INVALID, grouped ? "num_groups %d is outside 1..1024"
+                                         : "num_groups %d without offsets is not 1", E);
+  if (act < 0 || act >= kNumActs) return fail(MOE_ERR_INVALID, "unknown activation %d", act);
+  if (K > kMxMaxWidth || N > kMxMaxWidth)
+    return fail(MOE_ERR_UNSUPPORTED, "in_features %d or out_features %d is above %d", K, N, kMxMaxWidth);
+  if ((int64_t)K * N >= int64_t(1) << 30)
+    return fail(MOE_ERR_UNSUPPORTED, "a weight matrix reaches 2^30 elements");
+  if (M > (int64_t(1) << 26) || M * std::max(K, N) * elt_size(dtype) >= kMaxExtentBytes * 8)
+    return fail(MOE_ERR_UNSUPPORTED, "num_rows x max(in, out features) reaches 2^34 bytes");
+  return MOE_OK;
+}
+
+int mx_skinny_split(int K) { return K >= 8 * kMxChunk ? 4 : 2; }
+int64_t mx_skinny_slots(int64_t M, int E, bool grouped) {
+  return grouped ? std::min<int64_t>(E, M) + M / kLinearSkinnyRows : ceil_div(M, kLinearSkinnyRows);
+}
+int64_t mx_skinny_blocks(int64_t M, int K, int N, int E, bool grouped) {
+  return mx_skinny_slots(M, E, grouped) * ceil_div(N, 64 / mx_skinny_split(K)) + (grouped ? 64 : 0);
+}
+bool mx_skinny(int64_t M, int K, int N, int E, bool grouped) {
+  if (mx_skinny_blocks(M, K, N, E, grouped) * 256 >= kMaxGridThreads) return false;
+  return M <= 8 * (grouped ? std::min<int64_t>(E, M) : 4);
+}
+
+// Row tiles by height; prefixes of k_linear_prep.
+enum class MxTiles { kBig, kMid, kSmall };
+using MxBig = Tilings<bf16_t>::Big;
+using MxMid = Tilings<bf16_t>::BigMid;
+using MxSmall = Tilings<bf16_t>::BigSmall;
+MxTiles mx_tiles(bool grouped, int E, int64_t M, int N) {
+  const int groups = grouped ? (int)std::min<int64_t>(E, M) : 1;
+  auto count = [&](int bm, int bn) {
+    return (grouped ? group_row_tiles(groups, (double)M / groups, bm) : (double)ceil_div(M, bm)) * ceil_div(N, bn);
+  };
+  const double big = big_cost(count(256, 256), 10.0);
+  const double mid = round_cost(count(128, 128), {4.8, 6.3});
+  const double small = round_cost(count(64, 128), {2.9, 4.3});
+  return big <= std::min(mid, small) ? MxTiles::kBig : mid <= small ? MxTiles::kMid : MxTiles::kSmall;
+}
+template <class F>
+void with_mx_tiling(MxTiles kind, F&& f) {
+  if (kind == MxTiles::kMid) return f(MxMid{});
+  if (kind == MxTiles::kSmall) return f(MxSmall{});
+  f(MxBig{});
+}
+template <class C>
+int64_t mx_grid(bool grouped, int E, int64_t M, int N) {
+  if (!grouped) return (int64_t)ceil_div(M, C::BM) * ceil_div(N, C::BN);
+  return ((int64_t)(ceil_div(M, C::BM) + E) * ceil_div(N, C::BN) + 7) / 8 * 8;
+}
+moe_status check_mx_tiles(MxTiles kind, bool grouped, int E, int64_t M, int N) {
+  moe_status st = MOE_OK;
+  with_mx_tiling(kind, [&](auto c) {
+    using C = decltype(c);
+    st = check_grid(mx_grid<C>(grouped, E, M, N), C::THREADS);
+  });
+  return st;
+}
+moe_status check_mx_launches(bool backward, bool grouped, int E, int64_t M, int K, int N) {
+  if (backward) return check_mx_tiles(mx_tiles(grouped, E, M, K), grouped, E, M, K);
+  return mx_skinny(M, K, N, E, grouped) ? MOE_OK : check_mx_tiles(mx_tiles(grouped, E, M, N), grouped, E, M, N);
+}
+// Calls f(tiling, row groups, grid).
+template <class F>
+void with_mx_rows(MxTiles kind, const int* offsets, const int* prefixes, int E, int64_t M, int N, F&& f) {
+  with_mx_tiling(kind, [&](auto c) {
+    using C = decltype(c);
+    const bool grouped = offsets != nullptr;
+    const int grid = (int)mx_grid<C>(grouped, E, M, N);
+    if (!grouped) return f(c, RowGroups{nullptr, nullptr, nullptr, nullptr, 1, (int)M, 0, 0}, grid);
+    const int* tp = prefixes + prefix_slot(C::BM) * (E + 1);
+    constexpr bool big = std::is_same<C, MxBig>::value;
+    f(c, RowGroups{offsets, tp, tp + (E + 1), tp + 2 * (E + 1), E, (int)M, big && M >= 2 * (int64_t)C::BM * E,
+                   big ? tall_rows_for(C::BM) : 0}, grid);
+  });
+}
+
+struct MxWs {
+  size_t offs, prefixes, w_tab, dz, part, total;
+};
+int64_t mx_dz_chunks(int64_t M, int E, bool grouped) { return (M + kDzRows - 1) / kDzRows + (grouped ? E : 0); }
+MxWs mx_ws(int64_t M, int N, int E, bool grouped, int act, bool backward) {
+  MxWs w{};
+  Carve c;
+  if (grouped) {
+    w.offs = c.take((size_t)(E + 1) * 4);
+    w.prefixes = c.take((size_t)kNumTilePrefixes * (E + 1) * 4);
+    w.w_tab = c.take((size_t)E * sizeof(void*));
+  }
+  if (backward) {
+    if (act != kActNone) w.dz = c.take((size_t)M * N * 2);
+    w.part = c.take((size_t)mx_dz_chunks(M, E, grouped) * N * 4);
+  }
+  w.total = c.off;
+  return w;
+}
+
+constexpr int kMxPrepBlocks = 1 + 128;
+// Clean offsets, tile prefixes, and what belongs to no expert.
+template <typename T>
+void mx_prep(hipStream_t s, const int* offsets, int E, int64_t M, char* ws, const MxWs& L, const T* res, T* out,
+             T* out2, int cols) {
+  hipLaunchKernelGGL(k_linear_prep<T>, dim3(kMxPrepBlocks), dim3(1024), 0, s, offsets, E, (int)M,
+                     (int*)(ws + L.offs), (int*)(ws + L.prefixes), (const T*)nullptr, (T*)nullptr, (int64_t)0,
+                     (const T**)(ws + L.w_tab), (T**)nullptr, res, out, out2, cols);
+}
+
+template <bool X4, typename T>
+moe_status mx_forward(hipStream_t s, int64_t M, int E, const int* offsets, const void* x, const uint8_t* xs,
+                      const MxWeights& w, const LinearEpi<T>& epi, char* ws) {
+  const bool grouped = offsets != nullptr;
+  const int N = w.N, K = w.K;
+  if (mx_skinny(M, K, N, E, grouped)) {
+    const int nslot = (int)mx_skinny_slots(M, E, grouped);
+    const unsigned grid = (unsigned)mx_skinny_blocks(M, K, N, E, grouped);
+    auto go = [&](auto nc, auto ks) {
+      hipLaunchKernelGGL((k_mx_skinny<X4, T, decltype(nc)::value, decltype(ks)::value>), dim3(grid), dim3(256), 0, s,
+                         x, xs, offsets, E, (int)M, nslot, w, epi);
+    };
+    auto split = [&](auto nc) {
+      if (mx_skinny_split(K) == 4) go(nc, std::integral_constant<int, 4>());
+      else go(nc, std::integral_constant<int, 2>());
+    };
+    if (M <= 16) split(std::integral_constant<int, 1>());
+    else split(std::integral_constant<int, 4>());
+    LAUNCH_CHECK();
+    return MOE_OK;
+  }
+  const MxWs L = mx_ws(M, N, E, grouped, epi.act, false);
+  if (grouped) mx_prep<T>(s, offsets, E, M, ws, L, epi.res, epi.y, epi.pre, N);
+  with_mx_rows(mx_tiles(grouped, E, M, N), grouped ? (const int*)(ws + L.offs) : nullptr,
+               (const int*)(ws + L.prefixes), E, M, N, [&](auto c, const RowGroups& r, int grid) {
+    using C = decltype(c);
+    if constexpr (X4)
+      hipLaunchKernelGGL((k_mxmx_fwd<C, T>), dim3(grid), dim3(C::THREADS), 0, s, (const uint8_t*)x, xs, r, w, epi);
+    else
+      hipLaunchKernelGGL((k_mx_fwd<C>), dim3(grid), dim3(C::THREADS), 0, s, (const bf16_t*)x, r, w, epi);
+  });
+  LAUNCH_CHECK();
+  return MOE_OK;
+}
+
+moe_status mx_backward(hipStream_t s, int64_t M, int E, const int* offsets, const bf16_t* dy, const MxWeights& w,
+                       const bf16_t* pre, int act, bf16_t* dx, bf16_t* db, char* ws) {
+  const bool grouped = offsets != nullptr;
+  const int N = w.N, K = w.K;
+  const MxWs L = mx_ws(M, N, E, grouped, act, true);
+  const int* offs = grouped ? (const int*)(ws + L.offs) : nullptr;
+  const int* prefixes = (const int*)(ws + L.prefixes);
+  if (grouped) mx_prep<bf16_t>(s, offsets, E, M, ws, L, nullptr, dx, nullptr, K);
+  const RowGroups chunks{offs, prefixes, nullptr, nullptr, E, (int)M, 0, 0};
+  static_assert(prefix_slot(kDzRows) == 0, "the chunks' prefix is the first");
+  const bf16_t* dz = dy;
+  if (act != kActNone || db) {
+    bf16_t* out = (bf16_t*)(ws + L.dz);
+    float* part = db ? (float*)(ws + L.part) : nullptr;
+    hipLaunchKernelGGL(k_linear_dz<bf16_t>, dim3((unsigned)mx_dz_chunks(M, E, grouped), ceil_div(N, kDzCols)),
+                       dim3(256), 0, s, dy, pre, act, chunks, N, out, part);
+    if (act != kActNone) dz = out;
+    if (db)
+      hipLaunchKernelGGL(k_linear_db<bf16_t>, dim3(ceil_div(N, 64), E), dim3(256), 0, s, part, chunks, N, db);
+  }
+  if (dx)
+    with_mx_rows(mx_tiles(grouped, E, M, K), offs, prefixes, E, M, K, [&](auto c, const RowGroups& r, int grid) {
+      using C = decltype(c);
+      hipLaunchKernelGGL((k_mx_dgrad<C>), dim3(grid), dim3(C::THREADS), 0, s, dz, r, w, dx);
+    });
+  LAUNCH_CHECK();
+  return MOE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+moe_status moe_mx_quantize(int32_t device, void* stream, int32_t dtype, int64_t num_blocks, const void* x,
+                           uint8_t* codes, uint8_t* scales) {
+  moe_status st = check_mx(dtype, num_blocks);
+  if (st != MOE_OK || num_blocks == 0) return st;
+  if ((st = check_pointers({x, codes})) != MOE_OK || (st = check_ints({scales}, 1)) != MOE_OK) return st;
+  DeviceScope dev(device);
+  HIP_TRY(dev.enter());
+  const int64_t nvec = num_blocks * 4;
+  const dim3 grid((unsigned)((nvec + 255) / 256));
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == MOE_DTYPE_BF16)
+    hipLaunchKernelGGL(k_mx_quantize<bf16_t>, grid, dim3(256), 0, s, (const bf16_t*)x, nvec, (uint32_t*)codes, scales);
+  else
+    hipLaunchKernelGGL(k_mx_quantize<float>, grid, dim3(256), 0, s, (const float*)x, nvec, (uint32_t*)codes, scales);
+  LAUNCH_CHECK();
+  return MOE_OK;
+}
+
+moe_status moe_mx_dequantize(int32_t device, void* stream, int32_t dtype, int64_t num_blocks, const uint8_t* codes,
+                             const uint8_t* scales, void* y) {
+  moe_status st = check_mx(dtype, num_blocks);
+  if (st != MOE_OK || num_blocks == 0) return st;
+  if ((st = check_pointers({codes, y})) != MOE_OK || (st = check_ints({scales}, 1)) != MOE_OK) return st;
+  DeviceScope dev(device);
+  HIP_TRY(dev.enter());
+  const int64_t nvec = num_blocks * 4;
+  const dim3 grid((unsigned)((nvec + 255) / 256));
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == MOE_DTYPE_BF16)
+    hipLaunchKernelGGL(k_mx_dequantize<bf16_t>, grid, dim3(256), 0, s, (const uint32_t*)codes, scales, nvec, (bf16_t*)y);
+  else
+    hipLaunchKernelGGL(k_mx_dequantize<float>, grid, dim3(256), 0, s, (const uint32_t*)codes, scales, nvec, (float*)y);
+  LAUNCH_CHECK();
+  return MOE_OK;
+}
+
+size_t moe_mx_linear_workspace_bytes(int32_t x_format, int32_t dtype, int64_t M, int32_t K, int32_t N, int32_t E,
+                                     int32_t grouped, int32_t activation, int32_t backward) {
+  if (check_mx_linear(x_format, dtype, M, K, N, E, grouped != 0, activation) != MOE_OK) return 0;
+  if (M > 0 && check_mx_launches(backward != 0, grouped != 0, E, M, K, N) != MOE_OK) return 0;
+  return mx_ws(M, N, E, grouped != 0, activation, backward != 0).total;
+}
+
+moe_status moe_mx_linear_forward(int32_t device, void* stream, int32_t x_format, int32_t dtype, int64_t M, int32_t K,
+                                 int32_t N, int32_t E, const int32_t* offsets, const void* x, const uint8_t* x_scales,
+                                 const uint8_t* w_codes, const uint8_t* w_scales, const void* bias,
+                                 const void* residual, int32_t activation, void* y, void* pre_act, void* workspace) {
+  moe_status st = check_mx_linear(x_format, dtype, M, K, N, E, offsets != nullptr, activation);
+  if (st != MOE_OK || M == 0) return st;
+  if ((st = check_mx_launches(false, offsets != nullptr, E, M, K, N)) != MOE_OK) return st;
+  if ((st = check_pointers({x, w_codes, y}, {bias, residual, pre_act})) != MOE_OK) return st;
+  if ((st = check_ints({w_scales}, 1)) != MOE_OK) return st;
+  const bool four = x_format == MOE_MX_ROWS_FOUR_BIT;
+  if (four && (st = check_ints({x_scales}, 1)) != MOE_OK) return st;
+  if (offsets && ((st = check_ints({offsets})) != MOE_OK || (st = check_pointers({workspace})) != MOE_OK)) return st;
+  DeviceScope dev(device);
+  HIP_TRY(dev.enter());
+  hipStream_t s = (hipStream_t)stream;
+  const MxWeights w{w_codes, w_scales, N, K};
+  auto go = [&](auto x4, auto d) {
+    using D = decltype(d);
+    return mx_forward<decltype(x4)::value, D>(s, M, E, offsets, x, x_scales, w,
+                                              LinearEpi<D>{(const D*)bias, (const D*)residual, (D*)y, (D*)pre_act,
+                                                           activation, N}, (char*)workspace);
+  };
+  if (!four) return go(std::false_type(), bf16_t());
+  return dtype == MOE_DTYPE_BF16 ? go(std::true_type(), bf16_t()) : go(std::true_type(), float());
+}
+
+moe_status moe_mx_linear_backward(int32_t device, void* stream, int64_t M, int32_t K, int32_t N, int32_t E,
+                                  const int32_t* offsets, const void* d_y, const uint8_t* w_codes,
+                                  const uint8_t* w_scales, const void* pre_act, int32_t activation, void* dx,
+                                  void* d_bias, void* workspace) {
+  moe_status st = check_mx_linear(MOE_MX_ROWS_BF16, MOE_DTYPE_BF16, M, K, N, E, offsets != nullptr, activation);
+  if (st != MOE_OK) return st;
+  if ((st = check_pointers({}, {dx, d_bias, workspace})) != MOE_OK) return st;
+  if (M > 0) {
+    if ((st = check_mx_launches(true, offsets != nullptr, E, M, K, N)) != MOE_OK) return st;
+    if ((st = check_pointers({d_y, w_codes}, {pre_act})) != MOE_OK) return st;
+    if ((st = check_ints({w_scales}, 1)) != MOE_OK) return st;
+    if (activation != kActNone && !pre_act)
+      return fail(MOE_ERR_INVALID, "the activation's backward needs pre_act");
+    if (offsets && (st = check_ints({offsets})) != MOE_OK) return st;
+    if (!workspace) return fail(MOE_ERR_INVALID, "a required pointer is NULL");
+  }
+  DeviceScope dev(device);
+  HIP_TRY(dev.enter());
+  hipStream_t s = (hipStream_t)stream;
+  if (M == 0) return zero_async(s, d_bias, (size_t)E * N * 2);  // sums over no row
+  return mx_backward(s, M, E, offsets, (const bf16_t*)d_y, {w_codes, w_scales, N, K}, (const bf16_t*)pre_act,
+                     activation, (bf16_t*)dx, (bf16_t*)d_bias, (char*)workspace);
+}
+
+}  // extern "C"

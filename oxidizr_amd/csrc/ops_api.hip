@@ -2,65 +2,13 @@
 // expert products with bias, activation and residual, norms around a block.
 // Declared in include/moe_hip.h.  The calls keep no state: sizes in, device
 // pointers in, launches on the call's stream.
-#include "host.hpp"
+#include "entry.hpp"
 #include "linear.hpp"
 #include "ops.hpp"
 
 using namespace moe;
 
 namespace {
-
-// Makes `device` current for one call and the caller's device current after it.
-struct DeviceScope {
-  int before = -1, device;
-  bool changed = false;
-  explicit DeviceScope(int d) : device(d) {}
-  hipError_t enter() {
-    hipError_t e = hipGetDevice(&before);
-    if (e != hipSuccess || before == device) return e;
-    e = hipSetDevice(device);
-    changed = e == hipSuccess;
-    return e;
-  }
-  ~DeviceScope() {
-    if (changed) (void)hipSetDevice(before);
-  }
-};
-
-moe_status check_pointers(std::initializer_list<const void*> needed,
-                          std::initializer_list<const void*> optional = {}) {
-  for (const void* p : needed) {
-    if (!p) return fail(MOE_ERR_INVALID, "a required pointer is NULL");
-    if (!aligned16(p)) return fail(MOE_ERR_INVALID, "device pointers must be 16-byte aligned");
-  }
-  for (const void* p : optional)
-    if (p && !aligned16(p)) return fail(MOE_ERR_INVALID, "device pointers must be 16-byte aligned");
-  return MOE_OK;
-}
-
-moe_status check_dtype(int dtype) {
-  if (dtype != MOE_DTYPE_F32 && dtype != MOE_DTYPE_BF16)
-    return fail(MOE_ERR_INVALID, "unknown dtype %d", dtype);
-  return MOE_OK;
-}
-
-// Integer arrays (indices, orders, offsets) need their own alignment only: they may be
-// slices of one allocation.
-moe_status check_ints(std::initializer_list<const void*> needed, size_t bytes = 4) {
-  for (const void* p : needed) {
-    if (!p) return fail(MOE_ERR_INVALID, "a required pointer is NULL");
-    if ((uintptr_t)p % bytes) return fail(MOE_ERR_INVALID, "an integer array is not aligned");
-  }
-  return MOE_OK;
-}
-
-// Whether a launch of `blocks` workgroups of `threads` fits a grid.
-constexpr int64_t kMaxGridThreads = int64_t(1) << 32;
-moe_status check_grid(int64_t blocks, int threads) {
-  if (blocks * threads >= kMaxGridThreads)
-    return fail(MOE_ERR_UNSUPPORTED, "too many rows or tiles for one launch: split the batch");
-  return MOE_OK;
-}
 
 // ---- sort by expert
 constexpr int64_t kMaxAssignments = (int64_t(1) << 31) - 1;  // positions are int32

@@ -8,6 +8,14 @@ experts (src/model.rs:1416-1446), biases, other activations, norms on both sides
     y = unpermute_tokens(b, order, weights)               # back to [T, H], weighted
     h, n = residual_norm(h, y, post_weight, gate=g, next_weight=w)
 
+The router's losses over the same routing, and experts whose frozen weights are held in 4 bits (adapters are
+trained over such, prompts and decoding served from them):
+
+    losses = router_losses(logits, topk_idx)              # balance, z, counts
+    q1 = quantize_mxfp4(w1)                               # once
+    a = mx_linear(rows, q1, b1, offsets=order.offsets, activation="gelu")
+    a = mx_linear(quantize_mxfp4(rows), q1, b1, offsets=order.offsets, activation="gelu")  # both sides in 4 bits
+
 Every function takes float32 or bfloat16 CUDA tensors (one dtype to a call; routing weights are
 float32), runs on the current stream of their device, sums in fp32 in a fixed order and is
 differentiable once, backward; a forward-mode derivative and a trace (torch.jit.trace, make_fx) are
@@ -467,3 +475,288 @@ def residual_norm(h, y, post_weight=None, *, gate=None, next_weight=None, residu
         return _ResidualNorm.apply(h, y, post_weight, gate, next_weight, s)
     out, n, _, _ = _norm(_ready(h), _ready(y), _ready(post_weight), _ready(gate), _ready(next_weight), s, False)
     return out if n is None else (out, n)
+
+
+# ---------------------------------------------------------------- losses of a router
+
+SCORES = ("softmax", "sigmoid")  # moe_score's order
+MAX_SEQUENCES = (1 << 22) - 1
+
+
+class RouterLosses(NamedTuple):
+    """Losses of a routing (float32) and its counts (int32); a leading S with offsets."""
+    balance: torch.Tensor  # [] or [S]
+    z: torch.Tensor        # [] or [S]
+    counts: torch.Tensor   # [E] or [S, E] assignments of each expert
+
+
+class _RouterShape(NamedTuple):
+    T: int
+    E: int
+    k: int
+    S: int
+    score: int
+    temperature: float
+    switch_coef: float
+    sqprob_coef: float
+    shape: tuple  # of a loss
+
+
+def _router(logits, idx, offsets, s, keep):
+    L = _lib.load()
+    # one allocation for what a backward reads: slope, inv_real and lse
+    out = logits.new_empty(2, s.S, dtype=torch.float32)
+    counts = logits.new_empty(s.S, s.E, dtype=torch.int32)
+    kept = logits.new_empty(s.S * (s.E + 1) + s.T, dtype=torch.float32) if keep else None
+    at = kept.data_ptr() if keep else 0
+    ws = _workspace(L.moe_router_losses_workspace_bytes(s.T, s.E, s.S), logits)
+    _call(L.moe_router_losses, logits.get_device(), _dtype_code(logits.dtype), s.T, s.E, s.k, idx.element_size(),
+          logits.data_ptr(), idx.data_ptr(), s.score, s.temperature, s.switch_coef, s.sqprob_coef, _ptr(offsets), s.S,
+          out.data_ptr(), out.data_ptr() + 4 * s.S, counts.data_ptr(), at if keep else None,
+          at + 4 * s.S * s.E if keep else None, at + 4 * s.S * (s.E + 1) if keep else None, _ptr(ws))
+    balance, z = out.unbind(0)
+    return balance.view(s.shape), z.view(s.shape), counts.view(s.shape + (s.E,)), kept
+
+
+class _RouterLosses(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, idx, offsets, s):
+        ctx.set_materialize_grads(False)
+        logits = _ready(logits)
+        balance, z, counts, kept = _router(logits, idx, offsets, s, True)
+        ctx.save_for_backward(logits, idx, offsets, kept)
+        ctx.s = s
+        ctx.mark_non_differentiable(counts)
+        return balance, z, counts
+
+    @staticmethod
+    @_once
+    def backward(ctx, d_balance, d_z, _):
+        logits, idx, offsets, kept = ctx.saved_tensors
+        s = ctx.s
+        if d_balance is None and d_z is None:
+            return (None,) * 4
+        d_balance = None if d_balance is None else d_balance.contiguous()
+        d_z = None if d_z is None else d_z.contiguous()
+        d_logits = torch.empty_like(logits)
+        at = kept.data_ptr()
+        _call(_lib.load().moe_router_losses_backward, logits.get_device(), _dtype_code(logits.dtype), s.T, s.E, s.k,
+              idx.element_size(), logits.data_ptr(), idx.data_ptr(), s.score, s.temperature,
+              _ptr(offsets), s.S, at, at + 4 * s.S * s.E, at + 4 * s.S * (s.E + 1), _ptr(d_balance), _ptr(d_z), d_logits.data_ptr())
+        return d_logits, None, None, None
+
+
+def router_losses(logits, topk_idx, *, score: str = "softmax", temperature: float = 1.0, switch_coef: float = 1.0,
+                  sqprob_coef: float = 1.0, offsets=None) -> RouterLosses:
+    """The load-balance and z losses of a routing, and each expert's assignments:
+
+        x = logits / temperature,  q = softmax(x), or sigmoid(x) / sum sigmoid(x)
+        balance = E sum_e (switch_coef f_e P_e + sqprob_coef P_e^2),  P_e = mean_t q_te,  f_e = M_e / (k n)
+        z = mean_t logsumexp(x_t)^2
+
+    over the n tokens that have an expert; tokens all of whose topk_idx [T, k] (int32 or int64) lie outside [0, E) are
+    padding, whatever their logits [T, E] hold. With offsets (int32 [S + 1], ascending row offsets of sequences) each sequence
+    has losses and counts of its own; rows of none count nowhere. A sequence without tokens has losses 0. Differentiable in
+    logits; the counts M_e are not."""
+    if logits.dim() != 2:
+        raise ModelError(f"logits must be [T, E], got {list(logits.shape)}")
+    T, E = logits.shape
+    if topk_idx.dim() != 2 or topk_idx.shape[0] != T:
+        raise ModelError(f"topk_idx must be [{T}, k], got {list(topk_idx.shape)}")
+    if topk_idx.dtype not in (torch.int32, torch.int64):
+        raise ModelError(f"topk_idx must be int32 or int64, got {topk_idx.dtype}")
+    k = topk_idx.shape[1]
+    if not 1 <= k <= MAX_EXPERTS_PER_TOK:
+        raise ModelError(f"experts per token must be 1..{MAX_EXPERTS_PER_TOK}, got {k}")
+    if not 1 <= E <= MAX_EXPERTS:
+        raise ModelError(f"num_experts must be 1..{MAX_EXPERTS}, got {E}")
+    if score not in SCORES:
+        raise ModelError(f"score must be one of {SCORES}, got {score!r}")
+    if not 0.0 < temperature < float("inf"):
+        raise ModelError(f"temperature must be positive and finite, got {temperature}")
+    S = 1
+    if offsets is not None:
+        if offsets.dim() != 1 or offsets.dtype != torch.int32 or offsets.numel() < 1:
+            raise ModelError(f"offsets must be int32 [S + 1], got {offsets.dtype} {list(offsets.shape)}")
+        S = offsets.numel() - 1
+        if S > MAX_SEQUENCES:
+            raise ModelError(f"at most {MAX_SEQUENCES} sequences, got {S}")
+    _dtype_code(logits.dtype)
+    _on_device(logits, topk_idx, offsets)
+    s = _RouterShape(T, E, k, S, SCORES.index(score), float(temperature), float(switch_coef), float(sqprob_coef),
+                     () if offsets is None else (S,))
+    idx = topk_idx.contiguous()
+    offsets = None if offsets is None else offsets.contiguous()
+    if _derivable(logits):
+        return RouterLosses(*_RouterLosses.apply(logits, idx, offsets, s))
+    return RouterLosses(*_router(_ready(logits), idx, offsets, s, False)[:3])
+
+
+# ---------------------------------------------------------------- microscaled 4-bit numbers
+
+MX_BLOCK = 32
+
+
+class MxTensor(NamedTuple):
+    """A tensor [..., K] of OCP MXFP4 numbers: E2M1 elements, 32 along the last dimension under one
+    power of two. An element's four bits are its sign and one of 0 0.5 1 1.5 2 3 4 6; element 2 i is the low
+    half of byte i. A scale byte is the exponent plus 127 (255: NaN)."""
+    codes: torch.Tensor   # uint8 [..., K / 2]
+    scales: torch.Tensor  # uint8 [..., K / 32]
+
+
+def quantize_mxfp4(x) -> MxTensor:
+    """x [..., K] (float32 or bfloat16, K a multiple of 32) in 4 bits: a block's exponent is that of its largest
+    magnitude less 2, an element the nearest number (ties to the even code; what is above the largest becomes it). A block that
+    holds an infinity or a NaN becomes NaN. The result has no gradient."""
+    if x.dim() < 1 or x.shape[-1] < MX_BLOCK or x.shape[-1] % MX_BLOCK:
+        raise ModelError(f"expected [..., K] with K a positive multiple of {MX_BLOCK}, got {list(x.shape)}")
+    code = _dtype_code(x.dtype)
+    dev = _on_device(x)
+    x = _ready(x.detach())
+    lead, K = x.shape[:-1], x.shape[-1]
+    codes = x.new_empty(lead + (K // 2,), dtype=torch.uint8)
+    scales = x.new_empty(lead + (K // MX_BLOCK,), dtype=torch.uint8)
+    _call(_lib.load().moe_mx_quantize, dev, code, scales.numel(), x.data_ptr(), codes.data_ptr(), scales.data_ptr())
+    return MxTensor(codes, scales)
+
+
+def _check_mx(q, what):
+    if not isinstance(q, MxTensor):
+        raise ModelError(f"{what} must be an MxTensor (quantize_mxfp4)")
+    c, s = q
+    if c.dtype != torch.uint8 or s.dtype != torch.uint8:
+        raise ModelError(f"an MxTensor holds uint8 tensors, got {c.dtype} and {s.dtype}")
+    if not (c.dim() >= 1 and c.dim() == s.dim() and c.shape[:-1] == s.shape[:-1] and s.shape[-1] >= 1 and
+            c.shape[-1] == MX_BLOCK // 2 * s.shape[-1]):
+        raise ModelError(f"{what}: codes {list(c.shape)} and scales {list(s.shape)} do not go together "
+                         f"([..., K / 2] and [..., K / {MX_BLOCK}])")
+
+
+def dequantize_mxfp4(q: MxTensor, dtype=torch.bfloat16):
+    """The numbers [..., K] that q stands for, in dtype (float32 or bfloat16): exact."""
+    _check_mx(q, "q")
+    code = _dtype_code(dtype)
+    dev = _on_device(*q)
+    codes, scales = _ready(q.codes), q.scales.contiguous()
+    y = torch.empty(codes.shape[:-1] + (2 * codes.shape[-1],), dtype=dtype, device=codes.device)
+    _call(_lib.load().moe_mx_dequantize, dev, code, scales.numel(), codes.data_ptr(), scales.data_ptr(), y.data_ptr())
+    return y
+
+
+class _MxShape(NamedTuple):
+    M: int
+    K: int
+    N: int
+    groups: int
+    grouped: bool
+    act: int
+    rows: int          # moe_mx_rows
+    dtype: torch.dtype
+
+
+def _mx(x, x_scales, codes, scales, bias, offsets, residual, s, keep):
+    L = _lib.load()
+    code = _dtype_code(s.dtype)
+    y = torch.empty(s.M, s.N, dtype=s.dtype, device=x.device)
+    pre = torch.empty_like(y) if keep else None
+    ws = _workspace(L.moe_mx_linear_workspace_bytes(s.rows, code, s.M, s.K, s.N, s.groups, s.grouped, s.act, 0), x)
+    _call(L.moe_mx_linear_forward, x.get_device(), s.rows, code, s.M, s.K, s.N, s.groups, _ptr(offsets), x.data_ptr(),
+          _ptr(x_scales), codes.data_ptr(), scales.data_ptr(), _ptr(bias), _ptr(residual), s.act, y.data_ptr(),
+          _ptr(pre), _ptr(ws))
+    return y, pre
+
+
+class _MxLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, x_scales, bias, residual, codes, scales, offsets, s):
+        four = s.rows == _lib.MOE_MX_ROWS_FOUR_BIT
+        x, bias, residual = _ready(x), _ready(bias), _ready(residual)
+        products = ctx.needs_input_grad[0] or ctx.needs_input_grad[2]
+        if products:
+            L = _lib.load()
+            ctx.ws_bytes = L.moe_mx_linear_workspace_bytes(_lib.MOE_MX_ROWS_BF16, _lib.MOE_DTYPE_BF16, s.M, s.K, s.N,
+                                                           s.groups, s.grouped, s.act, 1)
+            if four or (ctx.ws_bytes == 0 and s.M > 0):
+                raise _lib.MoeError(_lib.MOE_ERR_UNSUPPORTED, "rows in 4 bits have no gradient of a bias" if four else
+                                    L.moe_last_error().decode())
+        y, pre = _mx(x, x_scales, codes, scales, bias, offsets, residual, s, products and s.act != 0)
+        ctx.save_for_backward(codes, scales, pre, offsets)
+        ctx.s = s
+        return y
+
+    @staticmethod
+    @_once
+    def backward(ctx, dy):
+        codes, scales, pre, offsets = ctx.saved_tensors
+        s, need_x, need_b, need_r = ctx.s, ctx.needs_input_grad[0], ctx.needs_input_grad[2], ctx.needs_input_grad[3]
+        dx = db = None
+        if need_x or need_b:
+            up = _ready(dy)
+            dx = up.new_empty(s.M, s.K) if need_x else None
+            db = up.new_empty((s.groups, s.N) if s.grouped else (s.N,)) if need_b else None
+            ws = _workspace(ctx.ws_bytes, up)
+            _call(_lib.load().moe_mx_linear_backward, up.get_device(), s.M, s.K, s.N, s.groups, _ptr(offsets),
+                  _ptr(up), codes.data_ptr(), scales.data_ptr(), _ptr(pre), s.act, _ptr(dx), _ptr(db), _ptr(ws))
+        return dx, None, db, dy if need_r else None, None, None, None, None
+
+
+def mx_linear(x, weight: MxTensor, bias=None, *, offsets=None, activation: str = "none", residual=None, dtype=None):
+    """activation(x W^T + bias) + residual, [M, N], as expert_linear, over 4-bit weights: an MxTensor [E, N, K], or
+    [N, K] without offsets. N is a multiple of 8, K of 32.
+
+    x [M, K] is bfloat16, as are bias, residual and the result, and the products are bf16 ones of the exact weights:
+    differentiable in x, bias and residual. Or x is an MxTensor [M, K]: products of 4-bit numbers, in bfloat16 or float32
+    (dtype; bias and residual too), with a gradient of the residual alone. Sums are fp32."""
+    if activation not in ACTIVATIONS:
+        raise ModelError(f"activation must be one of {ACTIVATIONS}, got {activation!r}")
+    _check_mx(weight, "weight")
+    four = isinstance(x, MxTensor)
+    if four:
+        _check_mx(x, "x")
+        rows, x_scales = x
+        dtype = torch.bfloat16 if dtype is None else dtype
+        _dtype_code(dtype)
+    else:
+        rows, x_scales = x, None
+        if x.dtype != torch.bfloat16:
+            raise ModelError(f"x must be bfloat16 or an MxTensor, got {x.dtype}")
+        if dtype is not None and dtype != torch.bfloat16:
+            raise ModelError(f"bfloat16 rows have bfloat16 results, got {dtype}")
+        dtype = torch.bfloat16
+    if rows.dim() != 2:
+        raise ModelError(f"x must be [M, K], got {list(rows.shape)}")
+    M, K = rows.shape[0], rows.shape[1] * (2 if four else 1)
+    codes, scales = weight
+    grouped = offsets is not None
+    if not (codes.dim() == (3 if grouped else 2) and 2 * codes.shape[-1] == K):
+        raise ModelError(f"weight must be {'[E, N' if grouped else '[N'}, {K}], got "
+                         f"{list(codes.shape[:-1]) + [2 * codes.shape[-1]]}")
+    groups, N = (codes.shape[0], codes.shape[1]) if grouped else (1, codes.shape[0])
+    if not (N >= 8 and N % 8 == 0):
+        raise ModelError(f"the output width must be a positive multiple of 8, got {N}")
+    if grouped:
+        if not 1 <= groups <= MAX_EXPERTS:
+            raise ModelError(f"num_experts must be 1..{MAX_EXPERTS}, got {groups}")
+        if not (offsets.dtype == torch.int32 and offsets.shape == (groups + 1,)):
+            raise ModelError(f"offsets must be int32 [{groups + 1}], got {offsets.dtype} {list(offsets.shape)}")
+    if bias is not None:
+        want = (groups, N) if grouped else (N,)
+        if bias.shape != want:
+            raise ModelError(f"bias must be {list(want)}, got {list(bias.shape)}")
+    if residual is not None and residual.shape != (M, N):
+        raise ModelError(f"residual must be [{M}, {N}], got {list(residual.shape)}")
+    for t in (bias, residual):
+        if not (t is None or t.dtype == dtype):
+            raise ModelError(f"bias and residual must be {dtype}, as the result")
+    if four and bias is not None and torch.is_grad_enabled() and bias.requires_grad:
+        raise ModelError("rows in 4 bits have no gradient of a bias: detach it")
+    _on_device(rows, codes, scales, x_scales, bias, offsets, residual)
+    s = _MxShape(M, K, N, groups, grouped, ACTIVATIONS.index(activation),
+                 _lib.MOE_MX_ROWS_FOUR_BIT if four else _lib.MOE_MX_ROWS_BF16, dtype)
+    offsets = offsets.contiguous() if grouped else None
+    codes, scales = _ready(codes), scales.contiguous()
+    x_scales = x_scales.contiguous() if four else None
+    if _derivable(rows, bias, residual):
+        return _MxLinear.apply(rows, x_scales, bias, residual, codes, scales, offsets, s)
+    return _mx(_ready(rows), x_scales, codes, scales, _ready(bias), offsets, _ready(residual), s, False)[0]

@@ -67,6 +67,14 @@ pub mod ffi {
     pub const MOE_GATE_TOKEN: i32 = 2;
     pub const MOE_GATE_FULL: i32 = 3;
 
+    /// `moe_score`.
+    pub const MOE_SCORE_SOFTMAX: i32 = 0;
+    pub const MOE_SCORE_SIGMOID: i32 = 1;
+
+    /// `moe_mx_rows`.
+    pub const MOE_MX_ROWS_BF16: i32 = 0;
+    pub const MOE_MX_ROWS_FOUR_BIT: i32 = 1;
+
     #[repr(C)]
     #[derive(Clone, Copy, Debug, Default)]
     pub struct MoeConfigC {
@@ -339,6 +347,123 @@ pub mod ffi {
             d_post_weight: *mut c_void,
             d_gate: *mut c_void,
             d_next_weight: *mut c_void,
+            workspace: *mut c_void,
+        ) -> MoeStatus;
+        pub fn moe_router_losses_workspace_bytes(
+            num_tokens: i64,
+            num_experts: i32,
+            num_sequences: i64,
+        ) -> usize;
+        pub fn moe_router_losses(
+            device: i32,
+            stream: *mut c_void,
+            dtype: i32,
+            num_tokens: i64,
+            num_experts: i32,
+            experts_per_tok: i32,
+            index_bytes: i32,
+            logits: *const c_void,
+            topk_idx: *const c_void,
+            score: i32,
+            temperature: f32,
+            switch_coef: f32,
+            sqprob_coef: f32,
+            offsets: *const i32,
+            num_sequences: i64,
+            balance: *mut f32,
+            z: *mut f32,
+            counts: *mut i32,
+            slope: *mut f32,
+            inv_real: *mut f32,
+            lse: *mut f32,
+            workspace: *mut c_void,
+        ) -> MoeStatus;
+        pub fn moe_router_losses_backward(
+            device: i32,
+            stream: *mut c_void,
+            dtype: i32,
+            num_tokens: i64,
+            num_experts: i32,
+            experts_per_tok: i32,
+            index_bytes: i32,
+            logits: *const c_void,
+            topk_idx: *const c_void,
+            score: i32,
+            temperature: f32,
+            offsets: *const i32,
+            num_sequences: i64,
+            slope: *const f32,
+            inv_real: *const f32,
+            lse: *const f32,
+            d_balance: *const f32,
+            d_z: *const f32,
+            d_logits: *mut c_void,
+        ) -> MoeStatus;
+        pub fn moe_mx_quantize(
+            device: i32,
+            stream: *mut c_void,
+            dtype: i32,
+            num_blocks: i64,
+            x: *const c_void,
+            codes: *mut u8,
+            scales: *mut u8,
+        ) -> MoeStatus;
+        pub fn moe_mx_dequantize(
+            device: i32,
+            stream: *mut c_void,
+            dtype: i32,
+            num_blocks: i64,
+            codes: *const u8,
+            scales: *const u8,
+            y: *mut c_void,
+        ) -> MoeStatus;
+        pub fn moe_mx_linear_workspace_bytes(
+            x_format: i32,
+            dtype: i32,
+            num_rows: i64,
+            in_features: i32,
+            out_features: i32,
+            num_groups: i32,
+            grouped: i32,
+            activation: i32,
+            backward: i32,
+        ) -> usize;
+        pub fn moe_mx_linear_forward(
+            device: i32,
+            stream: *mut c_void,
+            x_format: i32,
+            dtype: i32,
+            num_rows: i64,
+            in_features: i32,
+            out_features: i32,
+            num_groups: i32,
+            offsets: *const i32,
+            x: *const c_void,
+            x_scales: *const u8,
+            w_codes: *const u8,
+            w_scales: *const u8,
+            bias: *const c_void,
+            residual: *const c_void,
+            activation: i32,
+            y: *mut c_void,
+            pre_act: *mut c_void,
+            workspace: *mut c_void,
+        ) -> MoeStatus;
+        pub fn moe_mx_linear_backward(
+            device: i32,
+            stream: *mut c_void,
+            num_rows: i64,
+            in_features: i32,
+            out_features: i32,
+            num_groups: i32,
+            offsets: *const i32,
+            d_y: *const c_void,
+            w_codes: *const u8,
+            w_scales: *const u8,
+            pre_act: *const c_void,
+            activation: i32,
+            dx: *mut c_void,
+            d_bias: *mut c_void,
             workspace: *mut c_void,
         ) -> MoeStatus;
         pub fn moe_last_error() -> *const c_char;
