@@ -205,6 +205,15 @@ struct DmaStager {
           rs[seg], (lds_void_t*)(tile + (i * C::NW * RPI + wave * RPI) * C::BK), 16,
           kin ? (G ? vrow[i] : voff + i * step) : kOobOffset, soff, 0, 0);
   }
+  // Instruction i of issue(tile, k0, 0); without `more` there is no such k-tile, and it brings zeros.
+  MOE_DEV void issue_one(T* tile, int i, int k0, bool more) const {
+    static_assert(!G, "rows as they lie");
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool kin = more && k0 + kcol < k_valid[0];
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        rs[0], (lds_void_t*)(tile + (i * C::NW * RPI + wave * RPI) * C::BK), 16,
+        kin ? voff + i * step : kOobOffset, more ? (uint32_t)k0 * (uint32_t)sizeof(T) : 0u, 0, 0);
+  }
   MOE_DEV static u32x4 frag(const T* tile, int row, int kv) {
     return *reinterpret_cast<const u32x4*>(tile + row * C::BK + ((kv ^ swz(row)) * C::V));
   }

@@ -415,14 +415,14 @@ MOE_DEV bool skinny_slot(const int* __restrict__ offsets, int E, int M, int s, i
 // Rows of no expert, as block `block` of `blocks`: the residual, or zeros.
 template <typename T>
 MOE_DEV void skinny_no_group(const int* __restrict__ offsets, int E, int M, int N, int64_t block, int64_t blocks,
-                             const LinearEpi<T>& epi) {
+                             const LinearEpi<T>& epi, int threads = 256) {
   int m = 0;
   for (int e = threadIdx.x & 63; e <= E; e += 64) m = max(m, offsets[e]);
   m = min(wave_max(m), M);
   const int64_t head = (int64_t)min(max(offsets[0], 0), M) * N / 8, tail = (int64_t)m * N / 8;
   const int64_t none = head + (int64_t)M * N / 8 - tail;
-  const int64_t step = blocks * 256;
-  for (int64_t j = block * 256 + threadIdx.x; j < none; j += step) {
+  const int64_t step = blocks * threads;
+  for (int64_t j = block * threads + threadIdx.x; j < none; j += step) {
     const int64_t v = j < head ? j : j - head + tail;
     float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};

@@ -86,6 +86,92 @@ struct MxWeights {
   int N, K;
 };
 
+// Rows of a launch: groups by offsets [G + 1], or (null) M rows of one.
+struct MxRows {
+  const int* offsets;
+  int G, M;
+};
+
+// The tile of block blk of a launch with N output columns: group, first row, rows and first column, or false for a
+// block past the tiles.  Group by group, as resolve_rows has them, but from the offsets alone: lane l counts the
+// row tiles of groups l G / 64 .., a prefix sum over the lanes gives their number and the lane that holds the
+// block's, so a grouped call needs no launch before it (a kernel that writes prefixes takes 6 us, and finding a
+// group in them log2(G) loads one after another).  Offsets are clamped to 0 .. M and each group's end to its
+// start: whatever they hold, a tile's rows exist.
+template <int BM, int BN>
+MOE_DEV bool mx_tile(const MxRows& r, int N, int blk, int& grp, int& row0, int& mv, int& n0) {
+  const int nN = (N + BN - 1) / BN;
+  int id, mt, nt;
+  if (r.offsets == nullptr) {
+    const int nM = (r.M + BM - 1) / BM;
+    if (!xcd_slot(blk, nM * nN, id) || !tile_order(id, nM, nN, mt, nt)) return false;
+    grp = 0;
+    row0 = mt * BM;
+    mv = min(BM, r.M - row0);
+    n0 = nt * BN;
+    return true;
+  }
+  const int lane = threadIdx.x & 63, per = (r.G + 63) >> 6;
+  auto range = [&](int e, int& a, int& b) {
+    a = min(max(r.offsets[e], 0), r.M);
+    b = min(max(r.offsets[e + 1], a), r.M);
+  };
+  int n = 0;
+  for (int i = 0; i < per; ++i) {
+    int a, b;
+    if (lane * per + i < r.G) {
+      range(lane * per + i, a, b);
+      n += (b - a + BM - 1) / BM;
+    }
+  }
+  const int incl = wave_incl_scan(n);
+  const int total = __builtin_amdgcn_readlane(incl, 63);
+  if (!xcd_slot(blk, total * nN, id)) return false;
+  const int s = uni(id / nN);
+  const int l = __ffsll((unsigned long long)__ballot(incl > s)) - 1;
+  int first = __builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(n, l);
+  for (int i = 0; i < per; ++i) {  // the groups of lane l, walked by every lane
+    int a, b;
+    range(l * per + i, a, b);
+    a = uni(a);
+    b = uni(b);
+    const int c = (b - a + BM - 1) / BM;
+    if (s < first + c) {
+      if (!tile_order<kRowWalk>(id - first * nN, c, nN, mt, nt)) return false;
+      grp = l * per + i;
+      row0 = a + mt * BM;
+      mv = min(BM, b - row0);
+      n0 = nt * BN;
+      return true;
+    }
+    first += c;
+  }
+  return false;
+}
+
+// body(tiling): a BM/4- or BM/2-row tiling when that covers the mv valid rows, else the half-width tiling when at most
+// BN / 2 of the nv remaining columns are valid, else the 3BM/4-row tiling when that covers the rows, else C.
+template <class C, class F>
+MOE_DEV void with_mx_shape(int mv, int nv, F&& body) {
+  if constexpr (has_half_rows<bf16_t, C>()) {
+    if (mv <= C::BM / 4) return body(QuarterRows<C>{});
+    if (mv <= C::BM / 2) return body(HalfRows<C>{});
+    if (nv <= C::BN / 2) return body(HalfCols<C>{});
+    if (mv <= 3 * C::BM / 4) return body(ThreeQuarterRows<C>{});
+  }
+  body(C{});
+}
+constexpr int max_of(int a, int b) { return a > b ? a : b; }
+template <class C>
+constexpr int mx_smem_elems() {
+  int n = kernel_smem_elems<C, bf16_t, 1, 1, 1>();
+  if constexpr (has_half_rows<bf16_t, C>()) {
+    n = max_of(n, max_of(kernel_smem_elems<QuarterRows<C>, bf16_t, 1, 1, 1>(), kernel_smem_elems<HalfRows<C>, bf16_t, 1, 1, 1>()));
+    n = max_of(n, max_of(kernel_smem_elems<HalfCols<C>, bf16_t, 1, 1, 1>(), kernel_smem_elems<ThreeQuarterRows<C>, bf16_t, 1, 1, 1>()));
+  }
+  return n;
+}
+
 // One operand tile of 4-bit weights, staged through registers: a piece is a block of 32 elements, 16 bytes of
 // codes and a scale; a thread loads its pieces of a k-tile one k-tile ahead, and writes them as 4 x 16 bytes of bf16
 // into the LDS tile, laid out as the direct loads of a bf16 operand would have left it (gemm.hpp), so the
@@ -151,16 +237,17 @@ struct MxStager {
 // mainloop_dma, W through MxStager.  Per k-tile kt: the pieces of kt + 1, loaded during kt - 1, are written
 // to their stage (which was last read before the barrier that began kt), those of kt + 2 are requested, then
 // the k-steps run as in mainloop_dma.  The wait before the barrier leaves at most the direct loads of later k-tiles
-// outstanding, whatever the order in which the pieces' loads were issued among them.
+// outstanding, whatever the order in which the pieces' loads were issued among them.  One body serves all k-tiles (loads
+// behind the last one bring zeros): with bodies of their own for the last k-tiles, hipcc keeps the sums of the scaled MFMAs
+// (mainloop_mxmx) in two places and copies them at each k-tile, 100 to 400 spilled registers.
 template <class C, bool KM>
-MOE_DEV void mainloop_mx(f32x16 (&acc)[1][C::TN][C::TM], f32x16 (&xacc)[1][C::XTN], const OpDesc<bf16_t>& a,
-                         MxStager<C, C::BN, KM>& sb, int K, bf16_t* smem) {
+MOE_DEV void mainloop_mx(f32x16 (&acc)[1][C::TN][C::TM], const OpDesc<bf16_t>& a, MxStager<C, C::BN, KM>& sb, int K,
+                         bf16_t* smem) {
   using T = bf16_t;
-  constexpr int TILE_A = C::AR * C::BK, TILE_B = C::BN * C::BK, STAGE = TILE_A + TILE_B;
+  constexpr int TILE_A = C::BM * C::BK, TILE_B = C::BN * C::BK, STAGE = TILE_A + TILE_B;
   constexpr int NST = C::NST;
-  constexpr bool TALL = C::XR > 0;
-  static_assert(C::XR == 0 || C::XR == 64, "no 384-row tiles");
-  using SA = DmaStager<C, T, C::AR>;
+  static_assert(C::XR == 0, "no tall tiles");
+  using SA = DmaStager<C, T, C::BM>;
   using SBN = DmaStager<C, T, C::BN>;
   using SBT = DmaStagerT<C, T, C::BN>;
   constexpr int IPT = SA::PER;
@@ -171,23 +258,24 @@ MOE_DEV void mainloop_mx(f32x16 (&acc)[1][C::TN][C::TM], f32x16 (&xacc)[1][C::XT
   SA sa;
   sa.init(a, threadIdx.x);
   auto stage = [&](int kt) { return smem + (NST == 2 ? (kt & 1) : kt % NST) * STAGE; };
-  auto issue = [&](int kt) { sa.issue(stage(kt), kt * C::BK, 0); };
-  const int pro = min(NST - 1, nk);
-  for (int kt = 0; kt < pro; ++kt) issue(kt);
+  auto issue = [&](int kt) {
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) sa.issue_one(stage(kt), i, kt * C::BK, kt < nk);
+  };
+#pragma unroll
+  for (int kt = 0; kt < NST - 1; ++kt) issue(kt);
   sb.load(0);
   sb.write(stage(0) + TILE_A);
-  if (nk > 1) sb.load(C::BK);
-  constexpr int KSTEPS = C::BK / (2 * C::V);
+  sb.load(C::BK);
+  constexpr int KSTEPS = C::BK / (2 * C::V), LAST = KSTEPS - 1;
+  static_assert(KSTEPS == 4, "two sets of fragments");
   const int frag_row = lane & 31, frag_kv = lane >> 5;
-  u32x4 af[2][C::TM], bfr[2][C::TN], afx[2];
-  const int xrow = C::BM + 32 * (wm & 1) + frag_row;
-  const bool xhi = __builtin_amdgcn_readfirstlane(wm >> 1) != 0;
+  u32x4 af[2][C::TM], bfr[2][C::TN];
   auto read_frags = [&](const T* sA, int ks, int set) {
     const T* sB = sA + TILE_A;
     const int kv = ks * 2 + frag_kv;
 #pragma unroll
     for (int tm = 0; tm < C::TM; ++tm) af[set][tm] = SA::frag(sA, wm * C::WM + tm * 32 + frag_row, kv);
-    if constexpr (TALL) afx[set] = SA::frag(sA, xrow, kv);
 #pragma unroll
     for (int tn = 0; tn < C::TN; ++tn) {
       if constexpr (KM) bfr[set][tn] = SBT::frag(sB, wn * C::WN + tn * 32, ks * 2 * C::V);
@@ -196,93 +284,95 @@ MOE_DEV void mainloop_mx(f32x16 (&acc)[1][C::TN][C::TM], f32x16 (&xacc)[1][C::XT
   };
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   lds_barrier();
-  if (NST - 1 < nk) issue(NST - 1);
+  issue(NST - 1);
   read_frags(smem, 0, 0);
-  auto body = [&](int kt, auto phase_c) {
-    constexpr int phase = decltype(phase_c)::value;  // 0: refills a stage, 1: all issued, 2: the last
-    const T* sA = stage(kt);
-    if constexpr (phase < 2) {
-      sb.write(stage(kt + 1) + TILE_A);
-      if (kt + 2 < nk) sb.load((kt + 2) * C::BK);
-    }
+  int kt = 0;
+  do {
+    sb.write(stage(kt + 1) + TILE_A);
+    sb.load((kt + 2) * C::BK);
 #pragma unroll
     for (int ks = 0; ks < KSTEPS; ++ks) {
       const int cur = ks & 1;
-      if (ks + 1 < KSTEPS) {
-        read_frags(sA, ks + 1, cur ^ 1);
-      } else if constexpr (phase < 2) {
-        if constexpr (phase == 0) {
-          asm volatile("s_waitcnt vmcnt(%0)" :: "n"((NST - 2) * IPT) : "memory");
-        } else {
-          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        }
+      if (ks < LAST) {
+        read_frags(stage(kt), ks + 1, cur ^ 1);
+      } else {
+        asm volatile("s_waitcnt vmcnt(%0)" :: "n"((NST - 2) * IPT) : "memory");
         lds_barrier();
         read_frags(stage(kt + 1), 0, cur ^ 1);
-        if constexpr (phase == 0) issue(kt + NST);
       }
 #pragma unroll
       for (int tn = 0; tn < C::TN; ++tn)
 #pragma unroll
         for (int tm = 0; tm < C::TM; ++tm) mfma_frag(acc[0][tn][tm], bfr[cur][tn], af[cur][tm], T());
-      if constexpr (TALL) {
+      if (ks == LAST) {
+        issue(kt + NST);
+        // as in mainloop_dma: the fragments' reads, then a direct load after each MFMA while they last
+        constexpr int NM = C::TN * C::TM;
+        __builtin_amdgcn_sched_group_barrier(0x100, C::TM + C::TN * (KM ? 2 : 1), 0);
 #pragma unroll
-        for (int j = 0; j < C::XTN; ++j) {
-          const u32x4 bx = xhi ? bfr[cur][C::XTN + j] : bfr[cur][j];
-          mfma_frag(xacc[0][j], bx, afx[cur], T());
+        for (int i = 0; i < NM; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          if (i < IPT) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
         }
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-  };
-  int kt = 0;
-  for (; kt + NST < nk; ++kt) body(kt, std::integral_constant<int, 0>{});
-  for (; kt + 1 < nk; ++kt) body(kt, std::integral_constant<int, 1>{});
-  body(kt, std::integral_constant<int, 2>{});
+  } while (++kt < nk);
   __syncthreads();  // the caller's epilogue reuses the LDS
+}
+
+// Blocks from `tiles` on write the rows of no group.
+template <typename T>
+MOE_DEV bool mx_no_group(const MxRows& r, int tiles, const LinearEpi<T>& epi, int threads) {
+  if ((int)blockIdx.x < tiles) return false;
+  skinny_no_group(r.offsets, r.G, r.M, epi.N, (int64_t)blockIdx.x - tiles, (int64_t)gridDim.x - tiles, epi, threads);
+  return true;
 }
 
 // y tile by tile, bf16 rows.
 template <class C>
-__global__ __launch_bounds__(C::THREADS) void k_mx_fwd(const bf16_t* __restrict__ X, RowGroups groups, MxWeights w,
+__global__ __launch_bounds__(C::THREADS) void k_mx_fwd(const bf16_t* __restrict__ X, MxRows r, int tiles, MxWeights w,
                                                        LinearEpi<bf16_t> epi) {
-  __shared__ __align__(16) bf16_t smem[rowcol_smem_elems<bf16_t, C, 1, 1, 1>()];
+  __shared__ __align__(16) bf16_t smem[mx_smem_elems<C>()];
+  if (mx_no_group(r, tiles, epi, C::THREADS)) return;
   int grp, row0, mv, n0;
   const int N = w.N, K = w.K;
-  if (!resolve_rows(groups, N, C::AR, C::BN, grp, row0, mv, n0)) return;
+  if (!mx_tile<C::BM, C::BN>(r, N, (int)blockIdx.x, grp, row0, mv, n0)) return;
   const int64_t first = (int64_t)grp * N + n0;  // weight row
-  with_tile_shape<bf16_t, C>(mv, N - n0, [&](auto ct) {
+  with_mx_shape<C>(mv, N - n0, [&](auto ct) {
     using CT = decltype(ct);
     const OpDesc<bf16_t> a{X + (int64_t)row0 * K, K, mv, K};
     MxStager<CT, CT::BN, false> sb;
     sb.init(uni_ptr(w.codes + first * (K / 2)), uni_ptr(w.scales + first * (K / kMxBlock)), K, min(N - n0, CT::BN), K);
-    f32x16 acc[1][CT::TN][CT::TM], xacc[1][CT::XTN];
-    zero_acc<CT, 1>(acc, xacc);
-    mainloop_mx<CT, false>(acc, xacc, a, sb, K, smem);
+    f32x16 acc[1][CT::TN][CT::TM], none[1][CT::XTN];
+    zero_acc<CT, 1>(acc);
+    mainloop_mx<CT, false>(acc, a, sb, K, smem);
     static_assert(epi_lds_floats<CT, 1>() * 4 <= (int)sizeof(smem), "epilogue LDS");
-    linear_epilogue<CT>(acc, xacc, epi, epi.bias ? epi.bias + first : nullptr, row0, mv, n0,
+    linear_epilogue<CT>(acc, none, epi, epi.bias ? epi.bias + first : nullptr, row0, mv, n0,
                         reinterpret_cast<float*>(smem));
   });
 }
 
 // dx = dz W tile by tile: the contraction runs over the weight's rows.
 template <class C>
-__global__ __launch_bounds__(C::THREADS) void k_mx_dgrad(const bf16_t* __restrict__ dZ, RowGroups groups, MxWeights w,
+__global__ __launch_bounds__(C::THREADS) void k_mx_dgrad(const bf16_t* __restrict__ dZ, MxRows r, int tiles, MxWeights w,
                                                          bf16_t* __restrict__ dX) {
-  __shared__ __align__(16) bf16_t smem[rowcol_smem_elems<bf16_t, C, 1, 1, 1>()];
-  int grp, row0, mv, k0;
+  __shared__ __align__(16) bf16_t smem[mx_smem_elems<C>()];
   const int N = w.N, K = w.K;
-  if (!resolve_rows(groups, K, C::AR, C::BN, grp, row0, mv, k0)) return;
+  if (mx_no_group(r, tiles, LinearEpi<bf16_t>{nullptr, nullptr, dX, nullptr, kActNone, K}, C::THREADS)) return;
+  int grp, row0, mv, k0;
+  if (!mx_tile<C::BM, C::BN>(r, K, (int)blockIdx.x, grp, row0, mv, k0)) return;
   const int64_t first = (int64_t)grp * N;
-  with_tile_shape<bf16_t, C>(mv, K - k0, [&](auto ct) {
+  with_mx_shape<C>(mv, K - k0, [&](auto ct) {
     using CT = decltype(ct);
     const OpDesc<bf16_t> a{dZ + (int64_t)row0 * N, N, mv, N};
     MxStager<CT, CT::BN, true> sb;
     sb.init(uni_ptr(w.codes + first * (K / 2) + k0 / 2),
             uni_ptr(w.scales + first * (K / kMxBlock) + k0 / kMxBlock), K, N, min(K - k0, CT::BN));
-    f32x16 acc[1][CT::TN][CT::TM], xacc[1][CT::XTN];
-    zero_acc<CT, 1>(acc, xacc);
-    mainloop_mx<CT, true>(acc, xacc, a, sb, N, smem);
-    for_each_row8_x<CT, 1>(acc, xacc, reinterpret_cast<float*>(smem), [&](int m, int n, auto& v) {
+    f32x16 acc[1][CT::TN][CT::TM];
+    zero_acc<CT, 1>(acc);
+    mainloop_mx<CT, true>(acc, a, sb, N, smem);
+    for_each_row8<CT, 1>(acc, reinterpret_cast<float*>(smem), [&](int m, int n, auto& v) {
       if (m >= mv || k0 + n >= K) return;
       store8_stream(dX + ((int64_t)row0 + m) * K + k0 + n, v[0]);
     });
@@ -309,39 +399,46 @@ MOE_DEV void mfma_mx(f32x16& acc, u32x4 bt, u32x4 at, uint32_t sb, uint32_t sa, 
 
 // The scales of a tile's rows (AR of x, then BN of the weight), through registers: a thread loads the 16 of two
 // k-tiles at once from its rows (rows of K / 32 bytes have any alignment, and 8 bytes of a cache line a
-// k-tile would fetch each line many times) and writes 8 a k-tile to LDS.
+// k-tile would fetch each line many times) and writes 8 a k-tile to LDS.  A wave's 64 rows are all of one
+// operand's, so its base is scalar.
 template <class C>
 struct MxScaleStager {
   static constexpr int ROWS = C::AR + C::BN;
   static constexpr int PER = (ROWS + C::THREADS - 1) / C::THREADS;
-  const uint8_t* row[PER];  // null past the valid rows
-  int bytes;                // of a row
+  static_assert(C::AR % 64 == 0 && C::BN % 64 == 0, "a wave's rows are of one operand");
+  typedef const __attribute__((address_space(1))) uint8_t* bytes_t;
+  bytes_t base[PER];
+  int valid[PER];  // rows of the operand from the wave's first on
+  int bytes;       // of a row
   u32x4 s[PER];
   MOE_DEV void init(const uint8_t* xs, const uint8_t* ws, int mv, int nv, int K) {
     bytes = K / kMxBlock;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int r = threadIdx.x + i * C::THREADS;
-      row[i] = r < C::AR ? (r < mv ? xs + (int64_t)r * bytes : nullptr)
-                         : (r - C::AR < nv ? ws + (int64_t)(r - C::AR) * bytes : nullptr);
+      const int r = uni((threadIdx.x & ~63) + i * C::THREADS);
+      const bool a = r < C::AR;
+      base[i] = gptr(uni_ptr((a ? xs : ws) + (int64_t)(a ? r : r - C::AR) * bytes));
+      valid[i] = a ? mv - r : r < ROWS ? nv - (r - C::AR) : 0;
     }
   }
   // the 16 scales from byte `at` of each row on
   MOE_DEV void load(int at) {
-    const int left = bytes - at;
+    const int left = bytes - at, lane = threadIdx.x & 63;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       s[i] = u32x4{0, 0, 0, 0};
-      if (!row[i]) continue;
+      if (lane >= valid[i]) continue;
+      const uint32_t o = (uint32_t)(lane * bytes + at);
       if (left >= 16) {
         typedef u32x4 any_u32x4 __attribute__((aligned(1)));
-        s[i] = *(const __attribute__((address_space(1))) any_u32x4*)(row[i] + at);
+        s[i] = *(const __attribute__((address_space(1))) any_u32x4*)(base[i] + o);
       } else {
         for (int j = 0; j < left; ++j) {
-          const uint32_t b = gptr(row[i])[at + j];
-#pragma unroll
-          for (int d = 0; d < 4; ++d)
-            if (j >> 2 == d) s[i][d] |= b << (8 * (j & 3));
+          const uint32_t b = (uint32_t)base[i][o + j] << (8 * (j & 3));
+          if (j < 4) s[i].x |= b;
+          else if (j < 8) s[i].y |= b;
+          else if (j < 12) s[i].z |= b;
+          else s[i].w |= b;
         }
       }
     }
@@ -360,14 +457,13 @@ struct MxScaleStager {
 // As mainloop_dma, with scales.  OUT, the results' type, only sets the instantiations of two kernels apart: hipcc's host
 // pass takes the second use of one as an error.
 template <class C, typename OUT>
-MOE_DEV void mainloop_mxmx(f32x16 (&acc)[1][C::TN][C::TM], f32x16 (&xacc)[1][C::XTN], const OpDesc<bf16_t>& a,
-                           const OpDesc<bf16_t>& b, MxScaleStager<C>& ss, int K4, bf16_t* smem, u32x2* scales) {
+MOE_DEV void mainloop_mxmx(f32x16 (&acc)[1][C::TN][C::TM], const OpDesc<bf16_t>& a, const OpDesc<bf16_t>& b,
+                           MxScaleStager<C>& ss, int K4, bf16_t* smem, u32x2* scales) {
   using T = bf16_t;
-  constexpr int TILE_A = C::AR * C::BK, TILE_B = C::BN * C::BK, STAGE = TILE_A + TILE_B;
+  constexpr int TILE_A = C::BM * C::BK, TILE_B = C::BN * C::BK, STAGE = TILE_A + TILE_B;
   constexpr int NST = C::NST, ROWS = MxScaleStager<C>::ROWS;
-  constexpr bool TALL = C::XR > 0;
-  static_assert(C::XR == 0 || C::XR == 64, "no 384-row tiles");
-  using SA = DmaStager<C, T, C::AR>;
+  static_assert(C::XR == 0, "no tall tiles");
+  using SA = DmaStager<C, T, C::BM>;
   using SB = DmaStager<C, T, C::BN>;
   constexpr int IPT = SA::PER + SB::PER;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -380,132 +476,99 @@ MOE_DEV void mainloop_mxmx(f32x16 (&acc)[1][C::TN][C::TM], f32x16 (&xacc)[1][C::
   sb.init(b, threadIdx.x);
   auto stage = [&](int kt) { return smem + (NST == 2 ? (kt & 1) : kt % NST) * STAGE; };
   auto scales_of = [&](int kt) { return scales + (kt & 1) * ROWS; };
-  auto issue = [&](int kt) {
-    sa.issue(stage(kt), kt * C::BK, 0);
-    sb.issue(stage(kt) + TILE_A, kt * C::BK, 0);
+  auto issue = [&](int kt, int i) {
+    if (i < SA::PER) sa.issue_one(stage(kt), i, kt * C::BK, kt < nk);
+    else sb.issue_one(stage(kt) + TILE_A, i - SA::PER, kt * C::BK, kt < nk);
   };
-  const int pro = min(NST - 1, nk);
-  for (int kt = 0; kt < pro; ++kt) issue(kt);
+#pragma unroll
+  for (int kt = 0; kt < NST - 1; ++kt)
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) issue(kt, i);
   ss.load(0);
   ss.write(scales_of(0), false);
   constexpr int KSTEPS = C::BK / (2 * C::V);
   static_assert(KSTEPS == 4, "four scales to a dword");
   const int frag_row = lane & 31, half = lane >> 5;
-  u32x4 af[2][C::TM], bfr[2][C::TN], afx[2];
-  uint32_t as[2][C::TM], bs[2][C::TN], asx[2];  // of this k-tile and the next
-  const int xrow = C::BM + 32 * (wm & 1) + frag_row;
-  const bool xhi = __builtin_amdgcn_readfirstlane(wm >> 1) != 0;
-  auto read_scales = [&](int kt, int set) {
+  // one set of fragments of the weight: each is read again for the next k-step behind its last MFMA (two sets of both
+  // operands spill beside the scales)
+  u32x4 af[2][C::TM], bfr[C::TN];
+  uint32_t as[C::TM], bs[C::TN];
+  auto read_scales = [&](int kt) {
     const uint32_t* t = reinterpret_cast<const uint32_t*>(scales_of(kt)) + half;
 #pragma unroll
-    for (int tm = 0; tm < C::TM; ++tm) as[set][tm] = t[2 * (wm * C::WM + tm * 32 + frag_row)];
-    if constexpr (TALL) asx[set] = t[2 * xrow];
+    for (int tm = 0; tm < C::TM; ++tm) as[tm] = t[2 * (wm * C::WM + tm * 32 + frag_row)];
 #pragma unroll
-    for (int tn = 0; tn < C::TN; ++tn) bs[set][tn] = t[2 * (C::AR + wn * C::WN + tn * 32 + frag_row)];
+    for (int tn = 0; tn < C::TN; ++tn) bs[tn] = t[2 * (C::BM + wn * C::WN + tn * 32 + frag_row)];
   };
-  auto read_frags = [&](const T* sA, int ks, int set) {
-    const T* sB = sA + TILE_A;
-    const int kv = 4 * half + ks;
+  auto read_a = [&](const T* st, int ks, int set) {
 #pragma unroll
-    for (int tm = 0; tm < C::TM; ++tm) af[set][tm] = SA::frag(sA, wm * C::WM + tm * 32 + frag_row, kv);
-    if constexpr (TALL) afx[set] = SA::frag(sA, xrow, kv);
-#pragma unroll
-    for (int tn = 0; tn < C::TN; ++tn) bfr[set][tn] = SB::frag(sB, wn * C::WN + tn * 32 + frag_row, kv);
+    for (int tm = 0; tm < C::TM; ++tm) af[set][tm] = SA::frag(st, wm * C::WM + tm * 32 + frag_row, 4 * half + ks);
+  };
+  auto read_b = [&](const T* st, int ks, int tn) {
+    bfr[tn] = SB::frag(st + TILE_A, wn * C::WN + tn * 32 + frag_row, 4 * half + ks);
   };
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   lds_barrier();
-  if (NST - 1 < nk) issue(NST - 1);
-  read_frags(smem, 0, 0);
-  read_scales(0, 0);
-  // odd: which half of a load of scales, and register set, a k-tile has
-  auto body = [&](int kt, auto phase_c, auto odd_c) {
-    constexpr int phase = decltype(phase_c)::value;  // 0: refills a stage, 1: all issued, 2: the last
-    constexpr int odd = decltype(odd_c)::value;
-    const T* sA = stage(kt);
-    if constexpr (phase < 2) {
-      // the next k-tile's scales: the second half of a load, or the load that this k-tile's predecessor began
-      ss.write(scales_of(kt + 1), odd == 0);
-      if constexpr (odd == 0) {
-        if (kt + 2 < nk) ss.load((kt + 2) * 8);
-      }
-    }
+#pragma unroll
+  for (int i = 0; i < IPT; ++i) issue(NST - 1, i);
+  read_a(smem, 0, 0);
+#pragma unroll
+  for (int tn = 0; tn < C::TN; ++tn) read_b(smem, 0, tn);
+  read_scales(0);
+  int kt = 0;
+  do {
+    ss.write(scales_of(kt + 1), (kt & 1) == 0);
+    if ((kt & 1) == 0 && kt + 2 < nk) ss.load((kt + 2) * 8);
+    constexpr int M = KSTEPS - 1;
 #pragma unroll
     for (int ks = 0; ks < KSTEPS; ++ks) {
       const int cur = ks & 1;
-      if (ks + 1 < KSTEPS) {
-        read_frags(sA, ks + 1, cur ^ 1);
-      } else if constexpr (phase < 2) {
-        if constexpr (phase == 0) {
-          asm volatile("s_waitcnt vmcnt(%0)" :: "n"((NST - 2) * IPT) : "memory");
-        } else {
-          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        }
+      const T* next = ks < M ? stage(kt) : stage(kt + 1);
+      if (ks == M) {
+        asm volatile("s_waitcnt vmcnt(%0)" :: "n"((NST - 2) * IPT) : "memory");
         lds_barrier();
-        read_frags(stage(kt + 1), 0, cur ^ 1);
-        read_scales(kt + 1, odd ^ 1);
-        if constexpr (phase == 0) issue(kt + NST);
       }
+      read_a(next, (ks + 1) & M, cur ^ 1);
 #pragma unroll
-      for (int tn = 0; tn < C::TN; ++tn)
+      for (int tn = 0; tn < C::TN; ++tn) {
 #pragma unroll
-        for (int tm = 0; tm < C::TM; ++tm)
-          mfma_mx(acc[0][tn][tm], bfr[cur][tn], af[cur][tm], bs[odd][tn], as[odd][tm], ks);
-      if constexpr (TALL) {
+        for (int tm = 0; tm < C::TM; ++tm) mfma_mx(acc[0][tn][tm], bfr[tn], af[cur][tm], bs[tn], as[tm], ks);
+        read_b(next, (ks + 1) & M, tn);
+        // the refill of this k-tile's stage (its last reads are behind the barrier), shared out over the MFMAs
+        if (ks == M) {
 #pragma unroll
-        for (int j = 0; j < C::XTN; ++j) {
-          const u32x4 bx = xhi ? bfr[cur][C::XTN + j] : bfr[cur][j];
-          const uint32_t sx = xhi ? bs[odd][C::XTN + j] : bs[odd][j];
-          mfma_mx(xacc[0][j], bx, afx[cur], sx, asx[odd], ks);
+          for (int i = tn * IPT / C::TN; i < (tn + 1) * IPT / C::TN; ++i) issue(kt + NST, i);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);
     }
-  };
-  using Even = std::integral_constant<int, 0>;
-  using Odd = std::integral_constant<int, 1>;
-  auto run = [&](int kt, auto phase) {
-    if (kt & 1) body(kt, phase, Odd{});
-    else body(kt, phase, Even{});
-  };
-  int kt = 0;
-  for (; kt + NST + 1 < nk; kt += 2) {
-    body(kt, std::integral_constant<int, 0>{}, Even{});
-    body(kt + 1, std::integral_constant<int, 0>{}, Odd{});
-  }
-  if (kt + NST < nk) {
-    body(kt, std::integral_constant<int, 0>{}, Even{});
-    ++kt;
-  }
-  for (; kt + 1 < nk; ++kt) run(kt, std::integral_constant<int, 1>{});
-  run(kt, std::integral_constant<int, 2>{});
+    read_scales(kt + 1);
+  } while (++kt < nk);
   __syncthreads();
 }
 
-// Rows of scales in LDS: the most that a tile shape of C has, twice.
-template <class C>
-constexpr int mx_scale_rows() { return 2 * (C::BM + (has_half_rows<bf16_t, C>() ? C::BM / 4 : 0) + C::BN); }
-
 template <class C, typename T>
-__global__ __launch_bounds__(C::THREADS) void k_mxmx_fwd(const uint8_t* __restrict__ X, const uint8_t* __restrict__ XS,
-                                                         RowGroups groups, MxWeights w, LinearEpi<T> epi) {
-  __shared__ __align__(16) bf16_t smem[rowcol_smem_elems<bf16_t, C, 1, 1, 1>()];
-  __shared__ u32x2 scales[mx_scale_rows<C>()];
+__global__ __launch_bounds__(C::THREADS, 2) void k_mxmx_fwd(const uint8_t* __restrict__ X, const uint8_t* __restrict__ XS,
+                                                         MxRows r, int tiles, MxWeights w, LinearEpi<T> epi) {
+  __shared__ __align__(16) bf16_t smem[mx_smem_elems<C>()];
+  __shared__ u32x2 scales[2 * (C::BM + C::BN)];
+  if (mx_no_group(r, tiles, epi, C::THREADS)) return;
   int grp, row0, mv, n0;
   const int N = w.N, K = w.K, K4 = K / 4;
-  if (!resolve_rows(groups, N, C::AR, C::BN, grp, row0, mv, n0)) return;
+  if (!mx_tile<C::BM, C::BN>(r, N, (int)blockIdx.x, grp, row0, mv, n0)) return;
   const int64_t first = (int64_t)grp * N + n0;
-  with_tile_shape<bf16_t, C>(mv, N - n0, [&](auto ct) {
+  with_mx_shape<C>(mv, N - n0, [&](auto ct) {
     using CT = decltype(ct);
-    static_assert(2 * MxScaleStager<CT>::ROWS <= mx_scale_rows<C>(), "scales' LDS");
+    static_assert(CT::BM <= C::BM && CT::BN <= C::BN, "scales' LDS");
     const OpDesc<bf16_t> a{reinterpret_cast<const bf16_t*>(X + (int64_t)row0 * (K / 2)), K4, mv, K4};
     const OpDesc<bf16_t> b{reinterpret_cast<const bf16_t*>(w.codes + first * (K / 2)), K4, N - n0, K4};
     MxScaleStager<CT> ss;
     ss.init(XS + (int64_t)row0 * (K / kMxBlock), w.scales + first * (K / kMxBlock), mv, N - n0, K);
-    f32x16 acc[1][CT::TN][CT::TM], xacc[1][CT::XTN];
-    zero_acc<CT, 1>(acc, xacc);
-    mainloop_mxmx<CT, T>(acc, xacc, a, b, ss, K4, smem, scales);
+    f32x16 acc[1][CT::TN][CT::TM], none[1][CT::XTN];
+    zero_acc<CT, 1>(acc);
+    mainloop_mxmx<CT, T>(acc, a, b, ss, K4, smem, scales);
     static_assert(epi_lds_floats<CT, 1>() * 4 <= (int)sizeof(smem), "epilogue LDS");
-    linear_epilogue<CT>(acc, xacc, epi, epi.bias ? epi.bias + first : nullptr, row0, mv, n0,
+    linear_epilogue<CT>(acc, none, epi, epi.bias ? epi.bias + first : nullptr, row0, mv, n0,
                         reinterpret_cast<float*>(smem));
   });
 }

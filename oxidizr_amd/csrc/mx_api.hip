@@ -75,8 +75,10 @@ void with_mx_tiling(MxTiles kind, F&& f) {
   if (kind == MxTiles::kSmall) return f(MxSmall{});
   f(MxBig{});
 }
+// Blocks of tiles, and behind them (grouped) those for the rows of no group.
+constexpr int kMxNoGroupBlocks = 64;
 template <class C>
-int64_t mx_grid(bool grouped, int E, int64_t M, int N) {
+int64_t mx_tile_blocks(bool grouped, int E, int64_t M, int N) {
   if (!grouped) return (int64_t)ceil_div(M, C::BM) * ceil_div(N, C::BN);
   return ((int64_t)(ceil_div(M, C::BM) + E) * ceil_div(N, C::BN) + 7) / 8 * 8;
 }
@@ -84,7 +86,7 @@ moe_status check_mx_tiles(MxTiles kind, bool grouped, int E, int64_t M, int N) {
   moe_status st = MOE_OK;
   with_mx_tiling(kind, [&](auto c) {
     using C = decltype(c);
-    st = check_grid(mx_grid<C>(grouped, E, M, N), C::THREADS);
+    st = check_grid(mx_tile_blocks<C>(grouped, E, M, N) + kMxNoGroupBlocks, C::THREADS);
   });
   return st;
 }
@@ -92,54 +94,39 @@ moe_status check_mx_launches(bool backward, bool grouped, int E, int64_t M, int 
   if (backward) return check_mx_tiles(mx_tiles(grouped, E, M, K), grouped, E, M, K);
   return mx_skinny(M, K, N, E, grouped) ? MOE_OK : check_mx_tiles(mx_tiles(grouped, E, M, N), grouped, E, M, N);
 }
-// Calls f(tiling, row groups, grid).
+// Calls f(tiling, blocks of tiles, grid).
 template <class F>
-void with_mx_rows(MxTiles kind, const int* offsets, const int* prefixes, int E, int64_t M, int N, F&& f) {
+void with_mx_launch(MxTiles kind, const MxRows& r, int N, F&& f) {
   with_mx_tiling(kind, [&](auto c) {
-    using C = decltype(c);
-    const bool grouped = offsets != nullptr;
-    const int grid = (int)mx_grid<C>(grouped, E, M, N);
-    if (!grouped) return f(c, RowGroups{nullptr, nullptr, nullptr, nullptr, 1, (int)M, 0, 0}, grid);
-    const int* tp = prefixes + prefix_slot(C::BM) * (E + 1);
-    constexpr bool big = std::is_same<C, MxBig>::value;
-    f(c, RowGroups{offsets, tp, tp + (E + 1), tp + 2 * (E + 1), E, (int)M, big && M >= 2 * (int64_t)C::BM * E,
-                   big ? tall_rows_for(C::BM) : 0}, grid);
+    const bool grouped = r.offsets != nullptr;
+    const int tiles = (int)mx_tile_blocks<decltype(c)>(grouped, r.G, r.M, N);
+    f(c, tiles, dim3(tiles + (grouped ? kMxNoGroupBlocks : 0)));
   });
 }
 
+// Scratch of a backward with an activation or a bias gradient: k_linear_dz's chunks.
 struct MxWs {
   size_t offs, prefixes, w_tab, dz, part, total;
 };
 int64_t mx_dz_chunks(int64_t M, int E, bool grouped) { return (M + kDzRows - 1) / kDzRows + (grouped ? E : 0); }
 MxWs mx_ws(int64_t M, int N, int E, bool grouped, int act, bool backward) {
   MxWs w{};
+  if (!backward) return w;
   Carve c;
   if (grouped) {
     w.offs = c.take((size_t)(E + 1) * 4);
     w.prefixes = c.take((size_t)kNumTilePrefixes * (E + 1) * 4);
     w.w_tab = c.take((size_t)E * sizeof(void*));
   }
-  if (backward) {
-    if (act != kActNone) w.dz = c.take((size_t)M * N * 2);
-    w.part = c.take((size_t)mx_dz_chunks(M, E, grouped) * N * 4);
-  }
+  if (act != kActNone) w.dz = c.take((size_t)M * N * 2);
+  w.part = c.take((size_t)mx_dz_chunks(M, E, grouped) * N * 4);
   w.total = c.off;
   return w;
 }
 
-constexpr int kMxPrepBlocks = 1 + 128;
-// Clean offsets, tile prefixes, and what belongs to no expert.
-template <typename T>
-void mx_prep(hipStream_t s, const int* offsets, int E, int64_t M, char* ws, const MxWs& L, const T* res, T* out,
-             T* out2, int cols) {
-  hipLaunchKernelGGL(k_linear_prep<T>, dim3(kMxPrepBlocks), dim3(1024), 0, s, offsets, E, (int)M,
-                     (int*)(ws + L.offs), (int*)(ws + L.prefixes), (const T*)nullptr, (T*)nullptr, (int64_t)0,
-                     (const T**)(ws + L.w_tab), (T**)nullptr, res, out, out2, cols);
-}
-
 template <bool X4, typename T>
 moe_status mx_forward(hipStream_t s, int64_t M, int E, const int* offsets, const void* x, const uint8_t* xs,
-                      const MxWeights& w, const LinearEpi<T>& epi, char* ws) {
+                      const MxWeights& w, const LinearEpi<T>& epi) {
   const bool grouped = offsets != nullptr;
   const int N = w.N, K = w.K;
   if (mx_skinny(M, K, N, E, grouped)) {
@@ -158,15 +145,13 @@ moe_status mx_forward(hipStream_t s, int64_t M, int E, const int* offsets, const
     LAUNCH_CHECK();
     return MOE_OK;
   }
-  const MxWs L = mx_ws(M, N, E, grouped, epi.act, false);
-  if (grouped) mx_prep<T>(s, offsets, E, M, ws, L, epi.res, epi.y, epi.pre, N);
-  with_mx_rows(mx_tiles(grouped, E, M, N), grouped ? (const int*)(ws + L.offs) : nullptr,
-               (const int*)(ws + L.prefixes), E, M, N, [&](auto c, const RowGroups& r, int grid) {
+  const MxRows r{offsets, E, (int)M};
+  with_mx_launch(mx_tiles(grouped, E, M, N), r, N, [&](auto c, int tiles, dim3 grid) {
     using C = decltype(c);
     if constexpr (X4)
-      hipLaunchKernelGGL((k_mxmx_fwd<C, T>), dim3(grid), dim3(C::THREADS), 0, s, (const uint8_t*)x, xs, r, w, epi);
+      hipLaunchKernelGGL((k_mxmx_fwd<C, T>), grid, dim3(C::THREADS), 0, s, (const uint8_t*)x, xs, r, tiles, w, epi);
     else
-      hipLaunchKernelGGL((k_mx_fwd<C>), dim3(grid), dim3(C::THREADS), 0, s, (const bf16_t*)x, r, w, epi);
+      hipLaunchKernelGGL((k_mx_fwd<C>), grid, dim3(C::THREADS), 0, s, (const bf16_t*)x, r, tiles, w, epi);
   });
   LAUNCH_CHECK();
   return MOE_OK;
@@ -177,13 +162,17 @@ moe_status mx_backward(hipStream_t s, int64_t M, int E, const int* offsets, cons
   const bool grouped = offsets != nullptr;
   const int N = w.N, K = w.K;
   const MxWs L = mx_ws(M, N, E, grouped, act, true);
-  const int* offs = grouped ? (const int*)(ws + L.offs) : nullptr;
-  const int* prefixes = (const int*)(ws + L.prefixes);
-  if (grouped) mx_prep<bf16_t>(s, offsets, E, M, ws, L, nullptr, dx, nullptr, K);
-  const RowGroups chunks{offs, prefixes, nullptr, nullptr, E, (int)M, 0, 0};
-  static_assert(prefix_slot(kDzRows) == 0, "the chunks' prefix is the first");
+  const MxRows r{offsets, E, (int)M};
   const bf16_t* dz = dy;
   if (act != kActNone || db) {
+    int* offs = grouped ? (int*)(ws + L.offs) : nullptr;
+    int* prefixes = grouped ? (int*)(ws + L.prefixes) : nullptr;
+    if (grouped)  // the prefix of 64-row chunks; nothing to fill
+      hipLaunchKernelGGL(k_linear_prep<bf16_t>, dim3(1), dim3(1024), 0, s, offsets, E, (int)M, offs, prefixes,
+                         (const bf16_t*)nullptr, (bf16_t*)nullptr, (int64_t)0, (const bf16_t**)(ws + L.w_tab),
+                         (bf16_t**)nullptr, (const bf16_t*)nullptr, (bf16_t*)nullptr, (bf16_t*)nullptr, N);
+    const RowGroups chunks{offs, prefixes, nullptr, nullptr, E, (int)M, 0, 0};
+    static_assert(prefix_slot(kDzRows) == 0, "the chunks' prefix is the first");
     bf16_t* out = (bf16_t*)(ws + L.dz);
     float* part = db ? (float*)(ws + L.part) : nullptr;
     hipLaunchKernelGGL(k_linear_dz<bf16_t>, dim3((unsigned)mx_dz_chunks(M, E, grouped), ceil_div(N, kDzCols)),
@@ -193,9 +182,9 @@ moe_status mx_backward(hipStream_t s, int64_t M, int E, const int* offsets, cons
       hipLaunchKernelGGL(k_linear_db<bf16_t>, dim3(ceil_div(N, 64), E), dim3(256), 0, s, part, chunks, N, db);
   }
   if (dx)
-    with_mx_rows(mx_tiles(grouped, E, M, K), offs, prefixes, E, M, K, [&](auto c, const RowGroups& r, int grid) {
+    with_mx_launch(mx_tiles(grouped, E, M, K), r, K, [&](auto c, int tiles, dim3 grid) {
       using C = decltype(c);
-      hipLaunchKernelGGL((k_mx_dgrad<C>), dim3(grid), dim3(C::THREADS), 0, s, dz, r, w, dx);
+      hipLaunchKernelGGL((k_mx_dgrad<C>), grid, dim3(C::THREADS), 0, s, dz, r, tiles, w, dx);
     });
   LAUNCH_CHECK();
   return MOE_OK;
@@ -259,7 +248,7 @@ moe_status moe_mx_linear_forward(int32_t device, void* stream, int32_t x_format,
   if ((st = check_ints({w_scales}, 1)) != MOE_OK) return st;
   const bool four = x_format == MOE_MX_ROWS_FOUR_BIT;
   if (four && (st = check_ints({x_scales}, 1)) != MOE_OK) return st;
-  if (offsets && ((st = check_ints({offsets})) != MOE_OK || (st = check_pointers({workspace})) != MOE_OK)) return st;
+  if (offsets && (st = check_ints({offsets})) != MOE_OK) return st;
   DeviceScope dev(device);
   HIP_TRY(dev.enter());
   hipStream_t s = (hipStream_t)stream;
@@ -268,7 +257,7 @@ moe_status moe_mx_linear_forward(int32_t device, void* stream, int32_t x_format,
     using D = decltype(d);
     return mx_forward<decltype(x4)::value, D>(s, M, E, offsets, x, x_scales, w,
                                               LinearEpi<D>{(const D*)bias, (const D*)residual, (D*)y, (D*)pre_act,
-                                                           activation, N}, (char*)workspace);
+                                                           activation, N});
   };
   if (!four) return go(std::false_type(), bf16_t());
   return dtype == MOE_DTYPE_BF16 ? go(std::true_type(), bf16_t()) : go(std::true_type(), float());
