@@ -373,15 +373,15 @@ __global__ __launch_bounds__(C::THREADS) void k_linear_bwd(const T* __restrict__
 // experts of 4096 x 1536 bf16, 512 rows (1.61 GB) 231-240 us, 6.7-7.0 TB/s.
 constexpr int kLinearSkinnyRows = 64;  // rows of an expert that one workgroup takes
 constexpr int kSkinnyChunkBytes = 512;  // of a weight row, in one k-chunk
-// Slot s of a launch: the s-th (expert, 64 rows of it) pair with rows, experts
+// Slot s of a launch: the s-th (expert, R rows of it) pair with rows, experts
 // ascending.  Every wave finds its own from the offsets: lane l counts the chunks of
 // experts l E/64 .., a prefix sum over the lanes finds the lane that holds slot s.
 // False for a slot past the last.
+template <int R = kLinearSkinnyRows>
 MOE_DEV bool skinny_slot(const int* __restrict__ offsets, int E, int M, int s, int& grp, int& r0,
                          int& rows) {
   const int lane = threadIdx.x & 63;
   const int per = (E + 63) >> 6, e0 = lane * per;
-  constexpr int R = kLinearSkinnyRows;
   int n = 0;
   for (int i = 0; i < per; ++i) {
     const int e = e0 + i;

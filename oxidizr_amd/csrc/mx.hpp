@@ -384,7 +384,7 @@ __global__ __launch_bounds__(C::THREADS) void k_mx_dgrad(const bf16_t* __restric
 // loads, swizzles and fragments of gemm.hpp serve as they are, over rows of K / 4 two-byte units.
 // v_mfma_scale_f32_32x32x64_f8f6f4 takes such a vector of each operand and a scale for each.  Half h of a
 // wave reads vector 4 h + ks in k-step ks of a k-tile instead of 2 ks + h: its four scales of a row are then one dword,
-// of which step ks takes byte ks.
+// of which step ks takes byte ks (2 h + ks and two of them where k-tiles are half as deep).
 MOE_DEV void mfma_mx(f32x16& acc, u32x4 bt, u32x4 at, uint32_t sb, uint32_t sa, int ks) {
   typedef int i32x8 __attribute__((ext_vector_type(8)));
   const i32x8 b = {(int)bt.x, (int)bt.y, (int)bt.z, (int)bt.w, 0, 0, 0, 0};
@@ -397,59 +397,76 @@ MOE_DEV void mfma_mx(f32x16& acc, u32x4 bt, u32x4 at, uint32_t sb, uint32_t sa, 
   }
 }
 
-// The scales of a tile's rows (AR of x, then BN of the weight), through registers: a thread loads the 16 of two
-// k-tiles at once from its rows (rows of K / 32 bytes have any alignment, and 8 bytes of a cache line a
-// k-tile would fetch each line many times) and writes 8 a k-tile to LDS.  A wave's 64 rows are all of one
-// operand's, so its base is scalar.
+// The scales of a tile's rows (BM of x, then BN of the weight), through registers: a thread loads 16 of each of its
+// rows at once, those of LT k-tiles (rows of K / 32 bytes have any alignment, and a k-tile's few bytes of a cache line
+// would fetch each line many times), and writes a k-tile's, W dwords, to LDS.  No branch is between a load and its
+// use, or it would be waited for at once: a load that would leave the tensor (its last 15 bytes) is moved back into it and
+// shifted, and what is not the row's is masked.  A wave's 64 rows are all of one operand's, so its base is scalar.
+// Both tensors hold 16 bytes at least.
 template <class C>
 struct MxScaleStager {
-  static constexpr int ROWS = C::AR + C::BN;
+  static constexpr int ROWS = C::BM + C::BN;
   static constexpr int PER = (ROWS + C::THREADS - 1) / C::THREADS;
-  static_assert(C::AR % 64 == 0 && C::BN % 64 == 0, "a wave's rows are of one operand");
-  typedef const __attribute__((address_space(1))) uint8_t* bytes_t;
-  bytes_t base[PER];
-  int valid[PER];  // rows of the operand from the wave's first on
-  int bytes;       // of a row
+  static constexpr int W = C::BK / C::V / 4, LT = 4 / W;
+  static_assert(C::BM % 64 == 0 && C::BN % 64 == 0, "a wave's rows are of one operand");
+  static_assert(W == 1 || W == 2, "four or eight vectors to a k-tile's row");
+  const __attribute__((address_space(1))) uint8_t* base[PER];
+  uint32_t last[PER];   // the last 16 bytes of the tensor, from base
+  uint32_t row[PER];    // the thread's row, from base
+  int bytes, valid;     // of a row; bit i: row i exists
   u32x4 s[PER];
-  MOE_DEV void init(const uint8_t* xs, const uint8_t* ws, int mv, int nv, int K) {
+  int at;               // where s begins in a row
+  // xs, ws: the tensors; the tile's rows from x0 (mv of them) and w0 (nv)
+  MOE_DEV void init(const uint8_t* xs, const uint8_t* ws, int64_t x0, int64_t w0, int64_t xrows, int64_t wrows, int mv, int nv,
+                    int K) {
     bytes = K / kMxBlock;
+    valid = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int r = uni((threadIdx.x & ~63) + i * C::THREADS);
-      const bool a = r < C::AR;
-      base[i] = gptr(uni_ptr((a ? xs : ws) + (int64_t)(a ? r : r - C::AR) * bytes));
-      valid[i] = a ? mv - r : r < ROWS ? nv - (r - C::AR) : 0;
+      const int r = uni((threadIdx.x & ~63) + i * C::THREADS), lane = threadIdx.x & 63;
+      const bool a = r < C::BM;
+      // a wave past the tile's rows stays at its first
+      const int64_t first = a ? (r < mv ? x0 + r : x0) : (r - C::BM < nv ? w0 + r - C::BM : w0);
+      const int left = a ? mv - r : nv - (r - C::BM);
+      base[i] = gptr(uni_ptr((a ? xs : ws) + first * bytes));
+      last[i] = (uint32_t)min(((a ? xrows : wrows) - first) * bytes - 16, (int64_t)INT_MAX);
+      if (r < ROWS && lane < left) valid |= 1 << i;
+      row[i] = (uint32_t)(lane * bytes);
     }
   }
-  // the 16 scales from byte `at` of each row on
-  MOE_DEV void load(int at) {
-    const int left = bytes - at, lane = threadIdx.x & 63;
+  MOE_DEV void load(int from) {
+    at = from;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      s[i] = u32x4{0, 0, 0, 0};
-      if (lane >= valid[i]) continue;
-      const uint32_t o = (uint32_t)(lane * bytes + at);
-      if (left >= 16) {
-        typedef u32x4 any_u32x4 __attribute__((aligned(1)));
-        s[i] = *(const __attribute__((address_space(1))) any_u32x4*)(base[i] + o);
-      } else {
-        for (int j = 0; j < left; ++j) {
-          const uint32_t b = (uint32_t)base[i][o + j] << (8 * (j & 3));
-          if (j < 4) s[i].x |= b;
-          else if (j < 8) s[i].y |= b;
-          else if (j < 12) s[i].z |= b;
-          else s[i].w |= b;
-        }
-      }
+      typedef u32x4 any_u32x4 __attribute__((aligned(1)));
+      s[i] = *(const __attribute__((address_space(1))) any_u32x4*)(base[i] + (int64_t)min((int)(row[i] + at), (int)last[i]));
     }
   }
-  // 8 bytes a row: the first or (hi) second k-tile of a load
-  MOE_DEV void write(u32x2* tile, bool hi) const {
+  // the scales of k-tile kt, the (kt % LT)-th of the load
+  MOE_DEV void write(uint32_t* tile, int kt) const {
+    const int j = kt % LT, left = bytes - at;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int r = threadIdx.x + i * C::THREADS;
       if (ROWS % C::THREADS != 0 && r >= ROWS) break;
-      tile[r] = hi ? u32x2{s[i].z, s[i].w} : u32x2{s[i].x, s[i].y};
+      const int d = max((int)(row[i] + at) - (int)last[i], 0);  // bytes moved back
+      u32x4 v = s[i];
+      if (__builtin_expect(__any(d > 0), 0)) {
+        if (d & 8) v = u32x4{v.z, v.w, 0, 0};
+        if (d & 4) v = u32x4{v.y, v.z, v.w, 0};
+        const int b = 8 * (d & 3);
+        v = u32x4{(uint32_t)((((uint64_t)v.y << 32) | v.x) >> b), (uint32_t)((((uint64_t)v.z << 32) | v.y) >> b),
+                  (uint32_t)((((uint64_t)v.w << 32) | v.z) >> b), v.w >> b};
+        if (d >= 16) v = u32x4{0, 0, 0, 0};
+      }
+      const bool in = valid >> i & 1;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        uint32_t q = W == 2 ? (j ? (w ? v.w : v.z) : (w ? v.y : v.x)) : j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w;
+        const int n = left - 4 * (j * W + w);  // bytes of the row from here
+        q &= n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1;
+        tile[r * W + w] = in ? q : 0u;
+      }
     }
   }
 };
@@ -458,10 +475,10 @@ struct MxScaleStager {
 // pass takes the second use of one as an error.
 template <class C, typename OUT>
 MOE_DEV void mainloop_mxmx(f32x16 (&acc)[1][C::TN][C::TM], const OpDesc<bf16_t>& a, const OpDesc<bf16_t>& b,
-                           MxScaleStager<C>& ss, int K4, bf16_t* smem, u32x2* scales) {
+                           MxScaleStager<C>& ss, int K4, bf16_t* smem, uint32_t* scales) {
   using T = bf16_t;
   constexpr int TILE_A = C::BM * C::BK, TILE_B = C::BN * C::BK, STAGE = TILE_A + TILE_B;
-  constexpr int NST = C::NST, ROWS = MxScaleStager<C>::ROWS;
+  constexpr int NST = C::NST, W = MxScaleStager<C>::W, LT = MxScaleStager<C>::LT, ROWS = MxScaleStager<C>::ROWS;
   static_assert(C::XR == 0, "no tall tiles");
   using SA = DmaStager<C, T, C::BM>;
   using SB = DmaStager<C, T, C::BN>;
@@ -475,7 +492,7 @@ MOE_DEV void mainloop_mxmx(f32x16 (&acc)[1][C::TN][C::TM], const OpDesc<bf16_t>&
   sa.init(a, threadIdx.x);
   sb.init(b, threadIdx.x);
   auto stage = [&](int kt) { return smem + (NST == 2 ? (kt & 1) : kt % NST) * STAGE; };
-  auto scales_of = [&](int kt) { return scales + (kt & 1) * ROWS; };
+  auto scales_of = [&](int kt) { return scales + (kt & 1) * ROWS * W; };
   auto issue = [&](int kt, int i) {
     if (i < SA::PER) sa.issue_one(stage(kt), i, kt * C::BK, kt < nk);
     else sb.issue_one(stage(kt) + TILE_A, i - SA::PER, kt * C::BK, kt < nk);
@@ -485,16 +502,17 @@ MOE_DEV void mainloop_mxmx(f32x16 (&acc)[1][C::TN][C::TM], const OpDesc<bf16_t>&
 #pragma unroll
     for (int i = 0; i < IPT; ++i) issue(kt, i);
   ss.load(0);
-  ss.write(scales_of(0), false);
-  constexpr int KSTEPS = C::BK / (2 * C::V);
-  static_assert(KSTEPS == 4, "four scales to a dword");
+  ss.write(scales_of(0), 0);
+  constexpr int KSTEPS = C::BK / (2 * C::V), M = KSTEPS - 1;
+  static_assert(KSTEPS == 2 * W, "a lane's scales: two or four neighbours");
   const int frag_row = lane & 31, half = lane >> 5;
   // one set of fragments of the weight: each is read again for the next k-step behind its last MFMA (two sets of both
   // operands spill beside the scales)
   u32x4 af[2][C::TM], bfr[C::TN];
   uint32_t as[C::TM], bs[C::TN];
   auto read_scales = [&](int kt) {
-    const uint32_t* t = reinterpret_cast<const uint32_t*>(scales_of(kt)) + half;
+    typedef typename std::conditional<W == 2, uint32_t, uint16_t>::type S;
+    const S* t = reinterpret_cast<const S*>(scales_of(kt)) + half;
 #pragma unroll
     for (int tm = 0; tm < C::TM; ++tm) as[tm] = t[2 * (wm * C::WM + tm * 32 + frag_row)];
 #pragma unroll
@@ -502,10 +520,10 @@ MOE_DEV void mainloop_mxmx(f32x16 (&acc)[1][C::TN][C::TM], const OpDesc<bf16_t>&
   };
   auto read_a = [&](const T* st, int ks, int set) {
 #pragma unroll
-    for (int tm = 0; tm < C::TM; ++tm) af[set][tm] = SA::frag(st, wm * C::WM + tm * 32 + frag_row, 4 * half + ks);
+    for (int tm = 0; tm < C::TM; ++tm) af[set][tm] = SA::frag(st, wm * C::WM + tm * 32 + frag_row, KSTEPS * half + ks);
   };
   auto read_b = [&](const T* st, int ks, int tn) {
-    bfr[tn] = SB::frag(st + TILE_A, wn * C::WN + tn * 32 + frag_row, 4 * half + ks);
+    bfr[tn] = SB::frag(st + TILE_A, wn * C::WN + tn * 32 + frag_row, KSTEPS * half + ks);
   };
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   lds_barrier();
@@ -517,30 +535,45 @@ MOE_DEV void mainloop_mxmx(f32x16 (&acc)[1][C::TN][C::TM], const OpDesc<bf16_t>&
   read_scales(0);
   int kt = 0;
   do {
-    ss.write(scales_of(kt + 1), (kt & 1) == 0);
-    if ((kt & 1) == 0 && kt + 2 < nk) ss.load((kt + 2) * 8);
-    constexpr int M = KSTEPS - 1;
+    // the next k-tile's scales, of a load that ended before this k-tile or began with the one before it
+    ss.write(scales_of(kt + 1), kt + 1);
+    if ((kt + 2) % LT == 0) ss.load((kt + 2) * (C::BK / C::V));
+    auto products = [&](int ks, int tn) {
 #pragma unroll
-    for (int ks = 0; ks < KSTEPS; ++ks) {
-      const int cur = ks & 1;
-      const T* next = ks < M ? stage(kt) : stage(kt + 1);
-      if (ks == M) {
-        asm volatile("s_waitcnt vmcnt(%0)" :: "n"((NST - 2) * IPT) : "memory");
-        lds_barrier();
-      }
-      read_a(next, (ks + 1) & M, cur ^ 1);
+      for (int tm = 0; tm < C::TM; ++tm) mfma_mx(acc[0][tn][tm], bfr[tn], af[ks & 1][tm], bs[tn], as[tm], ks);
+    };
+#pragma unroll
+    for (int ks = 0; ks < M; ++ks) {
+      read_a(stage(kt), ks + 1, (ks + 1) & 1);
 #pragma unroll
       for (int tn = 0; tn < C::TN; ++tn) {
-#pragma unroll
-        for (int tm = 0; tm < C::TM; ++tm) mfma_mx(acc[0][tn][tm], bfr[tn], af[cur][tm], bs[tn], as[tm], ks);
-        read_b(next, (ks + 1) & M, tn);
-        // the refill of this k-tile's stage (its last reads are behind the barrier), shared out over the MFMAs
-        if (ks == M) {
-#pragma unroll
-          for (int i = tn * IPT / C::TN; i < (tn + 1) * IPT / C::TN; ++i) issue(kt + NST, i);
-        }
+        products(ks, tn);
+        read_b(stage(kt), ks + 1, tn);
         __builtin_amdgcn_sched_barrier(0);
       }
+    }
+    // Last k-step, whose fragments are read.  Behind a first barrier no wave reads this k-tile's stage again, and
+    // its refill is issued over the first half of the step's products; behind a second one the next k-tile has landed,
+    // whose refill was issued a k-tile ago: two k-tiles' loads are in flight meanwhile.
+    constexpr int H = (C::TN + 1) / 2;
+    lds_barrier();
+#pragma unroll
+    for (int tn = 0; tn < H; ++tn) {
+      products(M, tn);
+#pragma unroll
+      for (int i = tn * IPT / H; i < (tn + 1) * IPT / H; ++i) issue(kt + NST, i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    asm volatile("s_waitcnt vmcnt(%0)" :: "n"((NST - 1) * IPT) : "memory");
+    lds_barrier();
+    read_a(stage(kt + 1), 0, 0);
+#pragma unroll
+    for (int tn = 0; tn < H; ++tn) read_b(stage(kt + 1), 0, tn);
+#pragma unroll
+    for (int tn = H; tn < C::TN; ++tn) {
+      products(M, tn);
+      read_b(stage(kt + 1), 0, tn);
+      __builtin_amdgcn_sched_barrier(0);
     }
     read_scales(kt + 1);
   } while (++kt < nk);
@@ -551,7 +584,7 @@ template <class C, typename T>
 __global__ __launch_bounds__(C::THREADS, 2) void k_mxmx_fwd(const uint8_t* __restrict__ X, const uint8_t* __restrict__ XS,
                                                          MxRows r, int tiles, MxWeights w, LinearEpi<T> epi) {
   __shared__ __align__(16) bf16_t smem[mx_smem_elems<C>()];
-  __shared__ u32x2 scales[2 * (C::BM + C::BN)];
+  __shared__ uint32_t scales[2 * (C::BM + C::BN) * MxScaleStager<C>::W];
   if (mx_no_group(r, tiles, epi, C::THREADS)) return;
   int grp, row0, mv, n0;
   const int N = w.N, K = w.K, K4 = K / 4;
@@ -563,7 +596,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void k_mxmx_fwd(const uint8_t* __res
     const OpDesc<bf16_t> a{reinterpret_cast<const bf16_t*>(X + (int64_t)row0 * (K / 2)), K4, mv, K4};
     const OpDesc<bf16_t> b{reinterpret_cast<const bf16_t*>(w.codes + first * (K / 2)), K4, N - n0, K4};
     MxScaleStager<CT> ss;
-    ss.init(XS + (int64_t)row0 * (K / kMxBlock), w.scales + first * (K / kMxBlock), mv, N - n0, K);
+    ss.init(XS, w.scales, row0, first, r.M, (int64_t)r.G * N, mv, N - n0, K);
     f32x16 acc[1][CT::TN][CT::TM], none[1][CT::XTN];
     zero_acc<CT, 1>(acc);
     mainloop_mxmx<CT, T>(acc, a, b, ss, K4, smem, scales);
@@ -575,98 +608,146 @@ __global__ __launch_bounds__(C::THREADS, 2) void k_mxmx_fwd(const uint8_t* __res
 
 // ------------------------------------------------------------------ few rows
 // As in k_linear_skinny a launch with few rows to an expert is the stream of the weights that it touches: a wave
-// multiplies 16 weight rows with the rows of the expert (up to four chunks of 16) straight from memory,
-// KS waves of a workgroup share 16 weight rows and take every KS-th k-chunk of kMxChunk elements.  Lane l supplies block
-// l / 16 + 4 q of weight row l % 16 in load q, so four lanes read 64 contiguous bytes.
+// multiplies RW blocks of 16 weight rows with 16 rows of the expert straight from memory (an expert's further rows are
+// other workgroups', which find the weight in the caches; 64 rows to a workgroup took 40 to 90 registers more and 10 to 60 % longer),
+// KS waves of a workgroup share the weight rows and take every KS-th k-chunk of 512 elements (1024: as many registers
+// too many, 20 to 100 % longer).  Lane l supplies block l / 16 + 4 q of weight row l % 16 in load q, so four lanes read
+// 64 contiguous bytes; it loads the 16 scales of its row at once, of which its blocks' are the bytes l / 16 of each dword (a
+// load for each: 10 % longer).
 // bf16 rows: the block becomes four 8-element vectors, multiplied with the four of the token row by 16 x 16 x 32 MFMAs.
 // 4-bit rows: one 16 x 16 x 128 scaled MFMA.
-constexpr int kMxChunk = 512;
-template <bool X4, typename T, int NC, int KS>
+
+constexpr int kMxSkinnyRows = 16;
+constexpr int kMxChunkLoads = 4;  // of 128 elements
+// The 16 scales of a chunk from p on; FULL: all in the row (any alignment), else the first `left` blocks' are.
+template <bool FULL>
+MOE_DEV void mx_row_scales(const uint8_t* p, int left, int g, uint32_t (&s)[kMxChunkLoads]) {
+  if constexpr (FULL) {
+    typedef u32x4 any_u32x4 __attribute__((aligned(1)));
+    const u32x4 v = *(const __attribute__((address_space(1))) any_u32x4*)p;
+#pragma unroll
+    for (int q = 0; q < kMxChunkLoads; ++q) s[q] = v[q] >> (8 * g);
+  } else {
+#pragma unroll
+    for (int q = 0; q < kMxChunkLoads; ++q) s[q] = 4 * q + g < left ? gptr(p)[4 * q + g] : 0u;
+  }
+}
+
+template <bool X4, typename T, int KS, int RW>
 __global__ __launch_bounds__(256) void k_mx_skinny(const void* __restrict__ X, const uint8_t* __restrict__ XS,
                                                    const int* __restrict__ offsets, int E, int M, int nslot,
                                                    MxWeights w, LinearEpi<T> epi) {
-  constexpr int RB = 4 / KS, Q = kMxChunk / 128;
-  __shared__ f32x4 red[(KS - 1) * RB * NC * 64];
+  constexpr int RB = 4 / KS, ROWS = 16 * RW, Q = kMxChunkLoads, KC = 128 * Q;
+  constexpr int XQ = RW == 4 ? 1 : 2;  // loads of the weight that are multiplied with theirs of the rows at once
+  typedef int i32x8 __attribute__((ext_vector_type(8)));
+  __shared__ f32x4 red[(KS - 1) * RB * RW * 64];
   const int N = w.N, K = w.K;
-  const int nNb = (N + 16 * RB - 1) / (16 * RB);
+  const int nNb = (N + ROWS * RB - 1) / (ROWS * RB);
   const int slot = uni(blockIdx.x / nNb), nb = uni(blockIdx.x % nNb);
   if (slot >= nslot) {
     skinny_no_group(offsets, E, M, N, (int64_t)blockIdx.x - (int64_t)nslot * nNb,
                     (int64_t)gridDim.x - (int64_t)nslot * nNb, epi);
     return;
   }
-  int grp = 0, r0 = slot * kLinearSkinnyRows, rows = min(kLinearSkinnyRows, M - r0);
-  if (offsets && !skinny_slot(offsets, E, M, slot, grp, r0, rows)) return;  // workgroup-uniform
+  int grp = 0, r0 = slot * kMxSkinnyRows, rows = min(kMxSkinnyRows, M - r0);
+  if (offsets && !skinny_slot<kMxSkinnyRows>(offsets, E, M, slot, grp, r0, rows)) return;  // workgroup-uniform
   grp = uni(grp); r0 = uni(r0); rows = uni(rows);
   const int wave = uni(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int rb = wave / KS, ks = wave % KS;
-  const int n0 = (nb * RB + rb) * 16;
-  const int nrows = uni(min(16, N - n0));
+  const int n0 = (nb * RB + rb) * ROWS;
+  const int nrows = uni(min(ROWS, N - n0));
   const int g = lane >> 4, rl = lane & 15;
-  const int nch = (rows + 15) / 16;
   const int bytes = K / 2, blocks = K / kMxBlock;
-  f32x4 acc[NC];
+  f32x4 acc[RW];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) acc[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i = 0; i < RW; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   if (nrows > 0) {
     const int xb = X4 ? bytes : 2 * K;  // bytes of a token row
     const rsrc_t rx = make_rsrc(uni_ptr((const uint8_t*)X + (int64_t)r0 * xb), (uint32_t)uni(rows * xb));
-    const rsrc_t rxs = make_rsrc(uni_ptr(X4 ? XS + (int64_t)r0 * blocks : w.scales), (uint32_t)uni(X4 ? rows * blocks : 0));
     const int64_t first = (int64_t)grp * N + n0;
     const rsrc_t rw = make_rsrc(uni_ptr(w.codes + first * bytes), (uint32_t)uni(nrows * bytes));
-    const rsrc_t rs = make_rsrc(uni_ptr(w.scales + first * blocks), (uint32_t)uni(nrows * blocks));
-    for (int kc = ks; kc * kMxChunk < K; kc += KS) {
-      u32x4 wa[Q];
-      uint32_t ws[Q];
+    const uint8_t* wscales = uni_ptr(w.scales + first * blocks);
+    uint32_t vw[RW];
 #pragma unroll
-      for (int q = 0; q < Q; ++q) {
-        const int b = kc * (kMxChunk / kMxBlock) + 4 * q + g;
-        const bool in = b < blocks;
-        wa[q] = buf_ld16(rw, in ? (uint32_t)(rl * bytes + 16 * b) : kOobOffset, 0);
-        ws[q] = __builtin_amdgcn_raw_buffer_load_b8(rs, in ? (uint32_t)(rl * blocks + b) : kOobOffset, 0, 0);
-      }
+    for (int i = 0; i < RW; ++i) vw[i] = 16 * i + rl < nrows ? (uint32_t)((16 * i + rl) * bytes + 16 * g) : kOobOffset;
+    const uint32_t vx = rl < rows ? (uint32_t)(rl * xb + (X4 ? 16 : 64) * g) : kOobOffset;
+    auto chunk = [&](int kc, auto full_c) {
+      constexpr bool FULL = decltype(full_c)::value;
+      const int b0 = kc * 4 * Q, left = blocks - b0;  // blocks
+      u32x4 wa[RW][Q];
+      uint32_t ws[RW][Q];
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        if (c >= nch) break;
-        const int t = c * 16 + rl;
+      for (int i = 0; i < RW; ++i)
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
-          const int b = kc * (kMxChunk / kMxBlock) + 4 * q + g;
-          const bool in = b < blocks && t < rows;
-          if constexpr (X4) {
-            typedef int i32x8 __attribute__((ext_vector_type(8)));
-            const u32x4 xa = buf_ld16(rx, in ? (uint32_t)(t * bytes + 16 * b) : kOobOffset, 0);
-            const uint32_t xs = __builtin_amdgcn_raw_buffer_load_b8(rxs, in ? (uint32_t)(t * blocks + b) : kOobOffset, 0, 0);
-            const i32x8 av = {(int)xa.x, (int)xa.y, (int)xa.z, (int)xa.w, 0, 0, 0, 0};
-            const i32x8 bv = {(int)wa[q].x, (int)wa[q].y, (int)wa[q].z, (int)wa[q].w, 0, 0, 0, 0};
-            acc[c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc[c], 4, 4, 0, (int)xs, 0, (int)ws[q]);
-          } else {
-            u32x4 xa[4];
+          const bool in = FULL || 4 * q + g < left;
+          wa[i][q] = buf_ld16(rw, in ? vw[i] + 64 * q : kOobOffset, (uint32_t)b0 * 16);
+        }
 #pragma unroll
-            for (int v = 0; v < 4; ++v)
-              xa[v] = buf_ld16(rx, in ? (uint32_t)(t * xb + 64 * b + 16 * v) : kOobOffset, 0);
-            const float s = mx_scale(ws[q]);
+      for (int i = 0; i < RW; ++i)  // rows past the weight's read its first row's scales (their codes are zeros)
+        mx_row_scales<FULL>(wscales + (16 * i + rl < nrows ? 16 * i + rl : 0) * blocks + b0, left, g, ws[i]);
+      if constexpr (X4) {
+        u32x4 xa[Q];
+        uint32_t xs[Q];
 #pragma unroll
-            for (int v = 0; v < 4; ++v) mfma16(acc[c], xa[v], mx_bf16x8(wa[q][v], s));
+        for (int q = 0; q < Q; ++q) {
+          const bool in = FULL || 4 * q + g < left;
+          xa[q] = buf_ld16(rx, in ? vx + 64 * q : kOobOffset, (uint32_t)b0 * 16);
+        }
+        mx_row_scales<FULL>(XS + ((int64_t)r0 + (rl < rows ? rl : 0)) * blocks + b0, left, g, xs);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+          const i32x8 av = {(int)xa[q].x, (int)xa[q].y, (int)xa[q].z, (int)xa[q].w, 0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < RW; ++i) {
+            const u32x4 v = wa[i][q];
+            const i32x8 bv = {(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
+            acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc[i], 4, 4, 0, (int)xs[q], 0, (int)ws[i][q]);
           }
         }
+      } else {
+#pragma unroll
+        for (int h = 0; h < Q; h += XQ) {
+          u32x4 xa[XQ][4];
+#pragma unroll
+          for (int q = 0; q < XQ; ++q) {
+            const bool in = FULL || 4 * (h + q) + g < left;
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+              xa[q][v] = buf_ld16(rx, in ? vx + 256 * (h + q) + 16 * v : kOobOffset, (uint32_t)b0 * 64);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int q = 0; q < XQ; ++q)
+#pragma unroll
+            for (int i = 0; i < RW; ++i) {
+              const float s = mx_scale(ws[i][h + q] & 255u);
+#pragma unroll
+              for (int v = 0; v < 4; ++v) mfma16(acc[i], xa[q][v], mx_bf16x8(wa[i][h + q][v], s));
+            }
+        }
       }
-    }
+    };
+    int kc = ks;
+    for (; (kc + 1) * KC <= K; kc += KS) chunk(kc, std::true_type());
+    if (kc * KC < K) chunk(kc, std::false_type());
   }
   if (ks > 0) {
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-      if (c < nch) red[((ks - 1) * RB + rb) * NC * 64 + c * 64 + lane] = acc[c];
+    for (int i = 0; i < RW; ++i) red[(((ks - 1) * RB + rb) * RW + i) * 64 + lane] = acc[i];
   }
   __syncthreads();
   if (ks > 0) return;
 #pragma unroll
   for (int q = 1; q < KS; ++q)
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-      if (c < nch) acc[c] += red[((q - 1) * RB + rb) * NC * 64 + c * 64 + lane];
-  if (rl >= nrows) return;
-  skinny_store<T, NC>(epi, acc, nch, r0, rows, n0 + rl, grp);
+    for (int i = 0; i < RW; ++i) acc[i] += red[(((q - 1) * RB + rb) * RW + i) * 64 + lane];
+#pragma unroll
+  for (int i = 0; i < RW; ++i) {
+    const f32x4 one[1] = {acc[i]};
+    if (16 * i + rl < nrows) skinny_store<T, 1>(epi, one, 1, r0, rows, n0 + 16 * i + rl, grp);
+  }
 }
 
 }  // namespace moe

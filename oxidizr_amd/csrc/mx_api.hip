@@ -18,6 +18,7 @@ moe_status check_mx(int dtype, int64_t blocks) {
 
 // ---- products
 constexpr int kMxMaxWidth = 1 << 20;
+constexpr int kMxNoGroupBlocks = 64;  // of a launch, for the rows of no group
 moe_status check_mx_linear(int x_format, int dtype, int64_t M, int K, int N, int E, bool grouped, int act) {
   moe_status st = check_dtype(dtype);
   if (st != MOE_OK) return st;
@@ -42,41 +43,69 @@ moe_status check_mx_linear(int x_format, int dtype, int64_t M, int K, int N, int
   return MOE_OK;
 }
 
-int mx_skinny_split(int K) { return K >= 8 * kMxChunk ? 4 : 2; }
+// Shape of a few-row launch: waves that share the K of their weight rows, blocks of 16 weight rows to a wave.  More
+// blocks read the token rows less often (bf16 rows are four times the weight's bytes), fewer make more workgroups, and so
+// do more waves.  us at (4 waves, 1 block) / (4, 2) / (2, 4), and with both sides in 4 bits (4, 1) / (4, 2) / (2, 2): 2 rows in
+// 16 experts of 1408 x 2048 4.1 / 5.1 / 9.3 and 3.9 / 4.7 / 5.5; one weight of 4096 x 4096, 16 rows 7.7 / 9.4 / 20.6 and 5.3 / 7.1
+// / 10.0, 32 rows 12.4 / 9.6 / 20.7 and 7.6 / 7.1 / 10.1; 128 rows in 16 experts 13.8 / 11.7 / 13.5 and 8.9 / 8.6 / 9.9; 512 in 128
+// of 1536 x 4096 131 / 101 / 92 and 89 / 77 / 76.
+struct MxSkinny {
+  int ks, rw;
+};
 int64_t mx_skinny_slots(int64_t M, int E, bool grouped) {
-  return grouped ? std::min<int64_t>(E, M) + M / kLinearSkinnyRows : ceil_div(M, kLinearSkinnyRows);
+  return grouped ? std::min<int64_t>(E, M) + M / kMxSkinnyRows : ceil_div(M, kMxSkinnyRows);
 }
-int64_t mx_skinny_blocks(int64_t M, int K, int N, int E, bool grouped) {
-  return mx_skinny_slots(M, E, grouped) * ceil_div(N, 64 / mx_skinny_split(K)) + (grouped ? 64 : 0);
+MxSkinny mx_skinny_shape(bool four, int64_t M, int N, int E, bool grouped) {
+  const int64_t blocks = mx_skinny_slots(M, E, grouped) * ceil_div(N, 16);
+  if (blocks < 512) return {4, 1};
+  if (blocks < 4096) return {4, 2};
+  return {2, four ? 2 : 4};
 }
-bool mx_skinny(int64_t M, int K, int N, int E, bool grouped) {
-  if (mx_skinny_blocks(M, K, N, E, grouped) * 256 >= kMaxGridThreads) return false;
-  return M <= 8 * (grouped ? std::min<int64_t>(E, M) : 4);
+// Calls f(waves, blocks), constants.
+template <bool X4, class F>
+void with_mx_skinny(const MxSkinny& p, F&& f) {
+  using std::integral_constant;
+  if (p.ks == 2) f(integral_constant<int, 2>(), integral_constant<int, X4 ? 2 : 4>());
+  else if (p.rw == 2) f(integral_constant<int, 4>(), integral_constant<int, 2>());
+  else f(integral_constant<int, 4>(), integral_constant<int, 1>());
+}
+int64_t mx_skinny_blocks(const MxSkinny& p, int64_t M, int N, int E, bool grouped) {
+  return mx_skinny_slots(M, E, grouped) * ceil_div(N, 64 / p.ks * p.rw) + (grouped ? kMxNoGroupBlocks : 0);
+}
+// Whether a forward runs as the stream of its weights.  us, tiles / this: bf16 rows, 512, 1024 and 2048 in 128 experts of 1536 x
+// 4096 161 / 92, 168 / 112, 176 / 148; 128, 256 and 512 in 16 of 1408 x 2048 18 / 12, 19 / 14, 19 / 22; 64, 128 and 256 of one weight
+// of 4096 x 4096 32 / 14, 33 / 21, 33 / 37.  Both sides in 4 bits: 85 / 76, 87 / 91, 89 / 109; 9.3 / 8.6, 9.2 / 10.5, 9.5 / 14;
+// 13 / 10, 13 / 16, 13 / 27.
+bool mx_skinny(bool four, int64_t M, int K, int N, int E, bool grouped) {
+  // the tiles' scales are loaded 16 bytes at once
+  if (four && std::min(M, (int64_t)E * N) * (K / kMxBlock) < 16) return true;
+  if (mx_skinny_blocks(mx_skinny_shape(four, M, N, E, grouped), M, N, E, grouped) * 256 >= kMaxGridThreads) return false;
+  return grouped ? M <= (four ? 7 : 20) * std::min<int64_t>(E, M) : M <= (four ? 80 : 160);
 }
 
-// Row tiles by height; prefixes of k_linear_prep.
+// Row tiles by height, by their cost in tenths of a full round of 256-row tiles.  us, 256 / 128 / 64 rows, over bf16 rows: 16384 rows
+// in 16 experts, 2048 -> 1408 106 / 118 / 152; 65536 in 128, 4096 -> 1536 865 / 1051 / 1382; 12000 in 12, 1376 -> 1368 82 / 77 / 82;
+// 8192 in 64, 2048 -> 1408 85 / 86 / 89; 2048 in 16 44 / 27 / 26; 1999 of one weight, 2784 -> 2056 57 / 46 / 56; 512 of 4096 -> 4096
+// 81 / 45 / 35; their input gradients 118 / 127 / 177, 909 / 1129 / 1559, 77 / 73 / 97, 92 / 83 / 106, 38 / 30 / 37, 52 / 40 / 51, 96 /
+// 53 / 42; both sides in 4 bits 48 / 50 / 65, 343 / 404 / 569, 51 / 48 / 44, 40 / 39 / 43, 20 / 14 / 13, 27 / 21 / 25, 30 / 17 / 18.
 enum class MxTiles { kBig, kMid, kSmall };
-using MxBig = Tilings<bf16_t>::Big;
-using MxMid = Tilings<bf16_t>::BigMid;
-using MxSmall = Tilings<bf16_t>::BigSmall;
 MxTiles mx_tiles(bool grouped, int E, int64_t M, int N) {
   const int groups = grouped ? (int)std::min<int64_t>(E, M) : 1;
   auto count = [&](int bm, int bn) {
     return (grouped ? group_row_tiles(groups, (double)M / groups, bm) : (double)ceil_div(M, bm)) * ceil_div(N, bn);
   };
-  const double big = big_cost(count(256, 256), 10.0);
-  const double mid = round_cost(count(128, 128), {4.8, 6.3});
-  const double small = round_cost(count(64, 128), {2.9, 4.3});
+  const double tiles = count(256, 256), big = tiles <= 128.0 ? 7.5 : big_cost(tiles, 10.0);
+  const double mid = round_cost(count(128, 128), {4.2, 7.0});
+  const double small = round_cost(count(64, 128), {3.0, 4.9});
   return big <= std::min(mid, small) ? MxTiles::kBig : mid <= small ? MxTiles::kMid : MxTiles::kSmall;
 }
 template <class F>
 void with_mx_tiling(MxTiles kind, F&& f) {
-  if (kind == MxTiles::kMid) return f(MxMid{});
-  if (kind == MxTiles::kSmall) return f(MxSmall{});
-  f(MxBig{});
+  if (kind == MxTiles::kMid) return f(Tilings<bf16_t>::BigMid{});
+  if (kind == MxTiles::kSmall) return f(Tilings<bf16_t>::BigSmall{});
+  f(Tilings<bf16_t>::Big{});
 }
 // Blocks of tiles, and behind them (grouped) those for the rows of no group.
-constexpr int kMxNoGroupBlocks = 64;
 template <class C>
 int64_t mx_tile_blocks(bool grouped, int E, int64_t M, int N) {
   if (!grouped) return (int64_t)ceil_div(M, C::BM) * ceil_div(N, C::BN);
@@ -90,9 +119,9 @@ moe_status check_mx_tiles(MxTiles kind, bool grouped, int E, int64_t M, int N) {
   });
   return st;
 }
-moe_status check_mx_launches(bool backward, bool grouped, int E, int64_t M, int K, int N) {
+moe_status check_mx_launches(bool backward, bool four, bool grouped, int E, int64_t M, int K, int N) {
   if (backward) return check_mx_tiles(mx_tiles(grouped, E, M, K), grouped, E, M, K);
-  return mx_skinny(M, K, N, E, grouped) ? MOE_OK : check_mx_tiles(mx_tiles(grouped, E, M, N), grouped, E, M, N);
+  return mx_skinny(four, M, K, N, E, grouped) ? MOE_OK : check_mx_tiles(mx_tiles(grouped, E, M, N), grouped, E, M, N);
 }
 // Calls f(tiling, blocks of tiles, grid).
 template <class F>
@@ -129,19 +158,14 @@ moe_status mx_forward(hipStream_t s, int64_t M, int E, const int* offsets, const
                       const MxWeights& w, const LinearEpi<T>& epi) {
   const bool grouped = offsets != nullptr;
   const int N = w.N, K = w.K;
-  if (mx_skinny(M, K, N, E, grouped)) {
+  if (mx_skinny(X4, M, K, N, E, grouped)) {
+    const MxSkinny p = mx_skinny_shape(X4, M, N, E, grouped);
     const int nslot = (int)mx_skinny_slots(M, E, grouped);
-    const unsigned grid = (unsigned)mx_skinny_blocks(M, K, N, E, grouped);
-    auto go = [&](auto nc, auto ks) {
-      hipLaunchKernelGGL((k_mx_skinny<X4, T, decltype(nc)::value, decltype(ks)::value>), dim3(grid), dim3(256), 0, s,
-                         x, xs, offsets, E, (int)M, nslot, w, epi);
-    };
-    auto split = [&](auto nc) {
-      if (mx_skinny_split(K) == 4) go(nc, std::integral_constant<int, 4>());
-      else go(nc, std::integral_constant<int, 2>());
-    };
-    if (M <= 16) split(std::integral_constant<int, 1>());
-    else split(std::integral_constant<int, 4>());
+    const dim3 grid((unsigned)mx_skinny_blocks(p, M, N, E, grouped));
+    with_mx_skinny<X4>(p, [&](auto ks, auto rw) {
+      hipLaunchKernelGGL((k_mx_skinny<X4, T, decltype(ks)::value, decltype(rw)::value>), grid, dim3(256), 0, s, x, xs,
+                         offsets, E, (int)M, nslot, w, epi);
+    });
     LAUNCH_CHECK();
     return MOE_OK;
   }
@@ -233,7 +257,7 @@ moe_status moe_mx_dequantize(int32_t device, void* stream, int32_t dtype, int64_
 size_t moe_mx_linear_workspace_bytes(int32_t x_format, int32_t dtype, int64_t M, int32_t K, int32_t N, int32_t E,
                                      int32_t grouped, int32_t activation, int32_t backward) {
   if (check_mx_linear(x_format, dtype, M, K, N, E, grouped != 0, activation) != MOE_OK) return 0;
-  if (M > 0 && check_mx_launches(backward != 0, grouped != 0, E, M, K, N) != MOE_OK) return 0;
+  if (M > 0 && check_mx_launches(backward != 0, x_format == MOE_MX_ROWS_FOUR_BIT, grouped != 0, E, M, K, N) != MOE_OK) return 0;
   return mx_ws(M, N, E, grouped != 0, activation, backward != 0).total;
 }
 
@@ -243,7 +267,7 @@ moe_status moe_mx_linear_forward(int32_t device, void* stream, int32_t x_format,
                                  const void* residual, int32_t activation, void* y, void* pre_act, void* workspace) {
   moe_status st = check_mx_linear(x_format, dtype, M, K, N, E, offsets != nullptr, activation);
   if (st != MOE_OK || M == 0) return st;
-  if ((st = check_mx_launches(false, offsets != nullptr, E, M, K, N)) != MOE_OK) return st;
+  if ((st = check_mx_launches(false, x_format == MOE_MX_ROWS_FOUR_BIT, offsets != nullptr, E, M, K, N)) != MOE_OK) return st;
   if ((st = check_pointers({x, w_codes, y}, {bias, residual, pre_act})) != MOE_OK) return st;
   if ((st = check_ints({w_scales}, 1)) != MOE_OK) return st;
   const bool four = x_format == MOE_MX_ROWS_FOUR_BIT;
@@ -271,7 +295,7 @@ moe_status moe_mx_linear_backward(int32_t device, void* stream, int64_t M, int32
   if (st != MOE_OK) return st;
   if ((st = check_pointers({}, {dx, d_bias, workspace})) != MOE_OK) return st;
   if (M > 0) {
-    if ((st = check_mx_launches(true, offsets != nullptr, E, M, K, N)) != MOE_OK) return st;
+    if ((st = check_mx_launches(true, false, offsets != nullptr, E, M, K, N)) != MOE_OK) return st;
     if ((st = check_pointers({d_y, w_codes}, {pre_act})) != MOE_OK) return st;
     if ((st = check_ints({w_scales}, 1)) != MOE_OK) return st;
     if (activation != kActNone && !pre_act)
