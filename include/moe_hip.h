@@ -420,7 +420,7 @@ moe_status moe_router_losses_backward(int32_t device, void* stream, int32_t dtyp
  * tensor [.., K], K a multiple of 32, is codes [.., K / 2] and scales [.., K / 32].  Quantising num_blocks blocks of
  * 32: s = floor(log2 of the largest magnitude) - 2, at least -127; to the nearest code, ties to the even one, what is
  * above the largest becomes it; a block with an infinity or a NaN becomes NaN (scale 255).  Codes are 16-byte
- * aligned, scales have any alignment.  num_blocks < 2^30. */
+ * aligned, scales have any alignment.  num_blocks < 2^29. */
 moe_status moe_mx_quantize(int32_t device, void* stream, int32_t dtype, int64_t num_blocks, const void* x,
                            uint8_t* codes, uint8_t* scales);
 /* The numbers that they stand for, in fp32 or bf16 (both hold them exactly but for 6 2^127 in bf16, which

@@ -12,8 +12,8 @@ moe_status check_mx(int dtype, int64_t blocks) {
   moe_status st = check_dtype(dtype);
   if (st != MOE_OK) return st;
   if (blocks < 0) return fail(MOE_ERR_INVALID, "num_blocks is negative");
-  // four lanes to a block
-  return blocks >= kMaxGridThreads / 4 ? fail(MOE_ERR_UNSUPPORTED, "num_blocks reaches 2^30: split the tensor") : MOE_OK;
+  // up to eight lanes to a block
+  return blocks >= kMaxGridThreads / 8 ? fail(MOE_ERR_UNSUPPORTED, "num_blocks reaches 2^29: split the tensor") : MOE_OK;
 }
 
 // ---- products
@@ -243,7 +243,7 @@ moe_status moe_mx_dequantize(int32_t device, void* stream, int32_t dtype, int64_
   if ((st = check_pointers({codes, y})) != MOE_OK || (st = check_ints({scales}, 1)) != MOE_OK) return st;
   DeviceScope dev(device);
   HIP_TRY(dev.enter());
-  const int64_t nvec = num_blocks * 4;
+  const int64_t nvec = num_blocks * (dtype == MOE_DTYPE_BF16 ? 4 : 8);  // 16 bytes each
   const dim3 grid((unsigned)((nvec + 255) / 256));
   hipStream_t s = (hipStream_t)stream;
   if (dtype == MOE_DTYPE_BF16)

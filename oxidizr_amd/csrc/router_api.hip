@@ -29,17 +29,18 @@ template <class F>
 void with_router_shape(int E, F&& f) {
   if (E % 4 == 0) {
     if (E <= 16) f(RouterShape<4, 4, 1>());
-    else if (E <= 32) f(RouterShape<4, 8, 1>());
-    else if (E <= 64) f(RouterShape<4, 16, 1>());
-    else if (E <= 128) f(RouterShape<4, 32, 1>());
-    else if (E <= 256) f(RouterShape<4, 64, 1>());
-    else if (E <= 512) f(RouterShape<4, 64, 2>());
+    else if (E <= 32) f(RouterShape<4, 4, 2>());
+    else if (E <= 64) f(RouterShape<4, 4, 4>());
+    else if (E <= 96) f(RouterShape<4, 8, 3>());
+    else if (E <= 128) f(RouterShape<4, 8, 4>());
+    else if (E <= 160) f(RouterShape<4, 8, 5>());
+    else if (E <= 256) f(RouterShape<4, 16, 4>());
+    else if (E <= 512) f(RouterShape<4, 32, 4>());
     else f(RouterShape<4, 64, 4>());
   } else {
-    if (E <= 64) f(RouterShape<1, 64, 1>());
-    else if (E <= 128) f(RouterShape<1, 64, 2>());
+    if (E <= 16) f(RouterShape<1, 16, 1>());
+    else if (E <= 64) f(RouterShape<1, 16, 4>());
     else if (E <= 256) f(RouterShape<1, 64, 4>());
-    else if (E <= 512) f(RouterShape<1, 64, 8>());
     else f(RouterShape<1, 64, 16>());
   }
 }
@@ -151,8 +152,9 @@ moe_status moe_router_losses_backward(int32_t device, void* stream, int32_t dtyp
     using I = decltype(i);
     with_router_shape(E, [&](auto c) {
       using C = decltype(c);
-      const int64_t step = (kRouterBwdBlock / 64) * C::RPW;  // rows of a block's step; within 2^20 blocks
-      const int64_t rpb = step * std::max<int64_t>(4, (T / step >> 20) + 1);
+      // rows of a block: some steps where there are enough of them for every CU; within 2^20 blocks
+      const int64_t step = (kRouterBwdBlock / 64) * C::RPW, steps = T / step;
+      const int64_t rpb = step * std::max(std::min<int64_t>(4, steps / 1024 + 1), (steps >> 20) + 1);
       hipLaunchKernelGGL((k_router_losses_bwd<C, D, I>), dim3((unsigned)((T + rpb - 1) / rpb)), dim3(kRouterBwdBlock), 0,
                          s, (router_rows<D, I>(logits, topk_idx, offsets, T, E, k, S, score, temperature)), rpb, slope,
                          inv_real, lse, d_balance, d_z, (D*)d_logits);

@@ -129,7 +129,7 @@ def test_c_entries_refuse_before_any_device_call():
 
     for f in (L.moe_mx_quantize, L.moe_mx_dequantize):
         for args, match, code in (((7, 4, P, P, P), "dtype", 1), ((F32, -1, P, P, P), "num_blocks", 1),
-                                  ((F32, 2 ** 30, P, P, P), "2^30", 4), ((F32, 4, None, P, P), "NULL", 1),
+                                  ((F32, 2 ** 29, P, P, P), "2^29", 4), ((F32, 4, None, P, P), "NULL", 1),
                                   ((F32, 4, P + 8, P, P), "16-byte", 1)):
             assert status(f(0, None, *args), match) == code
         assert f(0, None, F32, 0, None, None, None) == 0
