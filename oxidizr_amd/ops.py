@@ -504,18 +504,23 @@ class _RouterShape(NamedTuple):
 
 def _router(logits, idx, offsets, s, keep):
     L = _lib.load()
+    balance, z = logits.new_empty(s.shape, dtype=torch.float32), logits.new_empty(s.shape, dtype=torch.float32)
+    counts = logits.new_empty(s.shape + (s.E,), dtype=torch.int32)
     # one allocation for what a backward reads: slope, inv_real and lse
-    out = logits.new_empty(2, s.S, dtype=torch.float32)
-    counts = logits.new_empty(s.S, s.E, dtype=torch.int32)
-    kept = logits.new_empty(s.S * (s.E + 1) + s.T, dtype=torch.float32) if keep else None
-    at = kept.data_ptr() if keep else 0
+    kept, at = None, (None, None, None)
+    if keep:
+        kept = logits.new_empty(s.S * (s.E + 1) + s.T, dtype=torch.float32)
+        at = _kept_of_router(kept, s)
     ws = _workspace(L.moe_router_losses_workspace_bytes(s.T, s.E, s.S), logits)
     _call(L.moe_router_losses, logits.get_device(), _dtype_code(logits.dtype), s.T, s.E, s.k, idx.element_size(),
           logits.data_ptr(), idx.data_ptr(), s.score, s.temperature, s.switch_coef, s.sqprob_coef, _ptr(offsets), s.S,
-          out.data_ptr(), out.data_ptr() + 4 * s.S, counts.data_ptr(), at if keep else None,
-          at + 4 * s.S * s.E if keep else None, at + 4 * s.S * (s.E + 1) if keep else None, _ptr(ws))
-    balance, z = out.unbind(0)
-    return balance.view(s.shape), z.view(s.shape), counts.view(s.shape + (s.E,)), kept
+          balance.data_ptr(), z.data_ptr(), counts.data_ptr(), *at, _ptr(ws))
+    return balance, z, counts, kept
+
+
+def _kept_of_router(kept, s):
+    at = kept.data_ptr()
+    return at, at + 4 * s.S * s.E, at + 4 * s.S * (s.E + 1)
 
 
 class _RouterLosses(torch.autograd.Function):
@@ -539,10 +544,9 @@ class _RouterLosses(torch.autograd.Function):
         d_balance = None if d_balance is None else d_balance.contiguous()
         d_z = None if d_z is None else d_z.contiguous()
         d_logits = torch.empty_like(logits)
-        at = kept.data_ptr()
         _call(_lib.load().moe_router_losses_backward, logits.get_device(), _dtype_code(logits.dtype), s.T, s.E, s.k,
-              idx.element_size(), logits.data_ptr(), idx.data_ptr(), s.score, s.temperature,
-              _ptr(offsets), s.S, at, at + 4 * s.S * s.E, at + 4 * s.S * (s.E + 1), _ptr(d_balance), _ptr(d_z), d_logits.data_ptr())
+              idx.element_size(), logits.data_ptr(), idx.data_ptr(), s.score, s.temperature, _ptr(offsets), s.S,
+              *_kept_of_router(kept, s), _ptr(d_balance), _ptr(d_z), d_logits.data_ptr())
         return d_logits, None, None, None
 
 
