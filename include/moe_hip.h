@@ -432,19 +432,19 @@ moe_status moe_mx_dequantize(int32_t device, void* stream, int32_t dtype, int64_
  * (dtype bf16), or 4-bit rows x [M, K / 2] with x_scales [M, K / 32].  bias [G, N], residual, y and pre_act [M, N] are
  * of dtype.  in_features K is a multiple of 32, out_features N of 8; products are summed in fp32.  Refused with
  * MOE_ERR_UNSUPPORTED: a width above 2^20, a weight matrix of 2^30 elements, more than 2^26 rows, rows x max(K, N) of
- * 2^34 bytes, and more tiles than a launch holds.  moe_mx_linear_workspace_bytes is 0 for a refused call. */
+ * 2^34 bytes, and more tiles than a launch holds. */
 typedef enum { MOE_MX_ROWS_BF16 = 0, MOE_MX_ROWS_FOUR_BIT } moe_mx_rows;
-size_t moe_mx_linear_workspace_bytes(int32_t x_format, int32_t dtype, int64_t num_rows,
-                                     int32_t in_features, int32_t out_features, int32_t num_groups,
-                                     int32_t grouped, int32_t activation, int32_t backward);
 moe_status moe_mx_linear_forward(int32_t device, void* stream, int32_t x_format, int32_t dtype,
                                  int64_t num_rows, int32_t in_features, int32_t out_features,
                                  int32_t num_groups, const int32_t* offsets, const void* x,
                                  const uint8_t* x_scales, const uint8_t* w_codes,
                                  const uint8_t* w_scales, const void* bias, const void* residual,
-                                 int32_t activation, void* y, void* pre_act, void* workspace);
+                                 int32_t activation, void* y, void* pre_act);
 /* dx [M, K] (0 for rows of no group) and d_bias [G, N] (0 for a group without rows) in bf16, each written
- * unless NULL, of a forward over bf16 rows.  The residual's gradient is d_y; the weights have none. */
+ * unless NULL, of a forward over bf16 rows.  The residual's gradient is d_y; the weights have none.
+ * moe_mx_linear_workspace_bytes is 0 for a refused call. */
+size_t moe_mx_linear_workspace_bytes(int64_t num_rows, int32_t in_features, int32_t out_features,
+                                     int32_t num_groups, int32_t grouped, int32_t activation);
 moe_status moe_mx_linear_backward(int32_t device, void* stream, int64_t num_rows, int32_t in_features,
                                   int32_t out_features, int32_t num_groups, const int32_t* offsets,
                                   const void* d_y, const uint8_t* w_codes, const uint8_t* w_scales,

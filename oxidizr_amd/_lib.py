@@ -162,10 +162,10 @@ def load():
     L.moe_mx_quantize.restype = i32
     L.moe_mx_dequantize.argtypes = L.moe_mx_quantize.argtypes
     L.moe_mx_dequantize.restype = i32
-    L.moe_mx_linear_workspace_bytes.argtypes = [i32, i32, i64, i32, i32, i32, i32, i32, i32]
+    L.moe_mx_linear_workspace_bytes.argtypes = [i64, i32, i32, i32, i32, i32]
     L.moe_mx_linear_workspace_bytes.restype = sz
     L.moe_mx_linear_forward.argtypes = [i32, _vp, i32, i32, i64, i32, i32, i32, _vp, _vp, _vp, _vp, _vp, _vp,
-                                        _vp, i32, _vp, _vp, _vp]
+                                        _vp, i32, _vp, _vp]
     L.moe_mx_linear_forward.restype = i32
     L.moe_mx_linear_backward.argtypes = [i32, _vp, i64, i32, i32, i32, _vp, _vp, _vp, _vp, _vp, i32, _vp, _vp,
                                          _vp]

@@ -133,6 +133,7 @@ MOE_DEV bool mx_tile(const MxRows& r, int N, int blk, int& grp, int& row0, int& 
   int first = __builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(n, l);
   for (int i = 0; i < per; ++i) {  // the groups of lane l, walked by every lane
     int a, b;
+    if (l * per + i >= r.G) break;
     range(l * per + i, a, b);
     a = uni(a);
     b = uni(b);

@@ -133,14 +133,13 @@ void with_mx_launch(MxTiles kind, const MxRows& r, int N, F&& f) {
   });
 }
 
-// Scratch of a backward with an activation or a bias gradient: k_linear_dz's chunks.
+// Scratch of a backward: dz, and k_linear_dz's chunks.
 struct MxWs {
   size_t offs, prefixes, w_tab, dz, part, total;
 };
 int64_t mx_dz_chunks(int64_t M, int E, bool grouped) { return (M + kDzRows - 1) / kDzRows + (grouped ? E : 0); }
-MxWs mx_ws(int64_t M, int N, int E, bool grouped, int act, bool backward) {
+MxWs mx_ws(int64_t M, int N, int E, bool grouped, int act) {
   MxWs w{};
-  if (!backward) return w;
   Carve c;
   if (grouped) {
     w.offs = c.take((size_t)(E + 1) * 4);
@@ -185,7 +184,7 @@ moe_status mx_backward(hipStream_t s, int64_t M, int E, const int* offsets, cons
                        const bf16_t* pre, int act, bf16_t* dx, bf16_t* db, char* ws) {
   const bool grouped = offsets != nullptr;
   const int N = w.N, K = w.K;
-  const MxWs L = mx_ws(M, N, E, grouped, act, true);
+  const MxWs L = mx_ws(M, N, E, grouped, act);
   const MxRows r{offsets, E, (int)M};
   const bf16_t* dz = dy;
   if (act != kActNone || db) {
@@ -254,17 +253,16 @@ moe_status moe_mx_dequantize(int32_t device, void* stream, int32_t dtype, int64_
   return MOE_OK;
 }
 
-size_t moe_mx_linear_workspace_bytes(int32_t x_format, int32_t dtype, int64_t M, int32_t K, int32_t N, int32_t E,
-                                     int32_t grouped, int32_t activation, int32_t backward) {
-  if (check_mx_linear(x_format, dtype, M, K, N, E, grouped != 0, activation) != MOE_OK) return 0;
-  if (M > 0 && check_mx_launches(backward != 0, x_format == MOE_MX_ROWS_FOUR_BIT, grouped != 0, E, M, K, N) != MOE_OK) return 0;
-  return mx_ws(M, N, E, grouped != 0, activation, backward != 0).total;
+size_t moe_mx_linear_workspace_bytes(int64_t M, int32_t K, int32_t N, int32_t E, int32_t grouped, int32_t activation) {
+  if (check_mx_linear(MOE_MX_ROWS_BF16, MOE_DTYPE_BF16, M, K, N, E, grouped != 0, activation) != MOE_OK) return 0;
+  if (M > 0 && check_mx_launches(true, false, grouped != 0, E, M, K, N) != MOE_OK) return 0;
+  return mx_ws(M, N, E, grouped != 0, activation).total;
 }
 
 moe_status moe_mx_linear_forward(int32_t device, void* stream, int32_t x_format, int32_t dtype, int64_t M, int32_t K,
                                  int32_t N, int32_t E, const int32_t* offsets, const void* x, const uint8_t* x_scales,
                                  const uint8_t* w_codes, const uint8_t* w_scales, const void* bias,
-                                 const void* residual, int32_t activation, void* y, void* pre_act, void* workspace) {
+                                 const void* residual, int32_t activation, void* y, void* pre_act) {
   moe_status st = check_mx_linear(x_format, dtype, M, K, N, E, offsets != nullptr, activation);
   if (st != MOE_OK || M == 0) return st;
   if ((st = check_mx_launches(false, x_format == MOE_MX_ROWS_FOUR_BIT, offsets != nullptr, E, M, K, N)) != MOE_OK) return st;

@@ -660,30 +660,25 @@ class _MxShape(NamedTuple):
 
 
 def _mx(x, x_scales, codes, scales, bias, offsets, residual, s, keep):
-    L = _lib.load()
-    code = _dtype_code(s.dtype)
     y = torch.empty(s.M, s.N, dtype=s.dtype, device=x.device)
     pre = torch.empty_like(y) if keep else None
-    ws = _workspace(L.moe_mx_linear_workspace_bytes(s.rows, code, s.M, s.K, s.N, s.groups, s.grouped, s.act, 0), x)
-    _call(L.moe_mx_linear_forward, x.get_device(), s.rows, code, s.M, s.K, s.N, s.groups, _ptr(offsets), x.data_ptr(),
-          _ptr(x_scales), codes.data_ptr(), scales.data_ptr(), _ptr(bias), _ptr(residual), s.act, y.data_ptr(),
-          _ptr(pre), _ptr(ws))
+    _call(_lib.load().moe_mx_linear_forward, x.get_device(), s.rows, _dtype_code(s.dtype), s.M, s.K, s.N, s.groups,
+          _ptr(offsets), x.data_ptr(), _ptr(x_scales), codes.data_ptr(), scales.data_ptr(), _ptr(bias), _ptr(residual),
+          s.act, y.data_ptr(), _ptr(pre))
     return y, pre
 
 
 class _MxLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, x_scales, bias, residual, codes, scales, offsets, s):
-        four = s.rows == _lib.MOE_MX_ROWS_FOUR_BIT
         x, bias, residual = _ready(x), _ready(bias), _ready(residual)
         products = ctx.needs_input_grad[0] or ctx.needs_input_grad[2]
         if products:
+            # here, where a refused backward can still be told
             L = _lib.load()
-            ctx.ws_bytes = L.moe_mx_linear_workspace_bytes(_lib.MOE_MX_ROWS_BF16, _lib.MOE_DTYPE_BF16, s.M, s.K, s.N,
-                                                           s.groups, s.grouped, s.act, 1)
-            if four or (ctx.ws_bytes == 0 and s.M > 0):
-                raise _lib.MoeError(_lib.MOE_ERR_UNSUPPORTED, "rows in 4 bits have no gradient of a bias" if four else
-                                    L.moe_last_error().decode())
+            ctx.ws_bytes = L.moe_mx_linear_workspace_bytes(s.M, s.K, s.N, s.groups, s.grouped, s.act)
+            if ctx.ws_bytes == 0 and s.M > 0:
+                raise _lib.MoeError(_lib.MOE_ERR_UNSUPPORTED, L.moe_last_error().decode())
         y, pre = _mx(x, x_scales, codes, scales, bias, offsets, residual, s, products and s.act != 0)
         ctx.save_for_backward(codes, scales, pre, offsets)
         ctx.s = s

@@ -418,15 +418,12 @@ pub mod ffi {
             y: *mut c_void,
         ) -> MoeStatus;
         pub fn moe_mx_linear_workspace_bytes(
-            x_format: i32,
-            dtype: i32,
             num_rows: i64,
             in_features: i32,
             out_features: i32,
             num_groups: i32,
             grouped: i32,
             activation: i32,
-            backward: i32,
         ) -> usize;
         pub fn moe_mx_linear_forward(
             device: i32,
@@ -447,7 +444,6 @@ pub mod ffi {
             activation: i32,
             y: *mut c_void,
             pre_act: *mut c_void,
-            workspace: *mut c_void,
         ) -> MoeStatus;
         pub fn moe_mx_linear_backward(
             device: i32,

@@ -45,6 +45,16 @@ def sources(to):
                             "if (emu::tiles < 0) p.tiles = big <= tall ? RowTiles::kBig : RowTiles::kTall;")
             text = replaced(text, "(big && M >= 2 * (int64_t)C::BM * E)",
                             "(big && (emu::tiles < 0 ? M >= 2 * (int64_t)C::BM * E : emu::tiles == 0))")
+        if name == "mx_api.hip":
+            text = replaced(text, "MxTiles mx_tiles(bool grouped, int E, int64_t M, int N) {",
+                            "MxTiles mx_tiles(bool grouped, int E, int64_t M, int N) {\n"
+                            "  if (emu::tiles >= 0) return (MxTiles)emu::tiles;")
+            text = replaced(text, "bool mx_skinny(bool four, int64_t M, int K, int N, int E, bool grouped) {",
+                            "bool mx_skinny(bool four, int64_t M, int K, int N, int E, bool grouped) {\n"
+                            "  if (emu::tiles >= 0 && !(four && std::min(M, (int64_t)E * N) * (K / kMxBlock) < 16)) return false;\n"
+                            "  if (emu::tiles == -2) return true;")
+            # as many blocks for the rows of no group as show their loop
+            text = replaced(text, "constexpr int kMxNoGroupBlocks = 64;", "constexpr int kMxNoGroupBlocks = 2;")
         with open(os.path.join(src, name), "w") as f:
             f.write(text)
 

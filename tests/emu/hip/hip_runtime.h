@@ -116,6 +116,8 @@ template <int D> Pair swap_halves(unsigned a, unsigned b) {
   const unsigned pa = from<unsigned>(exchange(bits(a))[lane() ^ D]), pb = from<unsigned>(exchange(bits(b))[lane() ^ D]);
   return lane() & D ? Pair{{pb, b}} : Pair{{a, pa}};
 }
+// Keeps the load of a value that no address and no store depends on.
+template <class T> void use(const T& v) { asm volatile("" : : "r"(&v) : "memory"); }
 }  // namespace emu
 
 #define hipLaunchKernelGGL(kernel, grid, block, lds, stream, ...) \
@@ -128,6 +130,14 @@ template <int D> Pair swap_halves(unsigned a, unsigned b) {
 #define __builtin_amdgcn_raw_buffer_load_b32(r, v, s, aux) emu::load<uint32_t>(r, v, s)
 #define __builtin_amdgcn_raw_ptr_buffer_load_lds(r, lds, n, v, s, inst, aux) emu::load_lds(r, (void*)(lds), n, v, s)
 #define __builtin_amdgcn_ds_read_tr16_b64_v4i16(p) (*(p))
+#define __builtin_amdgcn_raw_buffer_load_b8(r, v, s, aux) emu::load<uint8_t>(r, v, s)
+#define __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, fa, fb, oa, sa, ob, sb) (emu::use(sa), emu::use(sb), c)
+#define __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, fa, fb, oa, sa, ob, sb) (emu::use(sa), emu::use(sb), c)
+#define __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, i) (emu::use(s), (uint32_t)((c) >> (8 * (i)) & 255u))
+#define __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, i) (f32x2{(float)((c) >> (8 * (i)) & 15u), (s)})
+#define __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x, y, s, i) ((uint32_t)(c) | (((x) > (y) ? 1u : 2u) << (8 * (i))))
+#define __builtin_amdgcn_exp2f(x) exp2f(x)
+#define __any(x) (__ballot(x) != 0)
 #define __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, x, y, z) (c)
 #define __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, x, y, z) (c)
 #define __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, x, y, z) (c)

@@ -136,8 +136,8 @@ def test_c_entries_refuse_before_any_device_call():
     assert status(L.moe_mx_quantize(0, None, F32, 4, P, P, None), "NULL") == 1
     assert status(L.moe_mx_dequantize(0, None, F32, 4, P, None, P), "NULL") == 1
 
-    def fwd(M=4, K=64, N=8, E=3, off=P, act=0, x=P, xs=None, wc=P, wsc=P, rows=ROWS_BF16, dtype=BF16, ws=P):
-        return L.moe_mx_linear_forward(0, None, rows, dtype, M, K, N, E, off, x, xs, wc, wsc, None, None, act, P, None, ws)
+    def fwd(M=4, K=64, N=8, E=3, off=P, act=0, x=P, xs=None, wc=P, wsc=P, rows=ROWS_BF16, dtype=BF16, y=P):
+        return L.moe_mx_linear_forward(0, None, rows, dtype, M, K, N, E, off, x, xs, wc, wsc, None, None, act, y, None)
 
     def bwd(M=4, K=64, N=8, E=3, off=P, act=0, x=P, pre=None, wc=P, wsc=P, ws=P):
         return L.moe_mx_linear_backward(0, None, M, K, N, E, off, x, wc, wsc, pre, act, P, P, ws)
@@ -154,12 +154,13 @@ def test_c_entries_refuse_before_any_device_call():
         assert status(f(N=2 ** 20 + 8), "above 1048576") == 4
         assert status(f(M=2 ** 27), "rows") == 4
         assert status(f(M=2 ** 26, K=256), "2^34") == 4
-        assert status(f(ws=P + 8), "16-byte") == 1
-        assert status(f(ws=None), "NULL") == 1
         assert status(f(x=None), "NULL") == 1
         assert status(f(wc=P + 8), "16-byte") == 1
         assert status(f(wsc=None), "NULL") == 1
         assert status(f(off=P + 2), "aligned") == 1
+    assert status(bwd(ws=P + 8), "16-byte") == 1
+    assert status(bwd(ws=None), "NULL") == 1
+    assert status(fwd(y=None), "NULL") == 1
     assert fwd(M=0) == 0
     assert status(fwd(rows=2), "row format") == 1
     assert status(fwd(dtype=F32), "bf16 results") == 1
@@ -171,11 +172,10 @@ def test_c_entries_refuse_before_any_device_call():
 def test_workspace_sizes():
     L = _lib.load()
     ws = L.moe_mx_linear_workspace_bytes
-    assert ws(ROWS_BF16, BF16, 4096, 512, 256, 1, 0, 0, 0) == 0
-    none, act = (ws(ROWS_BF16, BF16, 4096, 512, 256, 8, 1, a, 1) for a in (0, 1))
+    none, act = (ws(4096, 512, 256, 8, 1, a) for a in (0, 1))
     assert act - none == 4096 * 256 * 2 and none >= (4096 // 64 + 8) * 256 * 4
-    assert ws(ROWS_BF16, BF16, 4096, 500, 256, 8, 1, 0, 1) == 0
-    assert ws(ROWS_BF16, F32, 4096, 512, 256, 8, 1, 0, 0) == 0
+    assert ws(4096, 500, 256, 8, 1, 0) == 0
+    assert ws(2 ** 27, 512, 256, 8, 1, 0) == 0
     r = L.moe_router_losses_workspace_bytes
     assert r(8192, 256, 1) >= 257 * 256 * 8 and r(0, 8, 1) > 0 and r(8, 0, 1) == 0 and r(8, 8, -1) == 0
 
