@@ -397,8 +397,8 @@ moe_status moe_residual_norm_backward_from_input(int32_t device, void* stream, i
  *   x = logits / temperature, q = softmax(x) or sigmoid(x) / sum sigmoid(x), P_e = sum q_te / n, f_e = M_e / (k n),
  *   balance[s] = E sum_e (switch_coef f_e P_e + sqprob_coef P_e^2), z[s] = sum logsumexp(x_t)^2 / n
  * (0 for n = 0), counts [S, E] = M_e.  1 <= E <= 1024, 1 <= k <= 16, T k < 2^31, S < 2^22.  slope [S, E] (of
- * balance in q_te), inv_real [S] (1 / n, or 0) and lse [T]: kept for a backward, or NULL.  Offsets ascend within 0..T; with others no access
- * leaves the tensors, but the results are not defined. */
+ * balance in q_te) and inv_real [S] (1 / n, or 0): kept for a backward, or NULL.  Offsets ascend within 0..T; with
+ * others no access leaves the tensors, but the results are not defined. */
 typedef enum { MOE_SCORE_SOFTMAX = 0, MOE_SCORE_SIGMOID } moe_score;
 size_t moe_router_losses_workspace_bytes(int64_t num_tokens, int32_t num_experts, int64_t num_sequences);
 moe_status moe_router_losses(int32_t device, void* stream, int32_t dtype, int64_t num_tokens,
@@ -406,14 +406,14 @@ moe_status moe_router_losses(int32_t device, void* stream, int32_t dtype, int64_
                              const void* logits, const void* topk_idx, int32_t score, float temperature,
                              float switch_coef, float sqprob_coef, const int32_t* offsets,
                              int64_t num_sequences, float* balance, float* z, int32_t* counts,
-                             float* slope, float* inv_real, float* lse, void* workspace);
+                             float* slope, float* inv_real, void* workspace);
 /* d_logits [T, E] of d_balance and d_z [S] (either may be NULL: 0), for what the forward was given and kept. */
 moe_status moe_router_losses_backward(int32_t device, void* stream, int32_t dtype, int64_t num_tokens,
                                       int32_t num_experts, int32_t experts_per_tok, int32_t index_bytes,
                                       const void* logits, const void* topk_idx, int32_t score,
                                       float temperature, const int32_t* offsets, int64_t num_sequences,
-                                      const float* slope, const float* inv_real, const float* lse,
-                                      const float* d_balance, const float* d_z, void* d_logits);
+                                      const float* slope, const float* inv_real, const float* d_balance,
+                                      const float* d_z, void* d_logits);
 
 /* Microscaled 4-bit numbers (OCP MXFP4).  32 elements share a scale 2^s, a byte s + 127 (255: NaN); an element
  * is a sign (bit 3) and a code 0..7 of 0 0.5 1 1.5 2 3 4 6; element 2 i of a row is the low half of its byte i.  A

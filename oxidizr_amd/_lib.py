@@ -153,10 +153,10 @@ def load():
     L.moe_router_losses_workspace_bytes.argtypes = [i64, i32, i64]
     L.moe_router_losses_workspace_bytes.restype = sz
     L.moe_router_losses.argtypes = [i32, _vp, i32, i64, i32, i32, i32, _vp, _vp, i32, f32, f32, f32, _vp, i64,
-                                    _vp, _vp, _vp, _vp, _vp, _vp, _vp]
+                                    _vp, _vp, _vp, _vp, _vp, _vp]
     L.moe_router_losses.restype = i32
     L.moe_router_losses_backward.argtypes = [i32, _vp, i32, i64, i32, i32, i32, _vp, _vp, i32, f32, _vp, i64,
-                                             _vp, _vp, _vp, _vp, _vp, _vp]
+                                             _vp, _vp, _vp, _vp, _vp]
     L.moe_router_losses_backward.restype = i32
     L.moe_mx_quantize.argtypes = [i32, _vp, i32, i64, _vp, _vp, _vp]
     L.moe_mx_quantize.restype = i32

@@ -188,8 +188,7 @@ __global__ __launch_bounds__(kRouterBlock) void k_router_losses(RouterRows<T, I>
                                                                 float* __restrict__ part_q,
                                                                 int* __restrict__ part_c,
                                                                 float* __restrict__ part_z,
-                                                                int* __restrict__ part_n,
-                                                                float* __restrict__ lse_out) {
+                                                                int* __restrict__ part_n) {
   constexpr int NW = kRouterBlock / 64;
   __shared__ float cols[NW][S::COLS];
   __shared__ int hist[S::COLS];
@@ -221,7 +220,6 @@ __global__ __launch_bounds__(kRouterBlock) void k_router_losses(RouterRows<T, I>
           ++n;
         }
       }
-      if (lse_out && has && j == 0) lse_out[row] = lse;
     }
 #pragma unroll
     for (int i = 0; i < S::C; ++i) {
@@ -347,7 +345,6 @@ constexpr int kRouterBwdBlock = 256;
 template <class S, typename T, typename I>
 __global__ __launch_bounds__(kRouterBwdBlock) void k_router_losses_bwd(
     RouterRows<T, I> in, int64_t rpb, const float* __restrict__ slope, const float* __restrict__ inv_real,
-    const float* __restrict__ lse_in,
     const float* __restrict__ d_balance, const float* __restrict__ d_z, T* __restrict__ d_logits) {
   constexpr int NW = kRouterBwdBlock / 64;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, j = lane % S::LPR, sub = lane / S::LPR;
@@ -375,16 +372,12 @@ __global__ __launch_bounds__(kRouterBwdBlock) void k_router_losses_bwd(
       const int64_t row = base + sub;
       const bool has = row < b;
       const int64_t at = has ? row : b - 1;
-      float x[S::C], q[S::C], p[S::C], lse = lse_in[at], dot = 0.0f;
+      float x[S::C], q[S::C], p[S::C], lse, dot = 0.0f;
       router_load<S>(in.logits + at * E, E, j, x, in.inv_tau);
       const bool real = router_real<S>(in.idx + at * k, k, E, j, has, [](int) {});
-      if (in.score == kScoreSoftmax) {
-#pragma unroll
-        for (int i = 0; i < S::C; ++i) q[i] = p[i] = exp_of(x[i] - lse);
-      } else {
-        float unused;
-        router_scores<S>(x, in.score, q, p, unused);
-      }
+      // from the row's largest again, not from a kept lse: x - lse carries lse's rounding, |lse| 2^-24, which is all of log sum
+      // where a row's logits are large (1 in each p of a row of the type's lowest value)
+      router_scores<S>(x, in.score, q, p, lse);
 #pragma unroll
       for (int i = 0; i < S::C; ++i) dot += q[i] * g[i];
       dot = group_sum<S::LPR>(dot);

@@ -98,7 +98,7 @@ size_t moe_router_losses_workspace_bytes(int64_t T, int32_t E, int64_t S) {
 moe_status moe_router_losses(int32_t device, void* stream, int32_t dtype, int64_t T, int32_t E, int32_t k,
                              int32_t index_bytes, const void* logits, const void* topk_idx, int32_t score,
                              float temperature, float switch_coef, float sqprob_coef, const int32_t* offsets, int64_t S,
-                             float* balance, float* z, int32_t* counts, float* slope, float* inv_real, float* lse,
+                             float* balance, float* z, int32_t* counts, float* slope, float* inv_real,
                              void* workspace) {
   moe_status st = check_router(dtype, T, E, k, index_bytes, score, temperature, offsets != nullptr, S);
   if (st != MOE_OK || S == 0) return st;
@@ -119,7 +119,7 @@ moe_status moe_router_losses(int32_t device, void* stream, int32_t dtype, int64_
     with_router_shape(E, [&](auto c) {
       hipLaunchKernelGGL((k_router_losses<decltype(c), D, I>), dim3(p.blocks), dim3(kRouterBlock), 0, s,
                          (router_rows<D, I>(logits, topk_idx, offsets, T, E, k, S, score, temperature)), p.rpb, pq, pc,
-                         pz, pn, lse);
+                         pz, pn);
     });
   });
   if (E % 4 == 0)
@@ -135,12 +135,10 @@ moe_status moe_router_losses(int32_t device, void* stream, int32_t dtype, int64_
 moe_status moe_router_losses_backward(int32_t device, void* stream, int32_t dtype, int64_t T, int32_t E, int32_t k,
                                       int32_t index_bytes, const void* logits, const void* topk_idx, int32_t score,
                                       float temperature, const int32_t* offsets, int64_t S, const float* slope,
-                                      const float* inv_real, const float* lse, const float* d_balance,
-                                      const float* d_z, void* d_logits) {
+                                      const float* inv_real, const float* d_balance, const float* d_z, void* d_logits) {
   moe_status st = check_router(dtype, T, E, k, index_bytes, score, temperature, offsets != nullptr, S);
   if (st != MOE_OK || T == 0) return st;
-  if ((st = check_pointers({logits, d_logits})) != MOE_OK || (st = check_ints({topk_idx}, index_bytes)) != MOE_OK ||
-      (st = check_ints({lse})) != MOE_OK)
+  if ((st = check_pointers({logits, d_logits})) != MOE_OK || (st = check_ints({topk_idx}, index_bytes)) != MOE_OK)
     return st;
   if (S > 0 && (st = check_ints({slope, inv_real})) != MOE_OK) return st;
   if (offsets && (st = check_ints({offsets})) != MOE_OK) return st;
@@ -157,7 +155,7 @@ moe_status moe_router_losses_backward(int32_t device, void* stream, int32_t dtyp
       const int64_t rpb = step * std::max(std::min<int64_t>(4, steps / 1024 + 1), (steps >> 20) + 1);
       hipLaunchKernelGGL((k_router_losses_bwd<C, D, I>), dim3((unsigned)((T + rpb - 1) / rpb)), dim3(kRouterBwdBlock), 0,
                          s, (router_rows<D, I>(logits, topk_idx, offsets, T, E, k, S, score, temperature)), rpb, slope,
-                         inv_real, lse, d_balance, d_z, (D*)d_logits);
+                         inv_real, d_balance, d_z, (D*)d_logits);
     });
   });
   LAUNCH_CHECK();

@@ -506,10 +506,10 @@ def _router(logits, idx, offsets, s, keep):
     L = _lib.load()
     balance, z = logits.new_empty(s.shape, dtype=torch.float32), logits.new_empty(s.shape, dtype=torch.float32)
     counts = logits.new_empty(s.shape + (s.E,), dtype=torch.int32)
-    # one allocation for what a backward reads: slope, inv_real and lse
-    kept, at = None, (None, None, None)
+    # one allocation for what a backward reads: slope and inv_real
+    kept, at = None, (None, None)
     if keep:
-        kept = logits.new_empty(s.S * (s.E + 1) + s.T, dtype=torch.float32)
+        kept = logits.new_empty(s.S * (s.E + 1), dtype=torch.float32)
         at = _kept_of_router(kept, s)
     ws = _workspace(L.moe_router_losses_workspace_bytes(s.T, s.E, s.S), logits)
     _call(L.moe_router_losses, logits.get_device(), _dtype_code(logits.dtype), s.T, s.E, s.k, idx.element_size(),
@@ -520,7 +520,7 @@ def _router(logits, idx, offsets, s, keep):
 
 def _kept_of_router(kept, s):
     at = kept.data_ptr()
-    return at, at + 4 * s.S * s.E, at + 4 * s.S * (s.E + 1)
+    return at, at + 4 * s.S * s.E
 
 
 class _RouterLosses(torch.autograd.Function):

@@ -375,7 +375,6 @@ pub mod ffi {
             counts: *mut i32,
             slope: *mut f32,
             inv_real: *mut f32,
-            lse: *mut f32,
             workspace: *mut c_void,
         ) -> MoeStatus;
         pub fn moe_router_losses_backward(
@@ -394,7 +393,6 @@ pub mod ffi {
             num_sequences: i64,
             slope: *const f32,
             inv_real: *const f32,
-            lse: *const f32,
             d_balance: *const f32,
             d_z: *const f32,
             d_logits: *mut c_void,

@@ -125,6 +125,39 @@ def test_masked_experts(score, fill):
         assert torch.equal(out.balance, same.balance) and torch.equal(out.z, same.z)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("at", [32.0, 2.0 ** 15, -2.0 ** 15])
+def test_a_softmax_does_not_depend_on_a_rows_level(at, dtype):
+    # logits of few bits: x + at is exact, so each x less the largest is the same number, and so are all results but lse's
+    idx = problem(300, 48, 3, 8)[1]
+    step = 2.0 ** -4 if dtype == F32 else 2.0 ** (-2 if at == 32.0 else 8)
+    x = torch.randint(-4, 4, (300, 48), device="cuda", generator=gen(8)).double() * step
+    out = []
+    for level in (0.0, at):
+        logits = (x + level).to(dtype)
+        assert torch.equal(logits.double(), x + level)
+        logits.requires_grad_()
+        balance = ops.router_losses(logits, idx).balance
+        out.append((balance.detach(), torch.autograd.grad(balance, logits)[0]))
+    assert torch.equal(out[0][0], out[1][0]) and torch.equal(out[0][1], out[1][1])
+
+
+def test_rows_masked_whole_by_the_lowest_value():
+    logits, idx = problem(90, 24, 2, 9, pad=0.0)
+    logits[::3] = torch.finfo(F32).min
+    ref = logits.double().requires_grad_()
+    real = ((idx >= 0) & (idx < 24)).any(1)
+    P = torch.softmax(ref, 1)[real].mean(0)
+    f = torch.bincount(idx[(idx >= 0) & (idx < 24)].long(), minlength=24) / (2 * real.sum().double())
+    want, = torch.autograd.grad(24 * (f * P + P * P).sum(), ref)
+    x = logits.requires_grad_()
+    got, = torch.autograd.grad(ops.router_losses(x, idx).balance, x)
+    # g_e and its mean over p: some 200 roundings of what is at most max |g|
+    n = float(real.sum())
+    assert bool(((got.double() - want).abs() <= 200 * 2.0 ** -24 * float(24 * (f + 2 * P).max()) / n).all())
+    assert float(want[::3].abs().max()) > 1e-4
+
+
 def test_nothing_real():
     for T in (0, 1, 70):
         logits = torch.full((T, 24), float("nan"), device="cuda").requires_grad_()

@@ -98,10 +98,10 @@ def test_c_entries_refuse_before_any_device_call():
 
     def losses(T=4, E=6, k=2, nbytes=4, dtype=F32, x=P, idx=P, score=0, tau=1.0, off=None, S=1, out=P, ws=P):
         return L.moe_router_losses(0, None, dtype, T, E, k, nbytes, x, idx, score, tau, 1.0, 1.0, off, S, out, P, P, None,
-                                   None, None, ws)
+                                   None, ws)
 
     def losses_bwd(T=4, E=6, k=2, nbytes=4, dtype=F32, x=P, idx=P, score=0, tau=1.0, off=None, S=1, out=P):
-        return L.moe_router_losses_backward(0, None, dtype, T, E, k, nbytes, x, idx, score, tau, off, S, P, P, P, P, P, out)
+        return L.moe_router_losses_backward(0, None, dtype, T, E, k, nbytes, x, idx, score, tau, off, S, P, P, P, P, out)
     for f in (losses, losses_bwd):
         assert status(f(T=-1), "num_tokens") == 1
         assert status(f(T=2 ** 31), "num_tokens") == 1
