@@ -386,7 +386,7 @@ __global__ __launch_bounds__(C::THREADS) void k_mx_dgrad(const bf16_t* __restric
 // loads, swizzles and fragments of gemm.hpp serve as they are, over rows of K / 4 two-byte units.
 // v_mfma_scale_f32_32x32x64_f8f6f4 takes such a vector of each operand and a scale for each.  Half h of a
 // wave reads vector 4 h + ks in k-step ks of a k-tile instead of 2 ks + h: its four scales of a row are then one dword,
-// of which step ks takes byte ks (2 h + ks and two of them where k-tiles are half as deep).
+// of which step ks takes byte ks.
 MOE_DEV void mfma_mx(f32x16& acc, u32x4 bt, u32x4 at, uint32_t sb, uint32_t sa, int ks) {
   typedef int i32x8 __attribute__((ext_vector_type(8)));
   const i32x8 b = {(int)bt.x, (int)bt.y, (int)bt.z, (int)bt.w, 0, 0, 0, 0};
@@ -400,8 +400,8 @@ MOE_DEV void mfma_mx(f32x16& acc, u32x4 bt, u32x4 at, uint32_t sb, uint32_t sa, 
 }
 
 // The scales of a tile's rows (BM of x, then BN of the weight), through registers: a thread loads 16 of each of its
-// rows at once, those of LT k-tiles (rows of K / 32 bytes have any alignment, and a k-tile's few bytes of a cache line
-// would fetch each line many times), and writes a k-tile's, W dwords, to LDS.  No branch is between a load and its
+// rows at once, those of two k-tiles (rows of K / 32 bytes have any alignment, and a k-tile's few bytes of a cache line
+// would fetch each line many times), and writes a k-tile's, eight, to LDS.  No branch is between a load and its
 // use, or it would be waited for at once: a load that would leave the tensor (its last 15 bytes) is moved back into it and
 // shifted, and what is not the row's is masked.  A wave's 64 rows are all of one operand's, so its base is scalar.
 // Both tensors hold 16 bytes at least.
@@ -409,9 +409,8 @@ template <class C>
 struct MxScaleStager {
   static constexpr int ROWS = C::BM + C::BN;
   static constexpr int PER = (ROWS + C::THREADS - 1) / C::THREADS;
-  static constexpr int W = C::BK / C::V / 4, LT = 4 / W;
   static_assert(C::BM % 64 == 0 && C::BN % 64 == 0, "a wave's rows are of one operand");
-  static_assert(W == 1 || W == 2, "four or eight vectors to a k-tile's row");
+  static_assert(C::BK == 8 * C::V, "eight blocks to a k-tile's row");
   const __attribute__((address_space(1))) uint8_t* base[PER];
   uint32_t last[PER];   // the last 16 bytes of the tensor, from base
   uint32_t row[PER];    // the thread's row, from base
@@ -444,9 +443,9 @@ struct MxScaleStager {
       s[i] = *(const __attribute__((address_space(1))) any_u32x4*)(base[i] + (int64_t)min((int)(row[i] + at), (int)last[i]));
     }
   }
-  // the scales of k-tile kt, the (kt % LT)-th of the load
+  // the scales of k-tile kt, the load's first half or (kt odd) its second
   MOE_DEV void write(uint32_t* tile, int kt) const {
-    const int j = kt % LT, left = bytes - at;
+    const int j = kt & 1, left = bytes - at - 8 * j;  // bytes of the row from here
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int r = threadIdx.x + i * C::THREADS;
@@ -463,11 +462,11 @@ struct MxScaleStager {
       }
       const bool in = valid >> i & 1;
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        uint32_t q = W == 2 ? (j ? (w ? v.w : v.z) : (w ? v.y : v.x)) : j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w;
-        const int n = left - 4 * (j * W + w);  // bytes of the row from here
+      for (int w = 0; w < 2; ++w) {
+        uint32_t q = w ? (j ? v.w : v.y) : (j ? v.z : v.x);
+        const int n = left - 4 * w;
         q &= n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1;
-        tile[r * W + w] = in ? q : 0u;
+        tile[2 * r + w] = in ? q : 0u;
       }
     }
   }
@@ -480,7 +479,7 @@ MOE_DEV void mainloop_mxmx(f32x16 (&acc)[1][C::TN][C::TM], const OpDesc<bf16_t>&
                            MxScaleStager<C>& ss, int K4, bf16_t* smem, uint32_t* scales) {
   using T = bf16_t;
   constexpr int TILE_A = C::BM * C::BK, TILE_B = C::BN * C::BK, STAGE = TILE_A + TILE_B;
-  constexpr int NST = C::NST, W = MxScaleStager<C>::W, LT = MxScaleStager<C>::LT, ROWS = MxScaleStager<C>::ROWS;
+  constexpr int NST = C::NST, ROWS = MxScaleStager<C>::ROWS;
   static_assert(C::XR == 0, "no tall tiles");
   using SA = DmaStager<C, T, C::BM>;
   using SB = DmaStager<C, T, C::BN>;
@@ -494,7 +493,7 @@ MOE_DEV void mainloop_mxmx(f32x16 (&acc)[1][C::TN][C::TM], const OpDesc<bf16_t>&
   sa.init(a, threadIdx.x);
   sb.init(b, threadIdx.x);
   auto stage = [&](int kt) { return smem + (NST == 2 ? (kt & 1) : kt % NST) * STAGE; };
-  auto scales_of = [&](int kt) { return scales + (kt & 1) * ROWS * W; };
+  auto scales_of = [&](int kt) { return scales + (kt & 1) * ROWS * 2; };
   auto issue = [&](int kt, int i) {
     if (i < SA::PER) sa.issue_one(stage(kt), i, kt * C::BK, kt < nk);
     else sb.issue_one(stage(kt) + TILE_A, i - SA::PER, kt * C::BK, kt < nk);
@@ -506,15 +505,14 @@ MOE_DEV void mainloop_mxmx(f32x16 (&acc)[1][C::TN][C::TM], const OpDesc<bf16_t>&
   ss.load(0);
   ss.write(scales_of(0), 0);
   constexpr int KSTEPS = C::BK / (2 * C::V), M = KSTEPS - 1;
-  static_assert(KSTEPS == 2 * W, "a lane's scales: two or four neighbours");
+  static_assert(KSTEPS == 4, "a lane's scales of a row: a dword");
   const int frag_row = lane & 31, half = lane >> 5;
   // one set of fragments of the weight: each is read again for the next k-step behind its last MFMA (two sets of both
   // operands spill beside the scales)
   u32x4 af[2][C::TM], bfr[C::TN];
   uint32_t as[C::TM], bs[C::TN];
   auto read_scales = [&](int kt) {
-    typedef typename std::conditional<W == 2, uint32_t, uint16_t>::type S;
-    const S* t = reinterpret_cast<const S*>(scales_of(kt)) + half;
+    const uint32_t* t = scales_of(kt) + half;
 #pragma unroll
     for (int tm = 0; tm < C::TM; ++tm) as[tm] = t[2 * (wm * C::WM + tm * 32 + frag_row)];
 #pragma unroll
@@ -539,7 +537,7 @@ MOE_DEV void mainloop_mxmx(f32x16 (&acc)[1][C::TN][C::TM], const OpDesc<bf16_t>&
   do {
     // the next k-tile's scales, of a load that ended before this k-tile or began with the one before it
     ss.write(scales_of(kt + 1), kt + 1);
-    if ((kt + 2) % LT == 0) ss.load((kt + 2) * (C::BK / C::V));
+    if ((kt & 1) == 0) ss.load((kt + 2) * (C::BK / C::V));
     auto products = [&](int ks, int tn) {
 #pragma unroll
       for (int tm = 0; tm < C::TM; ++tm) mfma_mx(acc[0][tn][tm], bfr[tn], af[ks & 1][tm], bs[tn], as[tm], ks);
@@ -586,7 +584,7 @@ template <class C, typename T>
 __global__ __launch_bounds__(C::THREADS, 2) void k_mxmx_fwd(const uint8_t* __restrict__ X, const uint8_t* __restrict__ XS,
                                                          MxRows r, int tiles, MxWeights w, LinearEpi<T> epi) {
   __shared__ __align__(16) bf16_t smem[mx_smem_elems<C>()];
-  __shared__ uint32_t scales[2 * (C::BM + C::BN) * MxScaleStager<C>::W];
+  __shared__ uint32_t scales[2 * (C::BM + C::BN) * 2];
   if (mx_no_group(r, tiles, epi, C::THREADS)) return;
   int grp, row0, mv, n0;
   const int N = w.N, K = w.K, K4 = K / 4;
