@@ -540,22 +540,9 @@ __global__ __launch_bounds__(256) void k_linear_skinny(const T* __restrict__ X,
 constexpr int kDzRows = kF32RowTile;  // rows of a chunk: the prefix of 64-row tiles counts them
 constexpr int kDzCols = 64;
 template <typename T>
-__global__ __launch_bounds__(256) void k_linear_dz(const T* __restrict__ dY,
-                                                   const T* __restrict__ pre, int act, RowGroups g,
-                                                   int N, T* __restrict__ dZ,
-                                                   float* __restrict__ part) {
+MOE_DEV void dz_chunk(const T* __restrict__ dY, const T* __restrict__ pre, int act, int chunk, int r0, int rows, int N,
+                      T* __restrict__ dZ, float* __restrict__ part) {
   __shared__ float col[32][kDzCols];
-  int r0, rows;
-  const int chunk = blockIdx.x;
-  if (g.offsets) {
-    if (chunk >= g.tile_prefix[g.G]) return;
-    const int grp = uni(find_group(g.tile_prefix, g.G, chunk));
-    r0 = g.offsets[grp] + (chunk - g.tile_prefix[grp]) * kDzRows;
-    rows = min(kDzRows, g.offsets[grp + 1] - r0);
-  } else {
-    r0 = chunk * kDzRows;
-    rows = min(kDzRows, g.M - r0);
-  }
   const int rl = threadIdx.x >> 3, c8 = (threadIdx.x & 7) * 8;
   const int n = blockIdx.y * kDzCols + c8;
   float d[2][8], z[2][8], s[8];
@@ -589,16 +576,30 @@ __global__ __launch_bounds__(256) void k_linear_dz(const T* __restrict__ dY,
   for (int r = 0; r < 32; ++r) t += col[r][threadIdx.x];
   part[(int64_t)chunk * N + cc] = t;
 }
+template <typename T>
+__global__ __launch_bounds__(256) void k_linear_dz(const T* __restrict__ dY,
+                                                   const T* __restrict__ pre, int act, RowGroups g,
+                                                   int N, T* __restrict__ dZ,
+                                                   float* __restrict__ part) {
+  int r0, rows;
+  const int chunk = blockIdx.x;
+  if (g.offsets) {
+    if (chunk >= g.tile_prefix[g.G]) return;
+    const int grp = uni(find_group(g.tile_prefix, g.G, chunk));
+    r0 = g.offsets[grp] + (chunk - g.tile_prefix[grp]) * kDzRows;
+    rows = min(kDzRows, g.offsets[grp + 1] - r0);
+  } else {
+    r0 = chunk * kDzRows;
+    rows = min(kDzRows, g.M - r0);
+  }
+  dz_chunk(dY, pre, act, chunk, r0, rows, N, dZ, part);
+}
 
 // db[g] = the sum of group g's chunks, in order (zeros for a group without rows).
 // Block (group, 64 columns): four row lanes of 64 columns each.
 template <typename T>
-__global__ __launch_bounds__(256) void k_linear_db(const float* __restrict__ part, RowGroups g,
-                                                   int N, T* __restrict__ db) {
+MOE_DEV void db_columns(const float* __restrict__ part, int grp, int p0, int p1, int N, T* __restrict__ db) {
   __shared__ float col[4][64];
-  const int grp = blockIdx.y;
-  const int p0 = g.offsets ? g.tile_prefix[grp] : 0;
-  const int p1 = g.offsets ? g.tile_prefix[grp + 1] : (g.M + kDzRows - 1) / kDzRows;
   const int n = blockIdx.x * 64 + (threadIdx.x & 63), rl = threadIdx.x >> 6;
   float s = 0.0f;
   if (n < N) {
@@ -610,6 +611,14 @@ __global__ __launch_bounds__(256) void k_linear_db(const float* __restrict__ par
   if (rl != 0 || n >= N) return;
   db[(int64_t)grp * N + n] =
       from_f<T>((col[0][n & 63] + col[1][n & 63]) + (col[2][n & 63] + col[3][n & 63]));
+}
+template <typename T>
+__global__ __launch_bounds__(256) void k_linear_db(const float* __restrict__ part, RowGroups g,
+                                                   int N, T* __restrict__ db) {
+  const int grp = blockIdx.y;
+  const int p0 = g.offsets ? g.tile_prefix[grp] : 0;
+  const int p1 = g.offsets ? g.tile_prefix[grp + 1] : (g.M + kDzRows - 1) / kDzRows;
+  db_columns(part, grp, p0, p1, N, db);
 }
 
 }  // namespace moe

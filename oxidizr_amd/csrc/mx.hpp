@@ -93,62 +93,93 @@ struct MxRows {
   int G, M;
 };
 
+// Block blk's part of n tiles of BM rows, dealt over the XCDs as xcd_slot does.  An XCD's 32 CUs take 32 tiles of 256 rows at
+// once; where the tiles behind its last full 32 are few, each is cut into two or four parts of as many rows, for the
+// CUs that would stand by.
+MOE_DEV int mx_parts(int tail) { return tail <= 8 ? 4 : tail <= 16 ? 2 : 1; }
+template <int BM>
+MOE_DEV bool mx_slot(int blk, int n, int& id, int& part, int& parts) {
+  part = 0;
+  parts = 1;
+  if constexpr (BM != 256) return xcd_slot(blk, n, id);
+  const int x = blk & 7, j = blk >> 3, q = n >> 3, r = n & 7;
+  const int mine = q + (x < r ? 1 : 0), full = mine & ~31, tail = mine - full;
+  id = x * q + min(x, r) + j;
+  if (j < full) return true;
+  parts = mx_parts(tail);
+  const int t = j - full;
+  if (t >= tail * parts) return false;
+  id += t / parts - t;
+  part = t % parts;
+  return true;
+}
+
+// Row tiles of BM rows of a launch's groups, numbered group by group as resolve_rows has them, but from the offsets alone:
+// lane l counts those of groups l G / 64 .., a prefix sum over the lanes gives their number and the lane that holds a tile's
+// group, so a grouped call needs no launch before it (a kernel that writes prefixes takes 6 us, and finding a group in them
+// log2(G) loads one after another).  Offsets are clamped to 0 .. M and each group's end to its start: whatever they hold, a
+// tile's rows exist.
+template <int BM>
+struct MxTileScan {
+  MxRows r;
+  int per, n, incl, total;
+  MOE_DEV explicit MxTileScan(const MxRows& rows) : r(rows), per((rows.G + 63) >> 6), n(0) {
+    const int l = threadIdx.x & 63;
+    for (int i = 0; i < per; ++i) {
+      int a, b;
+      if (l * per + i < r.G) n += range(l * per + i, a, b);
+    }
+    incl = wave_incl_scan(n);
+    total = __builtin_amdgcn_readlane(incl, 63);
+  }
+  MOE_DEV int range(int e, int& a, int& b) const {  // its tiles
+    a = min(max(r.offsets[e], 0), r.M);
+    b = min(max(r.offsets[e + 1], a), r.M);
+    return (b - a + BM - 1) / BM;
+  }
+  // Walks lane l's groups until f(group, its first tile, its tiles, first row, end) is true.
+  template <class F>
+  MOE_DEV void walk(int l, F&& f) const {
+    int first = __builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(n, l);
+    for (int i = 0; i < per && l * per + i < r.G; ++i) {
+      int a, b;
+      const int c = uni(range(l * per + i, a, b));
+      if (f(l * per + i, first, c, uni(a), uni(b))) return;
+      first += c;
+    }
+  }
+  MOE_DEV int lane_of(int tile) const { return __ffsll((unsigned long long)__ballot(incl > tile)) - 1; }  // tile < total
+};
+
 // The tile of block blk of a launch with N output columns: group, first row, rows and first column, or false for a
-// block past the tiles.  Group by group, as resolve_rows has them, but from the offsets alone: lane l counts the
-// row tiles of groups l G / 64 .., a prefix sum over the lanes gives their number and the lane that holds the
-// block's, so a grouped call needs no launch before it (a kernel that writes prefixes takes 6 us, and finding a
-// group in them log2(G) loads one after another).  Offsets are clamped to 0 .. M and each group's end to its
-// start: whatever they hold, a tile's rows exist.
+// block past the tiles.
 template <int BM, int BN>
 MOE_DEV bool mx_tile(const MxRows& r, int N, int blk, int& grp, int& row0, int& mv, int& n0) {
   const int nN = (N + BN - 1) / BN;
-  int id, mt, nt;
+  int id, mt, nt, part, parts;
+  auto rows = [&](int first, int end) {  // the part's rows of a tile
+    row0 = first + mt * BM + part * (BM / parts);
+    mv = min(BM / parts, end - row0);
+    n0 = nt * BN;
+    return mv > 0;
+  };
   if (r.offsets == nullptr) {
     const int nM = (r.M + BM - 1) / BM;
-    if (!xcd_slot(blk, nM * nN, id) || !tile_order(id, nM, nN, mt, nt)) return false;
+    if (!mx_slot<BM>(blk, nM * nN, id, part, parts) || !tile_order(id, nM, nN, mt, nt)) return false;
     grp = 0;
-    row0 = mt * BM;
-    mv = min(BM, r.M - row0);
-    n0 = nt * BN;
-    return true;
+    return rows(0, r.M);
   }
-  const int lane = threadIdx.x & 63, per = (r.G + 63) >> 6;
-  auto range = [&](int e, int& a, int& b) {
-    a = min(max(r.offsets[e], 0), r.M);
-    b = min(max(r.offsets[e + 1], a), r.M);
-  };
-  int n = 0;
-  for (int i = 0; i < per; ++i) {
-    int a, b;
-    if (lane * per + i < r.G) {
-      range(lane * per + i, a, b);
-      n += (b - a + BM - 1) / BM;
-    }
-  }
-  const int incl = wave_incl_scan(n);
-  const int total = __builtin_amdgcn_readlane(incl, 63);
-  if (!xcd_slot(blk, total * nN, id)) return false;
+  const MxTileScan<BM> scan(r);
+  if (!mx_slot<BM>(blk, scan.total * nN, id, part, parts)) return false;
   const int s = uni(id / nN);
-  const int l = __ffsll((unsigned long long)__ballot(incl > s)) - 1;
-  int first = __builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(n, l);
-  for (int i = 0; i < per; ++i) {  // the groups of lane l, walked by every lane
-    int a, b;
-    if (l * per + i >= r.G) break;
-    range(l * per + i, a, b);
-    a = uni(a);
-    b = uni(b);
-    const int c = (b - a + BM - 1) / BM;
-    if (s < first + c) {
-      if (!tile_order<kRowWalk>(id - first * nN, c, nN, mt, nt)) return false;
-      grp = l * per + i;
-      row0 = a + mt * BM;
-      mv = min(BM, b - row0);
-      n0 = nt * BN;
-      return true;
-    }
-    first += c;
-  }
-  return false;
+  bool found = false;
+  scan.walk(scan.lane_of(s), [&](int e, int first, int c, int a, int b) {
+    if (s >= first + c) return false;
+    grp = e;
+    found = tile_order<kRowWalk>(id - first * nN, c, nN, mt, nt) && rows(a, b);
+    return true;
+  });
+  return found;
 }
 
 // body(tiling): a BM/4- or BM/2-row tiling when that covers the mv valid rows, else the half-width tiling when at most
@@ -379,6 +410,39 @@ __global__ __launch_bounds__(C::THREADS) void k_mx_dgrad(const bf16_t* __restric
       store8_stream(dX + ((int64_t)row0 + m) * K + k0 + n, v[0]);
     });
   });
+}
+
+// The element-wise part of a backward, as k_linear_dz and k_linear_db, their chunks found from the offsets: 12000 rows of
+// 1368 in 12 groups 22 us and 4.8, where prefixes from a launch before them made 18 and 4.7 and cost 5.2 and a gap (the whole forward
+// and backward 188 -> 176).  Bound by reading dy and z and writing dz, 98 MB.  chunks: those that `part` holds.
+static __global__ __launch_bounds__(256) void k_mx_dz(const bf16_t* __restrict__ dY, const bf16_t* __restrict__ pre, int act,
+                                                      MxRows r, int N, bf16_t* __restrict__ dZ, float* __restrict__ part) {
+  const int chunk = blockIdx.x;
+  if (!r.offsets) return dz_chunk(dY, pre, act, chunk, chunk * kDzRows, min(kDzRows, r.M - chunk * kDzRows), N, dZ, part);
+  const MxTileScan<kDzRows> scan(r);
+  if (chunk >= scan.total) return;
+  int r0 = 0, rows = 0;
+  scan.walk(scan.lane_of(chunk), [&](int, int first, int c, int a, int b) {
+    if (chunk >= first + c) return false;
+    r0 = a + (chunk - first) * kDzRows;
+    rows = min(kDzRows, b - r0);
+    return true;
+  });
+  dz_chunk(dY, pre, act, chunk, r0, rows, N, dZ, part);
+}
+static __global__ __launch_bounds__(256) void k_mx_db(const float* __restrict__ part, MxRows r, int chunks, int N,
+                                                      bf16_t* __restrict__ db) {
+  const int grp = blockIdx.y;
+  int p0 = 0, p1 = chunks;
+  if (r.offsets) {
+    const MxTileScan<kDzRows> scan(r);
+    scan.walk(grp / scan.per, [&](int e, int first, int c, int, int) {
+      p0 = min(first, chunks);
+      p1 = min(first + c, chunks);
+      return e == grp;
+    });
+  }
+  db_columns(part, grp, p0, p1, N, db);
 }
 
 // ------------------------------------------------------------------ tiled products, both sides in 4 bits
@@ -614,8 +678,11 @@ __global__ __launch_bounds__(C::THREADS, 2) void k_mxmx_fwd(const uint8_t* __res
 // too many, 20 to 100 % longer).  Lane l supplies block l / 16 + 4 q of weight row l % 16 in load q, so four lanes read
 // 64 contiguous bytes; it loads the 16 scales of its row at once, of which its blocks' are the bytes l / 16 of each dword (a
 // load for each: 10 % longer).
-// bf16 rows: the block becomes four 8-element vectors, multiplied with the four of the token row by 16 x 16 x 32 MFMAs.
-// 4-bit rows: one 16 x 16 x 128 scaled MFMA.
+// bf16 rows: the block becomes four 8-element vectors, multiplied with the four of the token row by 16 x 16 x 32 MFMAs; the row's
+// next four are requested before (3 %).  4-bit rows: one 16 x 16 x 128 scaled MFMA.
+// Bound by HBM where the weights outgrow the caches: 512 rows in 128 experts of 1536 x 4096 (428 MB) 96 us over bf16 rows (4.5 TB/s;
+// each workgroup also reads 128 KB of rows from L2) and 76 over 4-bit ones (5.6; with the nontemporal hint on the weights 106 and 91);
+// 64 rows in them 44 and 30.  Bound by a launch and one chain of loads otherwise: one row of 4096 x 4096 4.5 and 4.0.
 
 constexpr int kMxSkinnyRows = 16;
 constexpr int kMxChunkLoads = 4;  // of 128 elements
@@ -638,7 +705,6 @@ __global__ __launch_bounds__(256) void k_mx_skinny(const void* __restrict__ X, c
                                                    const int* __restrict__ offsets, int E, int M, int nslot,
                                                    MxWeights w, LinearEpi<T> epi) {
   constexpr int RB = 4 / KS, ROWS = 16 * RW, Q = kMxChunkLoads, KC = 128 * Q;
-  constexpr int XQ = RW == 4 ? 1 : 2;  // loads of the weight that are multiplied with theirs of the rows at once
   typedef int i32x8 __attribute__((ext_vector_type(8)));
   __shared__ f32x4 red[(KS - 1) * RB * RW * 64];
   const int N = w.N, K = w.K;
@@ -707,25 +773,24 @@ __global__ __launch_bounds__(256) void k_mx_skinny(const void* __restrict__ X, c
           }
         }
       } else {
+        u32x4 xa[2][4];  // the rows of one load of the weight, and of the next, requested before that is multiplied
+        auto load_x = [&](int q) {
+          const bool in = FULL || 4 * q + g < left;
 #pragma unroll
-        for (int h = 0; h < Q; h += XQ) {
-          u32x4 xa[XQ][4];
+          for (int v = 0; v < 4; ++v) xa[q & 1][v] = buf_ld16(rx, in ? vx + 256 * q + 16 * v : kOobOffset, (uint32_t)b0 * 64);
+          __builtin_amdgcn_sched_barrier(0);
+        };
+        load_x(0);
 #pragma unroll
-          for (int q = 0; q < XQ; ++q) {
-            const bool in = FULL || 4 * (h + q) + g < left;
+        for (int q = 0; q < Q; ++q) {
+          if (q + 1 < Q) load_x(q + 1);
 #pragma unroll
-            for (int v = 0; v < 4; ++v)
-              xa[q][v] = buf_ld16(rx, in ? vx + 256 * (h + q) + 16 * v : kOobOffset, (uint32_t)b0 * 64);
+          for (int i = 0; i < RW; ++i) {
+            const float s = mx_scale(ws[i][q] & 255u);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) mfma16(acc[i], xa[q & 1][v], mx_bf16x8(wa[i][q][v], s));
           }
           __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int q = 0; q < XQ; ++q)
-#pragma unroll
-            for (int i = 0; i < RW; ++i) {
-              const float s = mx_scale(ws[i][h + q] & 255u);
-#pragma unroll
-              for (int v = 0; v < 4; ++v) mfma16(acc[i], xa[q][v], mx_bf16x8(wa[i][h + q][v], s));
-            }
         }
       }
     };

@@ -83,20 +83,23 @@ bool mx_skinny(bool four, int64_t M, int K, int N, int E, bool grouped) {
   return grouped ? M <= (four ? 7 : 20) * std::min<int64_t>(E, M) : M <= (four ? 80 : 160);
 }
 
-// Row tiles by height, by their cost in tenths of a full round of 256-row tiles.  us, 256 / 128 / 64 rows, over bf16 rows: 16384 rows
-// in 16 experts, 2048 -> 1408 106 / 118 / 152; 65536 in 128, 4096 -> 1536 865 / 1051 / 1382; 12000 in 12, 1376 -> 1368 82 / 77 / 82;
-// 8192 in 64, 2048 -> 1408 85 / 86 / 89; 2048 in 16 44 / 27 / 26; 1999 of one weight, 2784 -> 2056 57 / 46 / 56; 512 of 4096 -> 4096
-// 81 / 45 / 35; their input gradients 118 / 127 / 177, 909 / 1129 / 1559, 77 / 73 / 97, 92 / 83 / 106, 38 / 30 / 37, 52 / 40 / 51, 96 /
-// 53 / 42; both sides in 4 bits 48 / 50 / 65, 343 / 404 / 569, 51 / 48 / 44, 40 / 39 / 43, 20 / 14 / 13, 27 / 21 / 25, 30 / 17 / 18.
+// Row tiles by height, by their cost in tenths of a full round of 256-row tiles; the tiles behind the last full round are cut
+// (mx_slot).  us, 256 / 128 / 64 rows, over bf16 rows: 16384 rows in 16 experts, 2048 -> 1408 102 / 112 / 146; 65536 in 128, 4096 ->
+// 1536 840 / 1028 / 1344; 12000 in 12, 1376 -> 1368 70 / 74 / 81 (uncut 82); 8192 in 64, 2048 -> 1408 85 / 86 / 88; 2048 in 16 32 / 27 /
+// 26 (44); 1999 of one weight, 2784 -> 2056 45 / 48 / 56 (57); 512 of 4096 -> 4096 50 / 45 / 35 (80); 1024 60 / 50 / 52 (81); their input
+// gradients 115 / 133 / 181 (120), 893 / 1107 / 1561, 66 / 75 / 98 (78), 92 / 83 / 107, 38 / 29 / 40, 42 / 38 / 59 (53), 65 / 54 / 43
+// (96), 66 / 54 / 59 (96).  Both sides in 4 bits 44 / 45 / 62, 343 / 402 / 571, 46 / 48 / 44 (51), 40 / 40 / 43, 16 / 14 / 13 (20), 22 / 21 / 25 (26), 18 / 17 / 18 (29), 20 / 22 /
+// 21 (31).
 enum class MxTiles { kBig, kMid, kSmall };
-MxTiles mx_tiles(bool grouped, int E, int64_t M, int N) {
+MxTiles mx_tiles(bool four, bool grouped, int E, int64_t M, int N) {
   const int groups = grouped ? (int)std::min<int64_t>(E, M) : 1;
   auto count = [&](int bm, int bn) {
     return (grouped ? group_row_tiles(groups, (double)M / groups, bm) : (double)ceil_div(M, bm)) * ceil_div(N, bn);
   };
-  const double tiles = count(256, 256), big = tiles <= 128.0 ? 7.5 : big_cost(tiles, 10.0);
-  const double mid = round_cost(count(128, 128), {4.2, 7.0});
-  const double small = round_cost(count(64, 128), {3.0, 4.9});
+  const double tiles = count(256, 256), full = std::floor(tiles / 256.0), rest = tiles - 256.0 * full;
+  const double big = 10.0 * full + (rest <= 0.0 ? 0.0 : rest <= 64.0 ? (four ? 4.6 : 5.6) : rest <= 128.0 ? 7.2 : 10.0);
+  const double mid = round_cost(count(128, 128), four ? TileCost{5.0, 5.9} : TileCost{4.2, 7.0});
+  const double small = round_cost(count(64, 128), four ? TileCost{4.2, 4.6} : TileCost{3.0, 4.9});
   return big <= std::min(mid, small) ? MxTiles::kBig : mid <= small ? MxTiles::kMid : MxTiles::kSmall;
 }
 template <class F>
@@ -108,8 +111,8 @@ void with_mx_tiling(MxTiles kind, F&& f) {
 // Blocks of tiles, and behind them (grouped) those for the rows of no group.
 template <class C>
 int64_t mx_tile_blocks(bool grouped, int E, int64_t M, int N) {
-  if (!grouped) return (int64_t)ceil_div(M, C::BM) * ceil_div(N, C::BN);
-  return ((int64_t)(ceil_div(M, C::BM) + E) * ceil_div(N, C::BN) + 7) / 8 * 8;
+  const int64_t xcd = ((int64_t)(ceil_div(M, C::BM) + (grouped ? E : 0)) * ceil_div(N, C::BN) + 7) / 8;  // tiles of one, at most
+  return 8 * (C::BM == 256 ? xcd / 32 * 32 + 32 : xcd);  // mx_slot: parts behind the last full 32
 }
 moe_status check_mx_tiles(MxTiles kind, bool grouped, int E, int64_t M, int N) {
   moe_status st = MOE_OK;
@@ -120,8 +123,8 @@ moe_status check_mx_tiles(MxTiles kind, bool grouped, int E, int64_t M, int N) {
   return st;
 }
 moe_status check_mx_launches(bool backward, bool four, bool grouped, int E, int64_t M, int K, int N) {
-  if (backward) return check_mx_tiles(mx_tiles(grouped, E, M, K), grouped, E, M, K);
-  return mx_skinny(four, M, K, N, E, grouped) ? MOE_OK : check_mx_tiles(mx_tiles(grouped, E, M, N), grouped, E, M, N);
+  if (backward) return check_mx_tiles(mx_tiles(false, grouped, E, M, K), grouped, E, M, K);
+  return mx_skinny(four, M, K, N, E, grouped) ? MOE_OK : check_mx_tiles(mx_tiles(four, grouped, E, M, N), grouped, E, M, N);
 }
 // Calls f(tiling, blocks of tiles, grid).
 template <class F>
@@ -133,19 +136,14 @@ void with_mx_launch(MxTiles kind, const MxRows& r, int N, F&& f) {
   });
 }
 
-// Scratch of a backward: dz, and k_linear_dz's chunks.
+// Scratch of a backward: dz, and the chunks' sums of it.
 struct MxWs {
-  size_t offs, prefixes, w_tab, dz, part, total;
+  size_t dz, part, total;
 };
 int64_t mx_dz_chunks(int64_t M, int E, bool grouped) { return (M + kDzRows - 1) / kDzRows + (grouped ? E : 0); }
 MxWs mx_ws(int64_t M, int N, int E, bool grouped, int act) {
   MxWs w{};
   Carve c;
-  if (grouped) {
-    w.offs = c.take((size_t)(E + 1) * 4);
-    w.prefixes = c.take((size_t)kNumTilePrefixes * (E + 1) * 4);
-    w.w_tab = c.take((size_t)E * sizeof(void*));
-  }
   if (act != kActNone) w.dz = c.take((size_t)M * N * 2);
   w.part = c.take((size_t)mx_dz_chunks(M, E, grouped) * N * 4);
   w.total = c.off;
@@ -169,7 +167,7 @@ moe_status mx_forward(hipStream_t s, int64_t M, int E, const int* offsets, const
     return MOE_OK;
   }
   const MxRows r{offsets, E, (int)M};
-  with_mx_launch(mx_tiles(grouped, E, M, N), r, N, [&](auto c, int tiles, dim3 grid) {
+  with_mx_launch(mx_tiles(X4, grouped, E, M, N), r, N, [&](auto c, int tiles, dim3 grid) {
     using C = decltype(c);
     if constexpr (X4)
       hipLaunchKernelGGL((k_mxmx_fwd<C, T>), grid, dim3(C::THREADS), 0, s, (const uint8_t*)x, xs, r, tiles, w, epi);
@@ -188,24 +186,15 @@ moe_status mx_backward(hipStream_t s, int64_t M, int E, const int* offsets, cons
   const MxRows r{offsets, E, (int)M};
   const bf16_t* dz = dy;
   if (act != kActNone || db) {
-    int* offs = grouped ? (int*)(ws + L.offs) : nullptr;
-    int* prefixes = grouped ? (int*)(ws + L.prefixes) : nullptr;
-    if (grouped)  // the prefix of 64-row chunks; nothing to fill
-      hipLaunchKernelGGL(k_linear_prep<bf16_t>, dim3(1), dim3(1024), 0, s, offsets, E, (int)M, offs, prefixes,
-                         (const bf16_t*)nullptr, (bf16_t*)nullptr, (int64_t)0, (const bf16_t**)(ws + L.w_tab),
-                         (bf16_t**)nullptr, (const bf16_t*)nullptr, (bf16_t*)nullptr, (bf16_t*)nullptr, N);
-    const RowGroups chunks{offs, prefixes, nullptr, nullptr, E, (int)M, 0, 0};
-    static_assert(prefix_slot(kDzRows) == 0, "the chunks' prefix is the first");
     bf16_t* out = (bf16_t*)(ws + L.dz);
     float* part = db ? (float*)(ws + L.part) : nullptr;
-    hipLaunchKernelGGL(k_linear_dz<bf16_t>, dim3((unsigned)mx_dz_chunks(M, E, grouped), ceil_div(N, kDzCols)),
-                       dim3(256), 0, s, dy, pre, act, chunks, N, out, part);
+    const int chunks = (int)mx_dz_chunks(M, E, grouped);
+    hipLaunchKernelGGL(k_mx_dz, dim3(chunks, ceil_div(N, kDzCols)), dim3(256), 0, s, dy, pre, act, r, N, out, part);
     if (act != kActNone) dz = out;
-    if (db)
-      hipLaunchKernelGGL(k_linear_db<bf16_t>, dim3(ceil_div(N, 64), E), dim3(256), 0, s, part, chunks, N, db);
+    if (db) hipLaunchKernelGGL(k_mx_db, dim3(ceil_div(N, 64), E), dim3(256), 0, s, part, r, chunks, N, db);
   }
   if (dx)
-    with_mx_launch(mx_tiles(grouped, E, M, K), r, K, [&](auto c, int tiles, dim3 grid) {
+    with_mx_launch(mx_tiles(false, grouped, E, M, K), r, K, [&](auto c, int tiles, dim3 grid) {
       using C = decltype(c);
       hipLaunchKernelGGL((k_mx_dgrad<C>), grid, dim3(C::THREADS), 0, s, dz, r, tiles, w, dx);
     });

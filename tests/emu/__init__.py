@@ -46,8 +46,8 @@ def sources(to):
             text = replaced(text, "(big && M >= 2 * (int64_t)C::BM * E)",
                             "(big && (emu::tiles < 0 ? M >= 2 * (int64_t)C::BM * E : emu::tiles == 0))")
         if name == "mx_api.hip":
-            text = replaced(text, "MxTiles mx_tiles(bool grouped, int E, int64_t M, int N) {",
-                            "MxTiles mx_tiles(bool grouped, int E, int64_t M, int N) {\n"
+            text = replaced(text, "MxTiles mx_tiles(bool four, bool grouped, int E, int64_t M, int N) {",
+                            "MxTiles mx_tiles(bool four, bool grouped, int E, int64_t M, int N) {\n"
                             "  if (emu::tiles >= 0) return (MxTiles)emu::tiles;")
             text = replaced(text, "bool mx_skinny(bool four, int64_t M, int K, int N, int E, bool grouped) {",
                             "bool mx_skinny(bool four, int64_t M, int K, int N, int E, bool grouped) {\n"

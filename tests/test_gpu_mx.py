@@ -101,6 +101,11 @@ MANY = [(200, 736, 136, None, 0, "silu", True, True), (513, 320, 264, None, 0, "
         (6000, 96, 136, [3000, 2990], 10, "none", False, True), (9000, 256, 1408, None, 0, "silu", True, False),
         (5000, 448, 2816, [1250] * 4, 0, "gelu", False, False), (777, 32, 8, [7, 700], 70, "none", True, False)]
 
+# 256-row tiles with some left behind an XCD's last 32, forward (wide N) or back (wide K): 5, 12 and 24 of them, and of groups
+CUT = [(9316, 64, 2048, None, 0, "silu", True, True), (11259, 2048, 96, None, 0, "none", False, False), (14300, 64, 2048, None, 0, "none", True, False),
+       (12050, 96, 1368, [0, 1, 255, 257, 3000, 511, 513, 1100, 2000, 1700, 963, 1700], 50, "gelu", True, True),
+       (9000, 1376, 1368, [600, 700, 800, 900, 1000, 1000, 1100, 900, 1000, 1000], 0, "silu", True, False)]
+
 
 def problem(case, seed, std=1.0):
     M, K, N, sizes, tail, act, has_b, has_r = case
@@ -125,7 +130,7 @@ def reference(x, w, b, r, offsets, act, dy, dtype):
     return ops_ref.linear(x, mx_ref.values(*w), f64(b), None if offsets is None else offsets.cpu(), act, f64(r), f64(dy), dtype)
 
 
-@pytest.mark.parametrize("case", FEW + MANY, ids=str)
+@pytest.mark.parametrize("case", FEW + MANY + CUT, ids=str)
 def test_bf16_rows(case):
     x, w, b, r, offsets, act = problem(case, len(str(case)))
     if offsets is not None and int(offsets[-1]) < x.shape[0]:
@@ -138,7 +143,7 @@ def test_bf16_rows(case):
     assert torch.equal(got, ops.mx_linear(x, w, b, offsets=offsets, activation=act, residual=r))
 
 
-@pytest.mark.parametrize("case", FEW + MANY, ids=str)
+@pytest.mark.parametrize("case", FEW + MANY + CUT, ids=str)
 def test_gradients(case):
     x, w, b, r, offsets, act = problem(case, len(str(case)) + 1)
     dy = normal(gen(9), x.shape[0], case[2], dtype=BF16)
@@ -157,7 +162,7 @@ def test_gradients(case):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("case", FEW + MANY, ids=str)
+@pytest.mark.parametrize("case", FEW + MANY + CUT, ids=str)
 def test_both_sides_in_four_bits(case, dtype):
     x, w, b, r, offsets, act = problem(case, len(str(case)) + 2)
     if offsets is not None and int(offsets[-1]) < x.shape[0]:
