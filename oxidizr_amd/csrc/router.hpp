@@ -14,7 +14,7 @@
 // up over the rows of its block; the blocks' sums are added in block order, so no result depends on
 // scheduling.  Exponentials are v_exp_f32 of x log2(e), off by |x| 2^-24 of themselves for the product's rounding and
 // a step more (exact to fp32 where they matter, near the largest), quotients v_rcp_f32: with the device library's expf and
-// divisions 65536 rows of 160 sigmoid scores took 45 us forward and 55 back.
+// divisions 65536 rows of 160 sigmoid scores took 45 us forward and 55 back (24 and 29 with these).
 #pragma once
 #include "kernels.hpp"
 
@@ -182,6 +182,9 @@ MOE_DEV void router_walk(const int* offsets, int S, int64_t r0, int64_t r1, F&& 
 // ------------------------------------------------------------------ forward
 // Block b takes rows [b rpb, (b + 1) rpb) and writes, for each sequence s that has rows there, its column sums
 // of q, its counts and (z sum, real tokens) to slot b + s: such pairs ascend in both, so no two share a slot.
+// Bound by arithmetic (an exponential and some ten operations an element; a sigmoid two and twenty) on long inputs, by a launch and one
+// round trip on short ones: 65536 x 160 bf16 sigmoid scores in 48 sequences 24 us (0.9 TB/s), 8192 x 256 fp32 softmax 5.0 (1.7 TB/s).
+// More rows to a block leave the reduction fewer slots and the CUs idle: one block to a CU.
 constexpr int kRouterBlock = 512;
 template <class S, typename T, typename I>
 __global__ __launch_bounds__(kRouterBlock) void k_router_losses(RouterRows<T, I> in, int64_t rpb,
@@ -251,7 +254,7 @@ __global__ __launch_bounds__(kRouterBlock) void k_router_losses(RouterRows<T, I>
 }
 
 // Sequence s = blockIdx.x: its blocks' parts added in 64 bits (in block order within kRouterParts interleaved sums),
-// and the losses.
+// and the losses.  One workgroup to a sequence, bound by its CU's reads: 256 slots of 256 experts (0.5 MB) 9.5 us, of 48 sequences 5.6.
 constexpr int kRouterParts = 32;
 template <int V>
 __global__ __launch_bounds__(1024) void k_router_reduce(const float* __restrict__ part_q, const int* __restrict__ part_c,
@@ -340,6 +343,7 @@ __global__ __launch_bounds__(1024) void k_router_reduce(const float* __restrict_
 }
 
 // ------------------------------------------------------------------ backward
+// As the forward bound by arithmetic: 65536 x 160 bf16 sigmoid scores 29 us, 8192 x 256 fp32 softmax 8.0 (2.1 TB/s).
 // Block b: rows [b rpb, (b + 1) rpb) over four waves.  slope: of balance in q, [S, E].  d_balance, d_z: [S], or null (0).
 constexpr int kRouterBwdBlock = 256;
 template <class S, typename T, typename I>
