@@ -683,28 +683,45 @@ __global__ __launch_bounds__(C::THREADS, 2) void k_mxmx_fwd(const uint8_t* __res
 // other workgroups', which find the weight in the caches; 64 rows to a workgroup took 40 to 90 registers more and 10 to 60 % longer),
 // KS waves of a workgroup share the weight rows and take every KS-th k-chunk of 512 elements (1024: as many registers
 // too many, 20 to 100 % longer).  Lane l supplies block l / 16 + 4 q of weight row l % 16 in load q, so four lanes read
-// 64 contiguous bytes; it loads the 16 scales of its row at once, of which its blocks' are the bytes l / 16 of each dword (a
-// load for each: 10 % longer).
+// 64 contiguous bytes.  The four lanes of a row load the scales of four chunks of it, 16 bytes each, and every
+// chunk's are handed round (ds_bpermute): with each lane loading its chunk's 16 the cache lines of scales were fetched again for each
+// chunk, 96 us instead of 86 below (a load for each byte: 10 % more).
 // bf16 rows: the block becomes four 8-element vectors, multiplied with the four of the token row by 16 x 16 x 32 MFMAs; the row's
 // next four are requested before (3 %).  4-bit rows: one 16 x 16 x 128 scaled MFMA.
-// Bound by HBM where the weights outgrow the caches: 512 rows in 128 experts of 1536 x 4096 (428 MB) 96 us over bf16 rows (4.5 TB/s;
-// each workgroup also reads 128 KB of rows from L2) and 76 over 4-bit ones (5.6; with the nontemporal hint on the weights 106 and 91);
-// 64 rows in them 44 and 30.  Bound by a launch and one chain of loads otherwise: one row of 4096 x 4096 4.5 and 4.0.
+// Bound by HBM where the weights outgrow the caches: 512 rows in 128 experts of 1536 x 4096 (428 MB) 86 us over bf16 rows (5.0 TB/s;
+// fewer rows to a wave or registers for more waves of them: 91 to 148) and 70 over 4-bit ones (6.1; with the nontemporal hint on the
+// weights a tenth more in both); 64 rows in them 38 and 29.  Bound by a launch and one chain of loads otherwise: one row of 4096 x
+// 4096 4.6 and 4.0.
 
 constexpr int kMxSkinnyRows = 16;
 constexpr int kMxChunkLoads = 4;  // of 128 elements
-// The 16 scales of a chunk from p on; FULL: all in the row (any alignment), else the first `left` blocks' are.
-template <bool FULL>
-MOE_DEV void mx_row_scales(const uint8_t* p, int left, int g, uint32_t (&s)[kMxChunkLoads]) {
-  if constexpr (FULL) {
-    typedef u32x4 any_u32x4 __attribute__((aligned(1)));
-    const u32x4 v = *(const __attribute__((address_space(1))) any_u32x4*)p;
-#pragma unroll
-    for (int q = 0; q < kMxChunkLoads; ++q) s[q] = v[q] >> (8 * g);
-  } else {
-#pragma unroll
-    for (int q = 0; q < kMxChunkLoads; ++q) s[q] = 4 * q + g < left ? gptr(p)[4 * q + g] : 0u;
+// Scales of a wave's next four chunks: lane 16 c + rl holds the 16 of chunk c of its row, from p on; `left` of them are in the row.
+template <typename V>
+MOE_DEV V ld_any(const uint8_t* p) {  // of any alignment
+  typedef V any_v __attribute__((aligned(1)));
+  return *(const __attribute__((address_space(1))) any_v*)p;
+}
+MOE_DEV u32x4 mx_row_scales(const uint8_t* p, int left) {
+  u32x4 v{0, 0, 0, 0};
+  if (left >= 16) {
+    v = ld_any<u32x4>(p);
+  } else if (left > 0) {  // 8, 4, 2 and 1 of them
+    const uint64_t a = left & 8 ? ld_any<uint64_t>(p) : 0;
+    const uint32_t b = left & 4 ? ld_any<uint32_t>(p + (left & 8)) : 0;
+    const uint32_t c = left & 2 ? ld_any<uint16_t>(p + (left & 12)) : 0;
+    const uint32_t d = left & 1 ? gptr(p)[left & 14] : 0;
+    const uint64_t rest = b | (uint64_t)(c | d << 8 * (left & 2)) << 8 * (left & 4);
+    const uint64_t lo = left & 8 ? a : rest, hi = left & 8 ? rest : 0;
+    v = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
   }
+  return v;
+}
+// Chunk c's, as the lanes of block l / 16 of each load take them: byte l / 16 of its dword, in the lowest byte.
+MOE_DEV void mx_chunk_scales(const u32x4& held, int c, uint32_t (&s)[kMxChunkLoads]) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int q = 0; q < kMxChunkLoads; ++q)
+    s[q] = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * (16 * c + (lane & 15)), (int)held[q]) >> (8 * (lane >> 4));
 }
 
 template <bool X4, typename T, int KS, int RW>
@@ -744,7 +761,8 @@ __global__ __launch_bounds__(256) void k_mx_skinny(const void* __restrict__ X, c
 #pragma unroll
     for (int i = 0; i < RW; ++i) vw[i] = 16 * i + rl < nrows ? (uint32_t)((16 * i + rl) * bytes + 16 * g) : kOobOffset;
     const uint32_t vx = rl < rows ? (uint32_t)(rl * xb + (X4 ? 16 : 64) * g) : kOobOffset;
-    auto chunk = [&](int kc, auto full_c) {
+    u32x4 ws_held[RW], xs_held;
+    auto chunk = [&](int kc, int at, auto full_c) {  // at: of the four whose scales are held
       constexpr bool FULL = decltype(full_c)::value;
       const int b0 = kc * 4 * Q, left = blocks - b0;  // blocks
       u32x4 wa[RW][Q];
@@ -757,8 +775,7 @@ __global__ __launch_bounds__(256) void k_mx_skinny(const void* __restrict__ X, c
           wa[i][q] = buf_ld16(rw, in ? vw[i] + 64 * q : kOobOffset, (uint32_t)b0 * 16);
         }
 #pragma unroll
-      for (int i = 0; i < RW; ++i)  // rows past the weight's read its first row's scales (their codes are zeros)
-        mx_row_scales<FULL>(wscales + (16 * i + rl < nrows ? 16 * i + rl : 0) * blocks + b0, left, g, ws[i]);
+      for (int i = 0; i < RW; ++i) mx_chunk_scales(ws_held[i], at, ws[i]);
       if constexpr (X4) {
         u32x4 xa[Q];
         uint32_t xs[Q];
@@ -767,7 +784,7 @@ __global__ __launch_bounds__(256) void k_mx_skinny(const void* __restrict__ X, c
           const bool in = FULL || 4 * q + g < left;
           xa[q] = buf_ld16(rx, in ? vx + 64 * q : kOobOffset, (uint32_t)b0 * 16);
         }
-        mx_row_scales<FULL>(XS + ((int64_t)r0 + (rl < rows ? rl : 0)) * blocks + b0, left, g, xs);
+        mx_chunk_scales(xs_held, at, xs);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
@@ -801,9 +818,30 @@ __global__ __launch_bounds__(256) void k_mx_skinny(const void* __restrict__ X, c
         }
       }
     };
-    int kc = ks;
-    for (; (kc + 1) * KC <= K; kc += KS) chunk(kc, std::true_type());
-    if (kc * KC < K) chunk(kc, std::false_type());
+    int kc = ks, at = 0;
+    auto hold = [&] {
+      const int b = (kc + g * KS) * 4 * Q, left = blocks - b;  // of the chunk whose scales this lane holds
+#pragma unroll
+      for (int i = 0; i < RW; ++i)  // rows past the weight's hold its first row's scales (their codes are zeros)
+        ws_held[i] = mx_row_scales(wscales + (int64_t)(16 * i + rl < nrows ? 16 * i + rl : 0) * blocks + b, left);
+      if constexpr (X4) xs_held = mx_row_scales(XS + ((int64_t)r0 + (rl < rows ? rl : 0)) * blocks + b, left);
+    };
+    hold();
+#pragma unroll 1
+    for (; (kc + 1) * KC <= K; kc += KS) {
+      if (at == 4) {
+        at = 0;
+        hold();
+      }
+      chunk(kc, at++, std::true_type());
+    }
+    if (kc * KC < K) {
+      if (at == 4) {
+        at = 0;
+        hold();
+      }
+      chunk(kc, at, std::false_type());
+    }
   }
   if (ks > 0) {
 #pragma unroll

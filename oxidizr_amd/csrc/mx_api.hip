@@ -46,9 +46,9 @@ moe_status check_mx_linear(int x_format, int dtype, int64_t M, int K, int N, int
 // Shape of a few-row launch: waves that share the K of their weight rows, blocks of 16 weight rows to a wave.  More
 // blocks read the token rows less often (bf16 rows are four times the weight's bytes), fewer make more workgroups, and so
 // do more waves.  us at (4 waves, 1 block) / (4, 2) / (2, 4), and with both sides in 4 bits (4, 1) / (4, 2) / (2, 2): 2 rows in
-// 16 experts of 1408 x 2048 4.1 / 5.1 / 9.3 and 3.9 / 4.7 / 5.5; one weight of 4096 x 4096, 16 rows 7.7 / 9.4 / 20.6 and 5.3 / 7.1
-// / 10.0, 32 rows 12.4 / 9.6 / 20.7 and 7.6 / 7.1 / 10.1; 128 rows in 16 experts 13.8 / 11.7 / 13.5 and 8.9 / 8.6 / 9.9; 512 in 128
-// of 1536 x 4096 131 / 101 / 92 and 89 / 77 / 76.
+// 16 experts of 1408 x 2048 4.2 / 4.8 / 9.3 and 3.8 / 4.5 / 5.4; one weight of 4096 x 4096, 16 rows 7.7 / 9.0 / 19.0 and 5.0 / 6.4
+// / 9.0, 32 rows 12.1 / 9.2 / 19.0 and 6.8 / 6.5 / 9.0, 64 rows 21 / 14 / 19 and 10.7 / 9.2 / 9.0; 128 rows in 16 experts 14.1 / 11.5 /
+// 13.3 and 8.7 / 8.2 / 9.3, 256 20 / 16 / 14 and 10.9 / 10.2 / 10.1; 512 in 128 of 1536 x 4096 125 / 95 / 85 and 82 / 70 / 70.
 struct MxSkinny {
   int ks, rw;
 };
@@ -58,7 +58,7 @@ int64_t mx_skinny_slots(int64_t M, int E, bool grouped) {
 MxSkinny mx_skinny_shape(bool four, int64_t M, int N, int E, bool grouped) {
   const int64_t blocks = mx_skinny_slots(M, E, grouped) * ceil_div(N, 16);
   if (blocks < 512) return {4, 1};
-  if (blocks < 4096) return {4, 2};
+  if (blocks < 2500) return {4, 2};
   return {2, four ? 2 : 4};
 }
 // Calls f(waves, blocks), constants.
@@ -73,14 +73,14 @@ int64_t mx_skinny_blocks(const MxSkinny& p, int64_t M, int N, int E, bool groupe
   return mx_skinny_slots(M, E, grouped) * ceil_div(N, 64 / p.ks * p.rw) + (grouped ? kMxNoGroupBlocks : 0);
 }
 // Whether a forward runs as the stream of its weights.  us, tiles / this: bf16 rows, 512, 1024 and 2048 in 128 experts of 1536 x
-// 4096 161 / 92, 168 / 112, 176 / 148; 128, 256 and 512 in 16 of 1408 x 2048 18 / 12, 19 / 14, 19 / 22; 64, 128 and 256 of one weight
-// of 4096 x 4096 32 / 14, 33 / 21, 33 / 37.  Both sides in 4 bits: 85 / 76, 87 / 91, 89 / 109; 9.3 / 8.6, 9.2 / 10.5, 9.5 / 14;
-// 13 / 10, 13 / 16, 13 / 27.
+// 4096 159 / 85, 167 / 104, 175 / 136; 128, 256 and 512 in 16 of 1408 x 2048 19 / 12, 19 / 14, 19 / 22; 64, 128 and 256 of one weight
+// of 4096 x 4096 32 / 14, 32 / 25, 32 / 34.  Both sides in 4 bits: 85 / 70, 87 / 80, 89 / 108; 9.4 / 8.2, 9.3 / 10.1, 9.6 / 16;
+// 13 / 9.2, 13 / 15, 14 / 26.
 bool mx_skinny(bool four, int64_t M, int K, int N, int E, bool grouped) {
   // the tiles' scales are loaded 16 bytes at once
   if (four && std::min(M, (int64_t)E * N) * (K / kMxBlock) < 16) return true;
   if (mx_skinny_blocks(mx_skinny_shape(four, M, N, E, grouped), M, N, E, grouped) * 256 >= kMaxGridThreads) return false;
-  return grouped ? M <= (four ? 7 : 20) * std::min<int64_t>(E, M) : M <= (four ? 80 : 160);
+  return grouped ? M <= (four ? 9 : 20) * std::min<int64_t>(E, M) : M <= (four ? 80 : 160);
 }
 
 // Row tiles by height, by their cost in tenths of a full round of 256-row tiles; the tiles behind the last full round are cut

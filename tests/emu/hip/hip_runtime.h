@@ -149,6 +149,7 @@ template <class T> void use(const T& v) { asm volatile("" : : "r"(&v) : "memory"
 #define __builtin_amdgcn_rcpf(x) (1.0f / (x))
 #define __builtin_amdgcn_readfirstlane(v) (v)  // the kernels give it wave-uniform values
 #define __builtin_amdgcn_readlane(v, l) emu::of_lane((int)(v), l)
+#define __builtin_amdgcn_ds_bpermute(a, v) emu::of_lane((int)(v), (a) / 4)
 #define __builtin_amdgcn_update_dpp(o, v, c, r, b, bc) emu::dpp(o, v, c, r, b, bc)
 #define __builtin_amdgcn_permlane32_swap(a, b, x, y) emu::swap_halves<32>(a, b)
 #define __builtin_amdgcn_permlane16_swap(a, b, x, y) emu::swap_halves<16>(a, b)
