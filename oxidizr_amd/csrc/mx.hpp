@@ -267,6 +267,13 @@ struct MxStager {
   }
 };
 
+// Behind a main loop that requests k-tiles past the last one: the zeros that these write have landed in every wave's part of
+// the LDS, which the epilogue reuses (__syncthreads alone need not wait for direct loads).
+MOE_DEV void direct_loads_done() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
 // acc += W-tile x A-tile over the contraction, A (bf16, K-contiguous) by direct-to-LDS loads as in
 // mainloop_dma, W through MxStager.  Per k-tile kt: the pieces of kt + 1, loaded during kt - 1, are written
 // to their stage (which was last read before the barrier that began kt), those of kt + 2 are requested, then
@@ -352,7 +359,7 @@ MOE_DEV void mainloop_mx(f32x16 (&acc)[1][C::TN][C::TM], const OpDesc<bf16_t>& a
       __builtin_amdgcn_sched_barrier(0);
     }
   } while (++kt < nk);
-  __syncthreads();  // the caller's epilogue reuses the LDS
+  direct_loads_done();
 }
 
 // Blocks from `tiles` on write the rows of no group.
@@ -648,7 +655,7 @@ MOE_DEV void mainloop_mxmx(f32x16 (&acc)[1][C::TN][C::TM], const OpDesc<bf16_t>&
     }
     read_scales(kt + 1);
   } while (++kt < nk);
-  __syncthreads();
+  direct_loads_done();
 }
 
 template <class C, typename T>

@@ -2,7 +2,8 @@
 AddressSanitizer), from copies of the sources in which only this is changed: waits and barriers in inline asm go,
 dynamic LDS comes from the emulator, names have internal linkage (the sanitizer leaves static arrays of
 others alone, and LDS arrays become such), and a caller may name the row tiles (and fewer blocks fill
-what belongs to no expert)."""
+what belongs to no expert).  With `waits` the waits and barriers in inline asm become the emulator's, whose direct-to-LDS
+loads then stay in flight until their wait."""
 import os
 import re
 import shutil
@@ -19,7 +20,16 @@ def replaced(text, old, new):
     return text.replace(old, new)
 
 
-def sources(to):
+def waiting(text):
+    """The waits and barriers of the direct-to-LDS pipeline in a source, as the emulator's."""
+    text = re.sub(r'asm volatile\("s_waitcnt vmcnt\(%0\)" :: "n"\((.*?)\) : "memory"\);', r"emu::wait_direct(\1);", text)
+    text = text.replace('asm volatile("s_waitcnt vmcnt(0)" ::: "memory");', "emu::wait_direct(0);")
+    text = text.replace('asm volatile("s_waitcnt lgkmcnt(0)\\n\\ts_barrier" ::: "memory");', "emu::barrier();")
+    assert "s_waitcnt" not in re.sub(r"//.*", "", text)
+    return text
+
+
+def sources(to, waits=False):
     """The csrc folder and the header, with the changes."""
     src = os.path.join(to, "oxidizr_amd", "csrc")
     os.makedirs(src)
@@ -29,6 +39,8 @@ def sources(to):
         if not name.endswith((".hpp", ".hip")):
             continue
         text = open(os.path.join(ROOT, "oxidizr_amd", "csrc", name)).read()
+        if waits:
+            text = waiting(text)
         text = re.sub(r"asm volatile\([^;]*\);", ";", text)
         text = re.sub(r"extern __shared__ int (\w+)\[\];", r"int* \1 = (int*)emu::dynamic_lds();", text)
         text = text.replace("namespace moe {", "namespace moe { namespace {").replace("}  // namespace moe", "} }")
@@ -59,15 +71,15 @@ def sources(to):
             f.write(text)
 
 
-def build(to, program):
+def build(to, program, waits=False):
     """The path of `program`.cpp, built in the folder `to`."""
     to = str(to)
-    sources(to)
+    sources(to, waits)
     objs = []
     procs = []
     for name in ("emu.cpp", program + ".cpp"):
         objs.append(os.path.join(to, name + ".o"))
-        cmd = [CLANG, *FLAGS, "-I", HERE, "-I", to, "-c", os.path.join(HERE, name), "-o", objs[-1]]
+        cmd = [CLANG, *FLAGS, *(["-DEMU_WAITS"] if waits else []), "-I", HERE, "-I", to, "-c", os.path.join(HERE, name), "-o", objs[-1]]
         procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
     for cmd, p in procs:
         out = p.communicate()[0]

@@ -6,6 +6,7 @@
 #include <sys/mman.h>
 #include <ucontext.h>
 #include <unistd.h>
+#include <deque>
 #include <string>
 #include <vector>
 
@@ -23,6 +24,7 @@ struct Fiber {
   void* fake = nullptr;
   State state = kEnded;
   unsigned tid = 0;
+  std::deque<std::pair<const void*, size_t>> direct;  // loads in flight, the oldest first
 };
 std::vector<Fiber> fibers(1024);
 void* scheduler[5];
@@ -48,6 +50,7 @@ void entry() {
   __sanitizer_finish_switch_fiber(nullptr, &scheduler_stack, &scheduler_size);
   for (;;) {
     (*body)();
+    wait_direct(0);
     current->state = kEnded;
     yield();
   }
@@ -139,6 +142,14 @@ const uint64_t* exchange(uint64_t v, uint64_t* live) {
   return slots[w][mine];
 }
 void* dynamic_lds() { return dynamic; }
+void direct_load(const void* to, size_t n) {
+  __asan_poison_memory_region(to, n);
+  current->direct.emplace_back(to, n);
+}
+void wait_direct(size_t left) {
+  auto& d = current->direct;
+  for (; d.size() > left; d.pop_front()) __asan_unpoison_memory_region(d.front().first, d.front().second);
+}
 void touch(const void* p, size_t n, bool) {
   if (void* bad = __asan_region_is_poisoned(const_cast<void*>(p), n)) {
     printf("kernel %s, block %u, thread %u\n", kernel.c_str(), blockIdx.x, threadIdx.x);

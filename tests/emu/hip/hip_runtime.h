@@ -3,6 +3,8 @@
 // across a wave.  Loads and stores go to host memory, so AddressSanitizer sees each of them, LDS
 // arrays are static, buffer loads are checked against their resource and against what they
 // reach.  Matrix instructions change nothing: no address depends on a product.
+// With EMU_WAITS direct-to-LDS loads stay in flight until their thread waits for them: what they
+// write may be neither read nor written before (an address in it is then out of bounds).
 #pragma once
 #include <stddef.h>
 #include <stdint.h>
@@ -49,6 +51,10 @@ void* dynamic_lds();
 [[noreturn]] void die(const char* what, long long a = 0, long long b = 0);
 void touch(const void* p, size_t n, bool write);  // dies unless [p, p + n) may be accessed
 void count_store(const void* p);
+// A direct load of the current thread is issued; all but its newest `left` ones have landed.  (On the device
+// loads to registers count too, so a wait for `left` may end later.  It never ends sooner.)
+void direct_load(const void* to, size_t n);
+void wait_direct(size_t left);
 inline int lane() { return threadIdx.x & 63; }
 
 struct Rsrc {
@@ -75,6 +81,9 @@ inline void load_lds(const Rsrc& r, void* lds, unsigned n, uint32_t voff, uint32
   char* to = (char*)lds + lane() * n;
   touch(to, n, true);
   buffer_at(r, voff, soff, n);
+#ifdef EMU_WAITS
+  direct_load(to, n);
+#endif
 }
 template <class P, class V> void nt_store(V v, P* p) {
   count_store((const void*)p);
