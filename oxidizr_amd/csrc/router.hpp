@@ -73,7 +73,7 @@ struct RouterShape {
 };
 
 template <class S, typename T>
-MOE_DEV void router_load(const T* row, int E, int j, float (&x)[S::C], float scale) {
+MOE_DEV void router_load(const T* row, int E, int j, float (&x)[S::C]) {
 #pragma unroll
   for (int i = 0; i < S::NCH; ++i) {
     const int c = (i * S::LPR + j) * S::V;
@@ -81,25 +81,27 @@ MOE_DEV void router_load(const T* row, int E, int j, float (&x)[S::C], float sca
       float f[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       if (c < E) load4(row + c, f);
 #pragma unroll
-      for (int v = 0; v < 4; ++v) x[4 * i + v] = f[v] * scale;
+      for (int v = 0; v < 4; ++v) x[4 * i + v] = f[v];
     } else {
-      x[i] = c < E ? to_f<T>(row[c]) * scale : -INFINITY;
+      x[i] = c < E ? to_f<T>(row[c]) : -INFINITY;
     }
   }
 }
 
-// Of a row whose columns' x are spread over S::LPR lanes: q and p (both times nothing: normalised), lse, and for
-// sigmoid scores 1 - sigmoid.
+// Of a row whose logits x are spread over S::LPR lanes: q and p, normalised, the largest logit m and the log of the sum, so
+// that lse = m / tau + log_sum.  The largest is taken off before the division by tau: logits of the type's lowest value
+// over a tau below 1 are beyond fp32, their differences are not.
 template <class S>
-MOE_DEV void router_scores(const float (&x)[S::C], int score, float (&q)[S::C], float (&p)[S::C], float& lse) {
-  float m = -INFINITY;
+MOE_DEV void router_scores(const float (&x)[S::C], int score, float inv_tau, float (&q)[S::C], float (&p)[S::C], float& m,
+                           float& log_sum) {
+  m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < S::C; ++i) m = fmaxf(m, x[i]);
   m = group_max<S::LPR>(m);
   float sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < S::C; ++i) {
-    p[i] = exp_of(x[i] - m);
+    p[i] = exp_of((x[i] - m) * inv_tau);
     sum += p[i];
   }
   if (score == kScoreSoftmax) {
@@ -111,12 +113,12 @@ MOE_DEV void router_scores(const float (&x)[S::C], int score, float (&q)[S::C], 
       q[i] = p[i];
     }
   } else {
-    // sigmoid(x) over sigmoid's size at the row's largest x, min(1, exp(m)): rows of very negative logits have
+    // sigmoid(x / tau) over sigmoid's size at the row's largest, min(1, exp(m / tau)): rows of very negative logits have
     // scores as well
     float total = 0.0f;
 #pragma unroll
     for (int i = 0; i < S::C; ++i) {
-      const float t = exp_of(-fabsf(x[i]));
+      const float t = exp_of(-fabsf(x[i] * inv_tau));
       q[i] = (x[i] > 0.0f ? 1.0f : m > 0.0f ? t : p[i]) * __builtin_amdgcn_rcpf(1.0f + t);
       total += q[i];
     }
@@ -129,7 +131,7 @@ MOE_DEV void router_scores(const float (&x)[S::C], int score, float (&q)[S::C], 
       q[i] *= rq;
     }
   }
-  lse = m + logf(sum);
+  log_sum = logf(sum);
 }
 
 // Whether the row's token is real (all lanes of a wave call this; `in`: there is a row), and f(e) for each of its
@@ -211,14 +213,15 @@ __global__ __launch_bounds__(kRouterBlock) void k_router_losses(RouterRows<T, I>
       const int64_t row = base + sub;
       const bool has = row < b;
       const int64_t at = has ? row : b - 1;
-      float x[S::C], q[S::C], p[S::C], lse;
-      router_load<S>(in.logits + at * E, E, j, x, in.inv_tau);
+      float x[S::C], q[S::C], p[S::C], m, log_sum;
+      router_load<S>(in.logits + at * E, E, j, x);
       const bool real = router_real<S>(in.idx + at * k, k, E, j, has, [&](int e) { atomicAdd(&hist[e], 1); });
-      router_scores<S>(x, in.score, q, p, lse);
+      router_scores<S>(x, in.score, in.inv_tau, q, p, m, log_sum);
       if (real) {
 #pragma unroll
         for (int i = 0; i < S::C; ++i) acc[i] += q[i];
         if (j == 0) {
+          const float lse = m * in.inv_tau + log_sum;
           z += lse * lse;
           ++n;
         }
@@ -376,12 +379,14 @@ __global__ __launch_bounds__(kRouterBwdBlock) void k_router_losses_bwd(
       const int64_t row = base + sub;
       const bool has = row < b;
       const int64_t at = has ? row : b - 1;
-      float x[S::C], q[S::C], p[S::C], lse, dot = 0.0f;
-      router_load<S>(in.logits + at * E, E, j, x, in.inv_tau);
+      float x[S::C], q[S::C], p[S::C], m, log_sum, dot = 0.0f;
+      router_load<S>(in.logits + at * E, E, j, x);
       const bool real = router_real<S>(in.idx + at * k, k, E, j, has, [](int) {});
       // from the row's largest again, not from a kept lse: x - lse carries lse's rounding, |lse| 2^-24, which is all of log sum
       // where a row's logits are large (1 in each p of a row of the type's lowest value)
-      router_scores<S>(x, in.score, q, p, lse);
+      router_scores<S>(x, in.score, in.inv_tau, q, p, m, log_sum);
+      // h lse; where lse is beyond fp32 the product need not be
+      const float lse = m * in.inv_tau + log_sum, hl = isinf(lse) ? h * in.inv_tau * m + h * log_sum : h * lse;
 #pragma unroll
       for (int i = 0; i < S::C; ++i) dot += q[i] * g[i];
       dot = group_sum<S::LPR>(dot);
@@ -390,10 +395,10 @@ __global__ __launch_bounds__(kRouterBwdBlock) void k_router_losses_bwd(
       for (int i = 0; i < S::C; ++i) {
         float t = q[i] * (g[i] - dot);
         if (in.score == kScoreSigmoid) {
-          const float e = exp_of(-fabsf(x[i]));
+          const float e = exp_of(-fabsf(x[i] * in.inv_tau));
           t *= (x[i] > 0.0f ? e : 1.0f) * __builtin_amdgcn_rcpf(1.0f + e);
         }
-        d[i] = real ? t + h * lse * p[i] : 0.0f;
+        d[i] = real ? t + hl * p[i] : 0.0f;
       }
       if (has) store(row, d);
     }

@@ -1,0 +1,59 @@
+"""router_losses over logits at the ends of their types' ranges."""
+import pytest
+import torch
+
+from oxidizr_amd import ops
+from tests import mx_ref
+from tests.ops_ref import U32
+from tests.test_gpu_router import problem
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("end", ["min", "max"])
+@pytest.mark.parametrize("tau", [0.5, 0.03])
+def test_rows_beyond_fp32_once_divided_by_the_temperature(tau, end, score, dtype):
+    # whole rows of a type's lowest or largest value: their scores are even, as at any other level
+    logits, idx = problem(90, 24, 2, 9, dtype, pad=0.1)
+    level = getattr(torch.finfo(dtype), end)
+    logits[::3] = level
+    logits[1::9, 4:20] = torch.finfo(dtype).min
+    # the level does not matter to a softmax; sigmoid and its slope are those of +-200 to 1e-80
+    ref = logits.double()
+    ref[::3] = 0.0 if score == "softmax" else 200.0 if level > 0 else -200.0
+    ref[1::9, 4:20] = -float("inf")
+    d_balance = torch.tensor([0.3], device="cuda")
+    want = mx_ref.losses(ref, idx, score, tau, 1.0, 1.0, None, d_balance, None)
+    x = logits.clone().requires_grad_()
+    out = ops.router_losses(x, idx, score=score, temperature=tau)
+    mx_ref.assert_close(out.balance.detach().view(1), *want["balance"], "balance")
+    assert torch.equal(out.counts.view(1, -1), want["counts"])
+    got, = torch.autograd.grad(out.balance, x, d_balance[0])
+    mx_ref.assert_close(got, *want["d"], "d_logits")
+    assert float(want["d"][0][::3].abs().max()) > (1e-5 if score == "softmax" or level < 0 else -1.0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("end", ["min", "max"])
+def test_gradient_of_z_where_the_log_sum_is_beyond_fp32(end, dtype):
+    logits, idx = problem(60, 24, 2, 4, dtype, pad=0.1)
+    logits[::3] = getattr(torch.finfo(dtype), end)
+    real = ((idx >= 0) & (idx < 24)).any(1)
+    up = 1e-6
+    ref = logits.double() / 0.5
+    # the formula, not autograd's: torch's gradient of logsumexp is exp(x - lse), 1 in each of 24 where lse rounds to x
+    want = 2 * up / real.sum() * torch.logsumexp(ref, 1, keepdim=True) * torch.softmax(ref, 1) / 0.5
+    x = logits.clone().requires_grad_()
+    out = ops.router_losses(x, idx, temperature=0.5)
+    got, = torch.autograd.grad(out.z, x, torch.tensor(up, device="cuda"))
+    # h has four roundings, its product with 1 / tau and m two, the sum one, p some 5 (the sum of 24 ones is exact), the last two;
+    # the slope of the balance is not asked for
+    rows = real.clone()
+    rows[1::3] = rows[2::3] = False
+    tol = 16 * U32 + torch.finfo(dtype).eps / 2
+    assert bool(rows.any()) and float(want[rows].abs().max()) < 3e38
+    assert bool(((got[rows].double() - want[rows]).abs() <= tol * want[rows].abs()).all())
+    assert bool(got.isfinite().all())
