@@ -90,7 +90,7 @@ MOE_DEV void router_load(const T* row, int E, int j, float (&x)[S::C]) {
 
 // Of a row whose logits x are spread over S::LPR lanes: q and p, normalised, the largest logit m and the log of the sum, so
 // that lse = m / tau + log_sum.  The largest is taken off before the division by tau: logits of the type's lowest value
-// over a tau below 1 are beyond fp32, their differences are not.
+// over a tau below 1 are beyond fp32, their differences are not.  Of an infinite m, p is NaN and lse m itself.
 template <class S>
 MOE_DEV void router_scores(const float (&x)[S::C], int score, float inv_tau, float (&q)[S::C], float (&p)[S::C], float& m,
                            float& log_sum) {
@@ -132,6 +132,13 @@ MOE_DEV void router_scores(const float (&x)[S::C], int score, float inv_tau, flo
     }
   }
   log_sum = logf(sum);
+  if (__any(isinf(m))) {  // sum is NaN there; the maximum passed over any NaN
+    float nan = 0.0f;
+#pragma unroll
+    for (int i = 0; i < S::C; ++i) nan += isnan(x[i]) ? x[i] : 0.0f;
+    nan = group_sum<S::LPR>(nan);
+    if (isinf(m)) log_sum = nan;
+  }
 }
 
 // Whether the row's token is real (all lanes of a wave call this; `in`: there is a row), and f(e) for each of its
@@ -367,13 +374,14 @@ __global__ __launch_bounds__(kRouterBwdBlock) void k_router_losses_bwd(
     }
   };
   router_walk(in.offsets, in.S, r0, r1, [&](int s, int64_t a, int64_t b) {
+    // a loss without an upstream gradient adds nothing, also where its own value is not finite
     const float gb = d_balance ? d_balance[s] * in.inv_tau : 0.0f;
     const float h = d_z ? 2.0f * d_z[s] * inv_real[s] * in.inv_tau : 0.0f;
     float g[S::C];
 #pragma unroll
     for (int i = 0; i < S::C; ++i) {
       const int c = ((i / S::V) * S::LPR + j) * S::V + i % S::V;
-      g[i] = c < E ? gb * slope[(int64_t)s * E + c] : 0.0f;
+      g[i] = c < E && gb != 0.0f ? gb * slope[(int64_t)s * E + c] : 0.0f;
     }
     for (int64_t base = a + wave * S::RPW; base < b; base += NW * S::RPW) {
       const int64_t row = base + sub;
@@ -398,7 +406,7 @@ __global__ __launch_bounds__(kRouterBwdBlock) void k_router_losses_bwd(
           const float e = exp_of(-fabsf(x[i] * in.inv_tau));
           t *= (x[i] > 0.0f ? e : 1.0f) * __builtin_amdgcn_rcpf(1.0f + e);
         }
-        d[i] = real ? t + hl * p[i] : 0.0f;
+        d[i] = !real ? 0.0f : h != 0.0f ? t + hl * p[i] : t;
       }
       if (has) store(row, d);
     }

@@ -57,3 +57,49 @@ def test_gradient_of_z_where_the_log_sum_is_beyond_fp32(end, dtype):
     assert bool(rows.any()) and float(want[rows].abs().max()) < 3e38
     assert bool(((got[rows].double() - want[rows]).abs() <= tol * want[rows].abs()).all())
     assert bool(got.isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("E", [24, 13, 160])
+def test_infinite_logits_of_sigmoid_scores(E, dtype):
+    # sigmoid(inf) = 1: the balance loss and its gradient are numbers
+    logits, idx = problem(200, E, 2, 6, dtype, pad=0.1)
+    logits[::4, 3] = float("inf")
+    logits[1::4, 5:12] = -float("inf")
+    logits[2::8, :10] = float("inf")
+    ref = torch.where(logits == float("inf"), 200.0, logits.double())
+    d_balance = torch.tensor([0.3], device="cuda")
+    want = mx_ref.losses(ref, idx, "sigmoid", 1.0, 1.0, 1.0, None, d_balance, None)
+    x = logits.clone().requires_grad_()
+    out = ops.router_losses(x, idx, score="sigmoid")
+    mx_ref.assert_close(out.balance.detach().view(1), *want["balance"], "balance")
+    got, = torch.autograd.grad(out.balance, x, d_balance[0], retain_graph=True)
+    mx_ref.assert_close(got, *want["d"], "d_logits")
+    again, = torch.autograd.grad((out.balance, out.z), x, (d_balance[0], torch.zeros_like(d_balance[0])))
+    assert torch.equal(got, again)
+    assert float(out.z.detach()) == float("inf")
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("value,z", [(float("inf"), float("inf")), (-float("inf"), float("inf")), (float("nan"), float("nan"))])
+def test_z_of_a_row_that_is_not_finite(value, z, score):
+    # one such row of the second sequence: z and its gradient of all other rows are as the definition has them
+    logits, idx = problem(90, 24, 2, 9, pad=0.1)
+    idx[50] = 3
+    offsets = torch.tensor([0, 40, 90], dtype=torch.int32, device="cuda")
+    up = torch.tensor([0.2, 0.4], device="cuda")
+    want = mx_ref.losses(logits.double(), idx, score, 1.0, 1.0, 1.0, offsets, None, up)
+    logits[50] = value if value == -float("inf") else torch.where(torch.arange(24, device="cuda") == 7, value, logits[50])
+    x = logits.clone().requires_grad_()
+    out = ops.router_losses(x, idx, score=score, offsets=offsets)
+    got_z = out.z.detach()
+    mx_ref.assert_close(got_z[:1], *(t[:1] for t in want["z"]), "z")
+    assert str(float(got_z[1])) == str(z)
+    got, = torch.autograd.grad(out.z, x, up)
+    ref, err = want["d"]
+    others = torch.arange(90, device="cuda") != 50
+    mx_ref.assert_close(got[others], ref[others], err[others], "d_logits")
+    if value == float("inf"):
+        both = logits.clone()
+        both[50, 2] = float("nan")
+        assert bool(ops.router_losses(both, idx, score=score, offsets=offsets).z[1].isnan())
