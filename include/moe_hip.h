@@ -423,8 +423,9 @@ moe_status moe_router_losses_backward(int32_t device, void* stream, int32_t dtyp
  * aligned, scales have any alignment.  num_blocks < 2^29. */
 moe_status moe_mx_quantize(int32_t device, void* stream, int32_t dtype, int64_t num_blocks, const void* x,
                            uint8_t* codes, uint8_t* scales);
-/* The numbers that they stand for, in fp32 or bf16 (both hold them exactly but for 6 2^127 in bf16, which
- * becomes infinite; no quantised block reaches it). */
+/* The numbers that they stand for, in fp32 or bf16: exact below 2^128, infinite from there on (2, 3, 4 and 6
+ * under the scale 254, 4 and 6 under 253; no quantised block has a scale above 252).  moe_mx_linear_forward takes
+ * weights over bf16 rows so too. */
 moe_status moe_mx_dequantize(int32_t device, void* stream, int32_t dtype, int64_t num_blocks,
                              const uint8_t* codes, const uint8_t* scales, void* y);
 

@@ -20,8 +20,8 @@ constexpr int kMxBlock = 32;  // elements under one scale
 // and 255 a NaN (which makes every element one).
 MOE_DEV float mx_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
 
-// Eight elements (a dword of codes) as bf16: exact (2 bits of mantissa, and bf16 has E8M0's range; 6 2^127, above the
-// largest bf16, becomes infinite, but no quantisation makes a scale above 2^125).
+// Eight elements (a dword of codes) as bf16: exact (2 bits of mantissa, and bf16 has E8M0's range); what is 2^128 or more, as in
+// fp32, becomes infinite, but no quantisation makes a scale above 2^125.
 MOE_DEV u32x4 mx_bf16x8(uint32_t c, float s) {
   u32x4 r;
   r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0));

@@ -638,7 +638,8 @@ def _check_mx(q, what):
 
 
 def dequantize_mxfp4(q: MxTensor, dtype=torch.bfloat16):
-    """The numbers [..., K] that q stands for, in dtype (float32 or bfloat16): exact."""
+    """The numbers [..., K] that q stands for, in dtype (float32 or bfloat16): exact, and infinite from 2^128 on (elements of 2
+    and more under the scale byte 254, of 4 and more under 253, which quantize_mxfp4 never makes)."""
     _check_mx(q, "q")
     code = _dtype_code(dtype)
     dev = _on_device(*q)
