@@ -396,9 +396,10 @@ moe_status moe_residual_norm_backward_from_input(int32_t device, void* stream, i
  * offsets[s + 1]; NULL: one sequence of all rows, S = 1) with n real tokens and M_e assignments to expert e:
  *   x = logits / temperature, q = softmax(x) or sigmoid(x) / sum sigmoid(x), P_e = sum q_te / n, f_e = M_e / (k n),
  *   balance[s] = E sum_e (switch_coef f_e P_e + sqprob_coef P_e^2), z[s] = sum logsumexp(x_t)^2 / n
- * (0 for n = 0), counts [S, E] = M_e.  1 <= E <= 1024, 1 <= k <= 16, T k < 2^31, S < 2^22.  slope [S, E] (of
- * balance in q_te) and inv_real [S] (1 / n, or 0): kept for a backward, or NULL.  Offsets ascend within 0..T; with
- * others no access leaves the tensors, but the results are not defined. */
+ * (0 for n = 0), counts [S, E] = M_e.  temperature and its inverse are positive and finite in fp32, 1 <= E <= 1024,
+ * 1 <= k <= 16, T k < 2^31, S < 2^22.  slope [S, E] (of balance in q_te) and inv_real [S] (1 / n, or 0): kept for a
+ * backward, or NULL.  Offsets ascend within 0..T; with others no access leaves the tensors, but the results are not
+ * defined. */
 typedef enum { MOE_SCORE_SOFTMAX = 0, MOE_SCORE_SIGMOID } moe_score;
 size_t moe_router_losses_workspace_bytes(int64_t num_tokens, int32_t num_experts, int64_t num_sequences);
 moe_status moe_router_losses(int32_t device, void* stream, int32_t dtype, int64_t num_tokens,
