@@ -160,9 +160,9 @@ MOE_DEV bool router_real(const I* idx, int k, int E, int j, bool in, F&& f) {
   return ((b >> (sub * S::LPR)) & mask) != 0;
 }
 
-// The first sequence that ends behind row r.
-MOE_DEV int router_first(const int* offsets, int S, int64_t r) {
-  int lo = 0, hi = S;
+// The first sequence, from lo on, that ends behind row r.
+MOE_DEV int router_first(const int* offsets, int S, int64_t r, int lo = 0) {
+  int hi = S;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
     if (offsets[mid + 1] > r) hi = mid;
@@ -171,14 +171,16 @@ MOE_DEV int router_first(const int* offsets, int S, int64_t r) {
   return lo;
 }
 // Calls f(sequence, first row, end) for the parts of sequences in rows [r0, r1), in order, and none(first row, end) for
-// rows of none.  Offsets of any values end the walk.
+// rows of none.  A run of empty sequences is walked for eight and then searched for its end: 131072 of them within a block's rows
+// took it 13 ms, a load after another.  Offsets of any values end the walk.
 template <class F, class G>
 MOE_DEV void router_walk(const int* offsets, int S, int64_t r0, int64_t r1, F&& f, G&& none) {
   if (!offsets) return f(0, r0, r1);
   int64_t r = r0;
   for (int s = uni(router_first(offsets, S, r0)); r < r1; ++s) {
     int64_t end = 0;
-    while (s < S && (end = uni(offsets[s + 1])) <= r) ++s;
+    for (int empty = 0; s < S && (end = uni(offsets[s + 1])) <= r; ++empty)
+      s = empty < 8 ? s + 1 : uni(router_first(offsets, S, r, s + 1));
     if (s >= S) break;
     const int64_t a = min(max(r, (int64_t)uni(offsets[s])), r1), b = min(r1, end);
     if (a > r) none(r, min(a, b));

@@ -103,3 +103,47 @@ def test_z_of_a_row_that_is_not_finite(value, z, score):
         both = logits.clone()
         both[50, 2] = float("nan")
         assert bool(ops.router_losses(both, idx, score=score, offsets=offsets).z[1].isnan())
+
+
+@pytest.mark.parametrize("runs", [[1], [3, 7, 8, 9, 10, 200], [5000, 1, 60000]])
+def test_runs_of_empty_sequences(runs):
+    # sequences of 7 rows with so many empty ones behind each
+    logits, idx = problem(7 * (len(runs) + 1), 16, 2, 5, pad=0.2)
+    ends = [0]
+    for i, n in enumerate(runs):
+        ends += [7 * (i + 1)] * (n + 1)
+    offsets = torch.tensor(ends + [logits.shape[0]], dtype=torch.int32, device="cuda")
+    full = torch.tensor([0] + [7 * (i + 1) for i in range(len(runs) + 1)], dtype=torch.int32, device="cuda")
+    has = offsets[1:] > offsets[:-1]
+    x = logits.clone().requires_grad_()
+    out, want = (ops.router_losses(x, idx, offsets=o) for o in (offsets, full))
+    for a, b in zip(out, want):
+        assert torch.equal(a[has], b) and not bool(a[~has].any())
+    g = torch.rand(has.shape, device="cuda")
+    assert torch.equal(torch.autograd.grad(out.balance, x, g)[0], torch.autograd.grad(want.balance, x, g[has])[0])
+
+
+def test_a_long_run_of_empty_sequences_does_not_hold_up_a_block():
+    # 2^22 - 1 sequences, of which two have rows: beside each other, or (one block walks them) at both ends
+    S, T = 2 ** 22 - 1, 64
+    logits, idx = problem(T, 4, 1, 3, pad=0.0)
+    beside, ends = (torch.full((S + 1,), n, dtype=torch.int32, device="cuda") for n in (T, 10))
+    beside[0], beside[1], ends[0], ends[-1] = 0, 10, 0, T
+    x = logits.clone().requires_grad_()
+    up = torch.ones(S, device="cuda")
+
+    def ms(offsets):
+        best = []
+        for _ in range(3):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            out = ops.router_losses(x, idx, offsets=offsets)
+            d, = torch.autograd.grad(out.balance, x, up)
+            b.record()
+            b.synchronize()
+            best.append(a.elapsed_time(b))
+        return min(best), d
+    (quick, a), (walked, b) = ms(beside), ms(ends)
+    assert torch.equal(a, b)
+    # 0.1 us a sequence and direction when each is loaded behind the other: 0.8 s, where the rest takes some 40 ms
+    assert walked < 3 * quick + 20, (quick, walked)
