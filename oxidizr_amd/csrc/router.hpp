@@ -12,15 +12,18 @@
 //
 // Each direction reads the logits once.  The forward keeps a lane's columns in registers and adds them
 // up over the rows of its block; the blocks' sums are added in block order, so no result depends on
-// scheduling.  Exponentials are v_exp_f32 of x log2(e), off by |x| 2^-24 of themselves for the product's rounding and
-// a step more (exact to fp32 where they matter, near the largest), quotients v_rcp_f32: with the device library's expf and
+// scheduling.  Exponentials are v_exp_f32 of a logit times log2(e) / tau, off by |x| 2^-23 of themselves for the two
+// products' roundings and a step more (exact to fp32 where they matter, near the largest), quotients v_rcp_f32: with the device library's expf and
 // divisions 65536 rows of 160 sigmoid scores took 45 us forward and 55 back (24 and 29 with these).
 #pragma once
 #include "kernels.hpp"
 
 namespace moe {
 
-MOE_DEV float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+constexpr float kLog2E = 1.4426950408889634f;
+
+// The larger, or NaN if one of them is (fmaxf passes over it).
+MOE_DEV float max_of_all(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 // v of lane l ^ X, any power of two below 64.
 template <int X>
@@ -49,7 +52,7 @@ MOE_DEV float group_reduce(float v, OP&& op) {
 template <int N>
 MOE_DEV float group_sum(float v) { return group_reduce<1, N>(v, [](float a, float b) { return a + b; }); }
 template <int N>
-MOE_DEV float group_max(float v) { return group_reduce<1, N>(v, [](float a, float b) { return fmaxf(a, b); }); }
+MOE_DEV float group_max(float v) { return group_reduce<1, N>(v, max_of_all); }
 
 enum { kScoreSoftmax = 0, kScoreSigmoid = 1 };
 
@@ -90,18 +93,18 @@ MOE_DEV void router_load(const T* row, int E, int j, float (&x)[S::C]) {
 
 // Of a row whose logits x are spread over S::LPR lanes: q and p, normalised, the largest logit m and the log of the sum, so
 // that lse = m / tau + log_sum.  The largest is taken off before the division by tau: logits of the type's lowest value
-// over a tau below 1 are beyond fp32, their differences are not.  Of an infinite m, p is NaN and lse m itself.
+// over a tau below 1 are beyond fp32, their differences are not.  Of an infinite m, p is NaN and lse m itself.  scale: log2(e) / tau.
 template <class S>
-MOE_DEV void router_scores(const float (&x)[S::C], int score, float inv_tau, float (&q)[S::C], float (&p)[S::C], float& m,
+MOE_DEV void router_scores(const float (&x)[S::C], int score, float scale, float (&q)[S::C], float (&p)[S::C], float& m,
                            float& log_sum) {
   m = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < S::C; ++i) m = fmaxf(m, x[i]);
+  for (int i = 0; i < S::C; ++i) m = max_of_all(m, x[i]);
   m = group_max<S::LPR>(m);
   float sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < S::C; ++i) {
-    p[i] = exp_of((x[i] - m) * inv_tau);
+    p[i] = __builtin_amdgcn_exp2f((x[i] - m) * scale);
     sum += p[i];
   }
   if (score == kScoreSoftmax) {
@@ -118,8 +121,9 @@ MOE_DEV void router_scores(const float (&x)[S::C], int score, float inv_tau, flo
     float total = 0.0f;
 #pragma unroll
     for (int i = 0; i < S::C; ++i) {
-      const float t = exp_of(-fabsf(x[i] * inv_tau));
-      q[i] = (x[i] > 0.0f ? 1.0f : m > 0.0f ? t : p[i]) * __builtin_amdgcn_rcpf(1.0f + t);
+      const float t = __builtin_amdgcn_exp2f(-fabsf(x[i]) * scale);
+      const float below = m > 0.0f ? t : p[i];
+      q[i] = (x[i] > 0.0f ? 1.0f : below) * __builtin_amdgcn_rcpf(1.0f + t);
       total += q[i];
     }
     sum = group_sum<S::LPR>(sum);
@@ -131,14 +135,7 @@ MOE_DEV void router_scores(const float (&x)[S::C], int score, float inv_tau, flo
       q[i] *= rq;
     }
   }
-  log_sum = logf(sum);
-  if (__any(isinf(m))) {  // sum is NaN there; the maximum passed over any NaN
-    float nan = 0.0f;
-#pragma unroll
-    for (int i = 0; i < S::C; ++i) nan += isnan(x[i]) ? x[i] : 0.0f;
-    nan = group_sum<S::LPR>(nan);
-    if (isinf(m)) log_sum = nan;
-  }
+  log_sum = isinf(m) ? 0.0f : logf(sum);
 }
 
 // Whether the row's token is real (all lanes of a wave call this; `in`: there is a row), and f(e) for each of its
@@ -210,6 +207,7 @@ __global__ __launch_bounds__(kRouterBlock) void k_router_losses(RouterRows<T, I>
   __shared__ int ns[NW];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, j = lane % S::LPR, sub = lane / S::LPR;
   const int E = in.E, k = in.k;
+  const float scale = in.inv_tau * kLog2E;
   const int64_t r0 = blockIdx.x * rpb, r1 = min(r0 + rpb, in.Tn);
   router_walk(in.offsets, in.S, r0, r1, [&](int s, int64_t a, int64_t b) {
     for (int e = tid; e < E; e += kRouterBlock) hist[e] = 0;
@@ -225,7 +223,7 @@ __global__ __launch_bounds__(kRouterBlock) void k_router_losses(RouterRows<T, I>
       float x[S::C], q[S::C], p[S::C], m, log_sum;
       router_load<S>(in.logits + at * E, E, j, x);
       const bool real = router_real<S>(in.idx + at * k, k, E, j, has, [&](int e) { atomicAdd(&hist[e], 1); });
-      router_scores<S>(x, in.score, in.inv_tau, q, p, m, log_sum);
+      router_scores<S>(x, in.score, scale, q, p, m, log_sum);
       if (real) {
 #pragma unroll
         for (int i = 0; i < S::C; ++i) acc[i] += q[i];
@@ -365,6 +363,7 @@ __global__ __launch_bounds__(kRouterBwdBlock) void k_router_losses_bwd(
   constexpr int NW = kRouterBwdBlock / 64;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, j = lane % S::LPR, sub = lane / S::LPR;
   const int E = in.E, k = in.k;
+  const float scale = in.inv_tau * kLog2E;
   const int64_t r0 = blockIdx.x * rpb, r1 = min(r0 + rpb, in.Tn);
   auto store = [&](int64_t row, const float (&d)[S::C]) {
 #pragma unroll
@@ -394,7 +393,7 @@ __global__ __launch_bounds__(kRouterBwdBlock) void k_router_losses_bwd(
       const bool real = router_real<S>(in.idx + at * k, k, E, j, has, [](int) {});
       // from the row's largest again, not from a kept lse: x - lse carries lse's rounding, |lse| 2^-24, which is all of log sum
       // where a row's logits are large (1 in each p of a row of the type's lowest value)
-      router_scores<S>(x, in.score, in.inv_tau, q, p, m, log_sum);
+      router_scores<S>(x, in.score, scale, q, p, m, log_sum);
       // h lse; where lse is beyond fp32 the product need not be
       const float lse = m * in.inv_tau + log_sum, hl = isinf(lse) ? h * in.inv_tau * m + h * log_sum : h * lse;
 #pragma unroll
@@ -405,7 +404,7 @@ __global__ __launch_bounds__(kRouterBwdBlock) void k_router_losses_bwd(
       for (int i = 0; i < S::C; ++i) {
         float t = q[i] * (g[i] - dot);
         if (in.score == kScoreSigmoid) {
-          const float e = exp_of(-fabsf(x[i] * in.inv_tau));
+          const float e = __builtin_amdgcn_exp2f(-fabsf(x[i]) * scale);
           t *= (x[i] > 0.0f ? e : 1.0f) * __builtin_amdgcn_rcpf(1.0f + e);
         }
         d[i] = !real ? 0.0f : h != 0.0f ? t + hl * p[i] : t;
