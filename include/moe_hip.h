@@ -396,7 +396,7 @@ moe_status moe_residual_norm_backward_from_input(int32_t device, void* stream, i
  * offsets[s + 1]; NULL: one sequence of all rows, S = 1) with n real tokens and M_e assignments to expert e:
  *   x = logits / temperature, q = softmax(x) or sigmoid(x) / sum sigmoid(x), P_e = sum q_te / n, f_e = M_e / (k n),
  *   balance[s] = E sum_e (switch_coef f_e P_e + sqprob_coef P_e^2), z[s] = sum logsumexp(x_t)^2 / n
- * (0 for n = 0), counts [S, E] = M_e.  temperature and its inverse are positive and finite in fp32, 1 <= E <= 1024,
+ * (0 for n = 0), counts [S, E] = M_e.  2^-126 <= temperature, finite; 1 <= E <= 1024,
  * 1 <= k <= 16, T k < 2^31, S < 2^22.  slope [S, E] (of balance in q_te) and inv_real [S] (1 / n, or 0): kept for a
  * backward, or NULL.  Offsets ascend within 0..T; with others no access leaves the tensors, but the results are not
  * defined. */

@@ -1,4 +1,6 @@
 // C ABI of the router's losses.  Declared in include/moe_hip.h.  The calls keep no state.
+#include <cfloat>
+
 #include "entry.hpp"
 #include "router.hpp"
 
@@ -17,9 +19,9 @@ moe_status check_router(int dtype, int64_t T, int E, int k, int index_bytes, int
   if (index_bytes != 4 && index_bytes != 8)
     return fail(MOE_ERR_INVALID, "index_bytes %d is neither 4 nor 8", index_bytes);
   if (score != kScoreSoftmax && score != kScoreSigmoid) return fail(MOE_ERR_INVALID, "unknown score %d", score);
-  // the kernels multiply by its inverse
-  if (!(tau > 0.0f) || !std::isfinite(tau) || !std::isfinite(1.0f / tau))
-    return fail(MOE_ERR_INVALID, "temperature must be positive and finite, its inverse too");
+  // the kernels multiply by log2(e) / tau
+  if (!(tau >= FLT_MIN) || !std::isfinite(tau))
+    return fail(MOE_ERR_INVALID, "temperature must be positive (at least 2^-126) and finite");
   if (offsets ? S < 0 : S != 1)
     return fail(MOE_ERR_INVALID, offsets ? "num_sequences is negative" : "num_sequences without offsets is not 1");
   if (S >= int64_t(1) << 22) return fail(MOE_ERR_UNSUPPORTED, "num_sequences reaches 2^22");

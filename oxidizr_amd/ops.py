@@ -576,9 +576,9 @@ def router_losses(logits, topk_idx, *, score: str = "softmax", temperature: floa
         raise ModelError(f"num_experts must be 1..{MAX_EXPERTS}, got {E}")
     if score not in SCORES:
         raise ModelError(f"score must be one of {SCORES}, got {score!r}")
-    # of float32, as its inverse
-    if not 2.0 ** -128 < temperature < 2.0 ** 128:
-        raise ModelError(f"temperature must be positive and finite, got {temperature}")
+    # as a float32, and its inverse
+    if not 2.0 ** -126 <= temperature < 2.0 ** 128:
+        raise ModelError(f"temperature must be positive (at least 2^-126) and finite, got {temperature}")
     S = 1
     if offsets is not None:
         if offsets.dim() != 1 or offsets.dtype != torch.int32 or offsets.numel() < 1:

@@ -147,3 +147,24 @@ def test_a_long_run_of_empty_sequences_does_not_hold_up_a_block():
     assert torch.equal(a, b)
     # 0.1 us a sequence and direction when each is loaded behind the other: 0.8 s, where the rest takes some 40 ms
     assert walked < 3 * quick + 20, (quick, walked)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("tau", [2.0 ** -126, 1e-30, 1e30, 3e38])
+def test_temperatures_at_the_ends_of_their_range(tau, score):
+    # whole numbers, and each row's largest alone: at the lowest temperatures all of its score (a sigmoid's: of each above 0),
+    # at the highest none of it
+    g = torch.Generator(device="cuda").manual_seed(3)
+    logits = torch.randint(-9, 8, (60, 24), device="cuda", generator=g).float()
+    logits[torch.arange(60), torch.randint(0, 24, (60,), device="cuda", generator=g)] = 8.0
+    idx = torch.randint(0, 24, (60, 2), device="cuda", generator=g)
+    out = ops.router_losses(logits, idx, score=score, temperature=tau, switch_coef=1.0, sqprob_coef=1.0)
+    if tau > 1:
+        q = torch.full((60, 24), 1 / 24, dtype=torch.float64, device="cuda")
+    else:
+        q = (logits == 8.0 if score == "softmax" else logits > 0).double() + 0.5 * (logits == 0) * (score == "sigmoid")
+        q = q / q.sum(1, keepdim=True)
+    P, f = q.mean(0), torch.bincount(idx.flatten(), minlength=24).double() / 120
+    want = float(24 * (f * P + P * P).sum())
+    # quotients, 60 additions and 24 terms in fp32
+    assert abs(float(out.balance) - want) <= 120 * U32 * want

@@ -8,9 +8,9 @@ from oxidizr_amd.moe import ModelError
 P = 1 << 20  # an aligned address that a refused call never touches
 
 
-@pytest.mark.parametrize("tau", [1e-60, 1e-45, 1e-39, 2.0 ** -128, 2.0 ** 128, 1e39])
+@pytest.mark.parametrize("tau", [1e-60, 1e-45, 1e-39, 2.0 ** -128, 2.0 ** -127, 1.1e-38, 2.0 ** 128, 1e39])
 def test_a_temperature_beyond_fp32_or_whose_inverse_is(tau):
-    # the scores were NaN: the kernels multiply by 1 / tau, and 0 times infinity is none
+    # the scores were NaN: the kernels multiply by log2(e) / tau, and 0 times infinity is none
     with pytest.raises(ModelError, match="temperature must be"):
         ops.router_losses(torch.zeros(4, 6), torch.zeros(4, 2, dtype=torch.int32), temperature=tau)
     L = _lib.load()
@@ -21,7 +21,7 @@ def test_a_temperature_beyond_fp32_or_whose_inverse_is(tau):
     assert b"temperature" in L.moe_last_error()
 
 
-@pytest.mark.parametrize("tau", [3e-39, 1e-38, 3e38])
+@pytest.mark.parametrize("tau", [2.0 ** -126, 1e-37, 3e38])
 def test_the_ends_are_accepted(tau):
     with pytest.raises(ModelError, match="CUDA"):  # the next check
         ops.router_losses(torch.zeros(4, 6), torch.zeros(4, 2, dtype=torch.int32), temperature=tau)
