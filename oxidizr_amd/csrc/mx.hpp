@@ -425,7 +425,8 @@ __global__ __launch_bounds__(C::THREADS) void k_mx_dgrad(const bf16_t* __restric
 
 // The element-wise part of a backward, as k_linear_dz and k_linear_db, their chunks found from the offsets: 12000 rows of
 // 1368 in 12 groups 22 us and 4.8, where prefixes from a launch before them made 18 and 4.7 and cost 5.2 and a gap (the whole forward
-// and backward 188 -> 176).  Bound by reading dy and z and writing dz, 98 MB.  chunks: those that `part` holds.
+// and backward 188 -> 176).  98 MB of reading dy and z and writing dz take 19 at a copy's rate; the scan, and a thread's two rows one
+// behind the other, are the rest.  chunks: those that `part` holds.
 static __global__ __launch_bounds__(256) void k_mx_dz(const bf16_t* __restrict__ dY, const bf16_t* __restrict__ pre, int act,
                                                       MxRows r, int N, bf16_t* __restrict__ dZ, float* __restrict__ part) {
   const int chunk = blockIdx.x;
@@ -548,7 +549,8 @@ struct MxScaleStager {
 };
 
 // As mainloop_dma, with scales.  A k-tile of 256 x 256 x 256 takes some 2.1 us: 1.13 of matrix instructions at their rate from registers
-// (7.6 PFLOP/s), 1.4 to 1.7 with the fragments' reads and no direct loads, the rest for those (64 KB into LDS).  65536 rows in 128
+// (7.6 PFLOP/s), 1.4 to 1.7 with the fragments' reads and no direct loads, the rest for those (64 KB into LDS), which are waited
+// for in every k-tile (below).  65536 rows in 128
 // experts, 4096 -> 1536, 343 us (2.4 PFLOP/s): with the next k-tile requested only behind the last k-step 392; k-tiles half as deep in
 // four stages 393 -> 439.  OUT, the results' type, only sets the instantiations of two kernels apart: hipcc's host
 // pass takes the second use of one as an error.
@@ -632,7 +634,9 @@ MOE_DEV void mainloop_mxmx(f32x16 (&acc)[1][C::TN][C::TM], const OpDesc<bf16_t>&
     }
     // Last k-step, whose fragments are read.  Behind a first barrier no wave reads this k-tile's stage again, and
     // its refill is issued over the first half of the step's products; behind a second one the next k-tile has landed,
-    // whose refill was issued a k-tile ago: two k-tiles' loads are in flight meanwhile.
+    // whose refill was issued a k-tile ago.  The counted wait would leave the refill in flight, but with the scales in an
+    // LDS array of their own hipcc puts a vmcnt(0) before the next k-tile's first fragment: the refill is waited for in
+    // full half a k-step behind its issue, and further stages hide nothing.
     constexpr int H = (C::TN + 1) / 2;
     lds_barrier();
 #pragma unroll

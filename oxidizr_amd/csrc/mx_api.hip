@@ -89,7 +89,9 @@ bool mx_skinny(bool four, int64_t M, int K, int N, int E, bool grouped) {
 // 26 (44); 1999 of one weight, 2784 -> 2056 45 / 48 / 56 (57); 512 of 4096 -> 4096 50 / 45 / 35 (80); 1024 60 / 50 / 52 (81); their input
 // gradients 115 / 133 / 181 (120), 893 / 1107 / 1561, 66 / 75 / 98 (78), 92 / 83 / 107, 38 / 29 / 40, 42 / 38 / 59 (53), 65 / 54 / 43
 // (96), 66 / 54 / 59 (96).  Both sides in 4 bits 44 / 45 / 62, 343 / 402 / 571, 46 / 48 / 44 (51), 40 / 40 / 43, 16 / 14 / 13 (20), 22 / 21 / 25 (26), 18 / 17 / 18 (29), 20 / 22 /
-// 21 (31).
+// 21 (31).  (Those are of the loop as it stands, which waits for all its loads in each k-tile: mainloop_mxmx.)
+// An input gradient takes tiles at any number of rows: 512 rows in 128 experts of 1536 x 4096 195 us, where the stream of few
+// rows gives the forward in 88; 64 rows there 87 and 39, 256 rows in 256 experts of 768 x 2048 69 and 32.
 enum class MxTiles { kBig, kMid, kSmall };
 MxTiles mx_tiles(bool four, bool grouped, int E, int64_t M, int N) {
   const int groups = grouped ? (int)std::min<int64_t>(E, M) : 1;

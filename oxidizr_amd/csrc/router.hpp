@@ -12,8 +12,9 @@
 //
 // Each direction reads the logits once.  The forward keeps a lane's columns in registers and adds them
 // up over the rows of its block; the blocks' sums are added in block order, so no result depends on
-// scheduling.  Exponentials are v_exp_f32 of a logit times log2(e) / tau, off by |x| 2^-23 of themselves for the two
-// products' roundings and a step more (exact to fp32 where they matter, near the largest), quotients v_rcp_f32: with the device library's expf and
+// scheduling.  Sums within a block are fp32 (some 1e-7 of a loss), those over blocks 64 bits.  Exponentials are v_exp_f32
+// of a logit times log2(e) / tau, off by |x| 2^-23 of themselves for the factor's and the product's roundings and a step
+// more (exact to fp32 where they matter, near the largest), quotients v_rcp_f32: with the device library's expf and
 // divisions 65536 rows of 160 sigmoid scores took 45 us forward and 55 back (24 and 29 with these).
 #pragma once
 #include "kernels.hpp"
@@ -75,6 +76,8 @@ struct RouterShape {
   static constexpr int COLS = C * LPR;        // columns held, E at most
 };
 
+// A row's chunks.  bf16 ones are converted where they are loaded, in a branch each, so hipcc waits for every chunk before the
+// next is requested; fp32 ones are in flight together.
 template <class S, typename T>
 MOE_DEV void router_load(const T* row, int E, int j, float (&x)[S::C]) {
 #pragma unroll
@@ -190,9 +193,10 @@ MOE_DEV void router_walk(const int* offsets, int S, int64_t r0, int64_t r1, F&& 
 // ------------------------------------------------------------------ forward
 // Block b takes rows [b rpb, (b + 1) rpb) and writes, for each sequence s that has rows there, its column sums
 // of q, its counts and (z sum, real tokens) to slot b + s: such pairs ascend in both, so no two share a slot.
-// Bound by arithmetic (an exponential and some ten operations an element; a sigmoid two and twenty) on long inputs, by a launch and one
-// round trip on short ones: 65536 x 160 bf16 sigmoid scores in 48 sequences 24 us (0.9 TB/s), 8192 x 256 fp32 softmax 5.0 (1.7 TB/s).
-// More rows to a block leave the reduction fewer slots and the CUs idle: one block to a CU.
+// Bound by round trips to memory: nothing of a step's rows is requested before the step, the indices are loaded behind the
+// logits, and bf16 rows' chunks (router_load) one behind the other: 65536 x 160 bf16 sigmoid scores in 48 sequences 24 us (0.9
+// TB/s; the loop's instructions some 9), 8192 x 256 fp32 softmax 5.1 (1.7 TB/s).  More rows to a block leave the reduction fewer
+// slots and the CUs idle: one block to a CU.
 constexpr int kRouterBlock = 512;
 template <class S, typename T, typename I>
 __global__ __launch_bounds__(kRouterBlock) void k_router_losses(RouterRows<T, I> in, int64_t rpb,
@@ -353,7 +357,7 @@ __global__ __launch_bounds__(1024) void k_router_reduce(const float* __restrict_
 }
 
 // ------------------------------------------------------------------ backward
-// As the forward bound by arithmetic: 65536 x 160 bf16 sigmoid scores 29 us, 8192 x 256 fp32 softmax 8.0 (2.1 TB/s).
+// As the forward bound by round trips: 65536 x 160 bf16 sigmoid scores 29 us, 8192 x 256 fp32 softmax 8.2 (2.0 TB/s).
 // Block b: rows [b rpb, (b + 1) rpb) over four waves.  slope: of balance in q, [S, E].  d_balance, d_z: [S], or null (0).
 constexpr int kRouterBwdBlock = 256;
 template <class S, typename T, typename I>

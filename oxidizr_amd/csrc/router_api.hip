@@ -28,7 +28,9 @@ moe_status check_router(int dtype, int64_t T, int E, int k, int index_bytes, int
   return MOE_OK;
 }
 
-// Calls f(shape) of the narrowest wave shape that holds E columns.
+// Calls f(shape) of the narrowest wave shape that holds E columns.  A width inside a step costs up to a sixth more an
+// element than at its end: 65536 rows of 160, 192 and 256 bf16 sigmoid scores 17, 22 and 25 us forward and 23, 31 and 34 back,
+// of 256, 384 and 512 25, 40 and 45, and 34, 51 and 56 (fp32 softmax 15, 22 and 25, and 28, 38 and 48).
 template <class F>
 void with_router_shape(int E, F&& f) {
   if (E % 4 == 0) {
